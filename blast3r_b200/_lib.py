@@ -10,7 +10,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libb3r.so')
 
 B3R_OK = 0
-B3R_F32, B3R_F64 = 0, 1
+B3R_F32, B3R_F64, B3R_BF16, B3R_F16 = 0, 1, 2, 3
+NORM_LAYER, NORM_RMS = 0, 1
 ENABLE_ALL, ENABLE_ZERO, ENABLE_MASK = 0, 1, 2
 PASS_PREP, PASS_POINTS, PASS_FACTOR, PASS_DIAG, PASS_PAIRS = 0, 1, 2, 3, 4
 PASS_ELIMINATE = PASS_FACTOR   # former name
@@ -63,6 +64,31 @@ class Outputs(C.Structure):
                 ('residuals', _vp), ('loss', _vp)]
 
 
+class RotaryPart(C.Structure):
+    _fields_ = [('x', _vp), ('out', _vp), ('x_batch', _i64), ('x_token', _i64), ('x_head', _i64),
+                ('out_batch', _i64), ('out_token', _i64), ('out_head', _i64), ('heads', _i32), ('reserved', _i32)]
+
+
+class ResidualNorm(C.Structure):
+    _fields_ = [('rows', _i64), ('rows_per_gate', _i64), ('C', _i32), ('kind', _i32), ('dtype', _i32),
+                ('stream_dtype', _i32), ('weight_dtype', _i32), ('post', _i32), ('pre', _i32), ('eps', _f32),
+                ('residual_scale', _f32), ('w_post', _vp), ('b_post', _vp), ('gate', _vp), ('w_pre', _vp),
+                ('b_pre', _vp)]
+
+
+class AttnTensor(C.Structure):
+    _fields_ = [('p', _vp), ('batch', _i64), ('row', _i64), ('head', _i64)]
+
+
+class AttentionDesc(C.Structure):
+    _fields_ = [('B', _i32), ('Lq', _i32), ('Lk', _i32), ('Hq', _i32), ('Hkv', _i32), ('D', _i32), ('dtype', _i32),
+                ('causal', _i32), ('Tq', _i64), ('Tk', _i64), ('scale', _f32), ('reserved', _i32),
+                ('q_lens', _vp), ('k_lens', _vp), ('cu_q', _vp), ('cu_k', _vp),
+                ('q', AttnTensor), ('k', AttnTensor), ('v', AttnTensor), ('o', AttnTensor), ('lse', AttnTensor),
+                ('d_o', AttnTensor), ('dq', AttnTensor), ('dk', AttnTensor), ('dv', AttnTensor),
+                ('work', _vp), ('status', _vp)]
+
+
 # name -> (restype, argtypes)
 _SIGS = {
     'b3r_last_error': (C.c_char_p, []),
@@ -106,6 +132,15 @@ _SIGS = {
     'b3r_tangent_prior': (C.c_int, [_vp, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _f64, _f64, _i32, _i32, _vp,
                                     _vp, _vp, _vp]),
     'b3r_lin_add_zprior': (C.c_int, [_vp, _vp, _vp, _vp, C.POINTER(Outputs), _vp]),
+    'b3r_rotary': (C.c_int, [C.POINTER(RotaryPart), C.c_int, _i64, _i64, C.c_int, C.c_int, _vp, C.c_int, C.c_int,
+                             C.c_int, _vp, C.c_int, _i64, _i64, C.c_int, C.c_int, _vp]),
+    'b3r_residual_norm_fwd': (C.c_int, [C.POINTER(ResidualNorm), _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
+    'b3r_residual_norm_work_bytes': (_i64, [C.POINTER(ResidualNorm)]),
+    'b3r_residual_norm_bwd': (C.c_int, [C.POINTER(ResidualNorm), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64] + [_vp] * 9),
+    'b3r_attention_fwd_work_bytes': (_i64, [C.POINTER(AttentionDesc)]),
+    'b3r_attention_fwd': (C.c_int, [C.POINTER(AttentionDesc), _vp]),
+    'b3r_attention_bwd_work_bytes': (_i64, [C.POINTER(AttentionDesc)]),
+    'b3r_attention_bwd': (C.c_int, [C.POINTER(AttentionDesc), _vp]),
     'b3r_pcg_ex': (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, _f64, C.c_int, _i64, C.c_int, _vp, _vp, _vp]),
 }
 

@@ -37,6 +37,8 @@ extern "C" {
 
 #define B3R_F32 0
 #define B3R_F64 1
+#define B3R_BF16 2
+#define B3R_F16 3
 
 /* Message of the last failed call on the calling thread ("" if none). */
 const char* b3r_last_error(void);
@@ -445,6 +447,111 @@ int b3r_schur_spmv_f64(const b3r_plan* plan, const float* S_vals, const double* 
  * delta_c: [n_cam_params]; delta_p: [n_points*3], only this rank's tracks written. */
 int b3r_backsub(b3r_plan* plan, const b3r_params* params, const b3r_lin_opts* opts, void* workspace,
                 const float* delta_c, float* delta_p, void* stream);
+
+/* ===================================================================================
+ * Part 5 -- operators of a transformer block
+ *
+ * The network whose depth channels the bundle adjustment refines runs on the same GPU, frame
+ * after frame.  These are the operators of one of its blocks that libraries leave in pieces:
+ * rotary positions, attention with the backward pass that recomputes the probabilities, and the
+ * norms around a residual connection.  dtype: B3R_BF16, B3R_F16 or, where stated, B3R_F32.
+ * Strides are in elements; the innermost dimension is contiguous.
+ * =================================================================================== */
+
+/* One tensor of a rotary call: [B, T, heads, D] in x, written to out (x itself for in place,
+ * with the same strides; other overlaps are not allowed). */
+typedef struct {
+    const void* x;
+    void* out;
+    int64_t x_batch, x_token, x_head;
+    int64_t out_batch, out_token, out_head;
+    int32_t heads, reserved;
+} b3r_rotary_part;
+
+/* Rotary positions of one or two tensors (queries and keys) in one launch.  The first
+ * axes * 2 * half elements of each head are `axes` sections; section a holds `half` pairs,
+ * (k, half + k) or, if interleaved, (2k, 2k + 1), and pair k turns by the angle whose (cosine,
+ * sine) is table[p][k], table float [n_pos, half, 2], p = positions[b * pos_batch +
+ * t * pos_token + a] (int32, or int64 if pos_is_64; pos_batch 0 shares them over the batch).
+ * inverse turns back, which is the gradient of the forward call.  Elements past the sections
+ * are copied.  A position outside of the table gives NaN in its section.  dtype B3R_F32,
+ * B3R_BF16 or B3R_F16; the arithmetic is float32, rounded once.  Interleaved pairs must be
+ * aligned to a pair (even strides). */
+int b3r_rotary(const b3r_rotary_part* parts, int n_parts, int64_t B, int64_t T, int D, int dtype, const float* table,
+               int n_pos, int half, int axes, const void* positions, int pos_is_64, int64_t pos_batch,
+               int64_t pos_token, int interleaved, int inverse, void* stream);
+
+#define B3R_NORM_LAYER 0
+#define B3R_NORM_RMS 1
+
+/* The norms before and after a block with its gate and residual scale, over rows of C channels:
+ *     n = post ? N(y; w_post, b_post) : y,   r = residual_scale * x + g n,   h = N(r; w_pre, b_pre)
+ * N: layer norm or root-mean-square norm with eps.  Weights and biases may be NULL (1 and 0).
+ * gate: [rows / rows_per_gate, C] or NULL (1): one row for all (a channel scale), one per sequence,
+ * or one per row.  y, h have dtype; x, r have stream_dtype (dtype or B3R_F32); weights, biases,
+ * gate and their gradients have weight_dtype (dtype or B3R_F32).  C <= 8192.  Sums are float32;
+ * h is computed from r before r is rounded.  Outputs are contiguous rows. */
+typedef struct {
+    int64_t rows, rows_per_gate;
+    int32_t C, kind, dtype, stream_dtype, weight_dtype, post, pre;
+    float eps, residual_scale;
+    const void *w_post, *b_post, *gate, *w_pre, *b_pre;
+} b3r_residual_norm;
+
+int b3r_residual_norm_fwd(const b3r_residual_norm* d, const void* y, int64_t y_row, const void* x, int64_t x_row,
+                          void* r, void* h, void* stream);
+
+/* Gradients, from dr (what reaches r past h), dh (NULL without the norm of r), y (NULL if there is
+ * neither a norm of y nor a gate) and r as the forward call wrote it: dx (stream_dtype), dy (dtype),
+ * dgate (as gate), and the column sums dw_post, db_post, dw_pre, db_pre (each may be NULL).  The
+ * statistics are recomputed.  The sums over rows are float32 in a fixed order (no atomics).
+ * Without rows the column sums are cleared and dgate is not written.
+ * work: 256-byte aligned, b3r_residual_norm_work_bytes(d) bytes (-1: bad descriptor). */
+int64_t b3r_residual_norm_work_bytes(const b3r_residual_norm* d);
+int b3r_residual_norm_bwd(const b3r_residual_norm* d, const void* dr, int64_t dr_row, const void* dh, int64_t dh_row,
+                          const void* y, int64_t y_row, const void* r, int64_t r_row, void* dx, void* dy, void* dgate,
+                          void* dw_post, void* db_post, void* dw_pre, void* db_pre, void* work, void* stream);
+
+/* Attention over B sequences with Hq query heads and Hkv key/value heads (Hq a multiple of Hkv;
+ * query head h uses head h / (Hq / Hkv)), head size D (a multiple of 8, at most 128), dtype B3R_BF16
+ * or B3R_F16:
+ *     S_ij = scale q_i . k_j,   lse_i = log sum_j exp S_ij,   o_i = sum_j exp(S_ij - lse_i) v_j
+ * over the keys j that query i sees: j < k_len and, if causal, j <= i + k_len - q_len (the last
+ * query sees the last key).  A query that sees none has o = 0, lse = -inf and zero gradients.
+ * Two layouts:
+ *   padded: sequence b is q[b, 0..q_len) of Lq rows and k[b, 0..k_len) of Lk; q_lens / k_lens (device
+ *     int32 [B]) or NULL (all of them).  Rows past q_len get o = 0, lse = -inf, dq = 0, rows
+ *     past k_len dk = dv = 0.
+ *   packed: cu_q, cu_k (device int32 [B + 1], not NULL) hold where each sequence begins and ends
+ *     among Tq / Tk rows; the batch strides are not used and Lq / Lk bound the lengths.
+ * What lies in rows past a sequence's end is not used, NaN included.  Lengths and offsets
+ * outside of the tensors are cut to them.  Strides (batch, row, head) in elements, multiples
+ * of 8, with 16-byte aligned bases; lse is float with strides of its own. */
+typedef struct {
+    const void* p;
+    int64_t batch, row, head;
+} b3r_attn_tensor;
+
+typedef struct {
+    int32_t B, Lq, Lk, Hq, Hkv, D, dtype, causal;
+    int64_t Tq, Tk;
+    float scale;
+    int32_t reserved;
+    const int32_t *q_lens, *k_lens, *cu_q, *cu_k;
+    b3r_attn_tensor q, k, v, o, lse;
+    b3r_attn_tensor d_o, dq, dk, dv; /* backward only */
+    void* work;                      /* 256-byte aligned, b3r_attention_*_work_bytes bytes */
+    int32_t* status;                 /* device int32 or NULL: set to 1 if a wait inside a kernel ran
+                                      * out (the outputs are then NaN) */
+} b3r_attention_desc;
+
+/* o and lse are outputs. */
+int64_t b3r_attention_fwd_work_bytes(const b3r_attention_desc* d);
+int b3r_attention_fwd(const b3r_attention_desc* d, void* stream);
+/* o and lse are the forward call's; dq, dk, dv are outputs.  The gradients of a shared head are
+ * summed in float32 in a fixed order (no atomics). */
+int64_t b3r_attention_bwd_work_bytes(const b3r_attention_desc* d);
+int b3r_attention_bwd(const b3r_attention_desc* d, void* stream);
 
 #ifdef __cplusplus
 }
