@@ -49,7 +49,7 @@ def _readable(t):
     """t itself where the kernels can read it: the head size contiguous, the other strides and the
     base multiples of 16 bytes; a copy otherwise."""
     if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n != 1) \
-            and all(s >= 0 for s in t.stride()):
+            and all(s > 0 for s, n in zip(t.stride(), t.shape) if n != 1):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -80,6 +80,8 @@ def _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k):
         raise RuntimeError(f'attention: the head size is a multiple of 8 up to 128, got {D}')
     if Hkv < 1 or Hq < 1 or Hq % Hkv:
         raise RuntimeError(f'attention: {Hq} query heads do not share {Hkv} key/value heads evenly')
+    if scale is not None and not scale > 0:
+        raise RuntimeError(f'attention: the scale must be positive, got {scale}')
     keep = []
     d = L.AttentionDesc(Hq=Hq, Hkv=Hkv, D=D, dtype=DTYPES[q.dtype], causal=int(bool(causal)),
                         scale=D ** -0.5 if scale is None else float(scale))

@@ -1,7 +1,4 @@
-// Part 5 of the C ABI: attention and its backward pass.
-//
-// Forward, per query row: the running maximum m and sum l of exp(S - m) over the keys, the
-// output rescaled when m grows; o = acc / l, lse = m + log l.  Backward, with P = exp(S - lse):
+// Part 5 of the C ABI: attention's argument checks and its backward pass, with P = exp(S - lse):
 //   delta = do . o,  dv = P^T do,  dP = do v^T,  dS = P (dP - delta),  dq = scale dS k,  dk = scale dS^T q
 // A warp owns a row: a query row forward and for dq, a key row for dk and dv, which walks over the
 // queries of all heads that share it.  Lanes own keys (queries) for the scores and
@@ -11,27 +8,66 @@
 
 namespace b3r {
 
-int attn_check(const b3r_attention_desc* d, bool backward) {
+int attn_check_sizes(const b3r_attention_desc* d) {
   B3R_REQUIRE(d, "attention: NULL descriptor");
   B3R_REQUIRE(d->dtype == B3R_BF16 || d->dtype == B3R_F16, "attention: dtype must be bf16 or f16");
   B3R_REQUIRE(d->B >= 0 && d->Lq >= 0 && d->Lk >= 0 && d->Tq >= 0 && d->Tk >= 0, "attention: negative size");
   B3R_REQUIRE(d->D >= 8 && d->D <= 128 && d->D % 8 == 0, "attention: the head size is a multiple of 8 up to 128, got %d", d->D);
   B3R_REQUIRE(d->Hq >= 1 && d->Hkv >= 1 && d->Hq % d->Hkv == 0, "attention: %d query heads do not share %d key/value heads evenly",
               d->Hq, d->Hkv);
+  // rows (queries x heads of a group) and the blocks' indices are 32-bit integers
+  B3R_REQUIRE(d->Tq <= 0x7fffffff && d->Tk <= 0x7fffffff && (int64_t)d->Lq * (d->Hq / d->Hkv) <= 0x7fffff00 && d->Lk <= 0x7fffff00,
+              "attention: more rows than 32-bit indices reach");
+  B3R_REQUIRE((int64_t)d->B * d->Hq <= 65535, "attention: more than 65535 sequences x heads");
+  return B3R_OK;
+}
+
+int attn_check(const b3r_attention_desc* d, bool backward) {
+  B3R_TRY(attn_check_sizes(d));
+  B3R_REQUIRE(d->scale > 0.f, "attention: the scale must be positive");
   B3R_REQUIRE((d->cu_q == nullptr) == (d->cu_k == nullptr), "attention: packed sequences need cu_q and cu_k");
   B3R_REQUIRE(!d->cu_q || (!d->q_lens && !d->k_lens), "attention: packed sequences have no q_lens or k_lens");
-  B3R_REQUIRE(d->Tq <= 0x7fffffff && d->Tk <= 0x7fffffff, "attention: more than 2^31 - 1 rows");
   const b3r_attn_tensor* ts[] = {&d->q, &d->k, &d->v, &d->o, &d->d_o, &d->dq, &d->dk, &d->dv};
-  const bool rows_q = d->B > 0 && (d->cu_q ? d->Tq : d->Lq) > 0, rows_k = d->B > 0 && (d->cu_q ? d->Tk : d->Lk) > 0;
+  const int64_t nq = d->cu_q ? d->Tq : d->Lq, nk = d->cu_q ? d->Tk : d->Lk;
   for (int i = 0; i < (backward ? 8 : 4); ++i) {
-    const bool of_k = i == 1 || i == 2 || i >= 6, any = of_k ? rows_k : rows_q;
-    B3R_REQUIRE(!any || ts[i]->p, "attention: NULL tensor");
+    const bool of_k = i == 1 || i == 2 || i >= 6;
+    const int64_t rows = of_k ? nk : nq, heads = of_k ? d->Hkv : d->Hq;
+    if (d->B == 0 || rows == 0) continue;
+    B3R_REQUIRE(ts[i]->p, "attention: NULL tensor");
     B3R_REQUIRE(((uintptr_t)ts[i]->p & 15) == 0, "attention: tensors must be 16-byte aligned");
-    B3R_REQUIRE((ts[i]->row % 8 == 0 || (of_k ? d->Lk : d->Lq) <= 1) && (ts[i]->head % 8 == 0 || (of_k ? d->Hkv : d->Hq) == 1) &&
-                    (ts[i]->batch % 8 == 0 || d->B <= 1),
-                "attention: strides must be multiples of 8 elements");
+    auto ok = [](int64_t stride, int64_t n) { return n <= 1 || (stride > 0 && stride % 8 == 0); };
+    B3R_REQUIRE(ok(ts[i]->row, rows) && ok(ts[i]->head, heads) && (d->cu_q || ok(ts[i]->batch, d->B)),
+                "attention: strides must be positive multiples of 8 elements");
   }
-  B3R_REQUIRE(!rows_q || d->lse.p, "attention: NULL lse");
+  B3R_REQUIRE(d->B == 0 || nq == 0 || d->lse.p, "attention: NULL lse");
+  return B3R_OK;
+}
+
+int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype) {
+  typedef CUresult (*encode_t)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const encode_t encode = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess)
+      f = nullptr;
+    return reinterpret_cast<encode_t>(f);
+  }();
+  if (!encode) return fail(B3R_E_CUDA, "attention: the driver has no cuTensorMapEncodeTiled");
+  if (rows == 0) {                     // no keys: no load is issued, the map is never read
+    *map = CUtensorMap{};
+    return B3R_OK;
+  }
+  // the stride of a dimension of one is not used, but has to be a valid one
+  const int64_t row = rows > 1 ? t.row : 128, head = heads > 1 ? t.head : 128, bat = batch > 1 ? t.batch : 128;
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
+  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)bat * 2};
+  const cuuint32_t box[4] = {64, 128, 1, 1}, step[4] = {1, 1, 1, 1};
+  const CUresult rc = encode(map, dtype == B3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
+                             const_cast<void*>(t.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return fail(B3R_E_CUDA, "attention: cuTensorMapEncodeTiled failed (%d)", (int)rc);
   return B3R_OK;
 }
 
@@ -50,50 +86,6 @@ __device__ __forceinline__ float dot(const T* a, const T* b, int D) {
     for (int j = 0; j < 8; ++j) s += f_of(x[j]) * f_of(y[j]);
   }
   return s;
-}
-
-__device__ __forceinline__ float warp_max(float x) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-  return x;
-}
-__device__ __forceinline__ float warp_sum(float x) {
-#pragma unroll
-  for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-  return x;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) k_attn_fwd_rows(const __grid_constant__ b3r_attention_desc d) {
-  const int lane = threadIdx.x & 31;
-  const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), h = blockIdx.y % d.Hq, b = blockIdx.y / d.Hq;
-  const AttnSeq s = attn_seq(d, b);
-  if (i >= (d.cu_q ? s.ql : d.Lq)) return;
-  const int kv = h / (d.Hq / d.Hkv), bound = i < s.ql ? attn_bound(s, i, d.causal) : 0;
-  const T* q = attn_row<const T>(d.q, b, s.q0 + i, h);
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int j0 = 0; j0 < bound; j0 += 32) {
-    const int j = j0 + lane;
-    const float x = j < bound ? d.scale * dot(q, attn_row<const T>(d.k, b, s.k0 + j, kv), d.D) : -INFINITY;
-    const float mn = fmaxf(m, warp_max(x)), base = mn == -INFINITY ? 0.f : mn;
-    const float p = j < bound ? expf(x - base) : 0.f, c = expf(m - base);
-    m = mn;
-    l = l * c + warp_sum(p);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) acc[k] *= c;
-    for (int t = 0; t < min(32, bound - j0); ++t) {
-      const float pt = __shfl_sync(0xffffffffu, p, t);
-      const T* v = attn_row<const T>(d.v, b, s.k0 + j0 + t, kv);
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (lane + 32 * k < d.D) acc[k] += pt * f_of(v[lane + 32 * k]);
-    }
-  }
-  T* o = attn_row<T>(d.o, b, s.q0 + i, h);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    if (lane + 32 * k < d.D) o[lane + 32 * k] = t_of<T>(bound > 0 ? acc[k] / l : 0.f);
-  if (lane == 0) *attn_row<float>(d.lse, b, s.q0 + i, h) = bound > 0 ? m + logf(l) : -INFINITY;
 }
 
 template <typename T>
@@ -193,23 +185,10 @@ int bwd_rows(const b3r_attention_desc& d, cudaStream_t s) {
 
 using namespace b3r;
 
-extern "C" int64_t b3r_attention_fwd_work_bytes(const b3r_attention_desc* d) { return d ? 0 : -1; }
-
-extern "C" int b3r_attention_fwd(const b3r_attention_desc* d, void* stream) {
-  B3R_TRY(attn_check(d, false));
-  if (d->B == 0 || d->Lq == 0) return B3R_OK;
-  B3R_REQUIRE((int64_t)d->B * d->Hq <= 65535, "attention: more than 65535 sequences x heads");
-  const dim3 grid((d->Lq + kWarps - 1) / kWarps, d->B * d->Hq);
-  if (d->dtype == B3R_BF16) k_attn_fwd_rows<__nv_bfloat16><<<grid, 32 * kWarps, 0, as_stream(stream)>>>(*d);
-  else k_attn_fwd_rows<__half><<<grid, 32 * kWarps, 0, as_stream(stream)>>>(*d);
-  return check_launch("attention");
-}
-
 extern "C" int64_t b3r_attention_bwd_work_bytes(const b3r_attention_desc* d) { return d ? 0 : -1; }
 
 extern "C" int b3r_attention_bwd(const b3r_attention_desc* d, void* stream) {
   B3R_TRY(attn_check(d, true));
   if (d->B == 0) return B3R_OK;
-  B3R_REQUIRE((int64_t)d->B * d->Hq <= 65535, "attention: more than 65535 sequences x heads");
   return d->dtype == B3R_BF16 ? bwd_rows<__nv_bfloat16>(*d, as_stream(stream)) : bwd_rows<__half>(*d, as_stream(stream));
 }

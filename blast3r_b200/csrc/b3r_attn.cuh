@@ -1,5 +1,6 @@
 // What the attention kernels share: a sequence's place in the tensors, and the argument checks.
 #pragma once
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "b3r_status.h"
@@ -51,7 +52,11 @@ __device__ __forceinline__ __nv_bfloat16 t_of<__nv_bfloat16>(float x) { return _
 template <>
 __device__ __forceinline__ __half t_of<__half>(float x) { return __float2half_rn(x); }
 
-// The argument checks of both directions; `empty`: nothing to do beyond clearing outputs.
+// The argument checks: of the sizes alone, and of everything that a direction reads or writes.
+int attn_check_sizes(const b3r_attention_desc* d);
 int attn_check(const b3r_attention_desc* d, bool backward);
+
+// The tensor map of a (D, rows, heads, batch) tensor in boxes of 64 elements x 128 rows.
+int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype);
 
 }  // namespace b3r

@@ -1,0 +1,157 @@
+// Blackwell building blocks of the attention kernels: bounded mbarrier waits, TMA tile loads,
+// tcgen05 matrix products with accumulators (and left operands) in tensor memory.
+//
+// Tiles in shared memory are rows of 64 16-bit elements (128 bytes) in the 128-byte swizzle that
+// TMA writes: the 16-byte chunk c of row r lies at chunk c ^ (r & 7).  A tile of 128 rows
+// and a head size above 64 is two such blocks, 16 KB apart.
+#pragma once
+#include <cuda.h>
+#include <cstdint>
+
+namespace b3r {
+
+constexpr int kTileRows = 128;
+constexpr int kBlockBytes = kTileRows * 128;   // 128 rows of 64 elements
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// ---- mbarriers.  No wait is endless: after its limit it raises `dead`, which ends the later
+// waits of every role at once; the loops all have fixed counts, so the kernel then runs to its
+// end, frees its tensor memory and reports the failure.
+__device__ __forceinline__ void mbar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.shared::cta.b64 t, [%0];\n\t}" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("{\n\t.reg .b64 t;\n\tmbarrier.arrive.expect_tx.shared::cta.b64 t, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+constexpr int kWaitLimit = 1 << 22;   // polls; seconds, where a wait takes microseconds
+__device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+  if (mbar_try(bar, parity)) return;
+  for (int n = 0; n < kWaitLimit; ++n) {
+    if (mbar_try(bar, parity)) return;
+    if ((n & 255) == 255 && *dead) return;
+  }
+  *dead = 1;
+}
+
+// ---- TMA: one box of 64 elements x 128 rows of a (D, rows, heads, batch) tensor
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int d0, int row, int head, int batch, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(d0), "r"(row), "r"(head), "r"(batch), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// ---- tcgen05
+__device__ __forceinline__ void tc_alloc(uint32_t where, int cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(cols) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tc_free(uint32_t tmem, int cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols));
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
+      "l"(b), "r"(idesc), "r"((int)acc)
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]: row i of A in lane i, two elements to a column
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
+      "l"(b), "r"(idesc), "r"((int)acc)
+      : "memory");
+}
+
+// Shared-memory operand descriptors (128-byte swizzle).
+// k-major: the product runs along the 64 elements of a row; 8-row groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+// mn-major: the product runs along the rows (8-row groups 1024 bytes apart); blocks of 64
+// elements of the other dimension lie kBlockBytes apart.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(kBlockBytes >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+         (uint64_t(2) << 61);
+}
+// Instruction descriptor: float32 accumulator, both operands bf16 or both f16.
+__host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int M, int N, bool b_mn) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(M >> 4) << 24);
+}
+
+#define B3R_R4(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3])
+#define B3R_R16(a, i) B3R_R4(a, i), B3R_R4(a, i + 4), B3R_R4(a, i + 8), B3R_R4(a, i + 12)
+#define B3R_W4(a, i) "r"(a[i]), "r"(a[i + 1]), "r"(a[i + 2]), "r"(a[i + 3])
+#define B3R_W16(a, i) B3R_W4(a, i), B3R_W4(a, i + 4), B3R_W4(a, i + 8), B3R_W4(a, i + 12)
+
+// 32 columns of this thread's lane (the warp's quarter of the 128 lanes).  The registers hold the
+// values only after tc_wait_ld().
+__device__ __forceinline__ void tc_ld32(uint32_t tmem, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : B3R_R16(r, 0), B3R_R16(r, 16)
+      : "r"(tmem));
+}
+__device__ __forceinline__ void tc_st32(uint32_t tmem, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::B3R_W16(r, 0),
+      B3R_W16(r, 16), "r"(tmem)
+      : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t tmem, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::B3R_W16(
+          r, 0),
+      "r"(tmem)
+      : "memory");
+}
+// Waits for this thread's loads.  The empty statements tie the registers' uses to after the wait.
+template <int N>
+__device__ __forceinline__ void tc_wait_ld(uint32_t (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+}  // namespace b3r
