@@ -1,9 +1,4 @@
-// Part 5 of the C ABI: attention's argument checks and its backward pass, with P = exp(S - lse):
-//   delta = do . o,  dv = P^T do,  dP = do v^T,  dS = P (dP - delta),  dq = scale dS k,  dk = scale dS^T q
-// A warp owns a row: a query row forward and for dq, a key row for dk and dv, which walks over the
-// queries of all heads that share it.  Lanes own keys (queries) for the scores and
-// dimensions for the sums, all in float32.
-#include <algorithm>
+// Part 5 of the C ABI, attention: what both passes check, and the tensor maps that they load by.
 #include "b3r_attn.cuh"
 
 namespace b3r {
@@ -54,6 +49,11 @@ int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads
       f = nullptr;
     return reinterpret_cast<encode_t>(f);
   }();
+  // the encoder wants a current context, which a thread that has made no runtime call yet (an
+  // autograd worker) does not have
+  int dev;
+  B3R_TRY(check_cuda(cudaGetDevice(&dev), "attention"));
+  B3R_TRY(check_cuda(cudaSetDevice(dev), "attention"));
   if (!encode) return fail(B3R_E_CUDA, "attention: the driver has no cuTensorMapEncodeTiled");
   if (rows == 0) {                     // no keys: no load is issued, the map is never read
     *map = CUtensorMap{};
@@ -71,124 +71,4 @@ int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads
   return B3R_OK;
 }
 
-namespace {
-
-constexpr int kWarps = 4;
-
-template <typename T>
-__device__ __forceinline__ float dot(const T* a, const T* b, int D) {
-  float s = 0.f;
-  for (int c = 0; c < D; c += 8) {
-    const uint4 ua = *reinterpret_cast<const uint4*>(a + c), ub = *reinterpret_cast<const uint4*>(b + c);
-    const T* x = reinterpret_cast<const T*>(&ua);
-    const T* y = reinterpret_cast<const T*>(&ub);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) s += f_of(x[j]) * f_of(y[j]);
-  }
-  return s;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) k_attn_dq_rows(const __grid_constant__ b3r_attention_desc d) {
-  const int lane = threadIdx.x & 31;
-  const int i = blockIdx.x * kWarps + (threadIdx.x >> 5), h = blockIdx.y % d.Hq, b = blockIdx.y / d.Hq;
-  const AttnSeq s = attn_seq(d, b);
-  if (i >= (d.cu_q ? s.ql : d.Lq)) return;
-  const int kv = h / (d.Hq / d.Hkv), bound = i < s.ql ? attn_bound(s, i, d.causal) : 0;
-  const T* q = attn_row<const T>(d.q, b, s.q0 + i, h);
-  const T* go = attn_row<const T>(d.d_o, b, s.q0 + i, h);
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  if (bound > 0) {
-    const float delta = dot(go, attn_row<const T>(d.o, b, s.q0 + i, h), d.D);
-    const float lse = *attn_row<const float>(d.lse, b, s.q0 + i, h);
-    for (int j0 = 0; j0 < bound; j0 += 32) {
-      const int j = j0 + lane;
-      float ds = 0.f;
-      if (j < bound) {
-        const float p = expf(d.scale * dot(q, attn_row<const T>(d.k, b, s.k0 + j, kv), d.D) - lse);
-        ds = p * (dot(go, attn_row<const T>(d.v, b, s.k0 + j, kv), d.D) - delta);
-      }
-      for (int t = 0; t < min(32, bound - j0); ++t) {
-        const float x = __shfl_sync(0xffffffffu, ds, t);
-        const T* k = attn_row<const T>(d.k, b, s.k0 + j0 + t, kv);
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (lane + 32 * c < d.D) acc[c] += x * f_of(k[lane + 32 * c]);
-      }
-    }
-  }
-  T* dq = attn_row<T>(d.dq, b, s.q0 + i, h);
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 32 * c < d.D) dq[lane + 32 * c] = t_of<T>(d.scale * acc[c]);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(32 * kWarps) k_attn_dkv_rows(const __grid_constant__ b3r_attention_desc d) {
-  const int lane = threadIdx.x & 31;
-  const int j = blockIdx.x * kWarps + (threadIdx.x >> 5), kv = blockIdx.y % d.Hkv, b = blockIdx.y / d.Hkv;
-  const AttnSeq s = attn_seq(d, b);
-  if (j >= (d.cu_q ? s.kl : d.Lk)) return;
-  const int G = d.Hq / d.Hkv;
-  float ak[4] = {0.f, 0.f, 0.f, 0.f}, av[4] = {0.f, 0.f, 0.f, 0.f};
-  if (j < s.kl) {
-    const T* k = attn_row<const T>(d.k, b, s.k0 + j, kv);
-    const T* v = attn_row<const T>(d.v, b, s.k0 + j, kv);
-    const int first = d.causal ? max(0, j - (s.kl - s.ql)) : 0;   // the first query that sees key j
-    for (int h = kv * G; h < kv * G + G; ++h)
-      for (int i0 = first; i0 < s.ql; i0 += 32) {
-        const int i = i0 + lane;
-        float p = 0.f, ds = 0.f;
-        if (i < s.ql) {
-          const T* go = attn_row<const T>(d.d_o, b, s.q0 + i, h);
-          p = expf(d.scale * dot(attn_row<const T>(d.q, b, s.q0 + i, h), k, d.D) - *attn_row<const float>(d.lse, b, s.q0 + i, h));
-          ds = p * (dot(go, v, d.D) - dot(go, attn_row<const T>(d.o, b, s.q0 + i, h), d.D));
-        }
-        for (int t = 0; t < min(32, s.ql - i0); ++t) {
-          const float pt = __shfl_sync(0xffffffffu, p, t), dt = __shfl_sync(0xffffffffu, ds, t);
-          const T* q = attn_row<const T>(d.q, b, s.q0 + i0 + t, h);
-          const T* go = attn_row<const T>(d.d_o, b, s.q0 + i0 + t, h);
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (lane + 32 * c < d.D) {
-              av[c] += pt * f_of(go[lane + 32 * c]);
-              ak[c] += dt * f_of(q[lane + 32 * c]);
-            }
-        }
-      }
-  }
-  T* dk = attn_row<T>(d.dk, b, s.k0 + j, kv);
-  T* dv = attn_row<T>(d.dv, b, s.k0 + j, kv);
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + 32 * c < d.D) {
-      dk[lane + 32 * c] = t_of<T>(d.scale * ak[c]);
-      dv[lane + 32 * c] = t_of<T>(av[c]);
-    }
-}
-
-template <typename T>
-int bwd_rows(const b3r_attention_desc& d, cudaStream_t s) {
-  if (d.Lq > 0) {
-    k_attn_dq_rows<T><<<dim3((d.Lq + kWarps - 1) / kWarps, d.B * d.Hq), 32 * kWarps, 0, s>>>(d);
-    B3R_TRY(check_launch("attention dq"));
-  }
-  if (d.Lk > 0) {
-    k_attn_dkv_rows<T><<<dim3((d.Lk + kWarps - 1) / kWarps, d.B * d.Hkv), 32 * kWarps, 0, s>>>(d);
-    B3R_TRY(check_launch("attention dk, dv"));
-  }
-  return B3R_OK;
-}
-
-}  // namespace
 }  // namespace b3r
-
-using namespace b3r;
-
-extern "C" int64_t b3r_attention_bwd_work_bytes(const b3r_attention_desc* d) { return d ? 0 : -1; }
-
-extern "C" int b3r_attention_bwd(const b3r_attention_desc* d, void* stream) {
-  B3R_TRY(attn_check(d, true));
-  if (d->B == 0) return B3R_OK;
-  return d->dtype == B3R_BF16 ? bwd_rows<__nv_bfloat16>(*d, as_stream(stream)) : bwd_rows<__half>(*d, as_stream(stream));
-}

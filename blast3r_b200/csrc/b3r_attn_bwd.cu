@@ -1,0 +1,643 @@
+// Attention's backward pass on the 5th-generation tensor cores, with P = exp(S - lse) recomputed:
+//   delta = do . o,  dv = P^T do,  dP = do v^T,  dS = P (dP - delta),  dq = scale dS k,  dk = scale dS^T q
+//
+// Two kernels, so that every sum has one owner and a fixed order (no atomics):
+//   k_attn_dq    a block owns 128 rows (queries x heads of a group) and walks over the keys; it
+//                computes delta on the way in and leaves it for the other kernel
+//   k_attn_dkv   a block owns 128 keys and walks over the queries of every head that shares them,
+//                with S^T = K Q^T and dP^T = V dO^T, so that P^T and dS^T have the keys' rows
+// In both, warp 8 loads tiles by TMA into a ring, warp 9 issues the products, and two warpgroups
+// do the elementwise part, one row and half of the columns to a thread.  P and dS go back to
+// tensor memory as 16-bit pairs and are read there as the left operands of the products that
+// follow; they are rounded to the operands' type for it.  S, dP, delta and the sums are float32.
+//
+// Splitting the pass in two computes S and dP twice (7 products instead of 5); the
+// alternative adds dq to memory from every key block, which needs atomics or an order to wait for.
+#include <algorithm>
+#include "b3r_attn.cuh"
+#include "b3r_tc.cuh"
+
+namespace b3r {
+namespace {
+
+constexpr int kThreads = 384;
+constexpr int kMaxStages = 8;
+
+// P^T is rounded to the operands' type for dv.  In float16 the small probabilities of long rows
+// would be subnormal, so P is carried 2^11 times as large (P <= 1); the factor is taken out of dS in
+// float32 and of dv at the end, both exactly.
+template <typename T>
+constexpr float kLogScaleP = __is_same(T, __half) ? 11.f : 0.f;
+template <typename T>
+constexpr float kScaleP = __is_same(T, __half) ? 2048.f : 1.f;
+
+struct alignas(64) BwdArgs {
+  CUtensorMap q, go, k, v;
+  b3r_attention_desc d;
+  int q_tiles, k_tiles;       // row tiles of a key/value head's queries, and key tiles, of the longest sequence
+  int q_splits, k_splits;     // blocks along the keys for dq, along the queries for dk and dv
+  int stages, group;
+  float* delta;               // [B][Hq][Lq]
+  float* part_q;              // [q_splits][B Hkv][rows][D]
+  float* part_k;              // [k_splits][2][B Hkv][Lk][D]: dk, dv
+};
+
+struct Shared {
+  uint64_t fix, own_full, full[kMaxStages], empty[kMaxStages], s_full[2], dp_full, dp_read, p_full, ds_full, done;
+  uint64_t st_full[2], st_empty[2];
+  uint32_t tmem;
+  int dead;
+  float delta[kTileRows];
+  float stat[2][2][kTileRows];   // k_attn_dkv: per stage, lse (log2) and delta of 128 queries
+};
+
+// Which head and tile a block works on: heads in groups whose tensors fit L2; `heavy_first`
+// says on which side of a causal triangle the long tiles lie.
+__device__ __forceinline__ void place(int id, int tiles, int group, int heads, bool last_first, int& head, int& tile) {
+  const int gsz = group * tiles, g = id / gsz, r = id - g * gsz, width = min(group, heads - g * group);
+  head = g * group + r % width;
+  tile = last_first ? tiles - 1 - r / width : r / width;
+}
+
+__device__ __forceinline__ void init_shared(Shared& sh, int stages, int own) {
+  mbar_init(smem_u32(&sh.fix), 1);
+  mbar_init(smem_u32(&sh.own_full), own);
+  for (int i = 0; i < stages; ++i) {
+    mbar_init(smem_u32(&sh.full[i]), 1);
+    mbar_init(smem_u32(&sh.empty[i]), 1);
+  }
+  for (int i = 0; i < 2; ++i) {
+    mbar_init(smem_u32(&sh.s_full[i]), 1);
+    mbar_init(smem_u32(&sh.st_full[i]), 32);
+    mbar_init(smem_u32(&sh.st_empty[i]), 256);
+  }
+  mbar_init(smem_u32(&sh.dp_full), 1);
+  mbar_init(smem_u32(&sh.dp_read), 256);
+  mbar_init(smem_u32(&sh.p_full), 256);
+  mbar_init(smem_u32(&sh.ds_full), 256);
+  mbar_init(smem_u32(&sh.done), 1);
+  sh.dead = 0;
+  fence_async();
+}
+
+__device__ __forceinline__ void finish(Shared& sh, int32_t* status, int warp, bool used) {
+  tc_fence_before();
+  __syncthreads();
+  if (*(volatile int*)&sh.dead) {                      // copies that a failed wait left behind
+    for (int t = 0; t < 100; ++t) __nanosleep(1000);
+    if (threadIdx.x == 0 && status) *status = 1;
+    __syncthreads();
+  }
+  if (warp == 9 && used) {
+    tc_fence_after();
+    tc_free(sh.tmem, 512);
+  }
+}
+
+// 32 columns of an accumulator, times f, to a row of 16-bit values or of float32 parts.
+template <typename T>
+__device__ __forceinline__ void write32(uint32_t tmem, bool has, float f, T* out, float* part, int D, int c0, bool row) {
+  float v[32];
+  if (has) {
+    uint32_t o[32];
+    tc_ld32(tmem, o);
+    tc_wait_ld(o);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[e] = 0.f;
+  }
+  if (!row) return;
+  if (part) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 4)
+      if (c0 + e < D) *reinterpret_cast<float4*>(part + c0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; e += 8)
+      if (c0 + e < D)
+        *reinterpret_cast<uint4*>(out + c0 + e) = make_uint4(pack2(v[e], v[e + 1], T()), pack2(v[e + 2], v[e + 3], T()),
+                                                             pack2(v[e + 4], v[e + 5], T()), pack2(v[e + 6], v[e + 7], T()));
+  }
+}
+
+// ---------------------------------------------------------------- dq
+// Tensor memory: S of even and odd tiles at 0 and 128, dP at 256, dq at 384.  dS overwrites the
+// S that it came from, each half in place, so dP of the next tile can start once dP is read.
+template <int DP, typename T>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__ BwdArgs a) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
+  constexpr bool kBf = __is_same(T, __nv_bfloat16);
+  const uint32_t sq = smem_u32(base), sgo = sq + kTile;
+  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.stages) * kTile);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const b3r_attention_desc& d = a.d;
+  const int G = d.Hq / d.Hkv, split = blockIdx.x % a.q_splits;
+  int head, tile;
+  place(blockIdx.x / a.q_splits, a.q_tiles, a.group, d.B * d.Hkv, true, head, tile);
+  const int b = head / d.Hkv, kv = head % d.Hkv;
+  const AttnSeq s = attn_seq(d, b);
+  const int rows = (d.cu_q ? s.ql : d.Lq) * G, m0 = tile * kTileRows;
+  if (m0 >= rows) return;
+  int n = 0, first = 0;
+  {
+    const int last = min(m0 + kTileRows, s.ql * G) - 1;
+    const int all = last < m0 ? 0 : (attn_bound(s, last / G, d.causal) + kTileRows - 1) / kTileRows;
+    const int per = (all + a.q_splits - 1) / a.q_splits;
+    first = split * per;
+    n = min(max(all - first, 0), per);
+  }
+  if (threadIdx.x == 0) init_shared(sh, a.stages, 256);
+  if (warp == 9 && n > 0) tc_alloc(smem_u32(&sh.tmem), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  volatile int* dead = &sh.dead;
+  const int steps = (d.D + 15) / 16;
+  Ring ring{sq + 2 * kTile, base + 2 * kTile, sh.full, sh.empty, a.stages};
+
+  if (warp == 8 && n > 0) {
+    int fixes = 0;
+    const int batch = d.cu_k ? 0 : b;
+    for (int it = 0; it < n; ++it) {
+      const int t = (first + it) * kTileRows;
+      // dS is zero past the last key and meets K's rows there, so they are cleared
+      ring_load<kBlocks>(ring, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks>(ring, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
+    }
+  } else if (warp == 9 && n > 0) {
+    if (lane == 0) {
+      const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
+      auto product = [&](uint32_t acc, uint32_t left, int stage) {   // acc = left K^T or V^T
+        for (int t = 0; t < steps; ++t) {
+          const uint32_t off = (t >> 2) * kBlockBytes + (t & 3) * 32;
+          tc_mma(acc, desc_k(left + off), desc_k(ring.data + stage * kTile + off), id_s, t > 0);
+        }
+      };
+      int sk[2], sv = 0, last_round = 0;
+      auto scores = [&](int it) {
+        sk[it & 1] = ring.next(dead);
+        tc_fence_after();
+        product(tmem + (it & 1) * 128, sq, sk[it & 1]);
+        tc_commit(smem_u32(&sh.s_full[it & 1]));
+      };
+      auto grads = [&]() {
+        last_round = ring.round;
+        sv = ring.next(dead);
+        tc_fence_after();
+        product(tmem + 256, sgo, sv);
+        tc_commit(smem_u32(&sh.dp_full));
+        tc_commit(smem_u32(&sh.empty[sv]));
+      };
+      mbar_wait(smem_u32(&sh.own_full), 0, dead);
+      tc_fence_after();
+      scores(0);
+      grads();
+      if (n > 1) scores(1);
+      for (int it = 0; it < n; ++it) {
+        if (it + 1 < n) {
+          mbar_wait(smem_u32(&sh.dp_read), it & 1, dead);
+          tc_fence_after();
+          grads();
+        }
+        mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
+        tc_fence_after();
+        const uint32_t ds = tmem + (it & 1) * 128, k = ring.data + sk[it & 1] * kTile;
+        for (int t = 0; t < 8; ++t)
+          tc_mma_ts(tmem + 384, ds + (t >> 2) * 64 + (t & 3) * 8, desc_mn(k + t * 2048), id_o, it > 0 || t > 0);
+        tc_commit(smem_u32(&sh.empty[sk[it & 1]]));
+        if (it + 2 < n) scores(it + 2);
+      }
+      tc_commit(smem_u32(&sh.done));
+      mbar_wait(smem_u32(&sh.empty[sv]), last_round & 1, dead);      // no arrival is left behind
+      mbar_wait(smem_u32(&sh.done), 0, dead);
+    }
+  } else if (warp < 8) {
+    const int w = warp >> 2, r = threadIdx.x & 127, m = m0 + r;
+    const int i = m / G, h = kv * G + m % G;
+    const bool row = m < rows, live = row && i < s.ql;
+    const int bound = live ? attn_bound(s, i, d.causal) : 0;
+    const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);
+    // one group brings the rows of Q, the other those of dO and, with O, delta
+    {
+      const int64_t qr = s.q0 + (live ? i : 0);
+      const int qh = live ? h : kv * G;
+      const uint4* src = reinterpret_cast<const uint4*>(attn_row<const T>(w ? d.d_o : d.q, b, qr, qh));
+      const uint4* out = reinterpret_cast<const uint4*>(attn_row<const T>(d.o, b, qr, qh));
+      uint8_t* dst = base + w * kTile + r * 128;
+      float dot = 0.f;
+#pragma unroll
+      for (int cb = 0; cb < DP / 8; ++cb) {
+        const bool in = live && cb * 8 < d.D;
+        const uint4 x = in ? src[cb] : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4)) = x;
+        if (w && in) {
+          const uint4 y = out[cb];
+          const T* xe = reinterpret_cast<const T*>(&x);
+          const T* ye = reinterpret_cast<const T*>(&y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot += f_of(xe[e]) * f_of(ye[e]);
+        }
+      }
+      fence_async();
+      if (w) {
+        sh.delta[r] = dot;
+        if (live && split == 0) a.delta[((int64_t)b * d.Hq + h) * d.Lq + i] = dot;
+      }
+      if (n > 0) mbar_arrive(smem_u32(&sh.own_full));
+      bar_sync(1, 256);
+    }
+    const float delta = sh.delta[r], c = d.scale * kLog2e;
+    float lse = bound > 0 ? *attn_row<const float>(d.lse, b, s.q0 + i, h) * kLog2e : 0.f;
+    if (lse == -INFINITY) lse = INFINITY;              // nothing seen: P = 0
+    const float2 cc = make_float2(c, c), ll = make_float2(-lse, -lse), dd = make_float2(-delta, -delta);
+    for (int it = 0; it < n; ++it) {
+      const int lim = bound - (first + it) * kTileRows - w * 64;     // of this thread's 64 keys, how many its row sees
+      const uint32_t at = quarter + (it & 1) * 128 + w * 64;
+      mbar_wait(smem_u32(&sh.s_full[it & 1]), (it >> 1) & 1, dead);
+      tc_fence_after();
+      uint32_t p[64], g[64];
+      tc_ld32(at, p);
+      tc_ld32(at + 32, p + 32);
+      tc_wait_ld(p);
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), cc, ll);
+        p[e] = __float_as_uint(ex2(x.x));
+        p[e + 1] = __float_as_uint(ex2(x.y));
+      }
+      mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
+      tc_fence_after();
+      tc_ld32(quarter + 256 + w * 64, g);
+      tc_ld32(quarter + 256 + w * 64 + 32, g + 32);
+      tc_wait_ld(g);
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sh.dp_read));
+      const bool whole = __all_sync(0xffffffffu, lim >= 64);
+      uint32_t ds[32];
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        float2 x = __fadd2_rn(make_float2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1])), dd);
+        x = __fmul2_rn(x, make_float2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1])));
+        if (!whole) {                                  // unseen keys: whatever their S and dP are
+          x.x = 2 * e < lim ? x.x : 0.f;
+          x.y = 2 * e + 1 < lim ? x.y : 0.f;
+        }
+        ds[e] = pack2(x.x, x.y, T());
+      }
+      tc_st32(at, ds);
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sh.ds_full));
+    }
+    if (n > 0) {
+      mbar_wait(smem_u32(&sh.done), 0, dead);
+      tc_fence_after();
+    }
+    const float f = *dead ? __int_as_float(0x7fffffff) : d.scale;
+    T* out = attn_row<T>(d.dq, b, s.q0 + (row ? i : 0), row ? h : 0);
+    float* part = a.q_splits > 1
+                      ? a.part_q + (((int64_t)split * d.B * d.Hkv + head) * ((int64_t)d.Lq * G) + m) * d.D
+                      : nullptr;
+#pragma unroll
+    for (int q = 0; q < DP / 2; q += 32) {
+      const int c0 = w * (DP / 2) + q;
+      if (c0 < d.D) write32<T>(quarter + 384 + c0, n > 0, f, out, part, d.D, c0, row);
+    }
+  }
+  finish(sh, d.status, warp, n > 0);
+}
+
+// ---------------------------------------------------------------- dk, dv
+// Tensor memory: S^T at 0, dP^T at 128, dv at 256, dk at 256 + DP.  P^T overwrites S^T and dS^T
+// dP^T, each half in place.  While the groups are at P of tile t, the tensor cores are at dk of
+// tile t - 1 and dP of tile t; while they are at dS of t, at dv of t and S of t + 1.
+template <int DP, typename T>
+__global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant__ BwdArgs a) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+  constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
+  constexpr bool kBf = __is_same(T, __nv_bfloat16);
+  const uint32_t sk = smem_u32(base), sv = sk + kTile;
+  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.stages) * kTile);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const b3r_attention_desc& d = a.d;
+  const int G = d.Hq / d.Hkv, split = blockIdx.x % a.k_splits;
+  int head, tile;
+  place(blockIdx.x / a.k_splits, a.k_tiles, a.group, d.B * d.Hkv, false, head, tile);
+  const int b = head / d.Hkv, kv = head % d.Hkv;
+  const AttnSeq s = attn_seq(d, b);
+  const int j0 = tile * kTileRows, keys = d.cu_k ? s.kl : d.Lk;
+  if (j0 >= keys) return;
+  // query tiles from the first that sees this tile's first key, of each head in turn
+  int t0 = 0, per_head = 0, first = 0, n = 0;
+  if (j0 < s.kl) {
+    t0 = d.causal ? max(0, j0 - (s.kl - s.ql)) / kTileRows : 0;
+    per_head = max(0, (s.ql + kTileRows - 1) / kTileRows - t0);
+    const int all = per_head * G, per = (all + a.k_splits - 1) / a.k_splits;
+    first = split * per;
+    n = min(max(all - first, 0), per);
+  }
+  if (threadIdx.x == 0) init_shared(sh, a.stages, 1);
+  if (warp == 9 && n > 0) tc_alloc(smem_u32(&sh.tmem), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sh.tmem;
+  volatile int* dead = &sh.dead;
+  const int steps = (d.D + 15) / 16;
+  Ring ring{sk + 2 * kTile, base + 2 * kTile, sh.full, sh.empty, a.stages};
+
+  if (warp == 8 && n > 0) {
+    int fixes = 0;
+    const int bk = d.cu_k ? 0 : b, bq = d.cu_q ? 0 : b;
+    if (lane == 0) {
+      const uint32_t bar = smem_u32(&sh.own_full);
+      mbar_expect(bar, 2 * kTile);
+#pragma unroll
+      for (int c = 0; c < kBlocks; ++c) {
+        tma_box(sk + c * kBlockBytes, &a.k, c * 64, (int)s.k0 + j0, kv, bk, bar);
+        tma_box(sv + c * kBlockBytes, &a.v, c * 64, (int)s.k0 + j0, kv, bk, bar);
+      }
+    }
+    for (int it = 0; it < n; ++it) {
+      const int u = first + it, h = kv * G + u / per_head, i0 = (t0 + u % per_head) * kTileRows;
+      // P and dS are zero past the last query and meet the rows of dO and Q there
+      ring_load<kBlocks>(ring, &a.q, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks>(ring, &a.go, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
+    }
+    if (*dead && lane == 0) mbar_wait(smem_u32(&sh.own_full), 0, dead);
+  } else if (warp == 9 && n > 0) {
+    if (lane == 0) {
+      const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
+      auto product = [&](uint32_t acc, uint32_t left, int stage) {   // acc = K Q^T or V dO^T
+        for (int t = 0; t < steps; ++t) {
+          const uint32_t off = (t >> 2) * kBlockBytes + (t & 3) * 32;
+          tc_mma(acc, desc_k(left + off), desc_k(ring.data + stage * kTile + off), id_s, t > 0);
+        }
+      };
+      auto gather = [&](uint32_t acc, uint32_t left, int stage, bool add) {   // acc += P^T dO or dS^T Q
+        const uint32_t x = ring.data + stage * kTile;
+        for (int t = 0; t < 8; ++t)
+          tc_mma_ts(acc, left + (t >> 2) * 64 + (t & 3) * 8, desc_mn(x + t * 2048), id_o, add || t > 0);
+        tc_commit(smem_u32(&sh.empty[stage]));
+      };
+      mbar_wait(smem_u32(&sh.own_full), 0, dead);
+      int xq = ring.next(dead), xg, last_round = 0;
+      tc_fence_after();
+      product(tmem, sk, xq);
+      tc_commit(smem_u32(&sh.s_full[0]));
+      last_round = ring.round;
+      xg = ring.next(dead);
+      product(tmem + 128, sv, xg);
+      tc_commit(smem_u32(&sh.dp_full));
+      for (int it = 0; it < n; ++it) {
+        const int cq = xq, cg = xg, round_g = last_round;
+        mbar_wait(smem_u32(&sh.p_full), it & 1, dead);
+        tc_fence_after();
+        gather(tmem + 256, tmem, cg, it > 0);                        // dv
+        if (it + 1 < n) {
+          xq = ring.next(dead);
+          product(tmem, sk, xq);
+          tc_commit(smem_u32(&sh.s_full[0]));
+        }
+        mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
+        tc_fence_after();
+        gather(tmem + 256 + DP, tmem + 128, cq, it > 0);             // dk
+        if (it + 1 < n) {
+          last_round = ring.round;
+          xg = ring.next(dead);
+          product(tmem + 128, sv, xg);
+          tc_commit(smem_u32(&sh.dp_full));
+        } else {
+          tc_commit(smem_u32(&sh.done));
+          mbar_wait(smem_u32(&sh.empty[cg]), round_g & 1, dead);     // no arrival is left behind
+          mbar_wait(smem_u32(&sh.done), 0, dead);
+        }
+      }
+    }
+  } else if (warp == 10 && n > 0) {
+    // the statistics of each tile's queries, two tiles ahead at most
+    for (int it = 0; it < n; ++it) {
+      const int st = it & 1, u = first + it, h = kv * G + u / per_head, i0 = (t0 + u % per_head) * kTileRows;
+      if (it >= 2) mbar_wait(smem_u32(&sh.st_empty[st]), ((it >> 1) - 1) & 1, dead);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int x = q * 32 + lane, i = i0 + x;
+        float l = -INFINITY, dl = 0.f;
+        if (i < s.ql) {
+          l = *attn_row<const float>(d.lse, b, s.q0 + i, h);
+          dl = a.delta[((int64_t)b * d.Hq + h) * d.Lq + i];
+        }
+        sh.stat[st][0][x] = l == -INFINITY ? -INFINITY : kLogScaleP<T> - l * kLog2e;   // nothing seen: P = 2^-inf
+        sh.stat[st][1][x] = l == -INFINITY ? 0.f : -dl * (1.f / kScaleP<T>);
+      }
+      mbar_arrive(smem_u32(&sh.st_full[st]));
+    }
+  } else if (warp < 8) {
+    const int w = warp >> 2, r = threadIdx.x & 127, j = j0 + r;
+    const bool row = j < keys;
+    const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);
+    const float c = d.scale * kLog2e;
+    const float2 cc = make_float2(c, c), unscale = make_float2(1.f / kScaleP<T>, 1.f / kScaleP<T>);
+    const int see = d.causal ? max(0, j - (s.kl - s.ql)) : 0;         // the first query that sees this key
+    for (int it = 0; it < n; ++it) {
+      const int st = it & 1, u = first + it, i0 = (t0 + u % per_head) * kTileRows + w * 64;
+      const float2* lse = reinterpret_cast<const float2*>(sh.stat[st][0] + w * 64);
+      const float2* dlt = reinterpret_cast<const float2*>(sh.stat[st][1] + w * 64);
+      mbar_wait(smem_u32(&sh.st_full[st]), (it >> 1) & 1, dead);
+      mbar_wait(smem_u32(&sh.s_full[0]), it & 1, dead);
+      tc_fence_after();
+      uint32_t p[64], g[64], h[32];
+      tc_ld32(quarter + w * 64, p);
+      tc_ld32(quarter + w * 64 + 32, p + 32);
+      tc_wait_ld(p);
+      const int hide = see - i0;                                     // columns before it do not see the key
+      const bool whole = __all_sync(0xffffffffu, hide <= 0);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        float2 x = __ffma2_rn(make_float2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1])), cc, lse[e]);
+        x.x = ex2(x.x);
+        x.y = ex2(x.y);
+        if (!whole) {
+          x.x = 2 * e >= hide ? x.x : 0.f;
+          x.y = 2 * e + 1 >= hide ? x.y : 0.f;
+        }
+        p[2 * e] = __float_as_uint(x.x);
+        p[2 * e + 1] = __float_as_uint(x.y);
+        h[e] = pack2(x.x, x.y, T());
+      }
+      tc_st32(quarter + w * 64, h);
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sh.p_full));
+      mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
+      tc_fence_after();
+      tc_ld32(quarter + 128 + w * 64, g);
+      tc_ld32(quarter + 128 + w * 64 + 32, g + 32);
+      tc_wait_ld(g);
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        float2 x = __ffma2_rn(make_float2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1])), unscale, dlt[e]);
+        x = __fmul2_rn(x, make_float2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1])));
+        if (!whole) {
+          x.x = 2 * e >= hide ? x.x : 0.f;
+          x.y = 2 * e + 1 >= hide ? x.y : 0.f;
+        }
+        h[e] = pack2(x.x, x.y, T());
+      }
+      tc_st32(quarter + 128 + w * 64, h);
+      tc_wait_st();
+      tc_fence_before();
+      mbar_arrive(smem_u32(&sh.ds_full));
+      mbar_arrive(smem_u32(&sh.st_empty[st]));
+    }
+    if (n > 0) {
+      mbar_wait(smem_u32(&sh.done), 0, dead);
+      tc_fence_after();
+    }
+    // one group writes dv, the other dk; keys past the sequence's end get zeros
+    float f = w ? d.scale : 1.f / kScaleP<T>;
+    if (*dead) f = __int_as_float(0x7fffffff);
+    const bool has = n > 0;
+    const b3r_attn_tensor& to = w ? d.dk : d.dv;
+    T* out = attn_row<T>(to, b, s.k0 + (row ? j : 0), kv);
+    float* part = a.k_splits > 1
+                      ? a.part_k + ((((int64_t)split * 2 + w) * d.B * d.Hkv + head) * (int64_t)d.Lk + j) * d.D
+                      : nullptr;
+#pragma unroll
+    for (int q = 0; q < DP; q += 32) {
+      if (q >= d.D) break;
+      if (row && j >= s.kl) write32<T>(0, false, f, out, part, d.D, q, true);
+      const bool mine = row && j < s.kl;
+      __syncwarp();
+      if (has) write32<T>(quarter + 256 + w * DP + q, true, f, out, part, d.D, q, mine);   // the whole warp
+      else if (mine) write32<T>(0, false, f, out, part, d.D, q, true);
+    }
+  }
+  finish(sh, d.status, warp, n > 0);
+}
+
+// Adds the float32 parts in their order.  One thread to four columns of a row.
+// WHICH 0: dq (rows of queries x heads of a group); 1, 2: dv, dk.
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_add(const __grid_constant__ BwdArgs a, int which) {
+  const b3r_attention_desc& d = a.d;
+  const int G = d.Hq / d.Hkv, head = blockIdx.y, b = head / d.Hkv, kv = head % d.Hkv, quads = d.D / 4;
+  const int64_t idx = (int64_t)blockIdx.x * 256 + threadIdx.x, m = idx / quads;
+  const int c = (int)(idx % quads) * 4;
+  const AttnSeq s = attn_seq(d, b);
+  const int64_t rows = which ? (int64_t)d.Lk : (int64_t)d.Lq * G;
+  const int64_t mine = which ? (d.cu_k ? s.kl : d.Lk) : (int64_t)(d.cu_q ? s.ql : d.Lq) * G;
+  if (m >= mine) return;
+  const float* p = which ? a.part_k + (((int64_t)(which == 2) * d.B * d.Hkv + head) * rows + m) * d.D
+                         : a.part_q + ((int64_t)head * rows + m) * d.D;
+  const int64_t step = (which ? 2 : 1) * (int64_t)d.B * d.Hkv * rows * d.D;
+  const int n = which ? a.k_splits : a.q_splits;
+  float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i = 0; i < n; ++i) {
+    const float4 x = *reinterpret_cast<const float4*>(p + i * step + c);
+    t.x += x.x;
+    t.y += x.y;
+    t.z += x.z;
+    t.w += x.w;
+  }
+  T* out = which ? attn_row<T>(which == 2 ? d.dk : d.dv, b, s.k0 + m, kv)
+                 : attn_row<T>(d.dq, b, s.q0 + m / G, kv * G + (int)(m % G));
+  *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2(t.x, t.y, T()), pack2(t.z, t.w, T()));
+}
+
+constexpr int kSms = 148;
+int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
+
+int64_t cut(BwdArgs& a) {     // returns the workspace's bytes
+  const b3r_attention_desc& d = a.d;
+  const int64_t G = d.Hq / d.Hkv, heads = (int64_t)d.B * d.Hkv;
+  a.q_tiles = (int)((d.Lq * G + kTileRows - 1) / kTileRows);
+  a.k_tiles = (d.Lk + kTileRows - 1) / kTileRows;
+  const int64_t q_blocks = a.q_tiles * heads, k_blocks = a.k_tiles * heads;
+  const int64_t k_walk = (int64_t)((d.Lq + kTileRows - 1) / kTileRows) * G;   // query tiles that a key block meets
+  // fewer blocks than SMs: the walk is split, at least two tiles to a block
+  auto split = [](int64_t blocks, int64_t walk) {
+    return blocks <= 0 || blocks >= kSms ? 1 : (int)std::max<int64_t>(1, std::min<int64_t>((kSms + blocks - 1) / blocks, walk / 2));
+  };
+  a.q_splits = split(q_blocks, a.k_tiles);
+  a.k_splits = split(k_blocks, k_walk);
+  const int dp = d.D <= 64 ? 64 : 128, tile = dp / 64 * kBlockBytes;
+  a.stages = std::min(kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - 2);
+  const int64_t head = std::max<int64_t>(1, ((int64_t)d.Lk + d.Lq * G) * d.D * 4);
+  a.group = (int)std::max<int64_t>(1, std::min<int64_t>(heads, (32 << 20) / head));
+  int64_t n = align256((int64_t)d.B * d.Hq * d.Lq * 4);
+  const int64_t q_off = n;
+  if (a.q_splits > 1) n += align256((int64_t)a.q_splits * heads * d.Lq * G * d.D * 4);
+  const int64_t k_off = n;
+  if (a.k_splits > 1) n += align256((int64_t)a.k_splits * 2 * heads * d.Lk * d.D * 4);
+  uint8_t* w = reinterpret_cast<uint8_t*>(d.work);
+  a.delta = reinterpret_cast<float*>(w);
+  a.part_q = reinterpret_cast<float*>(w + q_off);
+  a.part_k = reinterpret_cast<float*>(w + k_off);
+  return n;
+}
+
+template <int DP, typename T>
+int launch(const BwdArgs& a, cudaStream_t s) {
+  const b3r_attention_desc& d = a.d;
+  const int64_t G = d.Hq / d.Hkv, heads = (int64_t)d.B * d.Hkv;
+  const int smem = 1024 + (2 + a.stages) * (DP / 64) * kBlockBytes + (int)sizeof(Shared);
+  B3R_REQUIRE(a.q_tiles * heads * a.q_splits <= 0x7fffffff && a.k_tiles * heads * a.k_splits <= 0x7fffffff,
+              "attention backward: too many rows for one call");
+  if (a.q_tiles > 0 && (!d.cu_q || d.Tq > 0)) {
+    B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_dq<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention dq"));
+    k_attn_dq<DP, T><<<(unsigned)(a.q_tiles * heads * a.q_splits), kThreads, smem, s>>>(a);
+    B3R_TRY(check_launch("attention dq"));
+    if (a.q_splits > 1) {
+      k_attn_add<T><<<dim3((unsigned)((d.Lq * G * (d.D / 4) + 255) / 256), (unsigned)heads), 256, 0, s>>>(a, 0);
+      B3R_TRY(check_launch("attention dq sum"));
+    }
+  }
+  if (a.k_tiles > 0 && (!d.cu_k || d.Tk > 0)) {
+    B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_dkv<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention dk, dv"));
+    k_attn_dkv<DP, T><<<(unsigned)(a.k_tiles * heads * a.k_splits), kThreads, smem, s>>>(a);
+    B3R_TRY(check_launch("attention dk, dv"));
+    for (int which = 1; which <= 2 && a.k_splits > 1; ++which) {
+      k_attn_add<T><<<dim3((unsigned)(((int64_t)d.Lk * (d.D / 4) + 255) / 256), (unsigned)heads), 256, 0, s>>>(a, which);
+      B3R_TRY(check_launch("attention dk, dv sum"));
+    }
+  }
+  return B3R_OK;
+}
+
+}  // namespace
+}  // namespace b3r
+
+using namespace b3r;
+
+extern "C" int64_t b3r_attention_bwd_work_bytes(const b3r_attention_desc* d) {
+  if (attn_check_sizes(d) != B3R_OK) return -1;
+  if (d->B == 0) return 0;
+  BwdArgs a;
+  a.d = *d;
+  return cut(a);
+}
+
+extern "C" int b3r_attention_bwd(const b3r_attention_desc* d, void* stream) {
+  B3R_TRY(attn_check(d, true));
+  if (d->B == 0) return B3R_OK;
+  BwdArgs a;
+  a.d = *d;
+  if (cut(a) > 0)
+    B3R_REQUIRE(d->work && ((uintptr_t)d->work & 255) == 0, "attention backward: work buffer must be 256-byte aligned");
+  const int64_t nq = d->cu_q ? d->Tq : d->Lq, nk = d->cu_q ? d->Tk : d->Lk;
+  const int batch = d->cu_q ? 1 : d->B;
+  B3R_TRY(attn_map(&a.q, d->q, nq, d->Hq, batch, d->D, d->dtype));
+  B3R_TRY(attn_map(&a.go, d->d_o, nq, d->Hq, batch, d->D, d->dtype));
+  B3R_TRY(attn_map(&a.k, d->k, nk, d->Hkv, batch, d->D, d->dtype));
+  B3R_TRY(attn_map(&a.v, d->v, nk, d->Hkv, batch, d->D, d->dtype));
+  cudaStream_t s = as_stream(stream);
+  if (d->dtype == B3R_BF16) return d->D <= 64 ? launch<64, __nv_bfloat16>(a, s) : launch<128, __nv_bfloat16>(a, s);
+  return d->D <= 64 ? launch<64, __half>(a, s) : launch<128, __half>(a, s);
+}

@@ -101,10 +101,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
   const b3r_attention_desc& d = a.d;
   if (j.m0[0] >= j.rows) return;       // uniform: no rows of this sequence here
   const bool none = j.n[0] + j.n[1] == 0;
-  const uint32_t bar_q = smem_u32(&sh.q_full), bar_fix = smem_u32(&sh.fix);
+  const uint32_t bar_q = smem_u32(&sh.q_full);
   if (threadIdx.x == 0) {
     mbar_init(bar_q, 256);
-    mbar_init(bar_fix, 1);
+    mbar_init(smem_u32(&sh.fix), 1);
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(smem_u32(&sh.kv_full[i]), 1);
       mbar_init(smem_u32(&sh.kv_empty[i]), 1);
@@ -129,35 +129,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 8 && !none) {
     // ------------------------------------------------ loads
-    int stage = 0, round = 0, fixes = 0;
+    Ring ring{skv, base + q_tiles * kTile, sh.kv_full, sh.kv_empty, a.stages};
+    int fixes = 0;
     const int row0 = (int)j.s.k0, batch = d.cu_k ? 0 : j.b;
-    auto load = [&](const CUtensorMap* map, int tile, bool values) {
-      const uint32_t full = smem_u32(&sh.kv_full[stage]), dst = skv + stage * kTile;
-      const int valid = j.s.kl - tile * kTileRows;
-      // rows of V past the sequence's end meet zeros in P, but may hold NaN: they are cleared
-      const bool fix = values && valid < kTileRows;
-      if (round > 0) mbar_wait(smem_u32(&sh.kv_empty[stage]), (round - 1) & 1, dead);
-      if (lane == 0) {
-        const uint32_t bar = fix ? bar_fix : full;
-        mbar_expect(bar, kTile);
-#pragma unroll
-        for (int c = 0; c < kBlocks; ++c) tma_box(dst + c * kBlockBytes, map, c * 64, row0 + tile * kTileRows, j.kv, batch, bar);
-      }
-      if (fix) {
-        mbar_wait(bar_fix, fixes & 1, dead);
-        ++fixes;
-        for (int i = valid * 8 + lane; i < kTileRows * 8; i += 32)
-#pragma unroll
-          for (int c = 0; c < kBlocks; ++c)
-            *reinterpret_cast<uint4*>(base + (dst - sq) + c * kBlockBytes + i * 16) = make_uint4(0, 0, 0, 0);
-        fence_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full);
-      }
-      if (++stage == a.stages) {
-        stage = 0;
-        ++round;
-      }
+    auto load = [&](const CUtensorMap* map, int tile, bool values) {   // P is zero past the last key, so V is cleared there
+      ring_load<kBlocks>(ring, map, row0 + tile * kTileRows, j.kv, batch, j.s.kl - tile * kTileRows, values, &sh.fix, fixes, lane,
+                         dead);
     };
     if (a.one) {
       for (int w = 0; w < 2; ++w)
@@ -180,16 +157,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     if (lane == 0) {
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
       const int steps = (d.D + 15) / 16;
-      int stage = 0, round = 0, last = 0, last_round = 0;
-      auto next = [&]() {                              // the stage with the next tile, once it is there
-        mbar_wait(smem_u32(&sh.kv_full[stage]), round & 1, dead);
-        const int s = last = stage;
-        last_round = round;
-        if (++stage == a.stages) {
-          stage = 0;
-          ++round;
-        }
-        return s;
+      Ring ring{skv, base + q_tiles * kTile, sh.kv_full, sh.kv_empty, a.stages};
+      int last = 0, last_round = 0;
+      auto next = [&]() {
+        last_round = ring.round;
+        return last = ring.next(dead);
       };
       auto scores = [&](int w, int s) {                // S_w = Q_w K^T
         const uint32_t q = sq + (a.one ? 0 : w) * kTile, k = skv + s * kTile;

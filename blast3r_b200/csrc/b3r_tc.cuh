@@ -154,4 +154,56 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
+// ---- a ring of shared-memory stages, each one tile of 128 rows, filled by one warp
+struct Ring {
+  uint32_t data;              // shared address of stage 0
+  uint8_t* data_ptr;          // the same, as a pointer
+  const uint64_t *full, *empty;
+  int stages;
+  int stage = 0, round = 0;
+
+  __device__ __forceinline__ void step() {
+    if (++stage == stages) {
+      stage = 0;
+      ++round;
+    }
+  }
+  // Consumer: the stage with the next tile, once it is there.
+  __device__ __forceinline__ int next(volatile int* dead) {
+    mbar_wait(smem_u32(full + stage), round & 1, dead);
+    const int s = stage;
+    step();
+    return s;
+  }
+};
+
+// Producer (a whole warp): the next stage gets rows [row, row + 128) of a head.  Only `valid` of
+// them belong to the sequence; the others are the neighbours' or padding, and may hold NaN.  They
+// are cleared where `clear`: where they meet zeros in a product along the rows.
+template <int BLOCKS>
+__device__ __forceinline__ void ring_load(Ring& g, const CUtensorMap* map, int row, int head, int batch, int valid, bool clear,
+                                          uint64_t* fix, int& fixes, int lane, volatile int* dead) {
+  const uint32_t full = smem_u32(g.full + g.stage), bar_fix = smem_u32(fix);
+  const int at = g.stage * BLOCKS * kBlockBytes;
+  const bool cut = clear && valid < kTileRows;
+  if (g.round > 0) mbar_wait(smem_u32(g.empty + g.stage), (g.round - 1) & 1, dead);
+  if (lane == 0) {
+    const uint32_t bar = cut ? bar_fix : full;
+    mbar_expect(bar, BLOCKS * kBlockBytes);
+#pragma unroll
+    for (int c = 0; c < BLOCKS; ++c) tma_box(g.data + at + c * kBlockBytes, map, c * 64, row, head, batch, bar);
+  }
+  if (cut) {
+    mbar_wait(bar_fix, fixes & 1, dead);
+    ++fixes;
+    for (int i = max(valid, 0) * 8 + lane; i < kTileRows * 8; i += 32)
+#pragma unroll
+      for (int c = 0; c < BLOCKS; ++c) *reinterpret_cast<uint4*>(g.data_ptr + at + c * kBlockBytes + i * 16) = make_uint4(0, 0, 0, 0);
+    fence_async();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(full);
+  }
+  g.step();
+}
+
 }  // namespace b3r
