@@ -20,11 +20,14 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include "b3r_status.h"
+#include "b3r_tc.cuh"
 
 namespace b3r {
 namespace {
 
-constexpr int kE = 8;   // consecutive elements of one vector access
+constexpr int kE = 8;        // consecutive elements of one vector access
+constexpr int kP = kE / 2;   // in packed pairs
+constexpr int kMaxStages = 4;   // rows of the backward pass's ring
 
 __device__ __forceinline__ float ld1(const float* p) { return *p; }
 __device__ __forceinline__ float ld1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
@@ -33,70 +36,135 @@ __device__ __forceinline__ void st1(float* p, float x) { *p = x; }
 __device__ __forceinline__ void st1(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
 __device__ __forceinline__ void st1(__half* p, float x) { *p = __float2half_rn(x); }
 
-// Eight elements as they lie in memory (16 or 32 bytes).
+__device__ __forceinline__ float2 unpack(uint32_t x, __nv_bfloat16) {
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+__device__ __forceinline__ float2 unpack(uint32_t x, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+__device__ __forceinline__ uint32_t pack(float2 x, __nv_bfloat16) {
+  const __nv_bfloat162 t = __float22bfloat162_rn(x);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+__device__ __forceinline__ uint32_t pack(float2 x, __half) {
+  const __half2 t = __float22half2_rn(x);
+  return *reinterpret_cast<const uint32_t*>(&t);
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) { return __fmul2_rn(a, b); }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// Eight elements as they lie in memory: 16 bytes, or 32 of float32.
 template <typename T>
-struct alignas(16) Raw8 {
-  T v[kE];
+struct Raw8 {
+  uint32_t v[kE * sizeof(T) / 4];
 };
 
-// The columns of a thread: vector v of VPT holds columns (v * threads + tid) * 8 + j, aligned, or,
+// One access of 16 or 32 bytes, past L1: every row is used once.
+__device__ __forceinline__ void fetch8(Raw8<float>& d, const float* p) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(d.v[0]), "=r"(d.v[1]), "=r"(d.v[2]), "=r"(d.v[3]), "=r"(d.v[4]), "=r"(d.v[5]), "=r"(d.v[6]), "=r"(d.v[7])
+               : "l"(p));
+}
+template <typename T>
+__device__ __forceinline__ void fetch8(Raw8<T>& d, const T* p) {
+  asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(d.v[0]), "=r"(d.v[1]), "=r"(d.v[2]), "=r"(d.v[3])
+               : "l"(p));
+}
+__device__ __forceinline__ void put8(float* p, const float2 (&x)[kP]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(__float_as_uint(x[0].x)),
+               "r"(__float_as_uint(x[0].y)), "r"(__float_as_uint(x[1].x)), "r"(__float_as_uint(x[1].y)),
+               "r"(__float_as_uint(x[2].x)), "r"(__float_as_uint(x[2].y)), "r"(__float_as_uint(x[3].x)),
+               "r"(__float_as_uint(x[3].y))
+               : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void put8(T* p, const float2 (&x)[kP]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(pack(x[0], T()), pack(x[1], T()), pack(x[2], T()), pack(x[3], T()));
+}
+__device__ __forceinline__ void widen(float2 (&o)[kP], const Raw8<float>& d) {
+#pragma unroll
+  for (int j = 0; j < kP; ++j) o[j] = make_float2(__uint_as_float(d.v[2 * j]), __uint_as_float(d.v[2 * j + 1]));
+}
+template <typename T>
+__device__ __forceinline__ void widen(float2 (&o)[kP], const Raw8<T>& d) {
+#pragma unroll
+  for (int j = 0; j < kP; ++j) o[j] = unpack(d.v[j], T());
+}
+
+// The columns of a thread: vector v holds columns (v * threads + tid) * 8 + j, in one access, or,
 // where the row's length or an address does not allow vectors, (v * 8 + j) * threads + tid.
 template <bool VEC>
 __device__ __forceinline__ int col_of(int v, int j, int tid, int threads) {
   return VEC ? (v * threads + tid) * kE + j : (v * kE + j) * threads + tid;
 }
 
+// A vector of a row of T in float32; zeros past the row.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load8(Raw8<T>& d, const T* p, int v, int tid, int threads, int C) {
+__device__ __forceinline__ void load8(float2 (&o)[kP], const T* p, int v, int tid, int threads, int C) {
   if constexpr (VEC) {
-    const int c = (v * threads + tid) * kE;
-    if (c < C) d = *reinterpret_cast<const Raw8<T>*>(p + c);
-  } else {
-#pragma unroll
-    for (int j = 0; j < kE; ++j) {
-      const int c = col_of<false>(v, j, tid, threads);
-      if (c < C) d.v[j] = p[c];
-    }
-  }
-}
-
-template <typename T, bool VEC>
-__device__ __forceinline__ void store8(T* p, const float (&x)[kE], int v, int tid, int threads, int C) {
-  if constexpr (VEC) {
-    const int c = (v * threads + tid) * kE;
-    if (c < C) {
-      Raw8<T> d;
-#pragma unroll
-      for (int j = 0; j < kE; ++j) st1(&d.v[j], x[j]);
-      *reinterpret_cast<Raw8<T>*>(p + c) = d;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < kE; ++j) {
-      const int c = col_of<false>(v, j, tid, threads);
-      if (c < C) st1(p + c, x[j]);
-    }
-  }
-}
-
-// A vector of a weight, bias or gate row, float32 or the activations' type; `none` past the row.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load_w(float (&o)[kE], const void* p, bool f32, int v, int tid, int threads, int C) {
-  if (f32) {
-    Raw8<float> d{};
-    load8<float, VEC>(d, reinterpret_cast<const float*>(p), v, tid, threads, C);
-#pragma unroll
-    for (int j = 0; j < kE; ++j) o[j] = d.v[j];
-  } else {
     Raw8<T> d{};
-    load8<T, VEC>(d, reinterpret_cast<const T*>(p), v, tid, threads, C);
+    const int c = (v * threads + tid) * kE;
+    if (c < C) fetch8(d, p + c);
+    widen(o, d);
+  } else {
 #pragma unroll
-    for (int j = 0; j < kE; ++j) o[j] = ld1(&d.v[j]);
+    for (int j = 0; j < kP; ++j) {
+      const int c0 = col_of<false>(v, 2 * j, tid, threads), c1 = col_of<false>(v, 2 * j + 1, tid, threads);
+      o[j] = make_float2(c0 < C ? ld1(p + c0) : 0.f, c1 < C ? ld1(p + c1) : 0.f);
+    }
   }
 }
 
-// Sums of K values over the row's threads (a whole block of `warps` warps, or one warp of a block of
-// several rows).  `buf`: 2 x K x 32 floats, used in turn, so one barrier per call is enough.
+template <typename T, bool VEC>
+__device__ __forceinline__ void store8(T* p, const float2 (&x)[kP], int v, int tid, int threads, int C) {
+  if constexpr (VEC) {
+    const int c = (v * threads + tid) * kE;
+    if (c < C) put8(p + c, x);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kP; ++j) {
+      const int c0 = col_of<false>(v, 2 * j, tid, threads), c1 = col_of<false>(v, 2 * j + 1, tid, threads);
+      if (c0 < C) st1(p + c0, x[j].x);
+      if (c1 < C) st1(p + c1, x[j].y);
+    }
+  }
+}
+
+// A vector of a weight, bias or gate row, which is float32 or the activations' type.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_w(float2 (&o)[kP], const void* p, bool f32, int v, int tid, int threads, int C) {
+  if constexpr (VEC) {                             // cached: every row uses them
+    const int c = (v * threads + tid) * kE;
+#pragma unroll
+    for (int j = 0; j < kP; ++j) o[j] = both(0.f);
+    if (c >= C) return;
+    if (f32) {
+      const float4* q = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + c);
+      const float4 x = __ldg(q), y = __ldg(q + 1);
+      o[0] = make_float2(x.x, x.y), o[1] = make_float2(x.z, x.w), o[2] = make_float2(y.x, y.y), o[3] = make_float2(y.z, y.w);
+    } else if constexpr (sizeof(T) == 2) {
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p) + c));
+      o[0] = unpack(x.x, T()), o[1] = unpack(x.y, T()), o[2] = unpack(x.z, T()), o[3] = unpack(x.w, T());
+    }
+  } else {
+    if (f32) load8<float, false>(o, reinterpret_cast<const float*>(p), v, tid, threads, C);
+    else load8<T, false>(o, reinterpret_cast<const T*>(p), v, tid, threads, C);
+  }
+}
+
+// Whether the pair's columns lie in the row (1) or past it (0).
+template <bool VEC>
+__device__ __forceinline__ float2 inside(int v, int j, int tid, int threads, int C) {
+  return make_float2(col_of<VEC>(v, 2 * j, tid, threads) < C ? 1.f : 0.f, col_of<VEC>(v, 2 * j + 1, tid, threads) < C ? 1.f : 0.f);
+}
+
+constexpr int kSums = 4;   // values of one row_sum at most
+// Sums of K values over the row's threads: one warp by shuffles, several through `buf` (two sets
+// of kSums x 32 floats used in turn, so one barrier per call is enough), added in the warps' order.
 template <int K>
 __device__ __forceinline__ void row_sum(float (&s)[K], int warps, float* buf, int& turn) {
 #pragma unroll
@@ -104,7 +172,7 @@ __device__ __forceinline__ void row_sum(float (&s)[K], int warps, float* buf, in
 #pragma unroll
     for (int k = 0; k < K; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], d);
   if (warps == 1) return;
-  float* b = buf + turn * 4 * 32;
+  float* b = buf + turn * kSums * 32;
   turn ^= 1;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   if (lane == 0)
@@ -113,11 +181,16 @@ __device__ __forceinline__ void row_sum(float (&s)[K], int warps, float* buf, in
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    float t = lane < warps ? b[k * 32 + lane] : 0.f;
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+    float t = 0.f;
+    for (int q = 0; q < warps; q += 4) {           // entries past the last warp stay zero
+      const float4 x = *reinterpret_cast<const float4*>(b + k * 32 + q);
+      t += (x.x + x.y) + (x.z + x.w);
+    }
     s[k] = t;
   }
+}
+__device__ __forceinline__ void clear_sums(float* buf) {
+  for (int i = threadIdx.x; i < 2 * kSums * 32; i += blockDim.x) buf[i] = 0.f;
 }
 
 struct NormArgs {
@@ -130,86 +203,104 @@ struct NormArgs {
   void *r, *h, *dx, *dy;         // rows of C, contiguous
   float *part, *gpart;           // backward partials
   void* dgate;
-  int post, pre, want_cols, gate_direct;
+  int post, pre, want_cols, gate_direct, stages, biases;
 };
 
 // ---------------------------------------------------------------- forward
-template <typename TX, typename TY, int VPT, bool VEC>
+// POST: with a norm of y, y and x are both held until its statistics are known; without it, only r.
+template <typename TX, typename TY, int VPT, bool VEC, bool POST>
 __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormArgs a) {
-  __shared__ float buf[2 * 4 * 32];
+  __shared__ alignas(16) float buf[2 * kSums * 32];
   // blockDim.x threads to a row; blocks of several rows have one warp to a row
   const int threads = blockDim.x, tid = threadIdx.x, warps = threads >> 5, C = a.C;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (warps > 1) {
+    clear_sums(buf);
+    __syncthreads();
+  }
   if (row >= a.rows) return;                       // uniform over the row's threads
   int turn = 0;
   const TY* yp = reinterpret_cast<const TY*>(a.y) + row * a.y_row;
   const TX* xp = reinterpret_cast<const TX*>(a.x) + row * a.x_row;
-  Raw8<TY> yr[VPT];
-  Raw8<TX> xr[VPT];
-#pragma unroll
-  for (int v = 0; v < VPT; ++v) {
-    yr[v] = Raw8<TY>{};
-    xr[v] = Raw8<TX>{};
-    load8<TY, VEC>(yr[v], yp, v, tid, threads, C);
-    load8<TX, VEC>(xr[v], xp, v, tid, threads, C);
-  }
   const float inv = 1.f / C;
-  float n[VPT][kE];
-#pragma unroll
-  for (int v = 0; v < VPT; ++v)
-#pragma unroll
-    for (int j = 0; j < kE; ++j) n[v][j] = ld1(&yr[v].v[j]);
-
-  // normalises n in place: columns past C are zero before and are never stored
-  auto normalise = [&](const void* w, const void* bias) {
+  const char* gp = reinterpret_cast<const char*>(a.gate);
+  if (a.gate && a.rows_per_gate < a.rows)
+    gp += (int64_t)((uint64_t)row < (1ull << 32) && a.rows_per_gate < (1ll << 32) ? (uint32_t)row / (uint32_t)a.rows_per_gate
+                                                                              : row / a.rows_per_gate) *
+          C * (a.wf32 ? 4 : sizeof(TY));
+  float2 n[VPT][kP];
+  auto normalise = [&](const void* w, const void* bias) {   // n in place
     float mu = 0.f;
     if (a.layer) {
-      float s[1] = {0.f};
+      float2 t = both(0.f);
 #pragma unroll
       for (int v = 0; v < VPT; ++v)
 #pragma unroll
-        for (int j = 0; j < kE; ++j) s[0] += n[v][j];
+        for (int j = 0; j < kP; ++j) t = add2(t, n[v][j]);
+      float s[1] = {t.x + t.y};
       row_sum<1>(s, warps, buf, turn);
       mu = s[0] * inv;
     }
-    float q[1] = {0.f};
+    float2 t = both(0.f);
 #pragma unroll
     for (int v = 0; v < VPT; ++v)
 #pragma unroll
-      for (int j = 0; j < kE; ++j) {
-        const float d = n[v][j] - mu;
-        if (col_of<VEC>(v, j, tid, threads) < C) q[0] += d * d;
+      for (int j = 0; j < kP; ++j) {
+        n[v][j] = add2(n[v][j], both(-mu));
+        if (a.layer) n[v][j] = mul2(n[v][j], inside<VEC>(v, j, tid, threads, C));
+        t = fma2(n[v][j], n[v][j], t);
       }
+    float q[1] = {t.x + t.y};
     row_sum<1>(q, warps, buf, turn);
     const float rstd = 1.f / sqrtf(q[0] * inv + a.eps);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      float wv[kE], bv[kE];
 #pragma unroll
-      for (int j = 0; j < kE; ++j) { wv[j] = 1.f; bv[j] = 0.f; }
-      if (w) load_w<TY, VEC>(wv, w, a.wf32, v, tid, threads, C);
-      if (bias) load_w<TY, VEC>(bv, bias, a.wf32, v, tid, threads, C);
+      for (int j = 0; j < kP; ++j) n[v][j] = mul2(n[v][j], both(rstd));
+      if (w) {
+        float2 wv[kP];
+        load_w<TY, VEC>(wv, w, a.wf32, v, tid, threads, C);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) n[v][j] = (n[v][j] - mu) * rstd * wv[j] + bv[j];
+        for (int j = 0; j < kP; ++j) n[v][j] = mul2(n[v][j], wv[j]);
+      }
+      if (bias) {
+        float2 bv[kP];
+        load_w<TY, VEC>(bv, bias, a.wf32, v, tid, threads, C);
+#pragma unroll
+        for (int j = 0; j < kP; ++j) n[v][j] = add2(n[v][j], bv[j]);
+      }
     }
   };
-  if (a.post) normalise(a.w_post, a.b_post);
-  const int64_t grow = a.gate ? row / a.rows_per_gate : 0;
-#pragma unroll
-  for (int v = 0; v < VPT; ++v) {
-    float g[kE];
-#pragma unroll
-    for (int j = 0; j < kE; ++j) g[j] = 1.f;
+  auto join = [&](int v, const float2 (&x)[kP]) {           // n = alpha x + g n
     if (a.gate) {
-      const char* gp = reinterpret_cast<const char*>(a.gate) + grow * C * (a.wf32 ? 4 : sizeof(TY));
+      float2 g[kP];
       load_w<TY, VEC>(g, gp, a.wf32, v, tid, threads, C);
+#pragma unroll
+      for (int j = 0; j < kP; ++j) n[v][j] = mul2(n[v][j], g[j]);
     }
 #pragma unroll
-    for (int j = 0; j < kE; ++j) {
-      const float t = a.alpha * ld1(&xr[v].v[j]) + g[j] * n[v][j];
-      n[v][j] = col_of<VEC>(v, j, tid, threads) < C ? t : 0.f;
-    }
+    for (int j = 0; j < kP; ++j) n[v][j] = fma2(both(a.alpha), x[j], n[v][j]);
     store8<TX, VEC>(reinterpret_cast<TX*>(a.r) + row * C, n[v], v, tid, threads, C);
+  };
+  if constexpr (POST) {
+    float2 x[VPT][kP];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      load8<TY, VEC>(n[v], yp, v, tid, threads, C);
+      load8<TX, VEC>(x[v], xp, v, tid, threads, C);
+    }
+    normalise(a.w_post, a.b_post);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) join(v, x[v]);
+  } else {
+    float2 x[VPT][kP];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      load8<TY, VEC>(n[v], yp, v, tid, threads, C);
+      load8<TX, VEC>(x[v], xp, v, tid, threads, C);
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) join(v, x[v]);
   }
   if (!a.pre) return;
   // h is the norm of r before r's rounding to the stream's type
@@ -222,148 +313,238 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
 // Columns of the partial sums, in this order.
 enum { kDwPost, kDbPost, kDwPre, kDbPre, kCols };
 
-template <typename TX, typename TY, bool VEC, int MAXT>
+// Rows of the stages of the ring: dr, r (stream type), dh, y, one after the other.
+template <typename TX, typename TY>
+__host__ __device__ inline int stage_bytes(int C) {
+  return C * (2 * (int)sizeof(TX) + 2 * (int)sizeof(TY));
+}
+
+// FULL: with means (layer norm) or biases.  RING: rows come through a ring of `stages` rows in
+// shared memory, filled by bulk copies that run ahead of the arithmetic without holding registers;
+// else (two rows do not fit, or VEC does not hold) each thread reads its columns directly.  Weights
+// lie in shared memory as float32; a thread only touches its own columns of them.
+template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>
 __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormArgs a) {
-  __shared__ float buf[2 * 4 * 32];
+  extern __shared__ __align__(128) uint8_t dyn[];
+  __shared__ alignas(16) float buf[2 * kSums * 32];
+  __shared__ uint64_t full[kMaxStages];
+  __shared__ int dead_flag;
+  volatile int* dead = &dead_flag;
   const int threads = blockDim.x, tid = threadIdx.x, warps = threads >> 5, C = a.C;
   const int64_t first = a.rows * blockIdx.x / gridDim.x, last = a.rows * (blockIdx.x + 1) / gridDim.x;
-  const float inv = 1.f / C;
   int turn = 0;
-  float acc[kCols][kE], dg[kE];
+  const float inv = 1.f / C, inv_mean = a.layer ? inv : 0.f;
+  const int stride = threads * kE;                          // floats of one weight
+  float* const weights = reinterpret_cast<float*>(dyn);     // w_pre, w_post, gate, and b_post
+  uint8_t* const ring = dyn + (FULL ? 4 : 3) * stride * sizeof(float);
+  const bool need_y = a.post || a.gate;
+  const int bytes_x = C * (int)sizeof(TX), bytes_y = C * (int)sizeof(TY);
+  const uint32_t expect = bytes_x + (a.pre ? bytes_x + bytes_y : 0) + (need_y ? bytes_y : 0);
+  auto request = [&](int64_t row) {                         // one thread: the copies of a row
+    if (row >= last) return;
+    const int st = (int)((row - first) % a.stages);
+    const uint32_t bar = smem_u32(&full[st]);
+    uint8_t* to = ring + (size_t)st * stage_bytes<TX, TY>(C);
+    mbar_expect(bar, expect);
+    bulk_copy(smem_u32(to), reinterpret_cast<const TX*>(a.dr) + row * a.dr_row, bytes_x, bar);
+    if (a.pre) {
+      bulk_copy(smem_u32(to + bytes_x), reinterpret_cast<const TX*>(a.x) + row * a.x_row, bytes_x, bar);
+      bulk_copy(smem_u32(to + 2 * bytes_x), reinterpret_cast<const TY*>(a.dh) + row * a.dh_row, bytes_y, bar);
+    }
+    if (need_y) bulk_copy(smem_u32(to + 2 * bytes_x + bytes_y), reinterpret_cast<const TY*>(a.y) + row * a.y_row, bytes_y, bar);
+  };
+  clear_sums(buf);
+  if (RING && tid == 0) {
+    dead_flag = 0;
+    for (int i = 0; i < a.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
+    fence_async();
+  }
+  auto own = [&](int which) { return reinterpret_cast<float4*>(weights + which * stride + tid * kE); };
+  auto keep = [&](int which, const void* p, float none) {   // a weight's columns of this thread to shared memory
+    float2 t[kP];
+#pragma unroll
+    for (int j = 0; j < kP; ++j) t[j] = both(none);
+    if (p) load_w<TY, VEC>(t, p, a.wf32, 0, tid, threads, C);
+    own(which)[0] = make_float4(t[0].x, t[0].y, t[1].x, t[1].y);
+    own(which)[1] = make_float4(t[2].x, t[2].y, t[3].x, t[3].y);
+  };
+  auto weight = [&](int which, float2 (&o)[kP]) {
+    const float4 x = own(which)[0], y = own(which)[1];
+    o[0] = make_float2(x.x, x.y), o[1] = make_float2(x.z, x.w), o[2] = make_float2(y.x, y.y), o[3] = make_float2(y.z, y.w);
+  };
+  keep(0, a.w_pre, 1.f);
+  keep(1, a.w_post, 1.f);
+  if (FULL) keep(3, a.b_post, 0.f);
+  __syncthreads();
+  if (RING && tid == 0)
+    for (int i = 0; i < a.stages; ++i) request(first + i);
+
+  float2 acc[kCols][kP], dg[kP];                            // the biases' columns stay unused without FULL
 #pragma unroll
   for (int k = 0; k < kCols; ++k)
 #pragma unroll
-    for (int j = 0; j < kE; ++j) acc[k][j] = 0.f;
+    for (int j = 0; j < kP; ++j) acc[k][j] = both(0.f);
 #pragma unroll
-  for (int j = 0; j < kE; ++j) dg[j] = 0.f;
-  bool in[kE];
-#pragma unroll
-  for (int j = 0; j < kE; ++j) in[j] = col_of<VEC>(0, j, tid, threads) < C;
-
-  Raw8<TX> drr{}, rr{};
-  Raw8<TY> dhr{}, yr{};
-  const bool need_y = a.post || a.gate;
-  auto fetch = [&](int64_t row) {
-    load8<TX, VEC>(drr, reinterpret_cast<const TX*>(a.dr) + row * a.dr_row, 0, tid, threads, C);
-    if (a.pre) {
-      load8<TX, VEC>(rr, reinterpret_cast<const TX*>(a.x) + row * a.x_row, 0, tid, threads, C);
-      load8<TY, VEC>(dhr, reinterpret_cast<const TY*>(a.dh) + row * a.dh_row, 0, tid, threads, C);
-    }
-    if (need_y) load8<TY, VEC>(yr, reinterpret_cast<const TY*>(a.y) + row * a.y_row, 0, tid, threads, C);
-  };
-  if (first < last) fetch(first);
-  int64_t group = a.gate ? first / a.rows_per_gate : 0;
+  for (int j = 0; j < kP; ++j) dg[j] = both(0.f);
+  const bool cols = VEC ? tid * kE < C : true;              // whether this thread has columns at all
+  int64_t group = 0, group_end = a.rows;                    // the gate row at work, and where its rows end
+  if (a.gate) {
+    group = first / a.rows_per_gate;
+    group_end = (group + 1) * a.rows_per_gate;
+    keep(2, reinterpret_cast<const char*>(a.gate) + group * C * (a.wf32 ? 4 : sizeof(TY)), 1.f);
+  }
+  int st = 0, round = 0;
   for (int64_t row = first; row < last; ++row) {
-    float d[kE], r[kE], dh[kE], y[kE];
+    const uint8_t* at = ring + (size_t)st * stage_bytes<TX, TY>(C);
+    auto fetch = [&](float2 (&o)[kP], int off, auto type, const void* p, int64_t step, bool on) {
+      using T = decltype(type);
 #pragma unroll
-    for (int j = 0; j < kE; ++j) {
-      d[j] = ld1(&drr.v[j]);
-      r[j] = ld1(&rr.v[j]);
-      dh[j] = ld1(&dhr.v[j]);
-      y[j] = ld1(&yr.v[j]);
-    }
-    if (row + 1 < last) fetch(row + 1);            // in flight while this row is worked on
-    float z[kE];
-    {
-      float w[kE];
+      for (int j = 0; j < kP; ++j) o[j] = both(0.f);
+      if (!on) return;
+      if constexpr (RING) {
+        if (cols) {
+          Raw8<T> d;
+          const uint4* q = reinterpret_cast<const uint4*>(at + off + tid * kE * (int)sizeof(T));
+          *reinterpret_cast<uint4*>(d.v) = q[0];
+          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(d.v + 4) = q[1];
+          widen(o, d);
+        }
+      } else {
+        load8<T, VEC>(o, reinterpret_cast<const T*>(p) + row * step, 0, tid, threads, C);
+      }
+    };
+    if (RING) mbar_wait(smem_u32(&full[st]), round & 1, dead);
+    float2 r[kP], dh[kP], y[kP], z[kP], d[kP];
+    fetch(r, bytes_x, TX(), a.x, a.x_row, a.pre);
+    fetch(dh, 2 * bytes_x, TY(), a.dh, a.dh_row, a.pre);
+    fetch(y, 2 * bytes_x + bytes_y, TY(), a.y, a.y_row, need_y);
+    fetch(d, 0, TX(), a.dr, a.dr_row, true);
+    weight(0, z);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) w[j] = 1.f;
-      if (a.pre && a.w_pre) load_w<TY, VEC>(w, a.w_pre, a.wf32, 0, tid, threads, C);
-#pragma unroll
-      for (int j = 0; j < kE; ++j) z[j] = dh[j] * w[j];
-    }
+    for (int j = 0; j < kP; ++j) z[j] = mul2(dh[j], z[j]);
     // statistics of both rows together
-    float mu_r = 0.f, mu_y = 0.f, mean_z = 0.f;
-    if (a.layer) {
-      float s[3] = {0.f, 0.f, 0.f};
+    float mean_z = 0.f;
+    if (FULL) {
+      float2 t[3] = {both(0.f), both(0.f), both(0.f)};
 #pragma unroll
-      for (int j = 0; j < kE; ++j) { s[0] += r[j]; s[1] += y[j]; s[2] += z[j]; }
+      for (int j = 0; j < kP; ++j) {
+        t[0] = add2(t[0], r[j]);
+        t[1] = add2(t[1], y[j]);
+        t[2] = add2(t[2], z[j]);
+      }
+      float s[3] = {t[0].x + t[0].y, t[1].x + t[1].y, t[2].x + t[2].y};
       row_sum<3>(s, warps, buf, turn);
-      mu_r = s[0] * inv;
-      mu_y = s[1] * inv;
-      mean_z = s[2] * inv;
-    }
-    float q[3] = {0.f, 0.f, 0.f};
+      const float mu_r = -s[0] * inv_mean, mu_y = a.post ? -s[1] * inv_mean : 0.f;
+      mean_z = s[2] * inv_mean;
 #pragma unroll
-    for (int j = 0; j < kE; ++j) {
-      r[j] = in[j] ? r[j] - mu_r : 0.f;
-      y[j] = in[j] && a.post ? y[j] - mu_y : y[j];
-      q[0] += r[j] * r[j];
-      q[1] += y[j] * y[j];
-      q[2] += z[j] * r[j];
+      for (int j = 0; j < kP; ++j) {
+        const float2 in = inside<VEC>(0, j, tid, threads, C);
+        r[j] = mul2(add2(r[j], both(mu_r)), in);
+        y[j] = mul2(add2(y[j], both(mu_y)), in);
+      }
     }
+    float2 t[3] = {both(0.f), both(0.f), both(0.f)};
+#pragma unroll
+    for (int j = 0; j < kP; ++j) {
+      t[0] = fma2(r[j], r[j], t[0]);
+      t[1] = fma2(y[j], y[j], t[1]);
+      t[2] = fma2(z[j], r[j], t[2]);
+    }
+    float q[3] = {t[0].x + t[0].y, t[1].x + t[1].y, t[2].x + t[2].y};
     row_sum<3>(q, warps, buf, turn);
+    if (RING && tid == 0 && row > first) request(row - 1 + a.stages);   // every thread has left the row before
     if (a.pre) {
-      const float rstd = 1.f / sqrtf(q[0] * inv + a.eps), proj = q[2] * inv * rstd;   // mean(z rhat)
+      const float rstd = 1.f / sqrtf(q[0] * inv + a.eps), proj = -q[2] * inv * rstd;   // -mean(z rhat)
 #pragma unroll
-      for (int j = 0; j < kE; ++j) {
-        const float hat = r[j] * rstd;
-        acc[kDwPre][j] += dh[j] * hat;
-        acc[kDbPre][j] += dh[j];
-        d[j] += rstd * (z[j] - mean_z - hat * proj);
+      for (int j = 0; j < kP; ++j) {
+        const float2 hat = mul2(r[j], both(rstd));
+        acc[kDwPre][j] = fma2(dh[j], hat, acc[kDwPre][j]);
+        if (FULL) acc[kDbPre][j] = add2(acc[kDbPre][j], dh[j]);
+        const float2 v = fma2(hat, both(proj), FULL ? add2(z[j], both(-mean_z)) : z[j]);
+        d[j] = fma2(both(rstd), v, d[j]);
       }
     }
     {
-      float o[kE];
+      float2 o[kP];
 #pragma unroll
-      for (int j = 0; j < kE; ++j) o[j] = a.alpha * d[j];
+      for (int j = 0; j < kP; ++j) o[j] = mul2(both(a.alpha), d[j]);
       store8<TX, VEC>(reinterpret_cast<TX*>(a.dx) + row * C, o, 0, tid, threads, C);
     }
     const float rstd = a.post ? 1.f / sqrtf(q[1] * inv + a.eps) : 1.f;
-    float w[kE], b[kE], g[kE];
 #pragma unroll
-    for (int j = 0; j < kE; ++j) { w[j] = 1.f; b[j] = 0.f; g[j] = 1.f; }
-    if (a.post && a.w_post) load_w<TY, VEC>(w, a.w_post, a.wf32, 0, tid, threads, C);
+    for (int j = 0; j < kP; ++j) y[j] = mul2(y[j], both(rstd));        // yhat
+    float2 w[kP];
+    weight(1, w);
     if (a.gate) {
-      if (a.post && a.b_post) load_w<TY, VEC>(b, a.b_post, a.wf32, 0, tid, threads, C);
-      const int64_t grow = row / a.rows_per_gate;
-      if (grow != group) {                         // uniform: the block's rows enter another gate row
-        if (!a.gate_direct) {
+      if (row == group_end) {                      // uniform: the block's rows enter another gate row
+        if (!a.gate_direct && cols) {
 #pragma unroll
-          for (int j = 0; j < kE; ++j)
-            if (in[j]) a.gpart[(blockIdx.x + group) * C + col_of<VEC>(0, j, tid, threads)] = dg[j];
+          for (int j = 0; j < kE; ++j) {
+            const int c = col_of<VEC>(0, j, tid, threads);
+            if (c < C) a.gpart[(blockIdx.x + group) * C + c] = (j & 1) ? dg[j / 2].y : dg[j / 2].x;
+          }
         }
 #pragma unroll
-        for (int j = 0; j < kE; ++j) dg[j] = 0.f;
-        group = grow;
+        for (int j = 0; j < kP; ++j) dg[j] = both(0.f);
+        ++group;
+        group_end += a.rows_per_gate;
+        keep(2, reinterpret_cast<const char*>(a.gate) + group * C * (a.wf32 ? 4 : sizeof(TY)), 1.f);
       }
-      const char* gp = reinterpret_cast<const char*>(a.gate) + grow * C * (a.wf32 ? 4 : sizeof(TY));
-      load_w<TY, VEC>(g, gp, a.wf32, 0, tid, threads, C);
+      float2 g[kP], b[kP];
+      weight(2, g);
+      if (FULL) weight(3, b);
 #pragma unroll
-      for (int j = 0; j < kE; ++j) dg[j] += d[j] * (y[j] * rstd * w[j] + b[j]);
+      for (int j = 0; j < kP; ++j) {
+        const float2 n = FULL ? fma2(y[j], w[j], b[j]) : mul2(y[j], w[j]);
+        dg[j] = fma2(d[j], n, dg[j]);
+        d[j] = mul2(d[j], g[j]);
+      }
       if (a.gate_direct) {                         // one row to a gate row: no partials
         if (a.wf32) store8<float, VEC>(reinterpret_cast<float*>(a.dgate) + row * C, dg, 0, tid, threads, C);
         else store8<TY, VEC>(reinterpret_cast<TY*>(a.dgate) + row * C, dg, 0, tid, threads, C);
       }
     }
-    float s[2] = {0.f, 0.f};
+    if (a.post) {
+      float2 u[2] = {both(0.f), both(0.f)};
 #pragma unroll
-    for (int j = 0; j < kE; ++j) {
-      d[j] *= g[j];
-      if (a.post) {
-        y[j] *= rstd;                              // yhat
-        acc[kDwPost][j] += d[j] * y[j];
-        acc[kDbPost][j] += d[j];
-        d[j] *= w[j];
-        if (in[j]) { s[0] += d[j]; s[1] += d[j] * y[j]; }
+      for (int j = 0; j < kP; ++j) {
+        acc[kDwPost][j] = fma2(d[j], y[j], acc[kDwPost][j]);
+        if (FULL) acc[kDbPost][j] = add2(acc[kDbPost][j], d[j]);
+        d[j] = mul2(d[j], w[j]);
+        if (FULL) u[0] = add2(u[0], d[j]);
+        u[1] = fma2(d[j], y[j], u[1]);
+      }
+      float s[2] = {u[0].x + u[0].y, u[1].x + u[1].y};
+      row_sum<2>(s, warps, buf, turn);
+      const float mz = FULL ? -s[0] * inv_mean : 0.f, proj = -s[1] * inv;
+#pragma unroll
+      for (int j = 0; j < kP; ++j) {
+        const float2 v = fma2(y[j], both(proj), FULL ? add2(d[j], both(mz)) : d[j]);
+        d[j] = mul2(both(rstd), v);
       }
     }
-    if (a.post) {
-      row_sum<2>(s, warps, buf, turn);
-      const float mz = a.layer ? s[0] * inv : 0.f, proj = s[1] * inv;
-#pragma unroll
-      for (int j = 0; j < kE; ++j) d[j] = rstd * (d[j] - mz - y[j] * proj);
-    }
     store8<TY, VEC>(reinterpret_cast<TY*>(a.dy) + row * C, d, 0, tid, threads, C);
+    if (++st == a.stages) {
+      st = 0;
+      ++round;
+    }
+  }
+  if (RING && *dead) {                              // a copy never came: say so in every result
+#pragma unroll
+    for (int k = 0; k < kCols; ++k)
+#pragma unroll
+      for (int j = 0; j < kP; ++j) acc[k][j] = dg[j] = both(__int_as_float(0x7fffffff));
+    for (int t = 0; t < 100; ++t) __nanosleep(1000);
   }
 #pragma unroll
   for (int j = 0; j < kE; ++j) {
-    if (!in[j]) continue;
     const int c = col_of<VEC>(0, j, tid, threads);
+    if (c >= C) continue;
     if (a.want_cols)
 #pragma unroll
-      for (int k = 0; k < kCols; ++k) a.part[((int64_t)blockIdx.x * kCols + k) * C + c] = acc[k][j];
-    if (a.gate && !a.gate_direct && first < last) a.gpart[(blockIdx.x + group) * C + c] = dg[j];
+      for (int k = 0; k < kCols; ++k)
+        a.part[((int64_t)blockIdx.x * kCols + k) * C + c] = (j & 1) ? acc[k][j / 2].y : acc[k][j / 2].x;
+    if (a.gate && !a.gate_direct && first < last) a.gpart[(blockIdx.x + group) * C + c] = (j & 1) ? dg[j / 2].y : dg[j / 2].x;
   }
 }
 
@@ -432,6 +613,12 @@ constexpr int kMaxC = 8192;
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
+template <typename TX, typename TY, int VPT, bool VEC>
+void fwd_kernel(const NormArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
+  if (a.post) k_norm_fwd<TX, TY, VPT, VEC, true><<<grid, block, 0, s>>>(a);
+  else k_norm_fwd<TX, TY, VPT, VEC, false><<<grid, block, 0, s>>>(a);
+}
+
 template <typename TX, typename TY, bool VEC>
 int fwd_launch(const NormArgs& a, cudaStream_t s) {
   // One warp holds up to 1024 columns (32 a lane); longer rows take up to 8 warps.  Few rows
@@ -448,32 +635,48 @@ int fwd_launch(const NormArgs& a, cudaStream_t s) {
   const dim3 block(threads, threads == 32 ? 4 : 1);
   const int64_t grid = (a.rows + block.y - 1) / block.y;
   B3R_REQUIRE(grid <= 0x7fffffff, "residual_norm: too many rows for one call");
-  if (vpt == 1) k_norm_fwd<TX, TY, 1, VEC><<<(unsigned)grid, block, 0, s>>>(a);
-  else if (vpt == 2) k_norm_fwd<TX, TY, 2, VEC><<<(unsigned)grid, block, 0, s>>>(a);
-  else k_norm_fwd<TX, TY, 4, VEC><<<(unsigned)grid, block, 0, s>>>(a);
+  if (vpt == 1) fwd_kernel<TX, TY, 1, VEC>(a, (unsigned)grid, block, s);
+  else if (vpt == 2) fwd_kernel<TX, TY, 2, VEC>(a, (unsigned)grid, block, s);
+  else fwd_kernel<TX, TY, 4, VEC>(a, (unsigned)grid, block, s);
   return check_launch("residual_norm");
 }
 
 int bwd_threads(int C) { return (C + kE * 32 - 1) / (kE * 32) * 32; }
 
-// Blocks of the backward pass: as many as fit the 148 SMs at once, each with a run of rows.
-int bwd_blocks(int64_t rows, int C) {
-  const int per_sm = std::max(1, std::min(8, 512 / bwd_threads(C)));
-  return (int)std::min<int64_t>(rows, 148 * per_sm);
+// Blocks of the backward pass: as many as fit the 148 SMs at once (512 threads an SM, by their
+// registers), each with a run of rows.
+int bwd_per_sm(int C) { return std::max(1, std::min(16, 512 / bwd_threads(C))); }
+int bwd_blocks(int64_t rows, int C) { return (int)std::min<int64_t>(rows, 148 * bwd_per_sm(C)); }
+
+template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>
+int bwd_kernel(const NormArgs& a, int smem, cudaStream_t s) {
+  auto* f = k_norm_bwd<TX, TY, FULL, VEC, RING, MAXT>;
+  B3R_TRY(check_cuda(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "residual_norm backward"));
+  f<<<bwd_blocks(a.rows, a.C), bwd_threads(a.C), smem, s>>>(a);
+  return check_launch("residual_norm backward");
 }
 
-template <typename TX, typename TY, bool VEC>
-int bwd_launch(const NormArgs& a, cudaStream_t s) {
-  const int threads = bwd_threads(a.C), blocks = bwd_blocks(a.rows, a.C);
-  if (threads <= 512) k_norm_bwd<TX, TY, VEC, 512><<<blocks, threads, 0, s>>>(a);
-  else k_norm_bwd<TX, TY, VEC, 1024><<<blocks, threads, 0, s>>>(a);
-  return check_launch("residual_norm backward");
+template <typename TX, typename TY, bool FULL, bool VEC>
+int bwd_launch(NormArgs a, cudaStream_t s) {
+  const int threads = bwd_threads(a.C), stage = stage_bytes<TX, TY>(a.C);
+  const int weights = (FULL ? 4 : 3) * threads * kE * 4, room = (227 * 1024) / bwd_per_sm(a.C) - 3072;
+  a.stages = std::min(kMaxStages, (room - weights) / stage);
+  if (VEC && a.stages >= 2) {
+    const int smem = weights + a.stages * stage;
+    return threads <= 512 ? bwd_kernel<TX, TY, FULL, VEC, VEC, 512>(a, smem, s) : bwd_kernel<TX, TY, FULL, VEC, VEC, 1024>(a, smem, s);
+  }
+  return bwd_kernel<TX, TY, FULL, VEC, false, 1024>(a, weights, s);
 }
 
 template <bool FWD, typename TX, typename TY>
 int go2(const NormArgs& a, bool vec, cudaStream_t s) {
-  if constexpr (FWD) return vec ? fwd_launch<TX, TY, true>(a, s) : fwd_launch<TX, TY, false>(a, s);
-  else return vec ? bwd_launch<TX, TY, true>(a, s) : bwd_launch<TX, TY, false>(a, s);
+  if constexpr (FWD) {
+    return vec ? fwd_launch<TX, TY, true>(a, s) : fwd_launch<TX, TY, false>(a, s);
+  } else {
+    const bool full = a.layer || a.biases;
+    if (vec) return full ? bwd_launch<TX, TY, true, true>(a, s) : bwd_launch<TX, TY, false, true>(a, s);
+    return full ? bwd_launch<TX, TY, true, false>(a, s) : bwd_launch<TX, TY, false, false>(a, s);
+  }
 }
 
 template <bool FWD>
@@ -516,8 +719,8 @@ int common(const b3r_residual_norm* d, NormArgs& a) {
   return B3R_OK;
 }
 
-// Whether every row of `p` starts on 16 bytes (strides in elements of 2 or 4 bytes: multiples of 8).
-bool rows_ok(const void* p, int64_t stride) { return aligned16(p) && stride % kE == 0; }
+// Whether every row of `p` starts on a vector (16 bytes, 32 of float32; strides: multiples of 8).
+bool rows_ok(const void* p, int64_t stride, int type) { return ((uintptr_t)p & (type == B3R_F32 ? 31 : 15)) == 0 && stride % kE == 0; }
 
 bool weights_ok(const NormArgs& a) {
   return aligned16(a.w_post) && aligned16(a.b_post) && aligned16(a.gate) && aligned16(a.w_pre) && aligned16(a.b_pre);
@@ -542,7 +745,8 @@ extern "C" int b3r_residual_norm_fwd(const b3r_residual_norm* d, const void* y, 
   a.x_row = x_row;
   a.r = r;
   a.h = h;
-  const bool vec = a.C % kE == 0 && rows_ok(y, y_row) && rows_ok(x, x_row) && aligned16(r) && aligned16(h) && weights_ok(a);
+  const int st = d->stream_dtype, dt = d->dtype;
+  const bool vec = a.C % kE == 0 && rows_ok(y, y_row, dt) && rows_ok(x, x_row, st) && rows_ok(r, 0, st) && rows_ok(h, 0, dt) && weights_ok(a);
   return go<true>(a, d->stream_dtype, d->dtype, vec, as_stream(stream));
 }
 
@@ -588,14 +792,17 @@ extern "C" int b3r_residual_norm_bwd(const b3r_residual_norm* d, const void* dr,
   a.dx = dx;
   a.dy = dy;
   a.dgate = dgate;
+  const bool need_y = a.post || a.gate;
   a.gate_direct = a.gate && a.rows_per_gate == 1;
+  a.biases = a.b_post || db_post || db_pre;
   a.want_cols = dw_post || db_post || dw_pre || db_pre;
   const int blocks = bwd_blocks(a.rows, a.C);
   a.part = reinterpret_cast<float*>(work);
   a.gpart = reinterpret_cast<float*>(reinterpret_cast<char*>(work) + align256((int64_t)blocks * kCols * a.C * 4));
-  const bool vec = a.C % kE == 0 && rows_ok(dr, dr_row) && aligned16(dx) && aligned16(dy) && aligned16(dgate) &&
-                   weights_ok(a) && (!a.pre || (rows_ok(dh, dh_row) && rows_ok(r, r_row))) &&
-                   ((!a.post && !a.gate) || rows_ok(y, y_row));
+  const int st = d->stream_dtype, dt = d->dtype;
+  const bool vec = a.C % kE == 0 && rows_ok(dr, dr_row, st) && rows_ok(dx, 0, st) && rows_ok(dy, 0, dt) &&
+                   rows_ok(dgate, 0, d->weight_dtype) && weights_ok(a) &&
+                   (!a.pre || (rows_ok(dh, dh_row, dt) && rows_ok(r, r_row, st))) && (!need_y || rows_ok(y, y_row, dt));
   B3R_TRY(go<false>(a, d->stream_dtype, d->dtype, vec, s));
   RedArgs q{};
   q.part = a.part;

@@ -9,8 +9,8 @@
 //
 // One thread owns one slot of a token: V pairs, or V elements that pass through, with V the
 // widest vector that the layout and the alignment allow.  It reads the slot's cosines and
-// sines once and keeps them in registers while it walks over the heads of the queries and of
-// the keys, four heads' loads in flight at a time; neighbouring threads own neighbouring slots.
+// sines once and keeps them in registers while it walks over four heads, two heads' loads in
+// flight at a time; neighbouring threads own neighbouring slots.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -20,12 +20,15 @@ namespace b3r {
 namespace {
 
 constexpr int kRotThreads = 256;
-constexpr int kRotHeads = 4;   // heads whose loads a thread has in flight
+constexpr int kRotHeads = 4;   // heads that a thread walks over
+constexpr int kRotBatch = 2;   // of them, how many have their loads in flight at once
 
 struct RotArgs {
   b3r_rotary_part part[2];
-  int64_t tokens, T;             // B * T, and T
-  int D, half, axes, heads, lanes, n_pos, slots, rot_slots;
+  int64_t T;
+  uint32_t threads[2];           // work of each part: tokens * lanes * slots
+  int lanes[2];
+  int D, half, axes, n_pos, slots, rot_slots;
   const float2* table;
   const void* pos;
   int64_t pos_batch, pos_token;
@@ -50,17 +53,16 @@ template <>
 __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 
 // V: elements of one vector.  Half layout: a rotated slot is the vectors at e and e + half.
-// Interleaved: a rotated slot is the vector at e, V / 2 pairs (V >= 2).
+// Interleaved: a rotated slot is the vector at e, V / 2 pairs (V >= 2).  blockIdx.y: the part.
 template <typename T, int V, bool IL>
-__global__ void __launch_bounds__(kRotThreads) k_rotary(const __grid_constant__ RotArgs a) {
-  const int64_t i = (int64_t)blockIdx.x * kRotThreads + threadIdx.x;
-  const int slot = (int)(i % a.slots);
-  const int64_t rest = i / a.slots;
-  const int lane = (int)(rest % a.lanes);
-  const int64_t tok = rest / a.lanes;
-  if (tok >= a.tokens) return;
-  const int64_t b = tok / a.T, t = tok - b * a.T;
-  const bool turns = slot < a.rot_slots;
+__global__ void __launch_bounds__(kRotThreads, 4) k_rotary(const __grid_constant__ RotArgs a) {
+  const int part = blockIdx.y, lanes = a.lanes[part];
+  const uint32_t i = blockIdx.x * kRotThreads + threadIdx.x;
+  if (i >= a.threads[part]) return;
+  const uint32_t rest = i / (uint32_t)a.slots, slot = i - rest * a.slots;
+  const uint32_t tok = rest / (uint32_t)lanes, lane = rest - tok * lanes;
+  const uint32_t b = tok / (uint32_t)a.T, t = tok - b * (uint32_t)a.T;
+  const bool turns = (int)slot < a.rot_slots;
   constexpr int NP = IL ? V / 2 : V;   // pairs of a slot
   float c[NP], s[NP];
   int e;                               // the slot's first element
@@ -68,54 +70,51 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const __grid_constant__ 
     if constexpr (IL) {
       e = slot * V;
     } else {
-      const int per = a.half / V, sec = slot / per;
-      e = sec * 2 * a.half + (slot - sec * per) * V;
+      const int per = a.half / V, sec = (int)slot / per;
+      e = sec * 2 * a.half + ((int)slot - sec * per) * V;
     }
-    int last_ax = -1;
-    int64_t p = 0;
-    float2 cs[NP];
+    // a vector of the half layout lies in one section; one of the interleaved layout may span two
+    int ax = e / (2 * a.half), k = e - ax * 2 * a.half;
+    if (IL) k /= 2;
+    const int64_t at = b * a.pos_batch + t * a.pos_token;
+    auto position = [&](int x) -> int64_t {
+      return a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[at + x] : (int64_t) reinterpret_cast<const int32_t*>(a.pos)[at + x];
+    };
+    int64_t p = position(ax);
+    const float sign = a.inverse ? -1.f : 1.f;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-      const int el = IL ? e + 2 * j : e + j;
-      const int ax = el / (2 * a.half), k = IL ? (el - ax * 2 * a.half) / 2 : el - ax * 2 * a.half;
-      if (ax != last_ax) {             // a vector of the interleaved layout may span two sections
-        const int64_t at = b * a.pos_batch + t * a.pos_token + ax;
-        p = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[at] : reinterpret_cast<const int32_t*>(a.pos)[at];
-        last_ax = ax;
+      if (IL && k == a.half) {
+        k = 0;
+        p = position(++ax);
       }
       // a position outside of the table has no angle: its pairs come out as NaN
       const float nan = __int_as_float(0x7fffffff);
-      cs[j] = (p >= 0 && p < a.n_pos) ? __ldg(a.table + p * a.half + k) : make_float2(nan, nan);
-    }
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-      c[j] = cs[j].x;
-      s[j] = a.inverse ? -cs[j].y : cs[j].y;
+      const float2 cs = (p >= 0 && p < a.n_pos) ? __ldg(a.table + p * a.half + k) : make_float2(nan, nan);
+      c[j] = cs.x;
+      s[j] = sign * cs.y;
+      ++k;
     }
   } else {
-    e = a.axes * 2 * a.half + (slot - a.rot_slots) * V;
+    e = a.axes * 2 * a.half + ((int)slot - a.rot_slots) * V;
   }
   using W = Vec<T, V>;
-  for (int h0 = lane; h0 < a.heads; h0 += a.lanes * kRotHeads) {
-    W lo[kRotHeads], hi[kRotHeads];
-    T* to[kRotHeads];
+  const b3r_rotary_part& pt = a.part[part];
+  const T* from = reinterpret_cast<const T*>(pt.x) + b * pt.x_batch + t * pt.x_token + lane * pt.x_head + e;
+  T* to = reinterpret_cast<T*>(pt.out) + b * pt.out_batch + t * pt.out_token + lane * pt.out_head + e;
+  const int64_t from_step = lanes * pt.x_head, to_step = lanes * pt.out_head;
+  for (int h = lane; h < pt.heads; h += lanes * kRotBatch) {
+    W lo[kRotBatch], hi[kRotBatch];
 #pragma unroll
-    for (int q = 0; q < kRotHeads; ++q) {
-      const int h = h0 + q * a.lanes;
-      to[q] = nullptr;
-      if (h < a.heads) {
-        const bool second = h >= a.part[0].heads;
-        const b3r_rotary_part& pt = second ? a.part[1] : a.part[0];
-        const int hh = second ? h - a.part[0].heads : h;
-        const T* from = reinterpret_cast<const T*>(pt.x) + b * pt.x_batch + t * pt.x_token + hh * pt.x_head + e;
-        to[q] = reinterpret_cast<T*>(pt.out) + b * pt.out_batch + t * pt.out_token + hh * pt.out_head + e;
-        lo[q] = *reinterpret_cast<const W*>(from);
-        if (!IL && turns) hi[q] = *reinterpret_cast<const W*>(from + a.half);
+    for (int q = 0; q < kRotBatch; ++q)
+      if (h + q * lanes < pt.heads) {
+        lo[q] = *reinterpret_cast<const W*>(from + q * from_step);
+        if (!IL && turns) hi[q] = *reinterpret_cast<const W*>(from + q * from_step + a.half);
       }
-    }
 #pragma unroll
-    for (int q = 0; q < kRotHeads; ++q) {
-      if (!to[q]) continue;
+    for (int q = 0; q < kRotBatch; ++q) {
+      if (h + q * lanes >= pt.heads) break;
+      T* o = to + q * to_step;
       if (turns) {
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
@@ -125,10 +124,12 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary(const __grid_constant__ 
           ru = from_f<T>(u * c[j] - w * s[j]);
           rw = from_f<T>(w * c[j] + u * s[j]);
         }
-        if (!IL) *reinterpret_cast<W*>(to[q] + a.half) = hi[q];
+        if (!IL) *reinterpret_cast<W*>(o + a.half) = hi[q];
       }
-      *reinterpret_cast<W*>(to[q]) = lo[q];
+      *reinterpret_cast<W*>(o) = lo[q];
     }
+    from += kRotBatch * from_step;
+    to += kRotBatch * to_step;
   }
 }
 
@@ -152,21 +153,26 @@ int rot_vector(const RotArgs& a, int n_parts, int esz, bool il) {
 }
 
 template <typename T, int V, bool IL>
-int rot_launch(RotArgs& a, cudaStream_t s) {
-  // Heads are spread over `lanes` threads of a slot: one thread walks over kRotHeads heads
-  // (their loads in flight at once) unless that would leave the SMs without threads.
-  const int64_t per_lane = a.tokens * a.slots;
-  int lanes = (a.heads + kRotHeads - 1) / kRotHeads;
-  if (per_lane * lanes < (int64_t)148 * 1024) lanes = a.heads;
-  a.lanes = lanes;
-  const int64_t blocks = (per_lane * lanes + kRotThreads - 1) / kRotThreads;
-  B3R_REQUIRE(blocks <= 0x7fffffff, "rotary: too many tokens for one call");
-  k_rotary<T, V, IL><<<(unsigned)blocks, kRotThreads, 0, s>>>(a);
+int rot_launch(RotArgs& a, int n_parts, int64_t tokens, cudaStream_t s) {
+  // A slot's heads are spread over threads of kRotHeads each, which share its cosines and sines
+  // through registers; where that leaves the SMs without threads, one head to a thread.
+  uint32_t most = 0;
+  for (int p = 0; p < n_parts; ++p) {
+    const int heads = a.part[p].heads;
+    int64_t lanes = (heads + kRotHeads - 1) / kRotHeads;
+    if (tokens * a.slots * lanes < (int64_t)148 * 1024) lanes = heads;
+    const int64_t n = tokens * a.slots * lanes;
+    B3R_REQUIRE(n <= 0x7fffff00, "rotary: too many tokens for one call");
+    a.lanes[p] = (int)lanes;
+    a.threads[p] = (uint32_t)n;
+    most = std::max(most, a.threads[p]);
+  }
+  k_rotary<T, V, IL><<<dim3((most + kRotThreads - 1) / kRotThreads, n_parts), kRotThreads, 0, s>>>(a);
   return check_launch("rotary");
 }
 
 template <typename T>
-int rot_run(RotArgs& a, int n_parts, bool il, bool copy_rest, cudaStream_t s) {
+int rot_run(RotArgs& a, int n_parts, int64_t tokens, bool il, bool copy_rest, cudaStream_t s) {
   const int rot = a.axes * 2 * a.half;
   int v = rot_vector(a, n_parts, sizeof(T), il);
   B3R_REQUIRE(!il || v >= 2, "rotary: interleaved pairs must be aligned to a pair (even strides and head size)");
@@ -174,12 +180,12 @@ int rot_run(RotArgs& a, int n_parts, bool il, bool copy_rest, cudaStream_t s) {
   a.slots = a.rot_slots + (copy_rest ? (a.D - rot) / v : 0);
   if (il) {
     if constexpr (sizeof(T) == 2)
-      if (v == 8) return rot_launch<T, 8, true>(a, s);
-    return v == 4 ? rot_launch<T, 4, true>(a, s) : rot_launch<T, 2, true>(a, s);
+      if (v == 8) return rot_launch<T, 8, true>(a, n_parts, tokens, s);
+    return v == 4 ? rot_launch<T, 4, true>(a, n_parts, tokens, s) : rot_launch<T, 2, true>(a, n_parts, tokens, s);
   }
   if constexpr (sizeof(T) == 2)
-    if (v == 8) return rot_launch<T, 8, false>(a, s);
-  return v == 4 ? rot_launch<T, 4, false>(a, s) : v == 2 ? rot_launch<T, 2, false>(a, s) : rot_launch<T, 1, false>(a, s);
+    if (v == 8) return rot_launch<T, 8, false>(a, n_parts, tokens, s);
+  return v == 4 ? rot_launch<T, 4, false>(a, n_parts, tokens, s) : v == 2 ? rot_launch<T, 2, false>(a, n_parts, tokens, s) : rot_launch<T, 1, false>(a, n_parts, tokens, s);
 }
 
 }  // namespace
@@ -193,25 +199,24 @@ extern "C" int b3r_rotary(const b3r_rotary_part* parts, int n_parts, int64_t B, 
   B3R_REQUIRE(parts && table, "rotary: NULL argument");
   B3R_REQUIRE(n_parts == 1 || n_parts == 2, "rotary: 1 or 2 parts, got %d", n_parts);
   B3R_REQUIRE(dtype == B3R_F32 || dtype == B3R_BF16 || dtype == B3R_F16, "rotary: dtype must be f32, bf16 or f16");
-  B3R_REQUIRE(B >= 0 && T >= 0 && D >= 2 && D <= 1024, "rotary: bad sizes (head size 2..1024)");
+  B3R_REQUIRE(B >= 0 && T >= 0 && T <= 0x7fffffff && D >= 2 && D <= 1024, "rotary: bad sizes (head size 2..1024)");
   B3R_REQUIRE(axes >= 1 && half >= 1 && (int64_t)axes * 2 * half <= D, "rotary: the rotated part exceeds the head");
   B3R_REQUIRE(n_pos >= 1, "rotary: empty table");
   B3R_REQUIRE(((uintptr_t)table & 7) == 0, "rotary: the table must be 8-byte aligned");
   RotArgs a{};
   bool in_place = true;
-  a.heads = 0;
+  int64_t heads = 0;
   for (int p = 0; p < n_parts; ++p) {
     B3R_REQUIRE(parts[p].heads >= 0 && (parts[p].heads == 0 || B * T == 0 || (parts[p].x && parts[p].out)),
                 "rotary: NULL tensor or negative head count");
     a.part[p] = parts[p];
-    a.heads += parts[p].heads;
+    heads += parts[p].heads;
     const bool same = parts[p].x == parts[p].out && parts[p].x_batch == parts[p].out_batch &&
                       parts[p].x_token == parts[p].out_token && parts[p].x_head == parts[p].out_head;
     in_place = in_place && same;
   }
-  if (B == 0 || T == 0 || a.heads == 0) return B3R_OK;
+  if (B == 0 || T == 0 || heads == 0) return B3R_OK;
   B3R_REQUIRE(positions, "rotary: NULL positions");
-  a.tokens = B * T;
   a.T = T;
   a.D = D;
   a.half = half;
@@ -225,7 +230,7 @@ extern "C" int b3r_rotary(const b3r_rotary_part* parts, int n_parts, int64_t B, 
   a.inverse = inverse;
   cudaStream_t s = as_stream(stream);
   // in place, the elements past the rotated part are where they belong already
-  if (dtype == B3R_F32) return rot_run<float>(a, n_parts, interleaved, !in_place, s);
-  if (dtype == B3R_BF16) return rot_run<__nv_bfloat16>(a, n_parts, interleaved, !in_place, s);
-  return rot_run<__half>(a, n_parts, interleaved, !in_place, s);
+  if (dtype == B3R_F32) return rot_run<float>(a, n_parts, B * T, interleaved, !in_place, s);
+  if (dtype == B3R_BF16) return rot_run<__nv_bfloat16>(a, n_parts, B * T, interleaved, !in_place, s);
+  return rot_run<__half>(a, n_parts, B * T, interleaved, !in_place, s);
 }

@@ -6,6 +6,8 @@
 // and a head size above 64 is two such blocks, 16 KB apart.
 #pragma once
 #include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cstdint>
 
 namespace b3r {
@@ -52,6 +54,12 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
       "l"(map), "r"(d0), "r"(row), "r"(head), "r"(batch), "r"(bar)
       : "memory");
+}
+// An untiled copy of `bytes` (a multiple of 16, both addresses 16-byte aligned).
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(bar)
+               : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
