@@ -6,6 +6,11 @@ There is no fallback: every op of this package raises if the library is missing.
 import ctypes as C
 import os
 
+try:                                   # the current stream's handle without building a Stream object
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    _raw_stream = None
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, 'libb3r.so')
 
@@ -180,3 +185,22 @@ def check(rc, what=''):
 
 def call(name, *args):
     return check(getattr(lib(), name)(*args), name)
+
+
+_fns = {}
+
+
+def call_on(index, name, *args):
+    """``call`` with the raw stream that is current on CUDA device `index` as its last argument,
+    on that device.  For calls of a few microseconds, where looking the function up and switching
+    to the device that is current already would cost as much as the launch."""
+    import torch
+    f = _fns.get(name)
+    if f is None:
+        f = _fns[name] = getattr(lib(), name)
+    if index == torch.cuda.current_device():
+        rc = f(*args, torch.cuda.current_stream(index).cuda_stream if _raw_stream is None else _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = f(*args, torch.cuda.current_stream(index).cuda_stream)
+    return rc if rc == B3R_OK else check(rc, name)

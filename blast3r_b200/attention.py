@@ -21,6 +21,8 @@ _status = {}    # device index -> int32 [1], raised by a kernel whose bounded wa
 def _status_of(dev):
     s = _status.get(dev.index)
     if s is None:
+        if torch.cuda.is_current_stream_capturing():
+            return None               # memory of a graph's pool would not outlive the graph
         s = _status[dev.index] = torch.zeros(1, dtype=torch.int32, device=dev)
     return s
 
@@ -36,35 +38,43 @@ def check_attention(device=None):
 
 
 def _tensor(t, packed):
-    return L.AttnTensor(t.data_ptr(), 0, t.stride(0), t.stride(1)) if packed else \
-        L.AttnTensor(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+    s = t.stride()
+    return (t.data_ptr(), 0, s[0], s[1]) if packed else (t.data_ptr(), s[0], s[1], s[2])
 
 
 def _lse_tensor(t, packed):
-    return L.AttnTensor(t.data_ptr(), 0, t.stride(1), t.stride(0)) if packed else \
-        L.AttnTensor(t.data_ptr(), t.stride(0), t.stride(2), t.stride(1))
+    s = t.stride()
+    return (t.data_ptr(), 0, s[1], s[0]) if packed else (t.data_ptr(), s[0], s[2], s[1])
 
 
 def _readable(t):
     """t itself where the kernels can read it: the head size contiguous, the other strides and the
     base multiples of 16 bytes; a copy otherwise."""
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and all(s % 8 == 0 for s, n in zip(t.stride()[:-1], t.shape) if n != 1) \
-            and all(s > 0 for s, n in zip(t.stride(), t.shape) if n != 1):
-        return t
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t
+        st = t.stride()
+        if st[-1] == 1:
+            for s, n in zip(st[:-1], t.shape):
+                if n != 1 and (s <= 0 or s % 8):
+                    break
+            else:
+                return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _index(t, name, n, dev):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != dev:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev:
         raise RuntimeError(f'attention: {name} is an int32 tensor of {n} elements on the tensors\' device')
     return t.contiguous()
 
 
 def _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k):
-    if not all(isinstance(t, torch.Tensor) and t.is_cuda for t in (q, k, v)):
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and
+            q.is_cuda and k.is_cuda and v.is_cuda):
         raise RuntimeError('attention runs on the GPU: pass CUDA tensors')
-    dev = q.device
-    if k.device != dev or v.device != dev:
+    dev = q.get_device()
+    if k.get_device() != dev or v.get_device() != dev:
         raise RuntimeError('attention: all tensors must be on one device')
     if q.dtype not in DTYPES or k.dtype != q.dtype or v.dtype != q.dtype:
         raise RuntimeError(f'attention takes bfloat16 or float16 tensors of one type, got {q.dtype}, {k.dtype}, {v.dtype}')
@@ -112,15 +122,16 @@ def _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k):
     return d, packed, keep
 
 
-def _launch(name, d, dev):
-    keep = _status_of(dev)
-    d.status = keep.data_ptr()
-    with torch.cuda.device(dev):
-        n = int(getattr(L.lib(), name + '_work_bytes')(C.byref(d)))
-        if n > 0:
-            work = torch.empty(n + 256, dtype=torch.uint8, device=dev)
-            d.work = work.data_ptr() + (-work.data_ptr()) % 256
-        L.call(name, C.byref(d), torch.cuda.current_stream(dev).cuda_stream)
+def _launch(name, d, dev, index):
+    status = _status_of(dev)
+    d.status = None if status is None else status.data_ptr()
+    ref = C.byref(d)
+    n = getattr(L.lib(), name + '_work_bytes')(ref)
+    if n > 0:
+        work = torch.empty(n + 256, dtype=torch.uint8, device=dev)
+        p = work.data_ptr()
+        d.work = p + (-p) % 256
+    L.call_on(index, name, ref)
 
 
 def attention_forward(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=None, cu_q=None, cu_k=None, max_q=None,
@@ -136,11 +147,11 @@ def attention_forward(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=
     the last key.  A query that sees no key has o = 0 and lse = -inf.  scale: D**-0.5."""
     d, packed, keep = _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k)
     q, k, v = _readable(q), _readable(k), _readable(v)
-    o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    o = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((d.Hq, d.Tq) if packed else (d.B, d.Hq, d.Lq), dtype=torch.float32, device=q.device)
     d.q, d.k, d.v, d.o, d.lse = _tensor(q, packed), _tensor(k, packed), _tensor(v, packed), _tensor(o, packed), \
         _lse_tensor(lse, packed)
-    _launch('b3r_attention_fwd', d, q.device)
+    _launch('b3r_attention_fwd', d, q.device, q.get_device())
     return o, lse
 
 
@@ -155,11 +166,11 @@ def attention_backward(do, q, k, v, o, lse, *, causal=False, scale=None, q_lens=
     if tuple(lse.shape) != want or lse.dtype != torch.float32 or lse.device != q.device:
         raise RuntimeError(f'attention backward: lse is the forward call\'s, float32 {want}')
     do, q, k, v, o = (_readable(t) for t in (do, q, k, v, o))
-    dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+    dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))
     for name, t in (('q', q), ('k', k), ('v', v), ('o', o), ('d_o', do), ('dq', dq), ('dk', dk), ('dv', dv)):
         setattr(d, name, _tensor(t, packed))
     d.lse = _lse_tensor(lse, packed)
-    _launch('b3r_attention_bwd', d, q.device)
+    _launch('b3r_attention_bwd', d, q.device, q.get_device())
     return dq, dk, dv
 
 

@@ -1,4 +1,5 @@
 // Part 5 of the C ABI, attention: what both passes check, and the tensor maps that they load by.
+#include <utility>
 #include "b3r_attn.cuh"
 
 namespace b3r {
@@ -38,7 +39,7 @@ int attn_check(const b3r_attention_desc* d, bool backward) {
   return B3R_OK;
 }
 
-int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype) {
+static int encode_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int G, int batch, int D, int dtype) {
   typedef CUresult (*encode_t)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -61,14 +62,28 @@ int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads
   }
   // the stride of a dimension of one is not used, but has to be a valid one
   const int64_t row = rows > 1 ? t.row : 128, head = heads > 1 ? t.head : 128, bat = batch > 1 ? t.batch : 128;
-  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
-  const cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)bat * 2};
-  const cuuint32_t box[4] = {64, 128, 1, 1}, step[4] = {1, 1, 1, 1};
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
+  cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)bat * 2};
+  cuuint32_t box[4] = {64, 128, 1, 1};
+  if (G > 0) {                         // heads before rows
+    std::swap(dims[1], dims[2]);
+    std::swap(strides[0], strides[1]);
+    box[1] = (cuuint32_t)G;
+    box[2] = (cuuint32_t)(128 / G);
+  }
+  const cuuint32_t step[4] = {1, 1, 1, 1};
   const CUresult rc = encode(map, dtype == B3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
                              const_cast<void*>(t.p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS) return fail(B3R_E_CUDA, "attention: cuTensorMapEncodeTiled failed (%d)", (int)rc);
   return B3R_OK;
+}
+
+int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype) {
+  return encode_map(map, t, rows, heads, 0, batch, D, dtype);
+}
+int attn_map_groups(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int G, int batch, int D, int dtype) {
+  return encode_map(map, t, rows, heads, G, batch, D, dtype);
 }
 
 }  // namespace b3r

@@ -68,13 +68,13 @@ __device__ __forceinline__ void init_shared(Shared& sh, int stages, int own) {
   }
   for (int i = 0; i < 2; ++i) {
     mbar_init(smem_u32(&sh.s_full[i]), 1);
-    mbar_init(smem_u32(&sh.st_full[i]), 32);
-    mbar_init(smem_u32(&sh.st_empty[i]), 256);
+    mbar_init(smem_u32(&sh.st_full[i]), 1);
+    mbar_init(smem_u32(&sh.st_empty[i]), 8);
   }
   mbar_init(smem_u32(&sh.dp_full), 1);
-  mbar_init(smem_u32(&sh.dp_read), 256);
-  mbar_init(smem_u32(&sh.p_full), 256);
-  mbar_init(smem_u32(&sh.ds_full), 256);
+  mbar_init(smem_u32(&sh.dp_read), 8);
+  mbar_init(smem_u32(&sh.p_full), 8);
+  mbar_init(smem_u32(&sh.ds_full), 8);
   mbar_init(smem_u32(&sh.done), 1);
   sh.dead = 0;
   fence_async();
@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
   const uint32_t sq = smem_u32(base), sgo = sq + kTile;
   Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.stages) * kTile);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
   const b3r_attention_desc& d = a.d;
   const int G = d.Hq / d.Hkv, split = blockIdx.x % a.q_splits;
   int head, tile;
@@ -150,12 +150,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     first = split * per;
     n = min(max(all - first, 0), per);
   }
-  if (threadIdx.x == 0) init_shared(sh, a.stages, 256);
+  if (threadIdx.x == 0) init_shared(sh, a.stages, 8);
   if (warp == 9 && n > 0) tc_alloc(smem_u32(&sh.tmem), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   volatile int* dead = &sh.dead;
   const int steps = (d.D + 15) / 16;
   Ring ring{sq + 2 * kTile, base + 2 * kTile, sh.full, sh.empty, a.stages};
@@ -170,28 +170,26 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       ring_load<kBlocks>(ring, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
     }
   } else if (warp == 9 && n > 0) {
-    if (lane == 0) {
+    {
+      const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
       auto product = [&](uint32_t acc, uint32_t left, int stage) {   // acc = left K^T or V^T
-        for (int t = 0; t < steps; ++t) {
-          const uint32_t off = (t >> 2) * kBlockBytes + (t & 3) * 32;
-          tc_mma(acc, desc_k(left + off), desc_k(ring.data + stage * kTile + off), id_s, t > 0);
-        }
+        tile_product<kBlocks>(acc, left, ring.data + stage * kTile, id_s, steps, on);
       };
       int sk[2], sv = 0, last_round = 0;
       auto scores = [&](int it) {
         sk[it & 1] = ring.next(dead);
         tc_fence_after();
         product(tmem + (it & 1) * 128, sq, sk[it & 1]);
-        tc_commit(smem_u32(&sh.s_full[it & 1]));
+        tc_commit(smem_u32(&sh.s_full[it & 1]), on);
       };
       auto grads = [&]() {
         last_round = ring.round;
         sv = ring.next(dead);
         tc_fence_after();
         product(tmem + 256, sgo, sv);
-        tc_commit(smem_u32(&sh.dp_full));
-        tc_commit(smem_u32(&sh.empty[sv]));
+        tc_commit(smem_u32(&sh.dp_full), on);
+        tc_commit(smem_u32(&sh.empty[sv]), on);
       };
       mbar_wait(smem_u32(&sh.own_full), 0, dead);
       tc_fence_after();
@@ -207,12 +205,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
         tc_fence_after();
         const uint32_t ds = tmem + (it & 1) * 128, k = ring.data + sk[it & 1] * kTile;
-        for (int t = 0; t < 8; ++t)
-          tc_mma_ts(tmem + 384, ds + (t >> 2) * 64 + (t & 3) * 8, desc_mn(k + t * 2048), id_o, it > 0 || t > 0);
-        tc_commit(smem_u32(&sh.empty[sk[it & 1]]));
+        tile_gather(tmem + 384, ds, 64, k, id_o, it > 0, on);
+        tc_commit(smem_u32(&sh.empty[sk[it & 1]]), on);
         if (it + 2 < n) scores(it + 2);
       }
-      tc_commit(smem_u32(&sh.done));
+      tc_commit(smem_u32(&sh.done), on);
       mbar_wait(smem_u32(&sh.empty[sv]), last_round & 1, dead);      // no arrival is left behind
       mbar_wait(smem_u32(&sh.done), 0, dead);
     }
@@ -248,7 +245,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         sh.delta[r] = dot;
         if (live && split == 0) a.delta[((int64_t)b * d.Hq + h) * d.Lq + i] = dot;
       }
-      if (n > 0) mbar_arrive(smem_u32(&sh.own_full));
+      __syncwarp();
+      if (n > 0 && lane == 0) mbar_arrive(smem_u32(&sh.own_full));
       bar_sync(1, 256);
     }
     const float delta = sh.delta[r], c = d.scale * kLog2e;
@@ -276,7 +274,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       tc_ld32(quarter + 256 + w * 64 + 32, g + 32);
       tc_wait_ld(g);
       tc_fence_before();
-      mbar_arrive(smem_u32(&sh.dp_read));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.dp_read));
       const bool whole = __all_sync(0xffffffffu, lim >= 64);
       uint32_t ds[32];
 #pragma unroll
@@ -292,7 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       tc_st32(at, ds);
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&sh.ds_full));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.ds_full));
     }
     if (n > 0) {
       mbar_wait(smem_u32(&sh.done), 0, dead);
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
   const uint32_t sk = smem_u32(base), sv = sk + kTile;
   Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.stages) * kTile);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
   const b3r_attention_desc& d = a.d;
   const int G = d.Hq / d.Hkv, split = blockIdx.x % a.k_splits;
   int head, tile;
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   volatile int* dead = &sh.dead;
   const int steps = (d.D + 15) / 16;
   Ring ring{sk + 2 * kTile, base + 2 * kTile, sh.full, sh.empty, a.stages};
@@ -372,29 +372,25 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     }
     if (*dead && lane == 0) mbar_wait(smem_u32(&sh.own_full), 0, dead);
   } else if (warp == 9 && n > 0) {
-    if (lane == 0) {
+    {
+      const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
       auto product = [&](uint32_t acc, uint32_t left, int stage) {   // acc = K Q^T or V dO^T
-        for (int t = 0; t < steps; ++t) {
-          const uint32_t off = (t >> 2) * kBlockBytes + (t & 3) * 32;
-          tc_mma(acc, desc_k(left + off), desc_k(ring.data + stage * kTile + off), id_s, t > 0);
-        }
+        tile_product<kBlocks>(acc, left, ring.data + stage * kTile, id_s, steps, on);
       };
       auto gather = [&](uint32_t acc, uint32_t left, int stage, bool add) {   // acc += P^T dO or dS^T Q
-        const uint32_t x = ring.data + stage * kTile;
-        for (int t = 0; t < 8; ++t)
-          tc_mma_ts(acc, left + (t >> 2) * 64 + (t & 3) * 8, desc_mn(x + t * 2048), id_o, add || t > 0);
-        tc_commit(smem_u32(&sh.empty[stage]));
+        tile_gather(acc, left, 64, ring.data + stage * kTile, id_o, add, on);
+        tc_commit(smem_u32(&sh.empty[stage]), on);
       };
       mbar_wait(smem_u32(&sh.own_full), 0, dead);
       int xq = ring.next(dead), xg, last_round = 0;
       tc_fence_after();
       product(tmem, sk, xq);
-      tc_commit(smem_u32(&sh.s_full[0]));
+      tc_commit(smem_u32(&sh.s_full[0]), on);
       last_round = ring.round;
       xg = ring.next(dead);
       product(tmem + 128, sv, xg);
-      tc_commit(smem_u32(&sh.dp_full));
+      tc_commit(smem_u32(&sh.dp_full), on);
       for (int it = 0; it < n; ++it) {
         const int cq = xq, cg = xg, round_g = last_round;
         mbar_wait(smem_u32(&sh.p_full), it & 1, dead);
@@ -403,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         if (it + 1 < n) {
           xq = ring.next(dead);
           product(tmem, sk, xq);
-          tc_commit(smem_u32(&sh.s_full[0]));
+          tc_commit(smem_u32(&sh.s_full[0]), on);
         }
         mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
         tc_fence_after();
@@ -412,9 +408,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
           last_round = ring.round;
           xg = ring.next(dead);
           product(tmem + 128, sv, xg);
-          tc_commit(smem_u32(&sh.dp_full));
+          tc_commit(smem_u32(&sh.dp_full), on);
         } else {
-          tc_commit(smem_u32(&sh.done));
+          tc_commit(smem_u32(&sh.done), on);
           mbar_wait(smem_u32(&sh.empty[cg]), round_g & 1, dead);     // no arrival is left behind
           mbar_wait(smem_u32(&sh.done), 0, dead);
         }
@@ -436,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         sh.stat[st][0][x] = l == -INFINITY ? -INFINITY : kLogScaleP<T> - l * kLog2e;   // nothing seen: P = 2^-inf
         sh.stat[st][1][x] = l == -INFINITY ? 0.f : -dl * (1.f / kScaleP<T>);
       }
-      mbar_arrive(smem_u32(&sh.st_full[st]));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.st_full[st]));
     }
   } else if (warp < 8) {
     const int w = warp >> 2, r = threadIdx.x & 127, j = j0 + r;
@@ -474,7 +471,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       tc_st32(quarter + w * 64, h);
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&sh.p_full));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
       mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
       tc_fence_after();
       tc_ld32(quarter + 128 + w * 64, g);
@@ -493,8 +491,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       tc_st32(quarter + 128 + w * 64, h);
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&sh.ds_full));
-      mbar_arrive(smem_u32(&sh.st_empty[st]));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.ds_full));
+      if (lane == 0) mbar_arrive(smem_u32(&sh.st_empty[st]));
     }
     if (n > 0) {
       mbar_wait(smem_u32(&sh.done), 0, dead);

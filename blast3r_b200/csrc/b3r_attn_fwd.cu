@@ -28,12 +28,13 @@ constexpr int kMaxStages = 8;
 constexpr float kGrow = 8.f;   // log2 of how far the maximum may grow before O is rescaled
 
 struct alignas(64) FwdArgs {
-  CUtensorMap k, v;
+  CUtensorMap q, k, v;
   b3r_attention_desc d;
   int tiles;        // pairs of row tiles (single ones when `one`) of the longest sequence
   int one;          // one tile of rows: the groups share it and split the keys
   int splits;       // blocks along the keys
   int stages, group;
+  int q_tma;        // the heads of a group divide 128: Q comes by TMA, a box of whole groups
   float* part_o;    // [splits][B Hkv][rows][D]
   float* part_l;    // [splits][B Hkv][rows]: log2 of the sum, -inf where a part sees nothing
 };
@@ -96,14 +97,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
   const int q_tiles = a.one ? 1 : 2;
   const uint32_t sq = smem_u32(base), skv = sq + q_tiles * kTile;
   Shared& sh = *reinterpret_cast<Shared*>(base + (q_tiles + a.stages) * kTile);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
+  if (warp == 9) tc_alloc(smem_u32(&sh.tmem), 512);   // first: it takes longer than the rest of the set-up
   const Job j = job_of(a);
   const b3r_attention_desc& d = a.d;
-  if (j.m0[0] >= j.rows) return;       // uniform: no rows of this sequence here
-  const bool none = j.n[0] + j.n[1] == 0;
+  const bool idle = j.m0[0] >= j.rows;                // no rows of this sequence here
+  const bool none = idle || j.n[0] + j.n[1] == 0;
   const uint32_t bar_q = smem_u32(&sh.q_full);
   if (threadIdx.x == 0) {
-    mbar_init(bar_q, 256);
+    mbar_init(bar_q, a.q_tma ? 1 : 8);
     mbar_init(smem_u32(&sh.fix), 1);
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(smem_u32(&sh.kv_full[i]), 1);
@@ -111,17 +113,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(smem_u32(&sh.s_full[w]), 1);
-      mbar_init(smem_u32(&sh.p_full[w]), 128);
+      mbar_init(smem_u32(&sh.p_full[w]), 4);
       mbar_init(smem_u32(&sh.o_done[w]), 1);
     }
     sh.dead = 0;
     fence_async();
   }
-  if (warp == 9 && !none) tc_alloc(smem_u32(&sh.tmem), 512);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = sh.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   volatile int* dead = &sh.dead;
   // a softmax thread holds a row of 128 scores: registers move over from the third warpgroup
   // (256 x 208 + 128 x 88 = 384 x 168, what the block was launched with)
@@ -131,6 +132,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     // ------------------------------------------------ loads
     Ring ring{skv, base + q_tiles * kTile, sh.kv_full, sh.kv_empty, a.stages};
     int fixes = 0;
+    if (a.q_tma && lane == 0) {        // whole groups of heads fill a tile: rows past the end only reach their own scores
+      mbar_expect(bar_q, q_tiles * kTile);
+      for (int w = 0; w < q_tiles; ++w)
+#pragma unroll
+        for (int c = 0; c < kBlocks; ++c)
+          tma_box(sq + w * kTile + c * kBlockBytes, &a.q, c * 64, j.kv * j.G, (int)j.s.q0 + j.m0[w] / j.G, d.cu_q ? 0 : j.b, bar_q);
+    }
     const int row0 = (int)j.s.k0, batch = d.cu_k ? 0 : j.b;
     auto load = [&](const CUtensorMap* map, int tile, bool values) {   // P is zero past the last key, so V is cleared there
       ring_load<kBlocks>(ring, map, row0 + tile * kTileRows, j.kv, batch, j.s.kl - tile * kTileRows, values, &sh.fix, fixes, lane,
@@ -154,7 +162,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     }
     } else if (warp == 9 && !none) {
     // ------------------------------------------------ matrix products
-    if (lane == 0) {
+    {
+      const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
       const int steps = (d.D + 15) / 16;
       Ring ring{skv, base + q_tiles * kTile, sh.kv_full, sh.kv_empty, a.stages};
@@ -165,20 +174,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       };
       auto scores = [&](int w, int s) {                // S_w = Q_w K^T
         const uint32_t q = sq + (a.one ? 0 : w) * kTile, k = skv + s * kTile;
-        for (int t = 0; t < steps; ++t) {
-          const uint32_t off = (t >> 2) * kBlockBytes + (t & 3) * 32;
-          tc_mma(tmem + w * 128, desc_k(q + off), desc_k(k + off), id_s, t > 0);
-        }
-        tc_commit(smem_u32(&sh.s_full[w]));
+        tile_product<kBlocks>(tmem + w * 128, q, k, id_s, steps, on);
+        tc_commit(smem_u32(&sh.s_full[w]), on);
       };
       auto output = [&](int w, int s, int i) {         // O_w += P_w V
         mbar_wait(smem_u32(&sh.p_full[w]), i & 1, dead);
         tc_fence_after();
-        for (int t = 0; t < 8; ++t)
-          tc_mma_ts(tmem + 256 + w * DP, tmem + w * 128 + t * 8, desc_mn(skv + s * kTile + t * 2048), id_o, i > 0 || t > 0);
-        tc_commit(smem_u32(&sh.o_done[w]));
+        tile_gather(tmem + 256 + w * DP, tmem + w * 128, 32, skv + s * kTile, id_o, i > 0, on);
+        tc_commit(smem_u32(&sh.o_done[w]), on);
       };
-      auto release = [&](int s) { tc_commit(smem_u32(&sh.kv_empty[s])); };
+      auto release = [&](int s) { tc_commit(smem_u32(&sh.kv_empty[s]), on); };
       mbar_wait(bar_q, 0, dead);
       tc_fence_after();
       if (a.one) {
@@ -231,18 +236,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     const int bound = row && i < j.s.ql ? attn_bound(j.s, i, d.causal) : 0;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);   // this warp's 32 lanes
     const float c = d.scale * kLog2e;
-    if (!none && (w == 0 || !a.one)) {
-      // the row of Q into the swizzled tile; zeros past D and past the rows
-      const uint4* q = reinterpret_cast<const uint4*>(attn_row<const T>(d.q, j.b, j.s.q0 + (row ? i : 0), row ? h : 0));
-      uint8_t* dst = base + w * kTile + r * 128;
+    if (!none && !a.q_tma) {
+      if (w == 0 || !a.one) {
+        // the row of Q into the swizzled tile; zeros past D and past the rows
+        const uint4* q = reinterpret_cast<const uint4*>(attn_row<const T>(d.q, j.b, j.s.q0 + (row ? i : 0), row ? h : 0));
+        uint8_t* dst = base + w * kTile + r * 128;
 #pragma unroll
-      for (int cb = 0; cb < DP / 8; ++cb) {
-        const uint4 x = (row && cb * 8 < d.D) ? q[cb] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4)) = x;
+        for (int cb = 0; cb < DP / 8; ++cb) {
+          const uint4 x = (row && cb * 8 < d.D) ? q[cb] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4)) = x;
+        }
+        fence_async();
       }
-      fence_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar_q);
     }
-    if (!none) mbar_arrive(bar_q);
     float mx = -INFINITY, l = 0.f;       // what the exponentials are taken against (log2), and their sum
     const int n = j.n[w];
     for (int it = 0; it < n; ++it) {
@@ -297,7 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       l += sum.x + sum.y;
       tc_wait_st();
       tc_fence_before();
-      mbar_arrive(smem_u32(&sh.p_full[w]));
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[w]));
     }
     if (n > 0) {
       mbar_wait(smem_u32(&sh.o_done[w]), (n - 1) & 1, dead);
@@ -326,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       f0 = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;     // NaN stays NaN
       lg = l == 0.f ? -INFINITY : mx + __log2f(l);
     }
-    if (w == 0 || !a.one) {
+    if (!idle && (w == 0 || !a.one)) {
       const bool has0 = n > 0, has1 = a.one && j.n[1] > 0;
       const int64_t at = ((int64_t)j.split * d.B * d.Hkv + (int64_t)j.b * d.Hkv + j.kv) * ((int64_t)d.Lq * j.G) + m;
       if (*dead) f0 = f1 = lg = __int_as_float(0x7fffffff);
@@ -380,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     if (threadIdx.x == 0 && d.status) *d.status = 1;
     __syncthreads();
   }
-  if (warp == 9 && !none) {
+  if (warp == 9) {
     tc_fence_after();
     tc_free(tmem, 512);
   }
@@ -494,6 +503,10 @@ extern "C" int b3r_attention_fwd(const b3r_attention_desc* d, void* stream) {
   }
   B3R_TRY(attn_map(&a.k, d->k, d->cu_q ? d->Tk : d->Lk, d->Hkv, d->cu_q ? 1 : d->B, d->D, d->dtype));
   B3R_TRY(attn_map(&a.v, d->v, d->cu_q ? d->Tk : d->Lk, d->Hkv, d->cu_q ? 1 : d->B, d->D, d->dtype));
+  const int G = d->Hq / d->Hkv;
+  a.q_tma = kTileRows % G == 0;
+  if (a.q_tma)
+    B3R_TRY(attn_map_groups(&a.q, d->q, d->cu_q ? d->Tq : d->Lq, d->Hq, G, d->cu_q ? 1 : d->B, d->D, d->dtype));
   cudaStream_t s = as_stream(stream);
   if (d->dtype == B3R_BF16) return d->D <= 64 ? launch<64, __nv_bfloat16>(a, s) : launch<128, __nv_bfloat16>(a, s);
   return d->D <= 64 ? launch<64, __half>(a, s) : launch<128, __half>(a, s);

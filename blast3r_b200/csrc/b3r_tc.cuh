@@ -73,21 +73,33 @@ __device__ __forceinline__ void tc_free(uint32_t tmem, int cols) {
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+// One lane of a converged warp.  The issuing warp stays converged, with uniform operands, and
+// this lane's predicate on the instructions themselves: issued from within a branch of one lane each
+// product took 75 to 140 cycles to issue, more than the tensor cores need for it.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(on));
+  return on;
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar, uint32_t on) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+      "r"(on)
+      : "memory");
 }
 // D[tmem] (+)= A[smem] B[smem]
-__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc, uint32_t on) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a),
-      "l"(b), "r"(idesc), "r"((int)acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((int)acc), "r"(on)
       : "memory");
 }
 // D[tmem] (+)= A[tmem] B[smem]: row i of A in lane i, two elements to a column
-__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void tc_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc, uint32_t on) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a),
-      "l"(b), "r"(idesc), "r"((int)acc)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((int)acc), "r"(on)
       : "memory");
 }
 
@@ -106,6 +118,24 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
 __host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int M, int N, bool b_mn) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
          ((uint32_t)(M >> 4) << 24);
+}
+
+// tile_product: acc = A B^T over the head size, both k-major tiles, in `steps` steps of 16.
+// tile_gather: acc (+)= A B over the 128 rows of tile b; A in tensor memory, steps 0-3 from `a`, 4-7
+// from `a + half`.  Offsets within a tile only change the descriptors' address field (units of 16 bytes).
+template <int BLOCKS>
+__device__ __forceinline__ void tile_product(uint32_t acc, uint32_t a, uint32_t b, uint32_t idesc, int steps, uint32_t on) {
+  const uint64_t da = desc_k(a), db = desc_k(b);
+#pragma unroll
+  for (int t = 0; t < BLOCKS * 4; ++t) {
+    const uint32_t off = ((t >> 2) * kBlockBytes + (t & 3) * 32) >> 4;
+    if (t < steps) tc_mma(acc, da + off, db + off, idesc, t > 0, on);
+  }
+}
+__device__ __forceinline__ void tile_gather(uint32_t acc, uint32_t a, int half, uint32_t b, uint32_t idesc, bool add, uint32_t on) {
+  const uint64_t db = desc_mn(b);
+#pragma unroll
+  for (int t = 0; t < 8; ++t) tc_mma_ts(acc, a + (t >> 2) * half + (t & 3) * 8, db + (t * 2048 >> 4), idesc, add || t > 0, on);
 }
 
 #define B3R_R4(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3])

@@ -36,7 +36,7 @@ def _rows(t):
     return t.contiguous(), t.shape[-1]
 
 
-def _pair(p, name, on):
+def _pair(p, name):
     if p is None:
         return False, None, None
     if p is True:
@@ -48,46 +48,67 @@ def _pair(p, name, on):
     return True, p[0], p[1]
 
 
+def _gate_rows(gate, shape):
+    """Rows of y, of `shape`, to a row of the gate; None where the two do not fit."""
+    if gate.shape[-1:] != shape[-1:]:
+        return None
+    g, lead = gate.shape[:-1], shape[:-1]
+    rows = 1
+    for n in lead:
+        rows *= n
+    k = len(g)
+    while k > 0 and g[k - 1] == 1 and (len(g) == len(lead) or k <= len(lead)) and lead[k - 1] != 1:
+        k -= 1                                       # (B, 1, C): one row for each of the first dimensions
+    if k > len(lead) or tuple(g[:k]) != tuple(lead[:k]):
+        return None
+    groups = 1
+    for n in g[:k]:
+        groups *= n
+    return max(rows // groups, 1) if groups else 1
+
+
 def _describe(y, x, kind, eps, post, gate, residual_scale, pre):
-    """(descriptor, its tensors, gate's tensor) after the checks of every argument."""
+    """(descriptor, its tensors in order: w_post, b_post, gate, w_pre, b_pre) after the checks of every argument."""
     if not (isinstance(y, torch.Tensor) and isinstance(x, torch.Tensor) and y.is_cuda and x.is_cuda):
         raise RuntimeError('residual_norm runs on the GPU: pass CUDA tensors')
-    if y.dim() < 1 or y.shape != x.shape:
-        raise RuntimeError(f'residual_norm: the block output {tuple(y.shape)} and the stream {tuple(x.shape)} differ in shape')
-    if y.dtype not in DTYPES or x.dtype not in (y.dtype, torch.float32):
+    shape, dt, sd, dev = y.shape, y.dtype, x.dtype, y.get_device()
+    if y.dim() < 1 or shape != x.shape:
+        raise RuntimeError(f'residual_norm: the block output {tuple(shape)} and the stream {tuple(x.shape)} differ in shape')
+    if dt not in DTYPES or (sd != dt and sd != torch.float32):
         raise RuntimeError(f'residual_norm: float32, bfloat16 or float16 block outputs and a stream of that type or '
-                           f'float32, got {y.dtype} and {x.dtype}')
+                           f'float32, got {dt} and {sd}')
     if kind not in KINDS:
         raise RuntimeError(f"residual_norm: kind is 'layer' or 'rms', got {kind!r}")
-    Cn = y.shape[-1]
-    has_post, w_post, b_post = _pair(post, 'post', y)
-    has_pre, w_pre, b_pre = _pair(pre, 'pre', y)
-    ws = [t for t in (w_post, b_post, w_pre, b_pre) if t is not None]
-    rows = y.numel() // Cn if Cn else 0
-    per = 1
+    Cn = shape[-1]
+    has_post, w_post, b_post = _pair(post, 'post')
+    has_pre, w_pre, b_pre = _pair(pre, 'pre')
+    rows, per = (y.numel() // Cn if Cn else 0), 1
     if gate is not None:
-        lead = y.shape[:-1]
-        if gate.shape[-1:] != y.shape[-1:]:
-            raise RuntimeError(f'residual_norm: a gate of shape {tuple(gate.shape)} for {Cn} channels')
-        g = gate.shape[:-1]
-        while g and g[-1] == 1 and len(g) > 0 and len(g) == len(lead) and lead[-1] != 1:
-            g, lead = g[:-1], lead[:-1]       # (B, 1, C): one row for each of the first dimensions
-        if g != lead[:len(g)] and any(n != 1 for n in g):
+        per = _gate_rows(gate, shape)
+        if per is None:
             raise RuntimeError(f'residual_norm: the gate {tuple(gate.shape)} is (C,), (B, C), (B, 1, C) or the shape of '
-                               f'the block output {tuple(y.shape)}')
-        groups = gate.numel() // Cn if Cn else 1
-        per = max(rows // groups, 1) if groups else 1
-    if any(t.dim() != 1 or t.shape[0] != Cn for t in ws):
-        raise RuntimeError(f'residual_norm: weights and biases have {Cn} elements')
-    params = ws + ([gate] if gate is not None else [])
-    if any(not t.is_cuda or t.device != y.device for t in params + [x]):
+                               f'the block output {tuple(shape)}')
+    wt, keep, ptrs = None, [], []
+    for t in (w_post, b_post, gate, w_pre, b_pre):
+        if t is not None:
+            if t is not gate and (t.dim() != 1 or t.shape[0] != Cn):
+                raise RuntimeError(f'residual_norm: weights and biases have {Cn} elements')
+            if t.get_device() != dev:
+                raise RuntimeError('residual_norm: all tensors must be on one CUDA device')
+            if wt is None:
+                wt = t.dtype
+            if t.dtype != wt or (wt != dt and wt != torch.float32):
+                raise RuntimeError(f'residual_norm: weights, biases and gate share one type, {dt} or float32')
+            if not t.is_contiguous():
+                t = t.contiguous()
+            ptrs.append(t.data_ptr())
+        else:
+            ptrs.append(None)
+        keep.append(t)
+    if x.get_device() != dev:
         raise RuntimeError('residual_norm: all tensors must be on one CUDA device')
-    wt = params[0].dtype if params else y.dtype
-    if any(t.dtype != wt for t in params) or wt not in (y.dtype, torch.float32):
-        raise RuntimeError(f'residual_norm: weights, biases and gate share one type, {y.dtype} or float32')
-    keep = [None if t is None else t.detach().contiguous() for t in (w_post, b_post, gate, w_pre, b_pre)]
-    d = L.ResidualNorm(rows, per, Cn, KINDS[kind], DTYPES[y.dtype], DTYPES[x.dtype], DTYPES[wt], int(has_post),
-                       int(has_pre), float(eps), float(residual_scale), *[None if t is None else t.data_ptr() for t in keep])
+    d = L.ResidualNorm(rows, per, Cn, KINDS[kind], DTYPES[dt], DTYPES[sd], DTYPES[wt or dt], has_post, has_pre, eps,
+                       residual_scale, *ptrs)
     return d, keep
 
 
@@ -99,11 +120,10 @@ def residual_norm_forward(y, x, *, kind='layer', eps=1e-6, post=None, gate=None,
     bfloat16 or float16 blocks; r has x's type, h has y's.  1 to 8192 channels."""
     d, keep = _describe(y, x, kind, eps, post, gate, residual_scale, pre)
     (yt, ys), (xt, xs) = _rows(y), _rows(x)
-    r = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(y.shape, dtype=y.dtype, device=y.device) if d.pre else None
-    with torch.cuda.device(y.device):
-        L.call('b3r_residual_norm_fwd', C.byref(d), yt.data_ptr(), ys, xt.data_ptr(), xs, r.data_ptr(),
-               None if h is None else h.data_ptr(), torch.cuda.current_stream(y.device).cuda_stream)
+    r = torch.empty_like(x, memory_format=torch.contiguous_format)
+    h = torch.empty_like(y, memory_format=torch.contiguous_format) if d.pre else None
+    L.call_on(y.get_device(), 'b3r_residual_norm_fwd', C.byref(d), yt.data_ptr(), ys, xt.data_ptr(), xs, r.data_ptr(),
+              None if h is None else h.data_ptr())
     return r, h
 
 
@@ -117,9 +137,9 @@ def residual_norm_backward(dr, dh, y, r, *, kind='layer', eps=1e-6, post=None, g
     if d.pre and (not isinstance(dh, torch.Tensor) or not dh.is_cuda or dh.shape != y.shape or dh.dtype != y.dtype):
         raise RuntimeError('residual_norm backward: dh has the shape and type of y')
     ts = [_rows(t) if t is not None else (None, 0) for t in (dr, dh if d.pre else None, y, r)]
-    new = lambda t: None if t is None else torch.empty(t.shape, dtype=t.dtype, device=y.device)   # noqa: E731
+    new = lambda t: None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)   # noqa: E731
     w_post, b_post, g, w_pre, b_pre = keep
-    dx, dy = torch.empty(r.shape, dtype=r.dtype, device=r.device), torch.empty(y.shape, dtype=y.dtype, device=y.device)
+    dx, dy = new(r), new(y)
     out = NormGrads(dx, dy, new(g), new(w_post), new(b_post), new(w_pre), new(b_pre))
     work = torch.empty(max(int(L.lib().b3r_residual_norm_work_bytes(C.byref(d))), 0) + 256, dtype=torch.uint8, device=y.device)
     wp = work.data_ptr()
@@ -128,9 +148,7 @@ def residual_norm_backward(dr, dh, y, r, *, kind='layer', eps=1e-6, post=None, g
         out.dgate.zero_()                # the library sees no rows and does not know the gate's
     ptr = lambda t: None if t is None else t.data_ptr()                                           # noqa: E731
     args = [a for t, s in ts for a in (ptr(t), s)]
-    with torch.cuda.device(y.device):
-        L.call('b3r_residual_norm_bwd', C.byref(d), *args, *[ptr(t) for t in out], wp,
-               torch.cuda.current_stream(y.device).cuda_stream)
+    L.call_on(y.get_device(), 'b3r_residual_norm_bwd', C.byref(d), *args, *[ptr(t) for t in out], wp)
     return out
 
 
@@ -157,8 +175,8 @@ class _ResidualNorm(torch.autograd.Function):
 
 def residual_norm(y, x, *, kind='layer', eps=1e-6, post=None, gate=None, residual_scale=1.0, pre=None):
     """``residual_norm_forward``, differentiable in y, x, the gate, the weights and the biases."""
-    has_post, w_post, b_post = _pair(post, 'post', y)
-    has_pre, w_pre, b_pre = _pair(pre, 'pre', y)
+    has_post, w_post, b_post = _pair(post, 'post')
+    has_pre, w_pre, b_pre = _pair(pre, 'pre')
     ts = (y, x, w_post, b_post, gate, w_pre, b_pre)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts):
         return _ResidualNorm.apply(*ts, has_post, has_pre, kind, eps, residual_scale)

@@ -13,6 +13,7 @@ import torch
 
 from . import _lib as L
 
+_PARTS = {n: L.RotaryPart * n for n in (1, 2)}
 DTYPES = {torch.float32: L.B3R_F32, torch.bfloat16: L.B3R_BF16, torch.float16: L.B3R_F16}
 
 
@@ -52,53 +53,72 @@ def rotary_table(n_positions, dim, device='cuda', **kw):
     return (torch.stack([ang.cos(), ang.sin()], dim=-1) * amp).float().to(device).contiguous()
 
 
-def _strides(t):
-    """Strides of a (B, T, heads, D) tensor whose D is contiguous."""
-    return t.stride(0), t.stride(1), t.stride(2)
+def _bad(xs, table, positions):
+    """Why the arguments cannot be used."""
+    if not all(isinstance(x, torch.Tensor) and x.is_cuda for x in (*xs, table, positions)):
+        return 'rotary runs on the GPU: pass CUDA tensors'
+    if any(t.device != xs[0].device for t in (*xs, table, positions)):
+        return 'rotary: all tensors must be on one device'
+    if xs[0].dtype not in DTYPES or any(x.dtype != xs[0].dtype for x in xs):
+        return f'rotary takes float32, bfloat16 or float16 tensors of one type, got {[x.dtype for x in xs]}'
+    if any(x.dim() != 4 for x in xs) or any(x.shape[:2] != xs[0].shape[:2] or x.shape[3] != xs[0].shape[3] for x in xs):
+        return f'rotary takes (B, T, heads, D) tensors of one B, T and D, got {[tuple(x.shape) for x in xs]}'
+    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or not table.is_contiguous():
+        return 'rotary: the table is a contiguous float32 (positions, pairs, 2) tensor (rotary_table)'
+    return f'rotary: positions are int32 or int64, got {positions.dtype}'
 
 
 def _rotate(xs, table, positions, interleaved, inverse, inplace):
-    if not 1 <= len(xs) <= 2:
-        raise ValueError(f'one tensor or two (queries and keys), got {len(xs)}')
+    n = len(xs)
+    if not 1 <= n <= 2:
+        raise ValueError(f'one tensor or two (queries and keys), got {n}')
     x0 = xs[0]
-    if not all(isinstance(x, torch.Tensor) and x.is_cuda for x in (*xs, table, positions)):
-        raise RuntimeError('rotary runs on the GPU: pass CUDA tensors')
-    dev = x0.device
-    if any(t.device != dev for t in (*xs, table, positions)):
-        raise RuntimeError('rotary: all tensors must be on one device')
-    if x0.dtype not in DTYPES or any(x.dtype != x0.dtype for x in xs):
-        raise RuntimeError(f'rotary takes float32, bfloat16 or float16 tensors of one type, got {[x.dtype for x in xs]}')
-    if any(x.dim() != 4 or x.shape[:2] != x0.shape[:2] or x.shape[3] != x0.shape[3] for x in xs):
-        raise RuntimeError(f'rotary takes (B, T, heads, D) tensors of one B, T and D, got {[tuple(x.shape) for x in xs]}')
-    B, T, _, D = x0.shape
-    if table.dtype != torch.float32 or table.dim() != 3 or table.shape[2] != 2 or not table.is_contiguous():
-        raise RuntimeError('rotary: the table is a contiguous float32 (positions, pairs, 2) tensor (rotary_table)')
-    if positions.dtype not in (torch.int32, torch.int64):
-        raise RuntimeError(f'rotary: positions are int32 or int64, got {positions.dtype}')
+    ok = isinstance(x0, torch.Tensor) and isinstance(table, torch.Tensor) and isinstance(positions, torch.Tensor) and x0.is_cuda
+    if ok:
+        dev, dt, shape0, tshape, pt = x0.get_device(), x0.dtype, x0.shape, table.shape, positions.dtype
+        code, wide = DTYPES.get(dt), pt == torch.int64
+        ok = (code is not None and len(shape0) == 4 and table.dtype == torch.float32 and len(tshape) == 3 and
+              tshape[2] == 2 and table.is_contiguous() and table.get_device() == dev and positions.get_device() == dev and
+              (wide or pt == torch.int32))
+    if ok and n == 2:
+        x1 = xs[1]
+        ok = isinstance(x1, torch.Tensor) and x1.dtype == dt and x1.get_device() == dev
+        if ok:
+            s1 = x1.shape
+            ok = len(s1) == 4 and s1[0] == shape0[0] and s1[1] == shape0[1] and s1[3] == shape0[3]
+    if not ok:
+        raise RuntimeError(_bad(xs, table, positions))
+    B, T, _, D = shape0
     if positions.dim() == 2:                 # (T, axes), shared over the batch
         positions = positions.unsqueeze(0)
-    if positions.dim() != 3 or positions.shape[0] not in (1, B) or positions.shape[1] != T:
-        raise RuntimeError(f'rotary: positions are (T, axes) or (B, T, axes), got {tuple(positions.shape)} for B={B}, T={T}')
-    axes, half = positions.shape[2], table.shape[1]
+    shape = positions.shape
+    if len(shape) != 3 or shape[0] not in (1, B) or shape[1] != T:
+        raise RuntimeError(f'rotary: positions are (T, axes) or (B, T, axes), got {tuple(shape)} for B={B}, T={T}')
+    axes, n_pos, half = shape[2], tshape[0], tshape[1]
     if axes < 1 or half < 1 or axes * 2 * half > D:
         raise RuntimeError(f'rotary: {axes} sections of {2 * half} elements exceed the head size {D}')
-    if positions.stride(2) != 1:
+    ps = positions.stride()
+    if ps[2] != 1:
         positions = positions.contiguous()
-    parts = (L.RotaryPart * len(xs))()
-    outs = []
+        ps = positions.stride()
+    parts, outs, keep = _PARTS[n](), [], []
     for i, x in enumerate(xs):
-        if x.stride(3) != 1:
+        st = x.stride()
+        if st[3] != 1 and D > 1:
             if inplace:
                 raise RuntimeError('rotary in place needs tensors whose last dimension is contiguous')
             x = x.contiguous()
-        out = x if inplace else torch.empty(x.shape, dtype=x.dtype, device=dev)
-        parts[i] = L.RotaryPart(x.data_ptr(), out.data_ptr(), *_strides(x), *_strides(out), x.shape[2], 0)
+            st = x.stride()
+        if inplace:
+            out, so = x, st
+        else:
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
+            so = out.stride()
+        parts[i] = (x.data_ptr(), out.data_ptr(), st[0], st[1], st[2], so[0], so[1], so[2], x.shape[2], 0)
         outs.append(out)
-    with torch.cuda.device(dev):
-        L.call('b3r_rotary', parts, len(xs), B, T, D, DTYPES[x0.dtype], table.data_ptr(), table.shape[0], half, axes,
-               positions.data_ptr(), int(positions.dtype == torch.int64),
-               0 if positions.shape[0] == 1 else positions.stride(0), positions.stride(1), int(bool(interleaved)),
-               int(bool(inverse)), torch.cuda.current_stream(dev).cuda_stream)
+        keep.append(x)
+    L.call_on(dev, 'b3r_rotary', parts, n, B, T, D, code, table.data_ptr(), n_pos, half, axes, positions.data_ptr(), wide,
+              0 if shape[0] == 1 else ps[0], ps[1], bool(interleaved), bool(inverse))
     return outs
 
 
