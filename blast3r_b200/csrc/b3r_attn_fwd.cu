@@ -25,58 +25,80 @@ namespace {
 
 constexpr int kThreads = 384;   // three warpgroups: two of softmax, one of loads and products
 constexpr int kMaxStages = 8;
-constexpr float kGrow = 8.f;   // log2 of how far the maximum may grow before O is rescaled
+constexpr int kAskAhead = 4;    // key tiles before its end at which a job's successor is asked for
+constexpr float kGrow = 8.f;    // log2 of how far the maximum may grow before O is rescaled
 
 struct alignas(64) FwdArgs {
   CUtensorMap q, k, v;
   b3r_attention_desc d;
   int tiles;        // pairs of row tiles (single ones when `one`) of the longest sequence
   int one;          // one tile of rows: the groups share it and split the keys
-  int splits;       // blocks along the keys
+  int splits;       // jobs along the keys
+  int G, heads;     // query heads to a group; B x Hkv
+  uint32_t g_mul, g_shift;   // for divisions by G
   int stages, group;
   int q_tma;        // the heads of a group divide 128: Q comes by TMA, a box of whole groups
   float* part_o;    // [splits][B Hkv][rows][D]
   float* part_l;    // [splits][B Hkv][rows]: log2 of the sum, -inf where a part sees nothing
 };
 
+// Buffers of a head size: S has three where tensor memory holds them beside O (so that a group's
+// next scores are ready when it ends the last ones), Q two where shared memory does.
+template <int DP>
+struct Cfg {
+  static constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
+  static constexpr int kS = DP == 64 ? 3 : 2, kQ = DP == 64 ? 2 : 1;
+  static constexpr int kOut = kS * 128;   // O's first column
+};
+
+// One job: two tiles of rows (one) of a key/value head, and a range of its keys.
+struct Job {
+  int b, kv, split;
+  int q0, k0, ql, kl, rows;
+  int m0[2];         // first row of each group's tile
+  int first, n[2];   // first key tile, and how many each group takes; n[0] < 0: there are no more jobs
+  int buf;           // S buffer of its first step
+};
+
+constexpr int kJobs = 3;   // jobs that a block has in hand at most
+
+// The barriers of S and P are each group's own, one for each of its last kS steps: a group that takes
+// no part in a job must not meet a barrier that has turned twice since.
 struct Shared {
-  uint64_t q_full, fix, kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2], p_full[2], o_done[2];
+  uint64_t q_full[2], q_empty[2], fix, kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2][3], p_full[2][3], o_done[2];
+  uint64_t job_full[kJobs], job_empty[kJobs], want, cancel;
+  alignas(16) uint4 answer;
+  Job job[kJobs];
   uint32_t tmem;
   int dead;
-  float m[kTileRows], l[kTileRows];
+  float m[2][kTileRows], l[2][kTileRows];   // of the second group, where both share a tile; by turns
 };
 
-// What a block works on; the same in every role.
-struct Job {
-  AttnSeq s;
-  int b, kv, split, rows, G;
-  int m0[2];     // first row of each group's tile
-  int first, n[2];   // first key tile, and how many each group takes
-};
+__device__ __forceinline__ int div_g(const FwdArgs& a, int m) { return (int)((__umulhi((uint32_t)m, a.g_mul) + (uint32_t)m) >> a.g_shift); }
 
-__device__ __forceinline__ Job job_of(const FwdArgs& a) {
+__device__ __forceinline__ void decode(const FwdArgs& a, int id, Job& j) {
   const b3r_attention_desc& d = a.d;
-  Job j;
-  const int heads = d.B * d.Hkv;
-  int id = blockIdx.x;
   j.split = id % a.splits;
   id /= a.splits;
   // heads in groups whose keys and values fit L2; within a group the row tiles with most work first
   const int gsz = a.group * a.tiles, g = id / gsz, r = id - g * gsz;
-  const int width = min(a.group, heads - g * a.group);
+  const int width = min(a.group, a.heads - g * a.group);
   const int tile = a.tiles - 1 - r / width, head = g * a.group + r % width;
   j.b = head / d.Hkv;
-  j.kv = head % d.Hkv;
-  j.G = d.Hq / d.Hkv;
-  j.s = attn_seq(d, j.b);
-  j.rows = (d.cu_q ? j.s.ql : d.Lq) * j.G;
-  const int seen = j.s.ql * j.G;
+  j.kv = head - j.b * d.Hkv;
+  const AttnSeq s = attn_seq(d, j.b);
+  j.q0 = (int)s.q0;
+  j.k0 = (int)s.k0;
+  j.ql = s.ql;
+  j.kl = s.kl;
+  j.rows = (d.cu_q ? s.ql : d.Lq) * a.G;
+  const int seen = s.ql * a.G;
   int n[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     j.m0[w] = a.one ? tile * kTileRows : (2 * tile + w) * kTileRows;
     const int last = min(j.m0[w] + kTileRows, seen) - 1;
-    n[w] = last < j.m0[w] ? 0 : (attn_bound(j.s, last / j.G, d.causal) + kTileRows - 1) / kTileRows;
+    n[w] = last < j.m0[w] ? 0 : (attn_bound(s, div_g(a, last), d.causal) + kTileRows - 1) / kTileRows;
   }
   const int all = max(n[0], n[1]), per = (all + a.splits - 1) / a.splits;
   j.first = j.split * per;
@@ -85,37 +107,129 @@ __device__ __forceinline__ Job job_of(const FwdArgs& a) {
     const int mine = min(max(n[w] - j.first, 0), per);
     j.n[w] = a.one ? (mine + 1 - w) / 2 : mine;
   }
-  return j;
 }
+
+// Where row m of a job's tile goes.
+template <typename T>
+struct RowOut {
+  T* o;
+  float* lse;
+  float *part_o, *part_l;
+  __device__ __forceinline__ RowOut(const FwdArgs& a, const Job& j, int m) {
+    const b3r_attention_desc& d = a.d;
+    const int i = div_g(a, m), h = j.kv * a.G + m - i * a.G;
+    o = attn_row<T>(d.o, j.b, (int64_t)j.q0 + i, h);
+    lse = attn_row<float>(d.lse, j.b, (int64_t)j.q0 + i, h);
+    const int64_t at = ((int64_t)j.split * a.heads + (int64_t)j.b * d.Hkv + j.kv) * ((int64_t)d.Lq * a.G) + m;
+    part_o = a.part_o + at * d.D;
+    part_l = a.part_l + at;
+  }
+};
+
+// The next job of a block.  The grid has a block for every job; a block that runs takes jobs over from
+// blocks that have not begun, so the barriers, tensor memory and loads of one serve many, and work of
+// unequal lengths spreads by itself.  (One warp; returns -1 when there are none left.)
+__device__ __forceinline__ void ask_next(Shared& sh) {
+  mbar_expect(smem_u32(&sh.cancel), 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(
+                   smem_u32(&sh.answer)),
+               "r"(smem_u32(&sh.cancel))
+               : "memory");
+}
+__device__ __forceinline__ int read_next(Shared& sh) {
+  uint32_t ok, x;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\tld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, _, _, _}, r;\n\t}"
+      : "=r"(ok), "=r"(x)
+      : "r"(smem_u32(&sh.answer))
+      : "memory");
+  return ok ? (int)x : -1;
+}
+
+// Walks over the steps of a block's jobs: key tile by key tile, each group that has one.
+struct Walk {
+  Shared& sh;
+  int k = 0, slot = 0, round = 0;   // the job at work, its slot
+  int n0 = 0, n1 = 0, i = 0, w = 0;
+  int step = 0;
+  bool opened = false, live = true;
+
+  __device__ __forceinline__ explicit Walk(Shared& s) : sh(s) {}
+  __device__ __forceinline__ const Job& job() const { return sh.job[slot]; }
+  __device__ __forceinline__ void open(volatile int* dead) {   // waits for the job to be there
+    mbar_wait(smem_u32(&sh.job_full[slot]), round & 1, dead);
+    const Job& j = sh.job[slot];
+    n0 = j.n[0];
+    n1 = j.n[1];
+    live = n0 >= 0 && !*dead;
+    i = 0;
+    w = n0 > 0 ? 0 : 1;
+    opened = true;
+  }
+  __device__ __forceinline__ bool first_step() const { return i == 0 && (w == 0 || n0 == 0); }
+  // whether this step is the first / the last that uses its tile
+  __device__ __forceinline__ bool opens(int one) const { return one || w == 0 || i >= n0; }
+  __device__ __forceinline__ bool closes(int one) const { return one || w == 1 || i >= n1; }
+  __device__ __forceinline__ int tile(int one) const { return job().first + (one ? 2 * i + w : i); }
+  // Goes on; true where the job is done (the next is not opened yet).
+  __device__ __forceinline__ bool next() {
+    ++step;
+    if (w == 0 && i < n1) {
+      w = 1;
+      return false;
+    }
+    ++i;
+    if (i < n0) w = 0;
+    else if (i < n1) w = 1;
+    else {
+      opened = false;
+      ++k;
+      if (++slot == kJobs) {
+        slot = 0;
+        ++round;
+      }
+      return true;
+    }
+    return false;
+  }
+};
 
 template <int DP, typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant__ FwdArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-  constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
-  constexpr bool kBf = sizeof(T) == 2 && __is_same(T, __nv_bfloat16);
-  const int q_tiles = a.one ? 1 : 2;
-  const uint32_t sq = smem_u32(base), skv = sq + q_tiles * kTile;
-  Shared& sh = *reinterpret_cast<Shared*>(base + (q_tiles + a.stages) * kTile);
+  using X = Cfg<DP>;
+  constexpr int kTile = X::kTile;
+  constexpr bool kBf = __is_same(T, __nv_bfloat16);
+  const int q_tiles = a.one ? 1 : 2, q_bytes = q_tiles * kTile;
+  const uint32_t sq = smem_u32(base), skv = sq + X::kQ * q_bytes;
+  Shared& sh = *reinterpret_cast<Shared*>(base + X::kQ * q_bytes + a.stages * kTile);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
-  if (warp == 9) tc_alloc(smem_u32(&sh.tmem), 512);   // first: it takes longer than the rest of the set-up
-  const Job j = job_of(a);
   const b3r_attention_desc& d = a.d;
-  const bool idle = j.m0[0] >= j.rows;                // no rows of this sequence here
-  const bool none = idle || j.n[0] + j.n[1] == 0;
-  const uint32_t bar_q = smem_u32(&sh.q_full);
+  if (warp == 9) tc_alloc(smem_u32(&sh.tmem), 512);
   if (threadIdx.x == 0) {
-    mbar_init(bar_q, a.q_tma ? 1 : 8);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&sh.q_full[i]), a.q_tma ? 1 : 8);
+      mbar_init(smem_u32(&sh.q_empty[i]), 1);
+      mbar_init(smem_u32(&sh.o_done[i]), 1);
+    }
     mbar_init(smem_u32(&sh.fix), 1);
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(smem_u32(&sh.kv_full[i]), 1);
       mbar_init(smem_u32(&sh.kv_empty[i]), 1);
     }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(smem_u32(&sh.s_full[w]), 1);
-      mbar_init(smem_u32(&sh.p_full[w]), 4);
-      mbar_init(smem_u32(&sh.o_done[w]), 1);
+    for (int i = 0; i < 6; ++i) {
+      mbar_init(smem_u32(&sh.s_full[i / 3][i % 3]), 1);
+      mbar_init(smem_u32(&sh.p_full[i / 3][i % 3]), 4);
     }
+    for (int i = 0; i < kJobs; ++i) {
+      mbar_init(smem_u32(&sh.job_full[i]), 1);
+      mbar_init(smem_u32(&sh.job_empty[i]), 10);   // loads, products, eight softmax warps
+    }
+    mbar_init(smem_u32(&sh.want), 1);
+    mbar_init(smem_u32(&sh.cancel), 1);
     sh.dead = 0;
     fence_async();
   }
@@ -128,257 +242,344 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
   // (256 x 208 + 128 x 88 = 384 x 168, what the block was launched with)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8 && !none) {
-    // ------------------------------------------------ loads
-    Ring ring{skv, base + q_tiles * kTile, sh.kv_full, sh.kv_empty, a.stages};
-    int fixes = 0;
-    if (a.q_tma && lane == 0) {        // whole groups of heads fill a tile: rows past the end only reach their own scores
-      mbar_expect(bar_q, q_tiles * kTile);
-      for (int w = 0; w < q_tiles; ++w)
+    if (warp == 8) {
+      // ------------------------------------------------ loads, in the order of the products
+      Ring ring{skv, base + X::kQ * q_bytes, sh.kv_full, sh.kv_empty, a.stages};
+      int fixes = 0;
+      bool asked = false;
+      Walk h(sh), t(sh);
+      auto load = [&](const CUtensorMap* map, const Walk& x, bool values) {   // P is zero past the last key, so V is cleared there
+        const Job& j = x.job();
+        const int row = x.tile(a.one) * kTileRows;
+        ring_load<X::kBlocks>(ring, map, j.k0 + row, j.kv, d.cu_k ? 0 : j.b, j.kl - row, values, &sh.fix, fixes, lane, dead);
+      };
+      auto keys = [&]() {
+        if (a.q_tma && h.first_step()) {   // rows past the end only reach their own scores
+          const Job& j = h.job();
+          const int qb = h.k % X::kQ, use = h.k / X::kQ;
+          const uint32_t bar = smem_u32(&sh.q_full[qb]);
+          if (use > 0) mbar_wait(smem_u32(&sh.q_empty[qb]), (use - 1) & 1, dead);
+          if (lane == 0) {
+            mbar_expect(bar, q_bytes);
+            for (int w = 0; w < q_tiles; ++w)
 #pragma unroll
-        for (int c = 0; c < kBlocks; ++c)
-          tma_box(sq + w * kTile + c * kBlockBytes, &a.q, c * 64, j.kv * j.G, (int)j.s.q0 + j.m0[w] / j.G, d.cu_q ? 0 : j.b, bar_q);
-    }
-    const int row0 = (int)j.s.k0, batch = d.cu_k ? 0 : j.b;
-    auto load = [&](const CUtensorMap* map, int tile, bool values) {   // P is zero past the last key, so V is cleared there
-      ring_load<kBlocks>(ring, map, row0 + tile * kTileRows, j.kv, batch, j.s.kl - tile * kTileRows, values, &sh.fix, fixes, lane,
-                         dead);
-    };
-    if (a.one) {
-      for (int w = 0; w < 2; ++w)
-        if (j.n[w] > 0) load(&a.k, j.first + w, false);
-      for (int i = 0; i < j.n[0]; ++i)
-        for (int w = 0; w < 2; ++w) {
-          if (i < j.n[w]) load(&a.v, j.first + 2 * i + w, true);
-          if (i + 1 < j.n[w]) load(&a.k, j.first + 2 * (i + 1) + w, false);
+              for (int c = 0; c < X::kBlocks; ++c)
+                tma_box(sq + qb * q_bytes + w * kTile + c * kBlockBytes, &a.q, c * 64, j.kv * a.G, j.q0 + div_g(a, j.m0[w]),
+                        d.cu_q ? 0 : j.b, bar);
+          }
         }
-    } else {
-      const int n = max(j.n[0], j.n[1]);
-      load(&a.k, j.first, false);
-      for (int i = 0; i < n; ++i) {
-        load(&a.v, j.first + i, true);
-        if (i + 1 < n) load(&a.k, j.first + i + 1, false);
+        if (h.opens(a.one)) load(&a.k, h, false);
+        if (!asked && h.i + kAskAhead >= max(h.n0, h.n1)) {   // near the job's end: the next one, not sooner
+          asked = true;
+          if (lane == 0) mbar_arrive(smem_u32(&sh.want));
+        }
+        if (h.next()) asked = false;
+      };
+      // scores as far ahead as S has buffers, into the next job at most (the products follow the same
+      // rule); not into it where the softmax warps bring Q, which they do when they get there
+      auto ahead = [&]() {
+        while (h.live && h.step < t.step + X::kS && h.k <= t.k + a.q_tma) {
+          if (!h.opened) h.open(dead);
+          if (h.live) keys();
+        }
+      };
+      t.open(dead);
+      while (t.live) {
+        ahead();
+        if (t.opens(a.one)) load(&a.v, t, true);
+        const int slot = t.slot;
+        if (t.next()) {
+          if (lane == 0) mbar_arrive(smem_u32(&sh.job_empty[slot]));
+          t.open(dead);
+        }
       }
-    }
-    } else if (warp == 9 && !none) {
-    // ------------------------------------------------ matrix products
-    {
+    } else if (warp == 9) {
+      // ------------------------------------------------ matrix products
       const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
       const int steps = (d.D + 15) / 16;
-      Ring ring{skv, base + q_tiles * kTile, sh.kv_full, sh.kv_empty, a.stages};
-      int last = 0, last_round = 0;
-      auto next = [&]() {
-        last_round = ring.round;
-        return last = ring.next(dead);
-      };
-      auto scores = [&](int w, int s) {                // S_w = Q_w K^T
-        const uint32_t q = sq + (a.one ? 0 : w) * kTile, k = skv + s * kTile;
-        tile_product<kBlocks>(tmem + w * 128, q, k, id_s, steps, on);
-        tc_commit(smem_u32(&sh.s_full[w]), on);
-      };
-      auto output = [&](int w, int s, int i) {         // O_w += P_w V
-        mbar_wait(smem_u32(&sh.p_full[w]), i & 1, dead);
+      const uint32_t bar_s = smem_u32(sh.s_full), bar_p = smem_u32(sh.p_full), bar_o = smem_u32(sh.o_done),
+                     bar_e = smem_u32(sh.kv_empty);
+      Ring ring{skv, base + X::kQ * q_bytes, sh.kv_full, sh.kv_empty, a.stages};
+      int last = -1, last_round = 0, ks = 0, vs = 0, hb = 0, tb = 0;   // (hb, tb: buffers of the steps at h and t)
+      int h0 = 0, h1 = 0, t0 = 0, t1 = 0, r0 = 0, r1 = 0;   // each group's barrier at h and at t, and the latter's round
+      Walk h(sh), t(sh);
+      auto scores = [&]() {                            // S = Q_w K^T of the step at h
+        const int qb = h.k % X::kQ, w = h.w;
+        if (h.first_step()) mbar_wait(smem_u32(&sh.q_full[qb]), (h.k / X::kQ) & 1, dead);
+        if (h.opens(a.one)) ks = ring.next(dead);
         tc_fence_after();
-        tile_gather(tmem + 256 + w * DP, tmem + w * 128, 32, skv + s * kTile, id_o, i > 0, on);
-        tc_commit(smem_u32(&sh.o_done[w]), on);
+        tile_product<X::kBlocks>(tmem + hb * 128, sq + qb * q_bytes + (a.one ? 0 : w) * kTile, skv + ks * kTile, id_s, steps, on);
+        tc_commit(bar_s + (w * 3 + (w ? h1 : h0)) * 8, on);
+        if (h.closes(a.one)) tc_commit(bar_e + ks * 8, on);
+        if (w) h1 = h1 + 1 == X::kS ? 0 : h1 + 1;
+        else h0 = h0 + 1 == X::kS ? 0 : h0 + 1;
+        hb = hb + 1 == X::kS ? 0 : hb + 1;
+        if (h.next()) tc_commit(smem_u32(&sh.q_empty[qb]), on);
       };
-      auto release = [&](int s) { tc_commit(smem_u32(&sh.kv_empty[s]), on); };
-      mbar_wait(bar_q, 0, dead);
-      tc_fence_after();
-      if (a.one) {
-        for (int w = 0; w < 2; ++w)
-          if (j.n[w] > 0) {
-            const int s = next();
-            scores(w, s);
-            release(s);
-          }
-        for (int i = 0; i < j.n[0]; ++i)
-          for (int w = 0; w < 2; ++w) {
-            if (i < j.n[w]) {
-              const int s = next();
-              output(w, s, i);
-              release(s);
-            }
-            if (i + 1 < j.n[w]) {
-              const int s = next();
-              scores(w, s);
-              release(s);
-            }
-          }
-      } else {
-        const int n = max(j.n[0], j.n[1]);
-        int sk = next();
-        for (int w = 0; w < 2; ++w)
-          if (j.n[w] > 0) scores(w, sk);
-        release(sk);
-        for (int i = 0; i < n; ++i) {
-          const int sv = next();
-          sk = i + 1 < n ? next() : -1;
-          for (int w = 0; w < 2; ++w) {
-            if (i < j.n[w]) output(w, sv, i);
-            if (i + 1 < j.n[w]) scores(w, sk);
-          }
-          release(sv);
-          if (sk >= 0) release(sk);
+      auto ahead = [&]() {
+        while (h.live && h.step < t.step + X::kS && h.k <= t.k + a.q_tma) {
+          if (!h.opened) h.open(dead);
+          if (h.live) scores();
+        }
+      };
+      t.open(dead);
+      while (t.live) {                                 // O_w += P V of the step at t
+        ahead();                                       // (into the buffer that P was just read from)
+        const int w = t.w;
+        if (t.opens(a.one)) {
+          last_round = ring.round;
+          last = vs = ring.next(dead);
+        }
+        mbar_wait(bar_p + (w * 3 + (w ? t1 : t0)) * 8, (w ? r1 : r0) & 1, dead);
+        tc_fence_after();
+        tile_gather(tmem + X::kOut + w * DP, tmem + tb * 128, 32, skv + vs * kTile, id_o, t.i > 0, on);
+        tc_commit(bar_o + w * 8, on);
+        if (t.closes(a.one)) tc_commit(bar_e + vs * 8, on);
+        if (w) {
+          if (++t1 == X::kS) t1 = 0, ++r1;
+        } else {
+          if (++t0 == X::kS) t0 = 0, ++r0;
+        }
+        tb = tb + 1 == X::kS ? 0 : tb + 1;
+        const int slot = t.slot;
+        if (t.next()) {
+          if (lane == 0) mbar_arrive(smem_u32(&sh.job_empty[slot]));
+          t.open(dead);
         }
       }
-      mbar_wait(smem_u32(&sh.kv_empty[last]), last_round & 1, dead);   // no arrival is left behind
-    }
+      if (last >= 0) mbar_wait(bar_e + last * 8, last_round & 1, dead);   // no arrival is left behind
+    } else if (warp == 10) {
+      // ------------------------------------------------ jobs
+      int id = blockIdx.x, slot = 0, round = 0, buf = 0, asks = 0;
+      for (int k = 0;;) {
+        Job j;
+        if (id >= 0) {
+          decode(a, id, j);
+          if (j.m0[0] < j.rows && j.n[0] + j.n[1] == 0) {   // rows that see nothing: cleared here and now
+            const int last = min(j.m0[a.one ? 0 : 1] + kTileRows, j.rows);
+            for (int m = j.m0[0]; m < last; ++m) {
+              const RowOut<T> to(a, j, m);
+              if (a.splits > 1) {
+                if (lane == 0) *to.part_l = -INFINITY;   // the part itself is not read then
+              } else {
+                for (int c = lane * 8; c < d.D; c += 256) *reinterpret_cast<uint4*>(to.o + c) = make_uint4(0, 0, 0, 0);
+                if (lane == 0) *to.lse = -INFINITY;
+              }
+            }
+          }
+        } else {
+          j.n[0] = j.n[1] = -1;
+        }
+        if (id < 0 || j.n[0] + j.n[1] > 0) {
+          if (round > 0) mbar_wait(smem_u32(&sh.job_empty[slot]), (round - 1) & 1, dead);
+          j.buf = buf;
+          if (lane == 0) {
+            sh.job[slot] = j;
+            mbar_arrive(smem_u32(&sh.job_full[slot]));
+          }
+          __syncwarp();
+          if (id < 0 || *dead) break;
+          buf = (buf + j.n[0] + j.n[1]) % X::kS;
+          if (++slot == kJobs) {
+            slot = 0;
+            ++round;
+          }
+          mbar_wait(smem_u32(&sh.want), k & 1, dead);    // until the loads are near its end
+          ++k;
+        }
+        if (lane == 0) ask_next(sh);
+        __syncwarp();
+        mbar_wait(smem_u32(&sh.cancel), asks & 1, dead);
+        ++asks;
+        id = *dead ? -1 : read_next(sh);
+        fence_async();                                   // the answer is read before the next one is written
+        __syncwarp();
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ------------------------------------------------ softmax, one row to a thread
     const int w = warp >> 2, r = threadIdx.x & 127;
-    const int m = j.m0[a.one ? 0 : w] + r;
-    const int i = m / j.G, h = j.kv * j.G + m % j.G;
-    const bool row = m < j.rows;
-    const int bound = row && i < j.s.ql ? attn_bound(j.s, i, d.causal) : 0;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);   // this warp's 32 lanes
     const float c = d.scale * kLog2e;
-    if (!none && !a.q_tma) {
-      if (w == 0 || !a.one) {
-        // the row of Q into the swizzled tile; zeros past D and past the rows
-        const uint4* q = reinterpret_cast<const uint4*>(attn_row<const T>(d.q, j.b, j.s.q0 + (row ? i : 0), row ? h : 0));
-        uint8_t* dst = base + w * kTile + r * 128;
+    int mine = 0, slot = 0, round = 0;         // this group's steps so far
+    for (int k = 0;; ++k) {
+      mbar_wait(smem_u32(&sh.job_full[slot]), round & 1, dead);
+      const Job& j = sh.job[slot];
+      if (j.n[0] < 0 || *dead) break;
+      const int n = j.n[w], n0 = j.n[0], n1 = j.n[1], buf0 = j.buf, first = j.first;
+      const int m = j.m0[a.one ? 0 : w] + r;
+      const bool row = m < j.rows;
+      const int i = div_g(a, m);
+      AttnSeq sq_;
+      sq_.ql = j.ql;
+      sq_.kl = j.kl;
+      const int bound = row && i < j.ql ? attn_bound(sq_, i, d.causal) : 0;
+      if (!a.q_tma) {
+        if (w == 0 || !a.one) {
+          // the row of Q into the swizzled tile; zeros past D and past the rows
+          const int h = j.kv * a.G + m - i * a.G;
+          const uint4* q = reinterpret_cast<const uint4*>(attn_row<const T>(d.q, j.b, (int64_t)j.q0 + (row ? i : 0), row ? h : 0));
+          uint8_t* dst = base + (k % X::kQ) * q_bytes + w * kTile + r * 128;
 #pragma unroll
-        for (int cb = 0; cb < DP / 8; ++cb) {
-          const uint4 x = (row && cb * 8 < d.D) ? q[cb] : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dst + (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4)) = x;
+          for (int cb = 0; cb < DP / 8; ++cb) {
+            const uint4 x = (row && cb * 8 < d.D) ? q[cb] : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(dst + (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4)) = x;
+          }
+          fence_async();
         }
-        fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[k % X::kQ]));
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar_q);
-    }
-    float mx = -INFINITY, l = 0.f;       // what the exponentials are taken against (log2), and their sum
-    const int n = j.n[w];
-    for (int it = 0; it < n; ++it) {
-      const int lim = bound - (j.first + (a.one ? 2 * it + w : it)) * kTileRows;   // keys of this tile that the row sees
-      mbar_wait(smem_u32(&sh.s_full[w]), it & 1, dead);
-      tc_fence_after();
-      uint32_t s[128];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) tc_ld32(quarter + w * 128 + q * 32, s + q * 32);
-      tc_wait_ld(s);
-      if (!__all_sync(0xffffffffu, lim >= kTileRows)) {
-#pragma unroll
-        for (int q = 0; q < 128; ++q) s[q] = q < lim ? s[q] : 0xff800000u;
-      }
-      float t0 = __uint_as_float(s[0]), t1 = __uint_as_float(s[1]);
-#pragma unroll
-      for (int q = 2; q < 128; q += 2) {
-        t0 = fmaxf(t0, __uint_as_float(s[q]));
-        t1 = fmaxf(t1, __uint_as_float(s[q + 1]));
-      }
-      const float top = fmaxf(mx, fmaxf(t0, t1) * c);
-      const bool grow = top > mx + kGrow || mx == -INFINITY;   // (mx = -inf: nothing summed yet)
-      if (it > 0 && __any_sync(0xffffffffu, grow && top > mx)) {
-        const float f = grow && top > mx ? ex2(mx - top) : 1.f;      // 0 for the first key that the row sees
-        mbar_wait(smem_u32(&sh.o_done[w]), (it - 1) & 1, dead);
+      float mx = -INFINITY, l = 0.f;       // what the exponentials are taken against (log2), and their sum
+      for (int it = 0; it < n; ++it, ++mine) {
+        // the step's place among all steps of the block gives its buffer
+        const int g = buf0 + min(it, n0) + min(it, n1) + (w && it < n0), bar = mine % X::kS;
+        const uint32_t at = quarter + g % X::kS * 128;
+        const int lim = bound - (first + (a.one ? 2 * it + w : it)) * kTileRows;   // keys of this tile that the row sees
+        mbar_wait(smem_u32(&sh.s_full[w][bar]), (mine / X::kS) & 1, dead);
         tc_fence_after();
+        uint32_t s[128];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) tc_ld32(at + q * 32, s + q * 32);
+        tc_wait_ld(s);
+        if (!__all_sync(0xffffffffu, lim >= kTileRows)) {
+#pragma unroll
+          for (int q = 0; q < 128; ++q) s[q] = q < lim ? s[q] : 0xff800000u;
+        }
+        float t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[4 + e]));
+#pragma unroll
+        for (int q = 8; q < 128; q += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(t[e], __uint_as_float(s[q + e])), __uint_as_float(s[q + 4 + e]));
+        const float top = fmaxf(mx, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c);
+        const bool grow = top > mx + kGrow || mx == -INFINITY;   // (mx = -inf: nothing summed yet)
+        if (it > 0 && __any_sync(0xffffffffu, grow && top > mx)) {
+          const float f = grow && top > mx ? ex2(mx - top) : 1.f;      // 0 for the first key that the row sees
+          mbar_wait(smem_u32(&sh.o_done[w]), (mine - 1) & 1, dead);
+          tc_fence_after();
+#pragma unroll
+          for (int q = 0; q < DP; q += 32) {
+            uint32_t o[32];
+            tc_ld32(quarter + X::kOut + w * DP + q, o);
+            tc_wait_ld(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tc_st32(quarter + X::kOut + w * DP + q, o);
+          }
+          l *= f;
+        }
+        if (grow) mx = top;
+        const float2 cc = make_float2(c, c), mm = make_float2(mx == -INFINITY ? 0.f : -mx, mx == -INFINITY ? 0.f : -mx);
+        float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int q0 = 0; q0 < 64; q0 += 16) {
+          uint32_t p[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * (q0 + e)]), __uint_as_float(s[2 * (q0 + e) + 1])), cc, mm);
+            x.x = ex2(x.x);
+            x.y = ex2(x.y);
+            sum[e & 1] = __fadd2_rn(sum[e & 1], x);
+            p[e] = pack2(x.x, x.y, T());
+          }
+          tc_st16(at + q0, p);
+        }
+        tc_wait_st();
+        // the last step's product ends long before, but has to be seen: o_done's turns are met one by one
+        if (mine > 0) mbar_wait(smem_u32(&sh.o_done[w]), (mine - 1) & 1, dead);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[w][bar]));
+        sum[0] = __fadd2_rn(sum[0], sum[1]);
+        l += sum[0].x + sum[0].y;
+      }
+      if (n > 0) {
+        mbar_wait(smem_u32(&sh.o_done[w]), (mine - 1) & 1, dead);
+        tc_fence_after();
+      }
+      // ---------------------------------------------- output
+      float f0 = 0.f, f1 = 0.f, lg;                      // factors of O (and of the other group's O); log2 of the sum
+      if (a.one) {
+        const int turn = k & 1;
+        if (w == 1) {
+          sh.m[turn][r] = mx;
+          sh.l[turn][r] = l;
+        }
+        tc_fence_before();
+        bar_sync(1, 256);
+        tc_fence_after();
+        if (w == 0) {
+          const float m1 = sh.m[turn][r], l1 = sh.l[turn][r], top = fmaxf(mx, m1);
+          const float e0 = mx == -INFINITY ? 0.f : ex2(mx - top), e1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
+          const float sum = l * e0 + l1 * e1;
+          f0 = sum > 0.f ? e0 / sum : 0.f;
+          f1 = sum > 0.f ? e1 / sum : 0.f;
+          lg = sum != 0.f ? top + __log2f(sum) : -INFINITY;
+          if (isnan(sum)) f0 = f1 = lg = sum;
+        }
+      } else {
+        f0 = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;     // NaN stays NaN
+        lg = l == 0.f ? -INFINITY : mx + __log2f(l);
+      }
+      if (w == 0 || !a.one) {
+        const bool has0 = n > 0, has1 = a.one && n1 > 0;
+        const RowOut<T> to(a, j, row ? m : 0);
+        if (*dead) f0 = f1 = lg = __int_as_float(0x7fffffff);
 #pragma unroll
         for (int q = 0; q < DP; q += 32) {
+          if (q >= d.D) break;
           uint32_t o[32];
-          tc_ld32(quarter + 256 + w * DP + q, o);
-          tc_wait_ld(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-          tc_st32(quarter + 256 + w * DP + q, o);
-        }
-        l *= f;
-      }
-      if (grow) mx = top;
-      const float2 cc = make_float2(c, c), mm = make_float2(mx == -INFINITY ? 0.f : -mx, mx == -INFINITY ? 0.f : -mx);
-      float2 sum = make_float2(0.f, 0.f);
-      uint32_t p[64];
-#pragma unroll
-      for (int q = 0; q < 64; ++q) {
-        float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * q]), __uint_as_float(s[2 * q + 1])), cc, mm);
-        x.x = ex2(x.x);
-        x.y = ex2(x.y);
-        sum = __fadd2_rn(sum, x);
-        p[q] = pack2(x.x, x.y, T());
-      }
-      tc_st32(quarter + w * 128, p);
-      tc_st32(quarter + w * 128 + 32, p + 32);
-      l += sum.x + sum.y;
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[w]));
-    }
-    if (n > 0) {
-      mbar_wait(smem_u32(&sh.o_done[w]), (n - 1) & 1, dead);
-      tc_fence_after();
-    }
-    // ---------------------------------------------- output
-    float f0 = 0.f, f1 = 0.f, lg;                      // factors of O (and of the other group's O); log2 of the sum
-    if (a.one) {
-      if (w == 1) {
-        sh.m[r] = mx;
-        sh.l[r] = l;
-      }
-      bar_sync(1, 256);
-      if (w == 0) {
-        const float m1 = sh.m[r], l1 = sh.l[r], top = fmaxf(mx, m1);
-        const float e0 = mx == -INFINITY ? 0.f : ex2(mx - top), e1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
-        const float sum = l * e0 + l1 * e1;
-        f0 = sum > 0.f ? e0 / sum : 0.f;
-        f1 = sum > 0.f ? e1 / sum : 0.f;
-        lg = top + __log2f(sum);
-        if (!(sum != 0.f)) lg = -INFINITY;
-        if (isnan(sum)) f0 = f1 = lg = sum;
-      }
-      tc_fence_after();
-    } else {
-      f0 = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;     // NaN stays NaN
-      lg = l == 0.f ? -INFINITY : mx + __log2f(l);
-    }
-    if (!idle && (w == 0 || !a.one)) {
-      const bool has0 = n > 0, has1 = a.one && j.n[1] > 0;
-      const int64_t at = ((int64_t)j.split * d.B * d.Hkv + (int64_t)j.b * d.Hkv + j.kv) * ((int64_t)d.Lq * j.G) + m;
-      if (*dead) f0 = f1 = lg = __int_as_float(0x7fffffff);
-#pragma unroll
-      for (int q = 0; q < DP; q += 32) {
-        if (q >= d.D) break;
-        uint32_t o[32];
-        float v[32];
-#pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0.f;
-        if (has0) {
-          tc_ld32(quarter + 256 + w * DP + q, o);
-          tc_wait_ld(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * f0;
-        }
-        if (has1) {
-          tc_ld32(quarter + 256 + DP + q, o);
-          tc_wait_ld(o);
-#pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] += __uint_as_float(o[e]) * f1;
-        }
-        if (lg == -INFINITY)                           // a row that sees nothing
+          float v[32];
 #pragma unroll
           for (int e = 0; e < 32; ++e) v[e] = 0.f;
-        if (!row) continue;
-        if (a.splits > 1) {
-          float* out = a.part_o + at * d.D + q;
+          if (has0) {
+            tc_ld32(quarter + X::kOut + w * DP + q, o);
+            tc_wait_ld(o);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            if (q + e < d.D) *reinterpret_cast<float4*>(out + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-        } else {
-          T* out = attn_row<T>(d.o, j.b, j.s.q0 + i, h) + q;
+            for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * f0;
+          }
+          if (has1) {
+            tc_ld32(quarter + X::kOut + DP + q, o);
+            tc_wait_ld(o);
 #pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            if (q + e < d.D)
-              *reinterpret_cast<uint4*>(out + e) = make_uint4(pack2(v[e], v[e + 1], T()), pack2(v[e + 2], v[e + 3], T()),
-                                                              pack2(v[e + 4], v[e + 5], T()), pack2(v[e + 6], v[e + 7], T()));
+            for (int e = 0; e < 32; ++e) v[e] += __uint_as_float(o[e]) * f1;
+          }
+          if (lg == -INFINITY)                           // a row that sees nothing
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = 0.f;
+          if (row) {
+            if (a.splits > 1) {
+              float* out = to.part_o + q;
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                if (q + e < d.D) *reinterpret_cast<float4*>(out + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+            } else {
+              T* out = to.o + q;
+#pragma unroll
+              for (int e = 0; e < 32; e += 8)
+                if (q + e < d.D)
+                  *reinterpret_cast<uint4*>(out + e) = make_uint4(pack2(v[e], v[e + 1], T()), pack2(v[e + 2], v[e + 3], T()),
+                                                                  pack2(v[e + 4], v[e + 5], T()), pack2(v[e + 6], v[e + 7], T()));
+            }
+          }
+          __syncwarp();
+        }
+        if (row) {
+          if (a.splits > 1) *to.part_l = lg;
+          else *to.lse = lg * kLn2;
         }
       }
-      if (row) {
-        if (a.splits > 1) a.part_l[at] = lg;
-        else *attn_row<float>(d.lse, j.b, j.s.q0 + i, h) = lg * kLn2;
+      tc_fence_before();
+      if (a.one) bar_sync(2, 256);                       // the other group's O has been read
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.job_empty[slot]));
+      if (++slot == kJobs) {
+        slot = 0;
+        ++round;
       }
     }
   }
@@ -439,32 +640,38 @@ constexpr int kSms = 148;
 // How the work is cut, from the descriptor alone (the lengths on the device are not known here).
 void cut(FwdArgs& a) {
   const b3r_attention_desc& d = a.d;
-  const int64_t rows = (int64_t)d.Lq * (d.Hq / d.Hkv);
+  a.G = d.Hq / d.Hkv;
+  a.heads = d.B * d.Hkv;
+  // m / G = (umulhi(m, mul) + m) >> shift for 0 <= m < 2^31 (Granlund and Montgomery's division by an invariant)
+  a.g_shift = 0;
+  while ((1u << a.g_shift) < (uint32_t)a.G) ++a.g_shift;
+  a.g_mul = (uint32_t)(((uint64_t(1) << 32) * ((uint64_t(1) << a.g_shift) - a.G)) / a.G + 1);
+  const int64_t rows = (int64_t)d.Lq * a.G;
   a.one = rows <= kTileRows;
-  a.tiles = a.one ? 1 : (int)((rows + 2 * kTileRows - 1) / (2 * kTileRows));
-  const int64_t blocks = (int64_t)a.tiles * d.B * d.Hkv, keys = (d.Lk + kTileRows - 1) / kTileRows;
-  // Fewer blocks than SMs leave SMs idle: the keys are split, two tiles to a block at least (one
-  // for each group).  Sequences of different lengths make some of these blocks shorter, so long
-  // key ranges (8 tiles a block at least) are split into about four blocks an SM.
+  const int64_t job_rows = a.one ? kTileRows : 2 * kTileRows;
+  a.tiles = (int)((rows + job_rows - 1) / job_rows);
+  const int64_t jobs = (int64_t)a.tiles * d.B * d.Hkv, keys = (d.Lk + kTileRows - 1) / kTileRows;
+  // Fewer jobs than SMs leave SMs idle: the keys are split, two tiles to a job at least (one for
+  // each group).  Sequences of different lengths make some of these jobs shorter, so long key
+  // ranges (8 tiles a job at least) are split into about four jobs an SM.
   a.splits = 1;
-  if (blocks < kSms) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>((kSms + blocks - 1) / blocks, keys / 2));
-  if (blocks < 4 * kSms && a.one)
-    a.splits = (int)std::max<int64_t>(a.splits, std::min<int64_t>((4 * kSms + blocks - 1) / blocks, keys / 8));
-  const int dp = d.D <= 64 ? 64 : 128, tile = dp / 64 * kBlockBytes;
-  a.stages = std::min(kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - (a.one ? 1 : 2));
+  if (jobs < kSms) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / jobs, keys / 2));
+  if (jobs < 4 * kSms && a.one)
+    a.splits = (int)std::max<int64_t>(a.splits, std::min<int64_t>((4 * kSms + jobs - 1) / jobs, keys / 8));
+  const int dp = d.D <= 64 ? 64 : 128, tile = dp / 64 * kBlockBytes, q = (dp == 64 ? 2 : 1) * (a.one ? 1 : 2);
+  a.stages = std::min(kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - q);
   // heads whose keys and values are at work at the same time: about 32 MB of the 126 MB L2
   const int64_t head = std::max<int64_t>(1, (int64_t)d.Lk * d.D * 4);
   a.group = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)d.B * d.Hkv, (32 << 20) / head));
 }
 
 template <int DP, typename T>
-int launch(const FwdArgs& a, cudaStream_t s) {
-  const int tile = DP / 64 * kBlockBytes;
-  const int smem = 1024 + ((a.one ? 1 : 2) + a.stages) * tile + (int)sizeof(Shared);
+int launch(FwdArgs& a, cudaStream_t s) {
+  const int smem = 1024 + ((DP == 64 ? 2 : 1) * (a.one ? 1 : 2) + a.stages) * Cfg<DP>::kTile + (int)sizeof(Shared);
   B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_fwd<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention"));
-  const int64_t blocks = (int64_t)a.tiles * a.d.B * a.d.Hkv * a.splits;
-  B3R_REQUIRE(blocks <= 0x7fffffff, "attention: too many rows for one call");
-  k_attn_fwd<DP, T><<<(unsigned)blocks, kThreads, smem, s>>>(a);
+  const int64_t jobs = (int64_t)a.tiles * a.heads * a.splits;
+  B3R_REQUIRE(jobs <= 0x3fffffff, "attention: too many rows for one call");
+  k_attn_fwd<DP, T><<<(unsigned)jobs, kThreads, smem, s>>>(a);
   B3R_TRY(check_launch("attention"));
   if (a.splits > 1) {
     const int64_t rows = (int64_t)a.d.Lq * (a.d.Hq / a.d.Hkv);

@@ -38,7 +38,7 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-constexpr int kWaitLimit = 1 << 22;   // polls; seconds, where a wait takes microseconds
+constexpr int kWaitLimit = 1 << 18;   // polls; about a second, where a wait takes microseconds
 __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
   if (mbar_try(bar, parity)) return;
   for (int n = 0; n < kWaitLimit; ++n) {

@@ -109,6 +109,23 @@ def test_packed(causal, D, Hq, Hkv):
         assert torch.equal(dk[b], clean['dk'][b]) and torch.equal(dv[b], clean['dv'][b])
 
 
+@pytest.mark.parametrize('Lq,Lk,causal', [(257, 257, False), (129, 300, True), (257, 100, True), (1, 700, False), (40, 513, False)])
+@pytest.mark.parametrize('D', [64, 128])
+def test_more_work_than_blocks(Lq, Lk, causal, D):
+    """Many heads, so that a block gets several pieces of work one after the other, some of which
+    leave half of it idle: last tiles of one row, causal tiles that see nothing, lengths of zero."""
+    kl = [Lk, 0, Lk, 1, Lk // 2, Lk, Lk // 3, 130][:8]
+    kl = [min(n, Lk) for n in kl]
+    q, k, v, do = _dense(8, Lq, Lk, 42, 42, D, 'bf16')
+    _check(q, k, v, do, [(b, Lq, kl[b]) for b in range(8)], False, causal, k_lens=torch.tensor(kl, dtype=torch.int32, device='cuda'))
+
+
+@pytest.mark.parametrize('causal', [False, True])
+def test_more_work_than_blocks_three_heads_to_a_group(causal):
+    q, k, v, do = _dense(6, 130, 190, 90, 30, 64, 'f16')
+    _check(q, k, v, do, [(b, 130, 190) for b in range(6)], False, causal)
+
+
 def test_strides_and_scale():
     """The three parts of one projection, heads before rows, and a copy where D is not contiguous."""
     B, L, H, D = 2, 150, 3, 64
