@@ -4,8 +4,11 @@
 // kv G + m % G, so the heads that share keys and values fill one tile and read them once.  A
 // block owns two tiles of 128 rows, or one where there are no more rows, and walks over tiles of
 // 128 keys:
-//   warp 8    loads K and V tiles by TMA into a ring of stages
-//   warp 9    issues S_w = Q_w K^T (tensor memory) and O_w += P_w V, P_w read from tensor memory
+//   warp 8    loads Q, K and V tiles by TMA, K and V into rings of stages
+//   warp 9    issues S_w = Q_w K^T into one of the S buffers in tensor memory
+//   warp 11   issues O_w += P_w V, P_w read from tensor memory (in one warp, issuing both took longer
+//             than the products themselves: 2000 cycles a step against 750 to 1350)
+//   warp 10   finds and decodes the block's next job
 //   warps 0-3, 4-7: one group for each tile w; a thread owns a row, keeps its running maximum and
 //             sum, and writes P_w as 16-bit pairs over S_w
 // While one group is at its exponentials, the tensor cores work for the other.  With one tile of
@@ -36,7 +39,7 @@ struct alignas(64) FwdArgs {
   int splits;       // jobs along the keys
   int G, heads;     // query heads to a group; B x Hkv
   uint32_t g_mul, g_shift;   // for divisions by G
-  int stages, group;
+  int k_stages, v_stages, group;
   int q_tma;        // the heads of a group divide 128: Q comes by TMA, a box of whole groups
   float* part_o;    // [splits][B Hkv][rows][D]
   float* part_l;    // [splits][B Hkv][rows]: log2 of the sum, -inf where a part sees nothing
@@ -65,7 +68,8 @@ constexpr int kJobs = 3;   // jobs that a block has in hand at most
 // The barriers of S and P are each group's own, one for each of its last kS steps: a group that takes
 // no part in a job must not meet a barrier that has turned twice since.
 struct Shared {
-  uint64_t q_full[2], q_empty[2], fix, kv_full[kMaxStages], kv_empty[kMaxStages], s_full[2][3], p_full[2][3], o_done[2];
+  uint64_t q_full[2], q_empty[2], fix, k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+  uint64_t s_full[2][3], p_full[2][3], s_free[3], o_done[2];
   uint64_t job_full[kJobs], job_empty[kJobs], want, cancel;
   alignas(16) uint4 answer;
   Job job[kJobs];
@@ -148,51 +152,24 @@ __device__ __forceinline__ int read_next(Shared& sh) {
   return ok ? (int)x : -1;
 }
 
-// Walks over the steps of a block's jobs: key tile by key tile, each group that has one.
-struct Walk {
+// A role's place in the block's list of jobs.
+struct JobList {
   Shared& sh;
-  int k = 0, slot = 0, round = 0;   // the job at work, its slot
-  int n0 = 0, n1 = 0, i = 0, w = 0;
-  int step = 0;
-  bool opened = false, live = true;
-
-  __device__ __forceinline__ explicit Walk(Shared& s) : sh(s) {}
-  __device__ __forceinline__ const Job& job() const { return sh.job[slot]; }
-  __device__ __forceinline__ void open(volatile int* dead) {   // waits for the job to be there
+  int slot = 0, round = 0;
+  __device__ __forceinline__ explicit JobList(Shared& s) : sh(s) {}
+  // The next job, once it is there; nullptr after the last.
+  __device__ __forceinline__ const Job* get(volatile int* dead) {
     mbar_wait(smem_u32(&sh.job_full[slot]), round & 1, dead);
-    const Job& j = sh.job[slot];
-    n0 = j.n[0];
-    n1 = j.n[1];
-    live = n0 >= 0 && !*dead;
-    i = 0;
-    w = n0 > 0 ? 0 : 1;
-    opened = true;
+    return sh.job[slot].n[0] < 0 || *dead ? nullptr : &sh.job[slot];
   }
-  __device__ __forceinline__ bool first_step() const { return i == 0 && (w == 0 || n0 == 0); }
-  // whether this step is the first / the last that uses its tile
-  __device__ __forceinline__ bool opens(int one) const { return one || w == 0 || i >= n0; }
-  __device__ __forceinline__ bool closes(int one) const { return one || w == 1 || i >= n1; }
-  __device__ __forceinline__ int tile(int one) const { return job().first + (one ? 2 * i + w : i); }
-  // Goes on; true where the job is done (the next is not opened yet).
-  __device__ __forceinline__ bool next() {
-    ++step;
-    if (w == 0 && i < n1) {
-      w = 1;
-      return false;
+  // Ends the role's use of it (one lane of a warp that has read all it needs).
+  __device__ __forceinline__ void done(int lane) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh.job_empty[slot]));
+    if (++slot == kJobs) {
+      slot = 0;
+      ++round;
     }
-    ++i;
-    if (i < n0) w = 0;
-    else if (i < n1) w = 1;
-    else {
-      opened = false;
-      ++k;
-      if (++slot == kJobs) {
-        slot = 0;
-        ++round;
-      }
-      return true;
-    }
-    return false;
   }
 };
 
@@ -204,8 +181,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
   constexpr int kTile = X::kTile;
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
   const int q_tiles = a.one ? 1 : 2, q_bytes = q_tiles * kTile;
-  const uint32_t sq = smem_u32(base), skv = sq + X::kQ * q_bytes;
-  Shared& sh = *reinterpret_cast<Shared*>(base + X::kQ * q_bytes + a.stages * kTile);
+  const uint32_t sq = smem_u32(base), sk = sq + X::kQ * q_bytes, sv = sk + a.k_stages * kTile;
+  Shared& sh = *reinterpret_cast<Shared*>(base + X::kQ * q_bytes + (a.k_stages + a.v_stages) * kTile);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
   const b3r_attention_desc& d = a.d;
   if (warp == 9) tc_alloc(smem_u32(&sh.tmem), 512);
@@ -216,9 +193,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       mbar_init(smem_u32(&sh.o_done[i]), 1);
     }
     mbar_init(smem_u32(&sh.fix), 1);
-    for (int i = 0; i < a.stages; ++i) {
-      mbar_init(smem_u32(&sh.kv_full[i]), 1);
-      mbar_init(smem_u32(&sh.kv_empty[i]), 1);
+    for (int i = 0; i < a.k_stages; ++i) {
+      mbar_init(smem_u32(&sh.k_full[i]), 1);
+      mbar_init(smem_u32(&sh.k_empty[i]), 1);
+      mbar_init(smem_u32(&sh.v_full[i]), 1);
+      mbar_init(smem_u32(&sh.v_empty[i]), 1);
     }
     for (int i = 0; i < 6; ++i) {
       mbar_init(smem_u32(&sh.s_full[i / 3][i % 3]), 1);
@@ -226,7 +205,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     }
     for (int i = 0; i < kJobs; ++i) {
       mbar_init(smem_u32(&sh.job_full[i]), 1);
-      mbar_init(smem_u32(&sh.job_empty[i]), 10);   // loads, products, eight softmax warps
+      mbar_init(smem_u32(&sh.job_empty[i]), 11);   // loads, two warps of products, eight of softmax
+      mbar_init(smem_u32(&sh.s_free[i]), 1);
     }
     mbar_init(smem_u32(&sh.want), 1);
     mbar_init(smem_u32(&sh.cancel), 1);
@@ -243,20 +223,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     if (warp == 8) {
-      // ------------------------------------------------ loads, in the order of the products
-      Ring ring{skv, base + X::kQ * q_bytes, sh.kv_full, sh.kv_empty, a.stages};
-      int fixes = 0;
-      bool asked = false;
-      Walk h(sh), t(sh);
-      auto load = [&](const CUtensorMap* map, const Walk& x, bool values) {   // P is zero past the last key, so V is cleared there
-        const Job& j = x.job();
-        const int row = x.tile(a.one) * kTileRows;
-        ring_load<X::kBlocks>(ring, map, j.k0 + row, j.kv, d.cu_k ? 0 : j.b, j.kl - row, values, &sh.fix, fixes, lane, dead);
-      };
-      auto keys = [&]() {
-        if (a.q_tma && h.first_step()) {   // rows past the end only reach their own scores
-          const Job& j = h.job();
-          const int qb = h.k % X::kQ, use = h.k / X::kQ;
+      // ------------------------------------------------ loads
+      Ring kr{sk, base + X::kQ * q_bytes, sh.k_full, sh.k_empty, a.k_stages};
+      Ring vr{sv, base + X::kQ * q_bytes + a.k_stages * kTile, sh.v_full, sh.v_empty, a.v_stages};
+      int fixes = 0, k = 0;
+      JobList list(sh);
+      while (const Job* j = list.get(dead)) {
+        if (a.q_tma) {                         // rows past the end only reach their own scores
+          const int qb = k % X::kQ, use = k / X::kQ;
           const uint32_t bar = smem_u32(&sh.q_full[qb]);
           if (use > 0) mbar_wait(smem_u32(&sh.q_empty[qb]), (use - 1) & 1, dead);
           if (lane == 0) {
@@ -264,88 +238,110 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
             for (int w = 0; w < q_tiles; ++w)
 #pragma unroll
               for (int c = 0; c < X::kBlocks; ++c)
-                tma_box(sq + qb * q_bytes + w * kTile + c * kBlockBytes, &a.q, c * 64, j.kv * a.G, j.q0 + div_g(a, j.m0[w]),
-                        d.cu_q ? 0 : j.b, bar);
+                tma_box(sq + qb * q_bytes + w * kTile + c * kBlockBytes, &a.q, c * 64, j->kv * a.G, j->q0 + div_g(a, j->m0[w]),
+                        d.cu_q ? 0 : j->b, bar);
           }
         }
-        if (h.opens(a.one)) load(&a.k, h, false);
-        if (!asked && h.i + kAskAhead >= max(h.n0, h.n1)) {   // near the job's end: the next one, not sooner
-          asked = true;
-          if (lane == 0) mbar_arrive(smem_u32(&sh.want));
+        const int tiles = a.one ? j->n[0] + j->n[1] : max(j->n[0], j->n[1]);
+        const int ask = max(0, tiles - kAskAhead), batch = d.cu_k ? 0 : j->b;
+        for (int i = 0; i < tiles; ++i) {
+          const int row = (j->first + i) * kTileRows;
+          if (i == ask && lane == 0) mbar_arrive(smem_u32(&sh.want));   // near the job's end: the next one, not sooner
+          ring_load<X::kBlocks>(kr, &a.k, j->k0 + row, j->kv, batch, j->kl - row, false, &sh.fix, fixes, lane, dead);
+          // P is zero past the last key, so V is cleared there
+          ring_load<X::kBlocks>(vr, &a.v, j->k0 + row, j->kv, batch, j->kl - row, true, &sh.fix, fixes, lane, dead);
         }
-        if (h.next()) asked = false;
-      };
-      // scores as far ahead as S has buffers, into the next job at most (the products follow the same
-      // rule); not into it where the softmax warps bring Q, which they do when they get there
-      auto ahead = [&]() {
-        while (h.live && h.step < t.step + X::kS && h.k <= t.k + a.q_tma) {
-          if (!h.opened) h.open(dead);
-          if (h.live) keys();
-        }
-      };
-      t.open(dead);
-      while (t.live) {
-        ahead();
-        if (t.opens(a.one)) load(&a.v, t, true);
-        const int slot = t.slot;
-        if (t.next()) {
-          if (lane == 0) mbar_arrive(smem_u32(&sh.job_empty[slot]));
-          t.open(dead);
-        }
+        list.done(lane);
+        ++k;
       }
     } else if (warp == 9) {
-      // ------------------------------------------------ matrix products
-      const uint32_t on = elect_one();
-      const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
+      // ------------------------------------------------ scores: S = Q_w K^T, step by step
+      const uint32_t on = elect_one(), id_s = mma_idesc(kBf, 128, 128, false);
       const int steps = (d.D + 15) / 16;
-      const uint32_t bar_s = smem_u32(sh.s_full), bar_p = smem_u32(sh.p_full), bar_o = smem_u32(sh.o_done),
-                     bar_e = smem_u32(sh.kv_empty);
-      Ring ring{skv, base + X::kQ * q_bytes, sh.kv_full, sh.kv_empty, a.stages};
-      int last = -1, last_round = 0, ks = 0, vs = 0, hb = 0, tb = 0;   // (hb, tb: buffers of the steps at h and t)
-      int h0 = 0, h1 = 0, t0 = 0, t1 = 0, r0 = 0, r1 = 0;   // each group's barrier at h and at t, and the latter's round
-      Walk h(sh), t(sh);
-      auto scores = [&]() {                            // S = Q_w K^T of the step at h
-        const int qb = h.k % X::kQ, w = h.w;
-        if (h.first_step()) mbar_wait(smem_u32(&sh.q_full[qb]), (h.k / X::kQ) & 1, dead);
-        if (h.opens(a.one)) ks = ring.next(dead);
-        tc_fence_after();
-        tile_product<X::kBlocks>(tmem + hb * 128, sq + qb * q_bytes + (a.one ? 0 : w) * kTile, skv + ks * kTile, id_s, steps, on);
-        tc_commit(bar_s + (w * 3 + (w ? h1 : h0)) * 8, on);
-        if (h.closes(a.one)) tc_commit(bar_e + ks * 8, on);
-        if (w) h1 = h1 + 1 == X::kS ? 0 : h1 + 1;
-        else h0 = h0 + 1 == X::kS ? 0 : h0 + 1;
-        hb = hb + 1 == X::kS ? 0 : hb + 1;
-        if (h.next()) tc_commit(smem_u32(&sh.q_empty[qb]), on);
-      };
-      auto ahead = [&]() {
-        while (h.live && h.step < t.step + X::kS && h.k <= t.k + a.q_tma) {
-          if (!h.opened) h.open(dead);
-          if (h.live) scores();
+      const uint32_t bar_s = smem_u32(sh.s_full), bar_f = smem_u32(sh.s_free), bar_e = smem_u32(sh.k_empty);
+      Ring kr{sk, base + X::kQ * q_bytes, sh.k_full, sh.k_empty, a.k_stages};
+      int k = 0, buf = 0, uses = 0, b0 = 0, b1 = 0;    // S buffer and its turn; each group's barrier
+      int last_buf = -1, last_use = 0;
+      JobList list(sh);
+      while (const Job* j = list.get(dead)) {
+        const int n0 = j->n[0], n1 = j->n[1], n = max(n0, n1), qb = k % X::kQ;
+        list.done(lane);
+        mbar_wait(smem_u32(&sh.q_full[qb]), (k / X::kQ) & 1, dead);
+        const uint32_t q0 = sq + qb * q_bytes, q1 = a.one ? q0 : q0 + kTile;
+        auto product = [&](uint32_t q, int w, int& b, int st) {
+          if (uses > 0) mbar_wait(bar_f + buf * 8, (uses - 1) & 1, dead);   // until P has been read from it
+          tc_fence_after();
+          tile_product<X::kBlocks>(tmem + buf * 128, q, sk + st * kTile, id_s, steps, on);
+          tc_commit(bar_s + (w * 3 + b) * 8, on);
+          b = b + 1 == X::kS ? 0 : b + 1;
+          last_buf = buf;
+          last_use = uses;
+          if (++buf == X::kS) {
+            buf = 0;
+            ++uses;
+          }
+        };
+        for (int i = 0; i < n; ++i) {
+          int st = 0;
+          if (!a.one) st = kr.next(dead);
+          if (i < n0) {
+            if (a.one) st = kr.next(dead);
+            product(q0, 0, b0, st);
+            if (a.one) tc_commit(bar_e + st * 8, on);
+          }
+          if (i < n1) {
+            if (a.one) st = kr.next(dead);
+            product(q1, 1, b1, st);
+            if (a.one) tc_commit(bar_e + st * 8, on);
+          }
+          if (!a.one) tc_commit(bar_e + st * 8, on);
         }
-      };
-      t.open(dead);
-      while (t.live) {                                 // O_w += P V of the step at t
-        ahead();                                       // (into the buffer that P was just read from)
-        const int w = t.w;
-        if (t.opens(a.one)) {
-          last_round = ring.round;
-          last = vs = ring.next(dead);
-        }
-        mbar_wait(bar_p + (w * 3 + (w ? t1 : t0)) * 8, (w ? r1 : r0) & 1, dead);
-        tc_fence_after();
-        tile_gather(tmem + X::kOut + w * DP, tmem + tb * 128, 32, skv + vs * kTile, id_o, t.i > 0, on);
-        tc_commit(bar_o + w * 8, on);
-        if (t.closes(a.one)) tc_commit(bar_e + vs * 8, on);
-        if (w) {
-          if (++t1 == X::kS) t1 = 0, ++r1;
-        } else {
-          if (++t0 == X::kS) t0 = 0, ++r0;
-        }
-        tb = tb + 1 == X::kS ? 0 : tb + 1;
-        const int slot = t.slot;
-        if (t.next()) {
-          if (lane == 0) mbar_arrive(smem_u32(&sh.job_empty[slot]));
-          t.open(dead);
+        tc_commit(smem_u32(&sh.q_empty[qb]), on);
+        ++k;
+      }
+      // no arrival is left behind: the last step's P is read after all that was issued here
+      if (last_buf >= 0) mbar_wait(bar_f + last_buf * 8, last_use & 1, dead);
+    } else if (warp == 11) {
+      // ------------------------------------------------ outputs: O_w += P V, step by step
+      const uint32_t on = elect_one(), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
+      const uint32_t bar_p = smem_u32(sh.p_full), bar_f = smem_u32(sh.s_free), bar_o = smem_u32(sh.o_done), bar_e = smem_u32(sh.v_empty);
+      Ring vr{sv, base + X::kQ * q_bytes + a.k_stages * kTile, sh.v_full, sh.v_empty, a.v_stages};
+      int buf = 0, b0 = 0, b1 = 0, r0 = 0, r1 = 0;     // P's buffer; each group's barrier and its round
+      int last = -1, last_round = 0;
+      JobList list(sh);
+      while (const Job* j = list.get(dead)) {
+        const int n0 = j->n[0], n1 = j->n[1], n = max(n0, n1);
+        list.done(lane);
+        auto product = [&](int w, int& b, int& r, int st, bool add) {
+          mbar_wait(bar_p + (w * 3 + b) * 8, r & 1, dead);
+          tc_fence_after();
+          tile_gather(tmem + X::kOut + w * DP, tmem + buf * 128, 32, sv + st * kTile, id_o, add, on);
+          tc_commit(bar_o + w * 8, on);
+          tc_commit(bar_f + buf * 8, on);
+          if (++b == X::kS) {
+            b = 0;
+            ++r;
+          }
+          buf = buf + 1 == X::kS ? 0 : buf + 1;
+        };
+        for (int i = 0; i < n; ++i) {
+          int st = 0;
+          auto next = [&]() {
+            last_round = vr.round;
+            last = st = vr.next(dead);
+          };
+          if (!a.one) next();
+          if (i < n0) {
+            if (a.one) next();
+            product(0, b0, r0, st, i > 0);
+            if (a.one) tc_commit(bar_e + st * 8, on);
+          }
+          if (i < n1) {
+            if (a.one) next();
+            product(1, b1, r1, st, i > 0);
+            if (a.one) tc_commit(bar_e + st * 8, on);
+          }
+          if (!a.one) tc_commit(bar_e + st * 8, on);
         }
       }
       if (last >= 0) mbar_wait(bar_e + last * 8, last_round & 1, dead);   // no arrival is left behind
@@ -403,11 +399,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     const int w = warp >> 2, r = threadIdx.x & 127;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);   // this warp's 32 lanes
     const float c = d.scale * kLog2e;
-    int mine = 0, slot = 0, round = 0;         // this group's steps so far
+    int mine = 0;                              // this group's steps so far
+    JobList list(sh);
     for (int k = 0;; ++k) {
-      mbar_wait(smem_u32(&sh.job_full[slot]), round & 1, dead);
-      const Job& j = sh.job[slot];
-      if (j.n[0] < 0 || *dead) break;
+      const Job* jp = list.get(dead);
+      if (!jp) break;
+      const Job& j = *jp;
       const int n = j.n[w], n0 = j.n[0], n1 = j.n[1], buf0 = j.buf, first = j.first;
       const int m = j.m0[a.one ? 0 : w] + r;
       const bool row = m < j.rows;
@@ -575,12 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       }
       tc_fence_before();
       if (a.one) bar_sync(2, 256);                       // the other group's O has been read
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.job_empty[slot]));
-      if (++slot == kJobs) {
-        slot = 0;
-        ++round;
-      }
+      list.done(lane);
     }
   }
   tc_fence_before();
@@ -659,7 +651,9 @@ void cut(FwdArgs& a) {
   if (jobs < 4 * kSms && a.one)
     a.splits = (int)std::max<int64_t>(a.splits, std::min<int64_t>((4 * kSms + jobs - 1) / jobs, keys / 8));
   const int dp = d.D <= 64 ? 64 : 128, tile = dp / 64 * kBlockBytes, q = (dp == 64 ? 2 : 1) * (a.one ? 1 : 2);
-  a.stages = std::min(kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - q);
+  const int stages = std::min(kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - q);
+  a.k_stages = (stages + 1) / 2;       // K is needed first
+  a.v_stages = stages / 2;
   // heads whose keys and values are at work at the same time: about 32 MB of the 126 MB L2
   const int64_t head = std::max<int64_t>(1, (int64_t)d.Lk * d.D * 4);
   a.group = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)d.B * d.Hkv, (32 << 20) / head));
@@ -667,7 +661,7 @@ void cut(FwdArgs& a) {
 
 template <int DP, typename T>
 int launch(FwdArgs& a, cudaStream_t s) {
-  const int smem = 1024 + ((DP == 64 ? 2 : 1) * (a.one ? 1 : 2) + a.stages) * Cfg<DP>::kTile + (int)sizeof(Shared);
+  const int smem = 1024 + ((DP == 64 ? 2 : 1) * (a.one ? 1 : 2) + a.k_stages + a.v_stages) * Cfg<DP>::kTile + (int)sizeof(Shared);
   B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_fwd<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention"));
   const int64_t jobs = (int64_t)a.tiles * a.heads * a.splits;
   B3R_REQUIRE(jobs <= 0x3fffffff, "attention: too many rows for one call");
