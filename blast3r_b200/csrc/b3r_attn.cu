@@ -39,7 +39,7 @@ int attn_check(const b3r_attention_desc* d, bool backward) {
   return B3R_OK;
 }
 
-static int encode_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int G, int batch, int D, int dtype) {
+static int encode_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int G, int batch, int D, int dtype, int box_rows) {
   typedef CUresult (*encode_t)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -64,12 +64,12 @@ static int encode_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, 
   const int64_t row = rows > 1 ? t.row : 128, head = heads > 1 ? t.head : 128, bat = batch > 1 ? t.batch : 128;
   cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)rows, (cuuint64_t)heads, (cuuint64_t)batch};
   cuuint64_t strides[3] = {(cuuint64_t)row * 2, (cuuint64_t)head * 2, (cuuint64_t)bat * 2};
-  cuuint32_t box[4] = {64, 128, 1, 1};
+  cuuint32_t box[4] = {64, (cuuint32_t)box_rows, 1, 1};
   if (G > 0) {                         // heads before rows
     std::swap(dims[1], dims[2]);
     std::swap(strides[0], strides[1]);
     box[1] = (cuuint32_t)G;
-    box[2] = (cuuint32_t)(128 / G);
+    box[2] = (cuuint32_t)(box_rows / G);
   }
   const cuuint32_t step[4] = {1, 1, 1, 1};
   const CUresult rc = encode(map, dtype == B3R_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4,
@@ -79,11 +79,11 @@ static int encode_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, 
   return B3R_OK;
 }
 
-int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype) {
-  return encode_map(map, t, rows, heads, 0, batch, D, dtype);
+int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype, int box) {
+  return encode_map(map, t, rows, heads, 0, batch, D, dtype, box);
 }
 int attn_map_groups(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int G, int batch, int D, int dtype) {
-  return encode_map(map, t, rows, heads, G, batch, D, dtype);
+  return encode_map(map, t, rows, heads, G, batch, D, dtype, 128);
 }
 
 }  // namespace b3r

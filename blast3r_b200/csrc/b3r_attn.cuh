@@ -56,8 +56,8 @@ __device__ __forceinline__ __half t_of<__half>(float x) { return __float2half_rn
 int attn_check_sizes(const b3r_attention_desc* d);
 int attn_check(const b3r_attention_desc* d, bool backward);
 
-// The tensor map of a (D, rows, heads, batch) tensor in boxes of 64 elements x 128 rows.
-int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype);
+// The tensor map of a (D, rows, heads, batch) tensor in boxes of 64 elements x `box` rows.
+int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype, int box);
 // The same tensor as (D, heads, rows, batch), in boxes of 64 elements x G heads x 128 / G rows: row m
 // of a box is query m / G, head m % G.
 int attn_map_groups(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int G, int batch, int D, int dtype);

@@ -166,15 +166,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     for (int it = 0; it < n; ++it) {
       const int t = (first + it) * kTileRows;
       // dS is zero past the last key and meets K's rows there, so they are cleared
-      ring_load<kBlocks>(ring, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
-      ring_load<kBlocks>(ring, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks, kTileRows>(ring, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks, kTileRows>(ring, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
     }
   } else if (warp == 9 && n > 0) {
     {
       const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
       auto product = [&](uint32_t acc, uint32_t left, int stage) {   // acc = left K^T or V^T
-        tile_product<kBlocks>(acc, left, ring.data + stage * kTile, id_s, steps, on);
+        tile_product<kBlocks, kTileRows>(acc, left, ring.data + stage * kTile, id_s, steps, on);
       };
       int sk[2], sv = 0, last_round = 0;
       auto scores = [&](int it) {
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
         tc_fence_after();
         const uint32_t ds = tmem + (it & 1) * 128, k = ring.data + sk[it & 1] * kTile;
-        tile_gather(tmem + 384, ds, 64, k, id_o, it > 0, on);
+        tile_gather<kTileRows>(tmem + 384, ds, 64, k, id_o, it > 0, on);
         tc_commit(smem_u32(&sh.empty[sk[it & 1]]), on);
         if (it + 2 < n) scores(it + 2);
       }
@@ -367,8 +367,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     for (int it = 0; it < n; ++it) {
       const int u = first + it, h = kv * G + u / per_head, i0 = (t0 + u % per_head) * kTileRows;
       // P and dS are zero past the last query and meet the rows of dO and Q there
-      ring_load<kBlocks>(ring, &a.q, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
-      ring_load<kBlocks>(ring, &a.go, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks, kTileRows>(ring, &a.q, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks, kTileRows>(ring, &a.go, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
     }
     if (*dead && lane == 0) mbar_wait(smem_u32(&sh.own_full), 0, dead);
   } else if (warp == 9 && n > 0) {
@@ -376,10 +376,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
       auto product = [&](uint32_t acc, uint32_t left, int stage) {   // acc = K Q^T or V dO^T
-        tile_product<kBlocks>(acc, left, ring.data + stage * kTile, id_s, steps, on);
+        tile_product<kBlocks, kTileRows>(acc, left, ring.data + stage * kTile, id_s, steps, on);
       };
       auto gather = [&](uint32_t acc, uint32_t left, int stage, bool add) {   // acc += P^T dO or dS^T Q
-        tile_gather(acc, left, 64, ring.data + stage * kTile, id_o, add, on);
+        tile_gather<kTileRows>(acc, left, 64, ring.data + stage * kTile, id_o, add, on);
         tc_commit(smem_u32(&sh.empty[stage]), on);
       };
       mbar_wait(smem_u32(&sh.own_full), 0, dead);
@@ -632,10 +632,10 @@ extern "C" int b3r_attention_bwd(const b3r_attention_desc* d, void* stream) {
     B3R_REQUIRE(d->work && ((uintptr_t)d->work & 255) == 0, "attention backward: work buffer must be 256-byte aligned");
   const int64_t nq = d->cu_q ? d->Tq : d->Lq, nk = d->cu_q ? d->Tk : d->Lk;
   const int batch = d->cu_q ? 1 : d->B;
-  B3R_TRY(attn_map(&a.q, d->q, nq, d->Hq, batch, d->D, d->dtype));
-  B3R_TRY(attn_map(&a.go, d->d_o, nq, d->Hq, batch, d->D, d->dtype));
-  B3R_TRY(attn_map(&a.k, d->k, nk, d->Hkv, batch, d->D, d->dtype));
-  B3R_TRY(attn_map(&a.v, d->v, nk, d->Hkv, batch, d->D, d->dtype));
+  B3R_TRY(attn_map(&a.q, d->q, nq, d->Hq, batch, d->D, d->dtype, kTileRows));
+  B3R_TRY(attn_map(&a.go, d->d_o, nq, d->Hq, batch, d->D, d->dtype, kTileRows));
+  B3R_TRY(attn_map(&a.k, d->k, nk, d->Hkv, batch, d->D, d->dtype, kTileRows));
+  B3R_TRY(attn_map(&a.v, d->v, nk, d->Hkv, batch, d->D, d->dtype, kTileRows));
   cudaStream_t s = as_stream(stream);
   if (d->dtype == B3R_BF16) return d->D <= 64 ? launch<64, __nv_bfloat16>(a, s) : launch<128, __nv_bfloat16>(a, s);
   return d->D <= 64 ? launch<64, __half>(a, s) : launch<128, __half>(a, s);

@@ -3,7 +3,7 @@
 // Rows are (query, head of the group) pairs: row m of key/value head kv is query m / G with head
 // kv G + m % G, so the heads that share keys and values fill one tile and read them once.  A
 // block owns two tiles of 128 rows, or one where there are no more rows, and walks over tiles of
-// 128 keys:
+// keys:
 //   warp 8    loads Q, K and V tiles by TMA, K and V into rings of stages
 //   warp 9    issues S_w = Q_w K^T into one of the S buffers in tensor memory
 //   warp 11   issues O_w += P_w V, P_w read from tensor memory (in one warp, issuing both took longer
@@ -45,14 +45,21 @@ struct alignas(64) FwdArgs {
   float* part_l;    // [splits][B Hkv][rows]: log2 of the sum, -inf where a part sees nothing
 };
 
-// Buffers of a head size: S has three where tensor memory holds them beside O (so that a group's
-// next scores are ready when it ends the last ones), Q two where shared memory does.
+// Buffers of a head size.  Up to 64, tensor memory holds three buffers of S beside O, so that a
+// group's next scores are ready when it ends the last ones, and shared memory two of Q.  Above, S has one
+// for each group, and the next scores follow the product that reads P out of it; one warp issues
+// both, so that no barrier lies between them (3430 cycles a step of both groups against 3800).  Two
+// buffers of 64 keys instead took 4160: with its left operand in shared memory a product of N = 64
+// takes as long as one of N = 128, about 100 cycles for each 16 of the head size.
 template <int DP>
 struct Cfg {
   static constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
-  static constexpr int kS = DP == 64 ? 3 : 2, kQ = DP == 64 ? 2 : 1;
-  static constexpr int kOut = kS * 128;   // O's first column
+  static constexpr bool kOneIssuer = DP > 64;
+  static constexpr int kS = kOneIssuer ? 2 : 3, kQ = kOneIssuer ? 1 : 2;
+  static constexpr int kOut = kS * kTileRows;                              // O's first column
 };
+constexpr int kMaxS = 3;
+constexpr int kStage = 32 * 64;   // bytes of a softmax warp's rows on their way out: 32 rows of 32 columns
 
 // One job: two tiles of rows (one) of a key/value head, and a range of its keys.
 struct Job {
@@ -69,7 +76,7 @@ constexpr int kJobs = 3;   // jobs that a block has in hand at most
 // no part in a job must not meet a barrier that has turned twice since.
 struct Shared {
   uint64_t q_full[2], q_empty[2], fix, k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
-  uint64_t s_full[2][3], p_full[2][3], s_free[3], o_done[2];
+  uint64_t s_full[2][kMaxS], p_full[2][kMaxS], s_free[kMaxS], o_done[2];
   uint64_t job_full[kJobs], job_empty[kJobs], want, cancel;
   alignas(16) uint4 answer;
   Job job[kJobs];
@@ -182,7 +189,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
   const int q_tiles = a.one ? 1 : 2, q_bytes = q_tiles * kTile;
   const uint32_t sq = smem_u32(base), sk = sq + X::kQ * q_bytes, sv = sk + a.k_stages * kTile;
-  Shared& sh = *reinterpret_cast<Shared*>(base + X::kQ * q_bytes + (a.k_stages + a.v_stages) * kTile);
+  uint8_t* const stage = base + X::kQ * q_bytes + (a.k_stages + a.v_stages) * kTile;
+  Shared& sh = *reinterpret_cast<Shared*>(stage + 8 * kStage);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
   const b3r_attention_desc& d = a.d;
   if (warp == 9) tc_alloc(smem_u32(&sh.tmem), 512);
@@ -199,14 +207,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       mbar_init(smem_u32(&sh.v_full[i]), 1);
       mbar_init(smem_u32(&sh.v_empty[i]), 1);
     }
-    for (int i = 0; i < 6; ++i) {
-      mbar_init(smem_u32(&sh.s_full[i / 3][i % 3]), 1);
-      mbar_init(smem_u32(&sh.p_full[i / 3][i % 3]), 4);
+    for (int i = 0; i < kMaxS; ++i) {
+      for (int w = 0; w < 2; ++w) {
+        mbar_init(smem_u32(&sh.s_full[w][i]), 1);
+        mbar_init(smem_u32(&sh.p_full[w][i]), 4);
+      }
+      mbar_init(smem_u32(&sh.s_free[i]), 1);
     }
     for (int i = 0; i < kJobs; ++i) {
       mbar_init(smem_u32(&sh.job_full[i]), 1);
-      mbar_init(smem_u32(&sh.job_empty[i]), 11);   // loads, two warps of products, eight of softmax
-      mbar_init(smem_u32(&sh.s_free[i]), 1);
+      mbar_init(smem_u32(&sh.job_empty[i]), X::kOneIssuer ? 10 : 11);   // loads, products, eight softmax warps
     }
     mbar_init(smem_u32(&sh.want), 1);
     mbar_init(smem_u32(&sh.cancel), 1);
@@ -247,16 +257,88 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         for (int i = 0; i < tiles; ++i) {
           const int row = (j->first + i) * kTileRows;
           if (i == ask && lane == 0) mbar_arrive(smem_u32(&sh.want));   // near the job's end: the next one, not sooner
-          ring_load<X::kBlocks>(kr, &a.k, j->k0 + row, j->kv, batch, j->kl - row, false, &sh.fix, fixes, lane, dead);
+          ring_load<X::kBlocks, kTileRows>(kr, &a.k, j->k0 + row, j->kv, batch, j->kl - row, false, &sh.fix, fixes, lane, dead);
           // P is zero past the last key, so V is cleared there
-          ring_load<X::kBlocks>(vr, &a.v, j->k0 + row, j->kv, batch, j->kl - row, true, &sh.fix, fixes, lane, dead);
+          ring_load<X::kBlocks, kTileRows>(vr, &a.v, j->k0 + row, j->kv, batch, j->kl - row, true, &sh.fix, fixes, lane, dead);
         }
         list.done(lane);
         ++k;
       }
-    } else if (warp == 9) {
+    } else if (X::kOneIssuer && warp == 9) {
+      // ------------------------------------------------ scores and outputs, S_w = Q_w K^T after O_w += P_w V
+      const uint32_t on = elect_one();
+      const uint32_t id_s = mma_idesc(kBf, 128, kTileRows, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
+      const int steps = (d.D + 15) / 16;
+      const uint32_t bar_s = smem_u32(sh.s_full), bar_p = smem_u32(sh.p_full), bar_o = smem_u32(sh.o_done);
+      const uint32_t bar_k = smem_u32(sh.k_empty), bar_v = smem_u32(sh.v_empty);
+      Ring kr{sk, base + X::kQ * q_bytes, sh.k_full, sh.k_empty, a.k_stages};
+      Ring vr{sv, base + X::kQ * q_bytes + a.k_stages * kTile, sh.v_full, sh.v_empty, a.v_stages};
+      int k = 0, hs0 = 0, hs1 = 0, ts0 = 0, ts1 = 0;   // jobs; each group's steps whose S, and O, has been issued
+      int last = -1, last_round = 0;
+      JobList list(sh);
+      while (const Job* j = list.get(dead)) {
+        const int n0 = j->n[0], n1 = j->n[1], n = max(n0, n1);
+        list.done(lane);
+        mbar_wait(smem_u32(&sh.q_full[0]), k & 1, dead);
+        auto scores = [&](int w, int& hs, int st) {
+          tc_fence_after();
+          tile_product<X::kBlocks, kTileRows>(tmem + w * kTileRows, sq + (a.one ? 0 : w) * kTile, sk + st * kTile, id_s, steps, on);
+          tc_commit(bar_s + (w * kMaxS + (hs & 1)) * 8, on);
+          ++hs;
+        };
+        auto output = [&](int w, int& ts, int st, bool add) {
+          mbar_wait(bar_p + (w * kMaxS + (ts & 1)) * 8, (ts >> 1) & 1, dead);
+          tc_fence_after();
+          tile_gather<kTileRows>(tmem + X::kOut + w * DP, tmem + w * kTileRows, 32, sv + st * kTile, id_o, add, on);
+          tc_commit(bar_o + w * 8, on);
+          ++ts;
+        };
+        auto next_v = [&]() {
+          last_round = vr.round;
+          return last = vr.next(dead);
+        };
+        int st = 0, sw = 0;
+        if (!a.one) st = kr.next(dead);
+        if (n0 > 0) {
+          if (a.one) st = kr.next(dead);
+          scores(0, hs0, st);
+          if (a.one) tc_commit(bar_k + st * 8, on);
+        }
+        if (n1 > 0) {
+          if (a.one) st = kr.next(dead);
+          scores(1, hs1, st);
+          if (a.one) tc_commit(bar_k + st * 8, on);
+        }
+        if (!a.one) tc_commit(bar_k + st * 8, on);
+        for (int i = 0; i < n; ++i) {
+          if (!a.one) {
+            sw = next_v();
+            if (i + 1 < n) st = kr.next(dead);
+          }
+          auto group = [&](int w, int nw, int& hs, int& ts) {
+            if (i >= nw) return;
+            if (a.one) sw = next_v();
+            output(w, ts, sw, i > 0);
+            if (a.one) tc_commit(bar_v + sw * 8, on);
+            if (i + 1 >= nw) return;
+            if (a.one) st = kr.next(dead);
+            scores(w, hs, st);
+            if (a.one) tc_commit(bar_k + st * 8, on);
+          };
+          group(0, n0, hs0, ts0);
+          group(1, n1, hs1, ts1);
+          if (!a.one) {
+            if (i + 1 < n) tc_commit(bar_k + st * 8, on);
+            tc_commit(bar_v + sw * 8, on);
+          }
+          if (i + 2 == n || n == 1) tc_commit(smem_u32(&sh.q_empty[0]), on);   // the last scores are on their way
+        }
+        ++k;
+      }
+      if (last >= 0) mbar_wait(bar_v + last * 8, last_round & 1, dead);   // no arrival is left behind
+    } else if (!X::kOneIssuer && warp == 9) {
       // ------------------------------------------------ scores: S = Q_w K^T, step by step
-      const uint32_t on = elect_one(), id_s = mma_idesc(kBf, 128, 128, false);
+      const uint32_t on = elect_one(), id_s = mma_idesc(kBf, 128, kTileRows, false);
       const int steps = (d.D + 15) / 16;
       const uint32_t bar_s = smem_u32(sh.s_full), bar_f = smem_u32(sh.s_free), bar_e = smem_u32(sh.k_empty);
       Ring kr{sk, base + X::kQ * q_bytes, sh.k_full, sh.k_empty, a.k_stages};
@@ -271,8 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         auto product = [&](uint32_t q, int w, int& b, int st) {
           if (uses > 0) mbar_wait(bar_f + buf * 8, (uses - 1) & 1, dead);   // until P has been read from it
           tc_fence_after();
-          tile_product<X::kBlocks>(tmem + buf * 128, q, sk + st * kTile, id_s, steps, on);
-          tc_commit(bar_s + (w * 3 + b) * 8, on);
+          tile_product<X::kBlocks, kTileRows>(tmem + buf * kTileRows, q, sk + st * kTile, id_s, steps, on);
+          tc_commit(bar_s + (w * kMaxS + b) * 8, on);
           b = b + 1 == X::kS ? 0 : b + 1;
           last_buf = buf;
           last_use = uses;
@@ -301,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       }
       // no arrival is left behind: the last step's P is read after all that was issued here
       if (last_buf >= 0) mbar_wait(bar_f + last_buf * 8, last_use & 1, dead);
-    } else if (warp == 11) {
+    } else if (!X::kOneIssuer && warp == 11) {
       // ------------------------------------------------ outputs: O_w += P V, step by step
       const uint32_t on = elect_one(), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
       const uint32_t bar_p = smem_u32(sh.p_full), bar_f = smem_u32(sh.s_free), bar_o = smem_u32(sh.o_done), bar_e = smem_u32(sh.v_empty);
@@ -313,9 +395,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         const int n0 = j->n[0], n1 = j->n[1], n = max(n0, n1);
         list.done(lane);
         auto product = [&](int w, int& b, int& r, int st, bool add) {
-          mbar_wait(bar_p + (w * 3 + b) * 8, r & 1, dead);
+          mbar_wait(bar_p + (w * kMaxS + b) * 8, r & 1, dead);
           tc_fence_after();
-          tile_gather(tmem + X::kOut + w * DP, tmem + buf * 128, 32, sv + st * kTile, id_o, add, on);
+          tile_gather<kTileRows>(tmem + X::kOut + w * DP, tmem + buf * kTileRows, 32, sv + st * kTile, id_o, add, on);
           tc_commit(bar_o + w * 8, on);
           tc_commit(bar_f + buf * 8, on);
           if (++b == X::kS) {
@@ -433,23 +515,23 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       for (int it = 0; it < n; ++it, ++mine) {
         // the step's place among all steps of the block gives its buffer
         const int g = buf0 + min(it, n0) + min(it, n1) + (w && it < n0), bar = mine % X::kS;
-        const uint32_t at = quarter + g % X::kS * 128;
+        const uint32_t at = quarter + (X::kOneIssuer ? w : g % X::kS) * kTileRows;
         const int lim = bound - (first + (a.one ? 2 * it + w : it)) * kTileRows;   // keys of this tile that the row sees
         mbar_wait(smem_u32(&sh.s_full[w][bar]), (mine / X::kS) & 1, dead);
         tc_fence_after();
-        uint32_t s[128];
+        uint32_t s[kTileRows];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) tc_ld32(at + q * 32, s + q * 32);
+        for (int q = 0; q < kTileRows; q += 32) tc_ld32(at + q, s + q);
         tc_wait_ld(s);
         if (!__all_sync(0xffffffffu, lim >= kTileRows)) {
 #pragma unroll
-          for (int q = 0; q < 128; ++q) s[q] = q < lim ? s[q] : 0xff800000u;
+          for (int q = 0; q < kTileRows; ++q) s[q] = q < lim ? s[q] : 0xff800000u;
         }
         float t[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[4 + e]));
 #pragma unroll
-        for (int q = 8; q < 128; q += 8)
+        for (int q = 8; q < kTileRows; q += 8)
 #pragma unroll
           for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(t[e], __uint_as_float(s[q + e])), __uint_as_float(s[q + 4 + e]));
         const float top = fmaxf(mx, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c);
@@ -473,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         const float2 cc = make_float2(c, c), mm = make_float2(mx == -INFINITY ? 0.f : -mx, mx == -INFINITY ? 0.f : -mx);
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-        for (int q0 = 0; q0 < 64; q0 += 16) {
+        for (int q0 = 0; q0 < kTileRows / 2; q0 += 16) {
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
@@ -494,6 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         sum[0] = __fadd2_rn(sum[0], sum[1]);
         l += sum[0].x + sum[0].y;
       }
+      const RowOut<T> to(a, j, row ? m : 0);
       if (n > 0) {
         mbar_wait(smem_u32(&sh.o_done[w]), (mine - 1) & 1, dead);
         tc_fence_after();
@@ -524,7 +607,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       }
       if (w == 0 || !a.one) {
         const bool has0 = n > 0, has1 = a.one && n1 > 0;
-        const RowOut<T> to(a, j, row ? m : 0);
         if (*dead) f0 = f1 = lg = __int_as_float(0x7fffffff);
 #pragma unroll
         for (int q = 0; q < DP; q += 32) {
@@ -548,22 +630,29 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
           if (lg == -INFINITY)                           // a row that sees nothing
 #pragma unroll
             for (int e = 0; e < 32; ++e) v[e] = 0.f;
-          if (row) {
-            if (a.splits > 1) {
-              float* out = to.part_o + q;
+          if (a.splits > 1) {
+            if (row)
 #pragma unroll
               for (int e = 0; e < 32; e += 4)
-                if (q + e < d.D) *reinterpret_cast<float4*>(out + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-            } else {
-              T* out = to.o + q;
+                if (q + e < d.D) *reinterpret_cast<float4*>(to.part_o + q + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+          } else {
+            // through shared memory, so that four lanes write the 64 bytes of a row (a lane to a row took
+            // 2500 to 4000 cycles a job); chunk c of row x lies at c ^ (x / 2 % 4), out of banks' way
+            uint4* const box = reinterpret_cast<uint4*>(stage + warp * kStage);
+            __syncwarp();
 #pragma unroll
-              for (int e = 0; e < 32; e += 8)
-                if (q + e < d.D)
-                  *reinterpret_cast<uint4*>(out + e) = make_uint4(pack2(v[e], v[e + 1], T()), pack2(v[e + 2], v[e + 3], T()),
-                                                                  pack2(v[e + 4], v[e + 5], T()), pack2(v[e + 6], v[e + 7], T()));
+            for (int e = 0; e < 4; ++e)
+              box[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(pack2(v[8 * e], v[8 * e + 1], T()), pack2(v[8 * e + 2], v[8 * e + 3], T()),
+                                                                   pack2(v[8 * e + 4], v[8 * e + 5], T()), pack2(v[8 * e + 6], v[8 * e + 7], T()));
+            __syncwarp();
+#pragma unroll
+            for (int x = 0; x < 32; x += 8) {
+              const int y = x + (lane >> 2), c = lane & 3;
+              T* const out = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, row ? reinterpret_cast<uint64_t>(to.o) : 0, y));
+              const uint4 z = box[y * 4 + (c ^ ((y >> 1) & 3))];
+              if (out && q + c * 8 < d.D) *reinterpret_cast<uint4*>(out + q + c * 8) = z;
             }
           }
-          __syncwarp();
         }
         if (row) {
           if (a.splits > 1) *to.part_l = lg;
@@ -650,8 +739,10 @@ void cut(FwdArgs& a) {
   if (jobs < kSms) a.splits = (int)std::max<int64_t>(1, std::min<int64_t>(kSms / jobs, keys / 2));
   if (jobs < 4 * kSms && a.one)
     a.splits = (int)std::max<int64_t>(a.splits, std::min<int64_t>((4 * kSms + jobs - 1) / jobs, keys / 8));
-  const int dp = d.D <= 64 ? 64 : 128, tile = dp / 64 * kBlockBytes, q = (dp == 64 ? 2 : 1) * (a.one ? 1 : 2);
-  const int stages = std::min(kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - q);
+  const int fixed = 1024 + 8 * kStage + (int)sizeof(Shared), q_tiles = a.one ? 1 : 2;
+  const int room = d.D <= 64 ? (232448 - fixed) / Cfg<64>::kTile - Cfg<64>::kQ * q_tiles
+                             : (232448 - fixed) / Cfg<128>::kTile - Cfg<128>::kQ * q_tiles;
+  const int stages = std::min(2 * kMaxStages, room);
   a.k_stages = (stages + 1) / 2;       // K is needed first
   a.v_stages = stages / 2;
   // heads whose keys and values are at work at the same time: about 32 MB of the 126 MB L2
@@ -661,7 +752,8 @@ void cut(FwdArgs& a) {
 
 template <int DP, typename T>
 int launch(FwdArgs& a, cudaStream_t s) {
-  const int smem = 1024 + ((DP == 64 ? 2 : 1) * (a.one ? 1 : 2) + a.k_stages + a.v_stages) * Cfg<DP>::kTile + (int)sizeof(Shared);
+  const int smem = 1024 + Cfg<DP>::kQ * (a.one ? 1 : 2) * Cfg<DP>::kTile + (a.k_stages + a.v_stages) * Cfg<DP>::kTile + 8 * kStage +
+                   (int)sizeof(Shared);
   B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_fwd<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention"));
   const int64_t jobs = (int64_t)a.tiles * a.heads * a.splits;
   B3R_REQUIRE(jobs <= 0x3fffffff, "attention: too many rows for one call");
@@ -702,8 +794,8 @@ extern "C" int b3r_attention_fwd(const b3r_attention_desc* d, void* stream) {
     a.part_o = reinterpret_cast<float*>(d->work);
     a.part_l = a.part_o + part_rows(a) * d->D;
   }
-  B3R_TRY(attn_map(&a.k, d->k, d->cu_q ? d->Tk : d->Lk, d->Hkv, d->cu_q ? 1 : d->B, d->D, d->dtype));
-  B3R_TRY(attn_map(&a.v, d->v, d->cu_q ? d->Tk : d->Lk, d->Hkv, d->cu_q ? 1 : d->B, d->D, d->dtype));
+  B3R_TRY(attn_map(&a.k, d->k, d->cu_q ? d->Tk : d->Lk, d->Hkv, d->cu_q ? 1 : d->B, d->D, d->dtype, kTileRows));
+  B3R_TRY(attn_map(&a.v, d->v, d->cu_q ? d->Tk : d->Lk, d->Hkv, d->cu_q ? 1 : d->B, d->D, d->dtype, kTileRows));
   const int G = d->Hq / d->Hkv;
   a.q_tma = kTileRows % G == 0;
   if (a.q_tma)

@@ -3,7 +3,7 @@
 //
 // Tiles in shared memory are rows of 64 16-bit elements (128 bytes) in the 128-byte swizzle that
 // TMA writes: the 16-byte chunk c of row r lies at chunk c ^ (r & 7).  A tile of 128 rows
-// and a head size above 64 is two such blocks, 16 KB apart.
+// and a head size above 64 is two such blocks, one after the other; so are tiles of 64 rows.
 #pragma once
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -48,7 +48,7 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatil
   *dead = 1;
 }
 
-// ---- TMA: one box of 64 elements x 128 rows of a (D, rows, heads, batch) tensor
+// ---- TMA: one box of 64 elements x some rows of a (D, rows, heads, batch) tensor
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int d0, int row, int head, int batch, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
@@ -109,9 +109,9 @@ __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(1) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 // mn-major: the product runs along the rows (8-row groups 1024 bytes apart); blocks of 64
-// elements of the other dimension lie kBlockBytes apart.
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(kBlockBytes >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+// elements of the other dimension lie `block` bytes apart.
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr, int block) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(block >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(2) << 61);
 }
 // Instruction descriptor: float32 accumulator, both operands bf16 or both f16.
@@ -120,22 +120,24 @@ __host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int M, int N, bool b
          ((uint32_t)(M >> 4) << 24);
 }
 
-// tile_product: acc = A B^T over the head size, both k-major tiles, in `steps` steps of 16.
-// tile_gather: acc (+)= A B over the 128 rows of tile b; A in tensor memory, steps 0-3 from `a`, 4-7
-// from `a + half`.  Offsets within a tile only change the descriptors' address field (units of 16 bytes).
-template <int BLOCKS>
+// tile_product: acc = A B^T over the head size in `steps` steps of 16; A has 128 rows, B has ROWS, both k-major.
+// tile_gather: acc (+)= A B over the ROWS rows of tile b; A in tensor memory, its first 64 rows' steps
+// from `a`, the others' from `a + half`.  Offsets within a tile only change the descriptors' address field
+// (units of 16 bytes).
+template <int BLOCKS, int ROWS>
 __device__ __forceinline__ void tile_product(uint32_t acc, uint32_t a, uint32_t b, uint32_t idesc, int steps, uint32_t on) {
   const uint64_t da = desc_k(a), db = desc_k(b);
 #pragma unroll
-  for (int t = 0; t < BLOCKS * 4; ++t) {
-    const uint32_t off = ((t >> 2) * kBlockBytes + (t & 3) * 32) >> 4;
-    if (t < steps) tc_mma(acc, da + off, db + off, idesc, t > 0, on);
-  }
+  for (int t = 0; t < BLOCKS * 4; ++t)
+    if (t < steps)
+      tc_mma(acc, da + (((t >> 2) * kBlockBytes + (t & 3) * 32) >> 4), db + (((t >> 2) * ROWS * 128 + (t & 3) * 32) >> 4), idesc, t > 0,
+             on);
 }
+template <int ROWS>
 __device__ __forceinline__ void tile_gather(uint32_t acc, uint32_t a, int half, uint32_t b, uint32_t idesc, bool add, uint32_t on) {
-  const uint64_t db = desc_mn(b);
+  const uint64_t db = desc_mn(b, ROWS * 128);
 #pragma unroll
-  for (int t = 0; t < 8; ++t) tc_mma_ts(acc, a + (t >> 2) * half + (t & 3) * 8, db + (t * 2048 >> 4), idesc, add || t > 0, on);
+  for (int t = 0; t < ROWS / 16; ++t) tc_mma_ts(acc, a + (t >> 2) * half + (t & 3) * 8, db + (t * 2048 >> 4), idesc, add || t > 0, on);
 }
 
 #define B3R_R4(a, i) "=r"(a[i]), "=r"(a[i + 1]), "=r"(a[i + 2]), "=r"(a[i + 3])
@@ -192,7 +194,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
 }
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
-// ---- a ring of shared-memory stages, each one tile of 128 rows, filled by one warp
+// ---- a ring of shared-memory stages, each one tile of rows, filled by one warp
 struct Ring {
   uint32_t data;              // shared address of stage 0
   uint8_t* data_ptr;          // the same, as a pointer
@@ -215,28 +217,29 @@ struct Ring {
   }
 };
 
-// Producer (a whole warp): the next stage gets rows [row, row + 128) of a head.  Only `valid` of
+// Producer (a whole warp): the next stage gets rows [row, row + ROWS) of a head.  Only `valid` of
 // them belong to the sequence; the others are the neighbours' or padding, and may hold NaN.  They
 // are cleared where `clear`: where they meet zeros in a product along the rows.
-template <int BLOCKS>
+template <int BLOCKS, int ROWS>
 __device__ __forceinline__ void ring_load(Ring& g, const CUtensorMap* map, int row, int head, int batch, int valid, bool clear,
                                           uint64_t* fix, int& fixes, int lane, volatile int* dead) {
   const uint32_t full = smem_u32(g.full + g.stage), bar_fix = smem_u32(fix);
-  const int at = g.stage * BLOCKS * kBlockBytes;
-  const bool cut = clear && valid < kTileRows;
+  constexpr int kBytes = ROWS * 128;
+  const int at = g.stage * BLOCKS * kBytes;
+  const bool cut = clear && valid < ROWS;
   if (g.round > 0) mbar_wait(smem_u32(g.empty + g.stage), (g.round - 1) & 1, dead);
   if (lane == 0) {
     const uint32_t bar = cut ? bar_fix : full;
-    mbar_expect(bar, BLOCKS * kBlockBytes);
+    mbar_expect(bar, BLOCKS * kBytes);
 #pragma unroll
-    for (int c = 0; c < BLOCKS; ++c) tma_box(g.data + at + c * kBlockBytes, map, c * 64, row, head, batch, bar);
+    for (int c = 0; c < BLOCKS; ++c) tma_box(g.data + at + c * kBytes, map, c * 64, row, head, batch, bar);
   }
   if (cut) {
     mbar_wait(bar_fix, fixes & 1, dead);
     ++fixes;
-    for (int i = max(valid, 0) * 8 + lane; i < kTileRows * 8; i += 32)
+    for (int i = max(valid, 0) * 8 + lane; i < ROWS * 8; i += 32)
 #pragma unroll
-      for (int c = 0; c < BLOCKS; ++c) *reinterpret_cast<uint4*>(g.data_ptr + at + c * kBlockBytes + i * 16) = make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < BLOCKS; ++c) *reinterpret_cast<uint4*>(g.data_ptr + at + c * kBytes + i * 16) = make_uint4(0, 0, 0, 0);
     fence_async();
     __syncwarp();
     if (lane == 0) mbar_arrive(full);
