@@ -21,7 +21,11 @@ namespace b3r {
 namespace {
 
 constexpr int kThreads = 384;
-constexpr int kMaxStages = 8;
+constexpr int kMaxStages = 4;   // of each ring
+// an elementwise thread holds 64 columns of P and of dP: registers move over from the third warpgroup
+// (256 x 208 + 128 x 88 = 384 x 168, what the block was launched with)
+__device__ __forceinline__ void few_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 88;"); }
+__device__ __forceinline__ void many_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 208;"); }
 
 // P^T is rounded to the operands' type for dv.  In float16 the small probabilities of long rows
 // would be subnormal, so P is carried 2^11 times as large (P <= 1); the factor is taken out of dS in
@@ -36,19 +40,20 @@ struct alignas(64) BwdArgs {
   b3r_attention_desc d;
   int q_tiles, k_tiles;       // row tiles of a key/value head's queries, and key tiles, of the longest sequence
   int q_splits, k_splits;     // blocks along the keys for dq, along the queries for dk and dv
-  int stages, group;
+  int k_stages, v_stages, group;   // (k_attn_dkv: of Q, of dO)
+  int G;
   float* delta;               // [B][Hq][Lq]
   float* part_q;              // [q_splits][B Hkv][rows][D]
   float* part_k;              // [k_splits][2][B Hkv][Lk][D]: dk, dv
 };
 
 struct Shared {
-  uint64_t fix, own_full, full[kMaxStages], empty[kMaxStages], s_full[2], dp_full, dp_read, p_full, ds_full, done;
+  uint64_t fix, own_full, full[2][kMaxStages], empty[2][kMaxStages], s_full[2], dp_full, dp_read, p_full, ds_full, done;
   uint64_t st_full[2], st_empty[2];
   uint32_t tmem;
   int dead;
   float delta[kTileRows];
-  float stat[2][2][kTileRows];   // k_attn_dkv: per stage, lse (log2) and delta of 128 queries
+  alignas(16) float stat[2][2][kTileRows];   // k_attn_dkv: per stage, -lse (log2) and -delta of 128 queries
 };
 
 // Which head and tile a block works on: heads in groups whose tensors fit L2; `heavy_first`
@@ -59,13 +64,14 @@ __device__ __forceinline__ void place(int id, int tiles, int group, int heads, b
   tile = last_first ? tiles - 1 - r / width : r / width;
 }
 
-__device__ __forceinline__ void init_shared(Shared& sh, int stages, int own) {
+__device__ __forceinline__ void init_shared(Shared& sh, int own) {
   mbar_init(smem_u32(&sh.fix), 1);
   mbar_init(smem_u32(&sh.own_full), own);
-  for (int i = 0; i < stages; ++i) {
-    mbar_init(smem_u32(&sh.full[i]), 1);
-    mbar_init(smem_u32(&sh.empty[i]), 1);
-  }
+  for (int i = 0; i < kMaxStages; ++i)
+    for (int k = 0; k < 2; ++k) {
+      mbar_init(smem_u32(&sh.full[k][i]), 1);
+      mbar_init(smem_u32(&sh.empty[k][i]), 1);
+    }
   for (int i = 0; i < 2; ++i) {
     mbar_init(smem_u32(&sh.s_full[i]), 1);
     mbar_init(smem_u32(&sh.st_full[i]), 1);
@@ -94,31 +100,40 @@ __device__ __forceinline__ void finish(Shared& sh, int32_t* status, int warp, bo
   }
 }
 
-// 32 columns of an accumulator, times f, to a row of 16-bit values or of float32 parts.
+// A warp's 32 rows of 32 columns of an accumulator, times f: to rows of 16-bit values through the warp's
+// 2 KB of shared memory (four lanes write the 64 bytes of a row; chunk c of row x lies at c ^ (x / 2 % 4)),
+// or to rows of float32 parts.  `row`: whether this thread's row is written at all.
 template <typename T>
-__device__ __forceinline__ void write32(uint32_t tmem, bool has, float f, T* out, float* part, int D, int c0, bool row) {
+__device__ __forceinline__ void write32(uint32_t tmem, bool has, float f, T* out, float* part, int D, int c0, bool row, uint8_t* box_) {
+  const int lane = threadIdx.x & 31;
+  uint32_t o[32];
   float v[32];
   if (has) {
-    uint32_t o[32];
     tc_ld32(tmem, o);
     tc_wait_ld(o);
-#pragma unroll
-    for (int e = 0; e < 32; ++e) v[e] = __uint_as_float(o[e]) * f;
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) v[e] = 0.f;
   }
-  if (!row) return;
+#pragma unroll
+  for (int e = 0; e < 32; ++e) v[e] = has ? __uint_as_float(o[e]) * f : 0.f;
   if (part) {
+    if (row)
 #pragma unroll
-    for (int e = 0; e < 32; e += 4)
-      if (c0 + e < D) *reinterpret_cast<float4*>(part + c0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-  } else {
+      for (int e = 0; e < 32; e += 4)
+        if (c0 + e < D) *reinterpret_cast<float4*>(part + c0 + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    return;
+  }
+  uint4* const box = reinterpret_cast<uint4*>(box_);
+  __syncwarp();
 #pragma unroll
-    for (int e = 0; e < 32; e += 8)
-      if (c0 + e < D)
-        *reinterpret_cast<uint4*>(out + c0 + e) = make_uint4(pack2(v[e], v[e + 1], T()), pack2(v[e + 2], v[e + 3], T()),
-                                                             pack2(v[e + 4], v[e + 5], T()), pack2(v[e + 6], v[e + 7], T()));
+  for (int e = 0; e < 4; ++e)
+    box[lane * 4 + (e ^ ((lane >> 1) & 3))] = make_uint4(pack2(v[8 * e], v[8 * e + 1], T()), pack2(v[8 * e + 2], v[8 * e + 3], T()),
+                                                         pack2(v[8 * e + 4], v[8 * e + 5], T()), pack2(v[8 * e + 6], v[8 * e + 7], T()));
+  __syncwarp();
+#pragma unroll
+  for (int x = 0; x < 32; x += 8) {
+    const int y = x + (lane >> 2), c = lane & 3;
+    T* const to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, row ? reinterpret_cast<uint64_t>(out) : 0, y));
+    const uint4 z = box[y * 4 + (c ^ ((y >> 1) & 3))];
+    if (to && c0 + c * 8 < D) *reinterpret_cast<uint4*>(to + c0 + c * 8) = z;
   }
 }
 
@@ -132,10 +147,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
   constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
   const uint32_t sq = smem_u32(base), sgo = sq + kTile;
-  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.stages) * kTile);
+  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.k_stages + a.v_stages) * kTile);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
   const b3r_attention_desc& d = a.d;
-  const int G = d.Hq / d.Hkv, split = blockIdx.x % a.q_splits;
+  const int G = a.G, split = blockIdx.x % a.q_splits;
   int head, tile;
   place(blockIdx.x / a.q_splits, a.q_tiles, a.group, d.B * d.Hkv, true, head, tile);
   const int b = head / d.Hkv, kv = head % d.Hkv;
@@ -150,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     first = split * per;
     n = min(max(all - first, 0), per);
   }
-  if (threadIdx.x == 0) init_shared(sh, a.stages, 8);
+  if (threadIdx.x == 0) init_shared(sh, 8);
   if (warp == 9 && n > 0) tc_alloc(smem_u32(&sh.tmem), 512);
   tc_fence_before();
   __syncthreads();
@@ -158,93 +173,103 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   volatile int* dead = &sh.dead;
   const int steps = (d.D + 15) / 16;
-  Ring ring{sq + 2 * kTile, base + 2 * kTile, sh.full, sh.empty, a.stages};
+  Ring kr{sq + 2 * kTile, base + 2 * kTile, sh.full[0], sh.empty[0], a.k_stages};
+  Ring vr{sq + (2 + a.k_stages) * kTile, base + (2 + a.k_stages) * kTile, sh.full[1], sh.empty[1], a.v_stages};
 
-  if (warp == 8 && n > 0) {
+  if (warp >= 8) {
+    few_registers();
+    if (warp == 8 && n > 0) {
     int fixes = 0;
     const int batch = d.cu_k ? 0 : b;
     for (int it = 0; it < n; ++it) {
       const int t = (first + it) * kTileRows;
       // dS is zero past the last key and meets K's rows there, so they are cleared
-      ring_load<kBlocks, kTileRows>(ring, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
-      ring_load<kBlocks, kTileRows>(ring, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks, kTileRows>(kr, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks, kTileRows>(vr, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
     }
   } else if (warp == 9 && n > 0) {
     {
       const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
-      auto product = [&](uint32_t acc, uint32_t left, int stage) {   // acc = left K^T or V^T
-        tile_product<kBlocks, kTileRows>(acc, left, ring.data + stage * kTile, id_s, steps, on);
+      auto product = [&](uint32_t acc, uint32_t left, uint32_t right) {   // acc = left K^T or V^T
+        tile_product<kBlocks, kTileRows>(acc, left, right, id_s, steps, on);
       };
-      int sk[2], sv = 0, last_round = 0;
+      int k_now = 0, k_next = 0, sv = 0, last_round = 0;
       auto scores = [&](int it) {
-        sk[it & 1] = ring.next(dead);
+        k_next = kr.next(dead);
         tc_fence_after();
-        product(tmem + (it & 1) * 128, sq, sk[it & 1]);
+        product(tmem + (it & 1) * 128, sq, kr.data + k_next * kTile);
         tc_commit(smem_u32(&sh.s_full[it & 1]), on);
       };
       auto grads = [&]() {
-        last_round = ring.round;
-        sv = ring.next(dead);
+        last_round = vr.round;
+        sv = vr.next(dead);
         tc_fence_after();
-        product(tmem + 256, sgo, sv);
+        product(tmem + 256, sgo, vr.data + sv * kTile);
         tc_commit(smem_u32(&sh.dp_full), on);
-        tc_commit(smem_u32(&sh.empty[sv]), on);
+        tc_commit(smem_u32(&sh.empty[1][sv]), on);
       };
       mbar_wait(smem_u32(&sh.own_full), 0, dead);
       tc_fence_after();
       scores(0);
       grads();
-      if (n > 1) scores(1);
       for (int it = 0; it < n; ++it) {
+        k_now = k_next;
         if (it + 1 < n) {
+          scores(it + 1);
           mbar_wait(smem_u32(&sh.dp_read), it & 1, dead);
           tc_fence_after();
           grads();
         }
         mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
         tc_fence_after();
-        const uint32_t ds = tmem + (it & 1) * 128, k = ring.data + sk[it & 1] * kTile;
-        tile_gather<kTileRows>(tmem + 384, ds, 64, k, id_o, it > 0, on);
-        tc_commit(smem_u32(&sh.empty[sk[it & 1]]), on);
-        if (it + 2 < n) scores(it + 2);
+        tile_gather<kTileRows>(tmem + 384, tmem + (it & 1) * 128, 64, kr.data + k_now * kTile, id_o, it > 0, on);
+        tc_commit(smem_u32(&sh.empty[0][k_now]), on);
       }
       tc_commit(smem_u32(&sh.done), on);
-      mbar_wait(smem_u32(&sh.empty[sv]), last_round & 1, dead);      // no arrival is left behind
+      mbar_wait(smem_u32(&sh.empty[1][sv]), last_round & 1, dead);   // no arrival is left behind
       mbar_wait(smem_u32(&sh.done), 0, dead);
     }
-  } else if (warp < 8) {
+    }
+  } else {
+    many_registers();
     const int w = warp >> 2, r = threadIdx.x & 127, m = m0 + r;
     const int i = m / G, h = kv * G + m % G;
     const bool row = m < rows, live = row && i < s.ql;
     const int bound = live ? attn_bound(s, i, d.causal) : 0;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);
-    // one group brings the rows of Q, the other those of dO and, with O, delta
+    // One group brings the rows of Q, the other those of dO and, with O, delta: a warp brings its 32 rows,
+    // DP / 8 lanes to a row, so that whole lines are read (a lane to a row took 4000 to 17000 cycles).
     {
-      const int64_t qr = s.q0 + (live ? i : 0);
-      const int qh = live ? h : kv * G;
-      const uint4* src = reinterpret_cast<const uint4*>(attn_row<const T>(w ? d.d_o : d.q, b, qr, qh));
-      const uint4* out = reinterpret_cast<const uint4*>(attn_row<const T>(d.o, b, qr, qh));
-      uint8_t* dst = base + w * kTile + r * 128;
-      float dot = 0.f;
-#pragma unroll
-      for (int cb = 0; cb < DP / 8; ++cb) {
-        const bool in = live && cb * 8 < d.D;
-        const uint4 x = in ? src[cb] : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(dst + (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4)) = x;
-        if (w && in) {
-          const uint4 y = out[cb];
-          const T* xe = reinterpret_cast<const T*>(&x);
-          const T* ye = reinterpret_cast<const T*>(&y);
+      constexpr int kLanes = DP / 8, kRows = 32 / kLanes;
+      const int c = lane % kLanes, m1 = m0 + (warp & 3) * 32;
+      const bool in = c * 8 < d.D;
+#pragma unroll 4
+      for (int x = 0; x < 32; x += kRows) {
+        const int y = x + lane / kLanes, my = m1 + y;
+        const int iy = my / G, hy = kv * G + my - iy * G;
+        const bool ok = in && my < rows && iy < s.ql;
+        const int64_t qr = s.q0 + (ok ? iy : 0);
+        const int qh = ok ? hy : kv * G;
+        const uint4 v = ok ? reinterpret_cast<const uint4*>(attn_row<const T>(w ? d.d_o : d.q, b, qr, qh))[c] : make_uint4(0, 0, 0, 0);
+        const int ry = (warp & 3) * 32 + y;
+        *reinterpret_cast<uint4*>(base + w * kTile + (c >> 3) * kBlockBytes + ry * 128 + (((c & 7) ^ (ry & 7)) << 4)) = v;
+        if (w) {
+          const uint4 o = ok ? reinterpret_cast<const uint4*>(attn_row<const T>(d.o, b, qr, qh))[c] : make_uint4(0, 0, 0, 0);
+          const T* xe = reinterpret_cast<const T*>(&v);
+          const T* ye = reinterpret_cast<const T*>(&o);
+          float dot = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) dot += f_of(xe[e]) * f_of(ye[e]);
+#pragma unroll
+          for (int t = kLanes / 2; t > 0; t >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, t);
+          if (c == 0) {
+            sh.delta[ry] = dot;
+            if (ok && split == 0) a.delta[((int64_t)b * d.Hq + hy) * d.Lq + iy] = dot;
+          }
         }
       }
       fence_async();
-      if (w) {
-        sh.delta[r] = dot;
-        if (live && split == 0) a.delta[((int64_t)b * d.Hq + h) * d.Lq + i] = dot;
-      }
       __syncwarp();
       if (n > 0 && lane == 0) mbar_arrive(smem_u32(&sh.own_full));
       bar_sync(1, 256);
@@ -306,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
 #pragma unroll
     for (int q = 0; q < DP / 2; q += 32) {
       const int c0 = w * (DP / 2) + q;
-      if (c0 < d.D) write32<T>(quarter + 384 + c0, n > 0, f, out, part, d.D, c0, row);
+      if (c0 < d.D) write32<T>(quarter + 384 + c0, n > 0, f, out, part, d.D, c0, row, base + 2 * kTile + warp * 2048);   // (the rings are idle)
     }
   }
   finish(sh, d.status, warp, n > 0);
@@ -323,10 +348,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
   const uint32_t sk = smem_u32(base), sv = sk + kTile;
-  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.stages) * kTile);
+  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.k_stages + a.v_stages) * kTile);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
   const b3r_attention_desc& d = a.d;
-  const int G = d.Hq / d.Hkv, split = blockIdx.x % a.k_splits;
+  const int G = a.G, split = blockIdx.x % a.k_splits;
   int head, tile;
   place(blockIdx.x / a.k_splits, a.k_tiles, a.group, d.B * d.Hkv, false, head, tile);
   const int b = head / d.Hkv, kv = head % d.Hkv;
@@ -342,7 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     first = split * per;
     n = min(max(all - first, 0), per);
   }
-  if (threadIdx.x == 0) init_shared(sh, a.stages, 1);
+  if (threadIdx.x == 0) init_shared(sh, 1);
   if (warp == 9 && n > 0) tc_alloc(smem_u32(&sh.tmem), 512);
   tc_fence_before();
   __syncthreads();
@@ -350,9 +375,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   volatile int* dead = &sh.dead;
   const int steps = (d.D + 15) / 16;
-  Ring ring{sk + 2 * kTile, base + 2 * kTile, sh.full, sh.empty, a.stages};
+  Ring qr{sk + 2 * kTile, base + 2 * kTile, sh.full[0], sh.empty[0], a.k_stages};
+  Ring gr{sk + (2 + a.k_stages) * kTile, base + (2 + a.k_stages) * kTile, sh.full[1], sh.empty[1], a.v_stages};
 
-  if (warp == 8 && n > 0) {
+  if (warp >= 8) {
+    few_registers();
+    if (warp == 8 && n > 0) {
     int fixes = 0;
     const int bk = d.cu_k ? 0 : b, bq = d.cu_q ? 0 : b;
     if (lane == 0) {
@@ -364,136 +392,170 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         tma_box(sv + c * kBlockBytes, &a.v, c * 64, (int)s.k0 + j0, kv, bk, bar);
       }
     }
+    int h = kv * G + first / per_head, t = first % per_head;
     for (int it = 0; it < n; ++it) {
-      const int u = first + it, h = kv * G + u / per_head, i0 = (t0 + u % per_head) * kTileRows;
+      const int i0 = (t0 + t) * kTileRows;
       // P and dS are zero past the last query and meet the rows of dO and Q there
-      ring_load<kBlocks, kTileRows>(ring, &a.q, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
-      ring_load<kBlocks, kTileRows>(ring, &a.go, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks, kTileRows>(qr, &a.q, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
+      ring_load<kBlocks, kTileRows>(gr, &a.go, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
+      if (++t == per_head) {
+        t = 0;
+        ++h;
+      }
     }
     if (*dead && lane == 0) mbar_wait(smem_u32(&sh.own_full), 0, dead);
   } else if (warp == 9 && n > 0) {
     {
       const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
-      auto product = [&](uint32_t acc, uint32_t left, int stage) {   // acc = K Q^T or V dO^T
-        tile_product<kBlocks, kTileRows>(acc, left, ring.data + stage * kTile, id_s, steps, on);
+      auto product = [&](uint32_t acc, uint32_t left, uint32_t right) {   // acc = K Q^T or V dO^T
+        tile_product<kBlocks, kTileRows>(acc, left, right, id_s, steps, on);
       };
-      auto gather = [&](uint32_t acc, uint32_t left, int stage, bool add) {   // acc += P^T dO or dS^T Q
-        tile_gather<kTileRows>(acc, left, 64, ring.data + stage * kTile, id_o, add, on);
-        tc_commit(smem_u32(&sh.empty[stage]), on);
+      int xq, xg, last_round = 0;
+      auto scores = [&]() {
+        xq = qr.next(dead);
+        product(tmem, sk, qr.data + xq * kTile);
+        tc_commit(smem_u32(&sh.s_full[0]), on);
+      };
+      auto grads = [&]() {
+        last_round = gr.round;
+        xg = gr.next(dead);
+        product(tmem + 128, sv, gr.data + xg * kTile);
+        tc_commit(smem_u32(&sh.dp_full), on);
       };
       mbar_wait(smem_u32(&sh.own_full), 0, dead);
-      int xq = ring.next(dead), xg, last_round = 0;
       tc_fence_after();
-      product(tmem, sk, xq);
-      tc_commit(smem_u32(&sh.s_full[0]), on);
-      last_round = ring.round;
-      xg = ring.next(dead);
-      product(tmem + 128, sv, xg);
-      tc_commit(smem_u32(&sh.dp_full), on);
+      scores();
+      grads();
       for (int it = 0; it < n; ++it) {
         const int cq = xq, cg = xg, round_g = last_round;
         mbar_wait(smem_u32(&sh.p_full), it & 1, dead);
         tc_fence_after();
-        gather(tmem + 256, tmem, cg, it > 0);                        // dv
-        if (it + 1 < n) {
-          xq = ring.next(dead);
-          product(tmem, sk, xq);
-          tc_commit(smem_u32(&sh.s_full[0]), on);
-        }
+        tile_gather<kTileRows>(tmem + 256, tmem, 64, gr.data + cg * kTile, id_o, it > 0, on);             // dv += P^T dO
+        tc_commit(smem_u32(&sh.empty[1][cg]), on);
+        if (it + 1 < n) scores();
         mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
         tc_fence_after();
-        gather(tmem + 256 + DP, tmem + 128, cq, it > 0);             // dk
+        tile_gather<kTileRows>(tmem + 256 + DP, tmem + 128, 64, qr.data + cq * kTile, id_o, it > 0, on);  // dk += dS^T Q
+        tc_commit(smem_u32(&sh.empty[0][cq]), on);
         if (it + 1 < n) {
-          last_round = ring.round;
-          xg = ring.next(dead);
-          product(tmem + 128, sv, xg);
-          tc_commit(smem_u32(&sh.dp_full), on);
+          grads();
         } else {
           tc_commit(smem_u32(&sh.done), on);
-          mbar_wait(smem_u32(&sh.empty[cg]), round_g & 1, dead);     // no arrival is left behind
+          mbar_wait(smem_u32(&sh.empty[1][cg]), round_g & 1, dead);     // no arrival is left behind
           mbar_wait(smem_u32(&sh.done), 0, dead);
         }
       }
     }
-  } else if (warp == 10 && n > 0) {
+    } else if (warp == 10 && n > 0) {
     // the statistics of each tile's queries, two tiles ahead at most
+    int h = kv * G + first / per_head, t = first % per_head;
     for (int it = 0; it < n; ++it) {
-      const int st = it & 1, u = first + it, h = kv * G + u / per_head, i0 = (t0 + u % per_head) * kTileRows;
-      if (it >= 2) mbar_wait(smem_u32(&sh.st_empty[st]), ((it >> 1) - 1) & 1, dead);
+      const int st = it & 1, i0 = (t0 + t) * kTileRows;
+      const float* l = attn_row<const float>(d.lse, b, s.q0 + i0, h);
+      const float* dl = a.delta + ((int64_t)b * d.Hq + h) * d.Lq + i0;
+      float x[4], y[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int x = q * 32 + lane, i = i0 + x;
-        float l = -INFINITY, dl = 0.f;
-        if (i < s.ql) {
-          l = *attn_row<const float>(d.lse, b, s.q0 + i, h);
-          dl = a.delta[((int64_t)b * d.Hq + h) * d.Lq + i];
-        }
-        sh.stat[st][0][x] = l == -INFINITY ? -INFINITY : kLogScaleP<T> - l * kLog2e;   // nothing seen: P = 2^-inf
-        sh.stat[st][1][x] = l == -INFINITY ? 0.f : -dl * (1.f / kScaleP<T>);
+        const bool ok = i0 + q * 32 + lane < s.ql;
+        x[q] = ok ? l[(q * 32 + lane) * d.lse.row] : -INFINITY;
+        y[q] = ok ? dl[q * 32 + lane] : 0.f;
+      }
+      if (it >= 2) mbar_wait(smem_u32(&sh.st_empty[st]), ((it >> 1) - 1) & 1, dead);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {                                    // nothing seen: P = 2^-inf
+        sh.stat[st][0][q * 32 + lane] = x[q] == -INFINITY ? -INFINITY : kLogScaleP<T> - x[q] * kLog2e;
+        sh.stat[st][1][q * 32 + lane] = x[q] == -INFINITY ? 0.f : -y[q] * (1.f / kScaleP<T>);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.st_full[st]));
+      if (++t == per_head) {
+        t = 0;
+        ++h;
+      }
     }
-  } else if (warp < 8) {
+    }
+  } else {
+    many_registers();
     const int w = warp >> 2, r = threadIdx.x & 127, j = j0 + r;
     const bool row = j < keys;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);
     const float c = d.scale * kLog2e;
     const float2 cc = make_float2(c, c), unscale = make_float2(1.f / kScaleP<T>, 1.f / kScaleP<T>);
     const int see = d.causal ? max(0, j - (s.kl - s.ql)) : 0;         // the first query that sees this key
+    int t = n > 0 ? first % per_head : 0;
     for (int it = 0; it < n; ++it) {
-      const int st = it & 1, u = first + it, i0 = (t0 + u % per_head) * kTileRows + w * 64;
-      const float2* lse = reinterpret_cast<const float2*>(sh.stat[st][0] + w * 64);
-      const float2* dlt = reinterpret_cast<const float2*>(sh.stat[st][1] + w * 64);
+      const int st = it & 1, i0 = (t0 + t) * kTileRows + w * 64;
+      if (++t == per_head) t = 0;
+      // The queries' values, all on their way before the wait that follows: while the tensor cores read
+      // shared memory a load takes hundreds of cycles (fetched as they were needed, dS took 2100).
+      const float4* lse = reinterpret_cast<const float4*>(sh.stat[st][0] + w * 64);
+      const float4* dlt = reinterpret_cast<const float4*>(sh.stat[st][1] + w * 64);
+      float4 z[16];
       mbar_wait(smem_u32(&sh.st_full[st]), (it >> 1) & 1, dead);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z[e] = lse[e];
       mbar_wait(smem_u32(&sh.s_full[0]), it & 1, dead);
       tc_fence_after();
-      uint32_t p[64], g[64], h[32];
+      uint32_t p[64];
       tc_ld32(quarter + w * 64, p);
       tc_ld32(quarter + w * 64 + 32, p + 32);
       tc_wait_ld(p);
       const int hide = see - i0;                                     // columns before it do not see the key
       const bool whole = __all_sync(0xffffffffu, hide <= 0);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        float2 x = __ffma2_rn(make_float2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1])), cc, lse[e]);
-        x.x = ex2(x.x);
-        x.y = ex2(x.y);
-        if (!whole) {
-          x.x = 2 * e >= hide ? x.x : 0.f;
-          x.y = 2 * e + 1 >= hide ? x.y : 0.f;
-        }
-        p[2 * e] = __float_as_uint(x.x);
-        p[2 * e + 1] = __float_as_uint(x.y);
-        h[e] = pack2(x.x, x.y, T());
+      for (int e = 0; e < 64; e += 2) {
+        const float4 y = z[e >> 2];
+        const float2 x = __ffma2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), cc,
+                                    (e & 2) ? make_float2(y.z, y.w) : make_float2(y.x, y.y));
+        p[e] = __float_as_uint(ex2(x.x));
+        p[e + 1] = __float_as_uint(ex2(x.y));
       }
-      tc_st32(quarter + w * 64, h);
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 64; ++e) p[e] = e >= hide ? p[e] : 0u;
+      }
+      {
+        uint32_t h[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]), T());
+        tc_st32(quarter + w * 64, h);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) z[e] = dlt[e];
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
       mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
       tc_fence_after();
-      tc_ld32(quarter + 128 + w * 64, g);
-      tc_ld32(quarter + 128 + w * 64 + 32, g + 32);
-      tc_wait_ld(g);
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        float2 x = __ffma2_rn(make_float2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1])), unscale, dlt[e]);
-        x = __fmul2_rn(x, make_float2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1])));
-        if (!whole) {
-          x.x = 2 * e >= hide ? x.x : 0.f;
-          x.y = 2 * e + 1 >= hide ? x.y : 0.f;
+      for (int e0 = 0; e0 < 64; e0 += 32) {
+        uint32_t g[32], h[16];
+        tc_ld32(quarter + 128 + w * 64 + e0, g);
+        tc_wait_ld(g);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float4 y = z[(e0 + e) >> 2];
+          float2 x = __ffma2_rn(make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), unscale,
+                                (e & 2) ? make_float2(y.z, y.w) : make_float2(y.x, y.y));
+          x = __fmul2_rn(x, make_float2(__uint_as_float(p[e0 + e]), __uint_as_float(p[e0 + e + 1])));
+          if (!whole) {                                              // (dP may be anything there)
+            x.x = e0 + e >= hide ? x.x : 0.f;
+            x.y = e0 + e + 1 >= hide ? x.y : 0.f;
+          }
+          h[e >> 1] = pack2(x.x, x.y, T());
         }
-        h[e] = pack2(x.x, x.y, T());
+        // dS of these columns lies over dP of columns that have been read: 0-15 first, then 16-31
+        tc_st16(quarter + 128 + w * 64 + (e0 >> 1), h);
       }
-      tc_st32(quarter + 128 + w * 64, h);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.ds_full));
-      if (lane == 0) mbar_arrive(smem_u32(&sh.st_empty[st]));
+      if (lane == 0) {
+        mbar_arrive(smem_u32(&sh.ds_full));
+        mbar_arrive(smem_u32(&sh.st_empty[st]));
+      }
     }
     if (n > 0) {
       mbar_wait(smem_u32(&sh.done), 0, dead);
@@ -511,11 +573,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
 #pragma unroll
     for (int q = 0; q < DP; q += 32) {
       if (q >= d.D) break;
-      if (row && j >= s.kl) write32<T>(0, false, f, out, part, d.D, q, true);
-      const bool mine = row && j < s.kl;
-      __syncwarp();
-      if (has) write32<T>(quarter + 256 + w * DP + q, true, f, out, part, d.D, q, mine);   // the whole warp
-      else if (mine) write32<T>(0, false, f, out, part, d.D, q, true);
+      // keys past the sequence's end get zeros, whatever their rows of the accumulators hold
+      const uint32_t at = quarter + 256 + w * DP + q;
+      uint8_t* const box = base + 2 * kTile + warp * 2048;             // (the rings are idle)
+      if (__any_sync(0xffffffffu, row && j >= s.kl)) write32<T>(0, false, f, out, part, d.D, q, row && j >= s.kl, box);
+      if (__any_sync(0xffffffffu, row && j < s.kl)) write32<T>(at, has, f, out, part, d.D, q, row && j < s.kl, box);
     }
   }
   finish(sh, d.status, warp, n > 0);
@@ -567,7 +629,10 @@ int64_t cut(BwdArgs& a) {     // returns the workspace's bytes
   a.q_splits = split(q_blocks, a.k_tiles);
   a.k_splits = split(k_blocks, k_walk);
   const int dp = d.D <= 64 ? 64 : 128, tile = dp / 64 * kBlockBytes;
-  a.stages = std::min(kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - 2);
+  const int stages = std::min(2 * kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - 2);
+  a.k_stages = (stages + 1) / 2;   // K is kept for longer than V, and Q than dO
+  a.v_stages = stages / 2;
+  a.G = (int)G;
   const int64_t head = std::max<int64_t>(1, ((int64_t)d.Lk + d.Lq * G) * d.D * 4);
   a.group = (int)std::max<int64_t>(1, std::min<int64_t>(heads, (32 << 20) / head));
   int64_t n = align256((int64_t)d.B * d.Hq * d.Lq * 4);
@@ -586,7 +651,7 @@ template <int DP, typename T>
 int launch(const BwdArgs& a, cudaStream_t s) {
   const b3r_attention_desc& d = a.d;
   const int64_t G = d.Hq / d.Hkv, heads = (int64_t)d.B * d.Hkv;
-  const int smem = 1024 + (2 + a.stages) * (DP / 64) * kBlockBytes + (int)sizeof(Shared);
+  const int smem = 1024 + (2 + a.k_stages + a.v_stages) * (DP / 64) * kBlockBytes + (int)sizeof(Shared);
   B3R_REQUIRE(a.q_tiles * heads * a.q_splits <= 0x7fffffff && a.k_tiles * heads * a.k_splits <= 0x7fffffff,
               "attention backward: too many rows for one call");
   if (a.q_tiles > 0 && (!d.cu_q || d.Tq > 0)) {
