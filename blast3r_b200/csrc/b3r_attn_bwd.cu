@@ -36,11 +36,14 @@ template <typename T>
 constexpr float kScaleP = __is_same(T, __half) ? 2048.f : 1.f;
 
 struct alignas(64) BwdArgs {
-  CUtensorMap q, go, k, v;
+  CUtensorMap q, go, k, v;    // boxes of 128 rows of a head
+  CUtensorMap qg, gog, og;    // boxes of whole groups, where q_tma
   b3r_attention_desc d;
   int q_tiles, k_tiles;       // row tiles of a key/value head's queries, and key tiles, of the longest sequence
   int q_splits, k_splits;     // blocks along the keys for dq, along the queries for dk and dv
-  int k_stages, v_stages, group;   // (k_attn_dkv: of Q, of dO)
+  int dq_k_stages, dq_v_stages;    // rings of K and V in k_attn_dq
+  int q_stages, go_stages, group;  // rings of Q and dO in k_attn_dkv
+  int q_tma;                       // the heads of a group divide 128
   int G;
   float* delta;               // [B][Hq][Lq]
   float* part_q;              // [q_splits][B Hkv][rows][D]
@@ -48,7 +51,7 @@ struct alignas(64) BwdArgs {
 };
 
 struct Shared {
-  uint64_t fix, own_full, full[2][kMaxStages], empty[2][kMaxStages], s_full[2], dp_full, dp_read, p_full, ds_full, done;
+  uint64_t fix, own_full, full[2][kMaxStages], empty[2][kMaxStages], s_full, s_read, dp_full, p_full, ds_full, done, own_ready;
   uint64_t st_full[2], st_empty[2];
   uint32_t tmem;
   int dead;
@@ -64,21 +67,22 @@ __device__ __forceinline__ void place(int id, int tiles, int group, int heads, b
   tile = last_first ? tiles - 1 - r / width : r / width;
 }
 
-__device__ __forceinline__ void init_shared(Shared& sh, int own) {
+__device__ __forceinline__ void init_shared(Shared& sh) {
   mbar_init(smem_u32(&sh.fix), 1);
-  mbar_init(smem_u32(&sh.own_full), own);
+  mbar_init(smem_u32(&sh.own_full), 1);
+  mbar_init(smem_u32(&sh.own_ready), 8);
   for (int i = 0; i < kMaxStages; ++i)
     for (int k = 0; k < 2; ++k) {
       mbar_init(smem_u32(&sh.full[k][i]), 1);
       mbar_init(smem_u32(&sh.empty[k][i]), 1);
     }
   for (int i = 0; i < 2; ++i) {
-    mbar_init(smem_u32(&sh.s_full[i]), 1);
     mbar_init(smem_u32(&sh.st_full[i]), 1);
     mbar_init(smem_u32(&sh.st_empty[i]), 8);
   }
+  mbar_init(smem_u32(&sh.s_full), 1);
+  mbar_init(smem_u32(&sh.s_read), 8);
   mbar_init(smem_u32(&sh.dp_full), 1);
-  mbar_init(smem_u32(&sh.dp_read), 8);
   mbar_init(smem_u32(&sh.p_full), 8);
   mbar_init(smem_u32(&sh.ds_full), 8);
   mbar_init(smem_u32(&sh.done), 1);
@@ -138,16 +142,15 @@ __device__ __forceinline__ void write32(uint32_t tmem, bool has, float f, T* out
 }
 
 // ---------------------------------------------------------------- dq
-// Tensor memory: S of even and odd tiles at 0 and 128, dP at 256, dq at 384.  dS overwrites the
-// S that it came from, each half in place, so dP of the next tile can start once dP is read.
+// Tensor memory: S at 0, dP at 128, dq at 256, and the block's own rows of Q and dO after it, as left operands.
+// The next S starts as soon as this one has been read; dS overwrites dP, each half in place.
 template <int DP, typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__ BwdArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
-  constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
+  constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes, kQ = 256 + DP, kGo = kQ + DP / 2;
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
-  const uint32_t sq = smem_u32(base), sgo = sq + kTile;
-  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.k_stages + a.v_stages) * kTile);
+  Shared& sh = *reinterpret_cast<Shared*>(base + (a.dq_k_stages + a.dq_v_stages) * kTile);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
   const b3r_attention_desc& d = a.d;
   const int G = a.G, split = blockIdx.x % a.q_splits;
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     first = split * per;
     n = min(max(all - first, 0), per);
   }
-  if (threadIdx.x == 0) init_shared(sh, 8);
+  if (threadIdx.x == 0) init_shared(sh);
   if (warp == 9 && n > 0) tc_alloc(smem_u32(&sh.tmem), 512);
   tc_fence_before();
   __syncthreads();
@@ -173,120 +176,134 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   volatile int* dead = &sh.dead;
   const int steps = (d.D + 15) / 16;
-  Ring kr{sq + 2 * kTile, base + 2 * kTile, sh.full[0], sh.empty[0], a.k_stages};
-  Ring vr{sq + (2 + a.k_stages) * kTile, base + (2 + a.k_stages) * kTile, sh.full[1], sh.empty[1], a.v_stages};
+  Ring kr{smem_u32(base), base, sh.full[0], sh.empty[0], a.dq_k_stages};
+  Ring vr{smem_u32(base) + a.dq_k_stages * kTile, base + a.dq_k_stages * kTile, sh.full[1], sh.empty[1], a.dq_v_stages};
+  // the block's own rows pass through stages that the rings reach last: Q and O through K's, dO through V's
+  const int at_q = (a.dq_k_stages - 1) * kTile, at_o = (a.dq_k_stages - 2) * kTile, at_go = (a.dq_k_stages + a.dq_v_stages - 1) * kTile;
 
   if (warp >= 8) {
     few_registers();
     if (warp == 8 && n > 0) {
-    int fixes = 0;
-    const int batch = d.cu_k ? 0 : b;
-    for (int it = 0; it < n; ++it) {
-      const int t = (first + it) * kTileRows;
-      // dS is zero past the last key and meets K's rows there, so they are cleared
-      ring_load<kBlocks, kTileRows>(kr, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
-      ring_load<kBlocks, kTileRows>(vr, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
-    }
-  } else if (warp == 9 && n > 0) {
-    {
+      int fixes = 0;
+      const int batch = d.cu_k ? 0 : b;
+      if (a.q_tma && lane == 0) {      // rows past the end only reach their own row of dq
+        const uint32_t bar = smem_u32(&sh.own_full);
+        const int row = (int)s.q0 + m0 / G, bq = d.cu_q ? 0 : b;
+        mbar_expect(bar, 3 * kTile);
+#pragma unroll
+        for (int c = 0; c < kBlocks; ++c) {
+          tma_box(kr.data + at_q + c * kBlockBytes, &a.qg, c * 64, kv * G, row, bq, bar);
+          tma_box(kr.data + at_go + c * kBlockBytes, &a.gog, c * 64, kv * G, row, bq, bar);
+          tma_box(kr.data + at_o + c * kBlockBytes, &a.og, c * 64, kv * G, row, bq, bar);
+        }
+      }
+      const int free_until = min(a.dq_k_stages - 2, a.dq_v_stages - 1);
+      for (int it = 0; it < n; ++it) {
+        const int t = (first + it) * kTileRows;
+        if (it == free_until) mbar_wait(smem_u32(&sh.own_ready), 0, dead);
+        // dS is zero past the last key and meets K's rows there, so they are cleared
+        ring_load<kBlocks, kTileRows>(kr, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
+        ring_load<kBlocks, kTileRows>(vr, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
+      }
+    } else if (warp == 9 && n > 0) {
       const uint32_t on = elect_one();
       const uint32_t id_s = mma_idesc(kBf, 128, 128, false), id_o = mma_idesc(kBf, 128, (d.D + 15) & ~15, true);
-      auto product = [&](uint32_t acc, uint32_t left, uint32_t right) {   // acc = left K^T or V^T
-        tile_product<kBlocks, kTileRows>(acc, left, right, id_s, steps, on);
-      };
       int k_now = 0, k_next = 0, sv = 0, last_round = 0;
-      auto scores = [&](int it) {
+      auto scores = [&]() {                            // S = Q K^T
         k_next = kr.next(dead);
         tc_fence_after();
-        product(tmem + (it & 1) * 128, sq, kr.data + k_next * kTile);
-        tc_commit(smem_u32(&sh.s_full[it & 1]), on);
+        tile_product_ts<kBlocks, kTileRows>(tmem, tmem + kQ, kr.data + k_next * kTile, id_s, steps, on);
+        tc_commit(smem_u32(&sh.s_full), on);
       };
-      auto grads = [&]() {
+      auto grads = [&]() {                             // dP = dO V^T
         last_round = vr.round;
         sv = vr.next(dead);
         tc_fence_after();
-        product(tmem + 256, sgo, vr.data + sv * kTile);
+        tile_product_ts<kBlocks, kTileRows>(tmem + 128, tmem + kGo, vr.data + sv * kTile, id_s, steps, on);
         tc_commit(smem_u32(&sh.dp_full), on);
         tc_commit(smem_u32(&sh.empty[1][sv]), on);
       };
-      mbar_wait(smem_u32(&sh.own_full), 0, dead);
-      tc_fence_after();
-      scores(0);
+      mbar_wait(smem_u32(&sh.own_ready), 0, dead);
+      scores();
       grads();
       for (int it = 0; it < n; ++it) {
         k_now = k_next;
         if (it + 1 < n) {
-          scores(it + 1);
-          mbar_wait(smem_u32(&sh.dp_read), it & 1, dead);
-          tc_fence_after();
-          grads();
+          mbar_wait(smem_u32(&sh.s_read), it & 1, dead);
+          scores();
         }
         mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
         tc_fence_after();
-        tile_gather<kTileRows>(tmem + 384, tmem + (it & 1) * 128, 64, kr.data + k_now * kTile, id_o, it > 0, on);
+        tile_gather<kTileRows>(tmem + 256, tmem + 128, 64, kr.data + k_now * kTile, id_o, it > 0, on);   // dq += dS K
         tc_commit(smem_u32(&sh.empty[0][k_now]), on);
+        if (it + 1 < n) grads();
       }
       tc_commit(smem_u32(&sh.done), on);
       mbar_wait(smem_u32(&sh.empty[1][sv]), last_round & 1, dead);   // no arrival is left behind
       mbar_wait(smem_u32(&sh.done), 0, dead);
     }
-    }
   } else {
     many_registers();
     const int w = warp >> 2, r = threadIdx.x & 127, m = m0 + r;
-    const int i = m / G, h = kv * G + m % G;
+    const int i = m / G, h = kv * G + m - i * G;
     const bool row = m < rows, live = row && i < s.ql;
     const int bound = live ? attn_bound(s, i, d.causal) : 0;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);
-    // One group brings the rows of Q, the other those of dO and, with O, delta: a warp brings its 32 rows,
-    // DP / 8 lanes to a row, so that whole lines are read (a lane to a row took 4000 to 17000 cycles).
-    {
-      constexpr int kLanes = DP / 8, kRows = 32 / kLanes;
-      const int c = lane % kLanes, m1 = m0 + (warp & 3) * 32;
-      const bool in = c * 8 < d.D;
-#pragma unroll 4
-      for (int x = 0; x < 32; x += kRows) {
-        const int y = x + lane / kLanes, my = m1 + y;
-        const int iy = my / G, hy = kv * G + my - iy * G;
-        const bool ok = in && my < rows && iy < s.ql;
-        const int64_t qr = s.q0 + (ok ? iy : 0);
-        const int qh = ok ? hy : kv * G;
-        const uint4 v = ok ? reinterpret_cast<const uint4*>(attn_row<const T>(w ? d.d_o : d.q, b, qr, qh))[c] : make_uint4(0, 0, 0, 0);
-        const int ry = (warp & 3) * 32 + y;
-        *reinterpret_cast<uint4*>(base + w * kTile + (c >> 3) * kBlockBytes + ry * 128 + (((c & 7) ^ (ry & 7)) << 4)) = v;
-        if (w) {
-          const uint4 o = ok ? reinterpret_cast<const uint4*>(attn_row<const T>(d.o, b, qr, qh))[c] : make_uint4(0, 0, 0, 0);
-          const T* xe = reinterpret_cast<const T*>(&v);
-          const T* ye = reinterpret_cast<const T*>(&o);
-          float dot = 0.f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dot += f_of(xe[e]) * f_of(ye[e]);
-#pragma unroll
-          for (int t = kLanes / 2; t > 0; t >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, t);
-          if (c == 0) {
-            sh.delta[ry] = dot;
-            if (ok && split == 0) a.delta[((int64_t)b * d.Hq + hy) * d.Lq + iy] = dot;
-          }
-        }
-      }
-      fence_async();
-      __syncwarp();
-      if (n > 0 && lane == 0) mbar_arrive(smem_u32(&sh.own_full));
-      bar_sync(1, 256);
-    }
-    const float delta = sh.delta[r], c = d.scale * kLog2e;
+    const float c = d.scale * kLog2e;
     float lse = bound > 0 ? *attn_row<const float>(d.lse, b, s.q0 + i, h) * kLog2e : 0.f;
     if (lse == -INFINITY) lse = INFINITY;              // nothing seen: P = 0
+    // one group brings the rows of Q into tensor memory, the other those of dO and, with O, delta
+    {
+      uint4 x[DP / 8];
+      float dot = 0.f;
+      const bool staged = a.q_tma && n > 0;
+      if (staged) mbar_wait(smem_u32(&sh.own_full), 0, dead);
+      const int64_t qr = s.q0 + (live ? i : 0);
+      const int qh = live ? h : kv * G;
+      auto fetch = [&](int at, const b3r_attn_tensor& t, int cb) {
+        if (staged) return *reinterpret_cast<const uint4*>(base + at + (cb >> 3) * kBlockBytes + r * 128 + (((cb & 7) ^ (r & 7)) << 4));
+        return live && cb * 8 < d.D ? reinterpret_cast<const uint4*>(attn_row<const T>(t, b, qr, qh))[cb] : make_uint4(0, 0, 0, 0);
+      };
+#pragma unroll
+      for (int cb = 0; cb < DP / 8; ++cb) x[cb] = w ? fetch(at_go, d.d_o, cb) : fetch(at_q, d.q, cb);
+      if (w) {
+#pragma unroll
+        for (int cb = 0; cb < DP / 8; ++cb) {
+          const uint4 y = fetch(at_o, d.o, cb);
+          const T* xe = reinterpret_cast<const T*>(&x[cb]);
+          const T* ye = reinterpret_cast<const T*>(&y);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) dot += f_of(xe[e]) * f_of(ye[e]);
+        }
+        sh.delta[r] = dot;
+        if (live && split == 0) a.delta[((int64_t)b * d.Hq + h) * d.Lq + i] = dot;
+      }
+      if (n > 0) {
+#pragma unroll
+        for (int cb = 0; cb < DP / 8; cb += 8)
+          tc_st32(quarter + (w ? kGo : kQ) + cb * 4, reinterpret_cast<const uint32_t*>(x) + cb * 4);
+        tc_wait_st();
+        fence_async();                                 // the stages may be loaded again
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.own_ready));
+      }
+      bar_sync(1, 256);
+    }
+    const float delta = sh.delta[r];
     const float2 cc = make_float2(c, c), ll = make_float2(-lse, -lse), dd = make_float2(-delta, -delta);
     for (int it = 0; it < n; ++it) {
       const int lim = bound - (first + it) * kTileRows - w * 64;     // of this thread's 64 keys, how many its row sees
-      const uint32_t at = quarter + (it & 1) * 128 + w * 64;
-      mbar_wait(smem_u32(&sh.s_full[it & 1]), (it >> 1) & 1, dead);
+      const uint32_t at = quarter + w * 64;
+      mbar_wait(smem_u32(&sh.s_full), it & 1, dead);
       tc_fence_after();
       uint32_t p[64], g[64];
       tc_ld32(at, p);
       tc_ld32(at + 32, p + 32);
       tc_wait_ld(p);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&sh.s_read));
 #pragma unroll
       for (int e = 0; e < 64; e += 2) {
         const float2 x = __ffma2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), cc, ll);
@@ -295,12 +312,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       }
       mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
       tc_fence_after();
-      tc_ld32(quarter + 256 + w * 64, g);
-      tc_ld32(quarter + 256 + w * 64 + 32, g + 32);
+      tc_ld32(at + 128, g);
+      tc_ld32(at + 160, g + 32);
       tc_wait_ld(g);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.dp_read));
       const bool whole = __all_sync(0xffffffffu, lim >= 64);
       uint32_t ds[32];
 #pragma unroll
@@ -313,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         }
         ds[e] = pack2(x.x, x.y, T());
       }
-      tc_st32(at, ds);
+      tc_st32(at + 128, ds);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -331,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
 #pragma unroll
     for (int q = 0; q < DP / 2; q += 32) {
       const int c0 = w * (DP / 2) + q;
-      if (c0 < d.D) write32<T>(quarter + 384 + c0, n > 0, f, out, part, d.D, c0, row, base + 2 * kTile + warp * 2048);   // (the rings are idle)
+      if (c0 < d.D) write32<T>(quarter + 256 + c0, n > 0, f, out, part, d.D, c0, row, base + warp * 2048);   // (the rings are idle)
     }
   }
   finish(sh, d.status, warp, n > 0);
@@ -348,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
   const uint32_t sk = smem_u32(base), sv = sk + kTile;
-  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.k_stages + a.v_stages) * kTile);
+  Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.q_stages + a.go_stages) * kTile);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
   const b3r_attention_desc& d = a.d;
   const int G = a.G, split = blockIdx.x % a.k_splits;
@@ -367,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     first = split * per;
     n = min(max(all - first, 0), per);
   }
-  if (threadIdx.x == 0) init_shared(sh, 1);
+  if (threadIdx.x == 0) init_shared(sh);
   if (warp == 9 && n > 0) tc_alloc(smem_u32(&sh.tmem), 512);
   tc_fence_before();
   __syncthreads();
@@ -375,8 +389,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
   const uint32_t tmem = __shfl_sync(0xffffffffu, sh.tmem, 0);
   volatile int* dead = &sh.dead;
   const int steps = (d.D + 15) / 16;
-  Ring qr{sk + 2 * kTile, base + 2 * kTile, sh.full[0], sh.empty[0], a.k_stages};
-  Ring gr{sk + (2 + a.k_stages) * kTile, base + (2 + a.k_stages) * kTile, sh.full[1], sh.empty[1], a.v_stages};
+  Ring qr{sk + 2 * kTile, base + 2 * kTile, sh.full[0], sh.empty[0], a.q_stages};
+  Ring gr{sk + (2 + a.q_stages) * kTile, base + (2 + a.q_stages) * kTile, sh.full[1], sh.empty[1], a.go_stages};
 
   if (warp >= 8) {
     few_registers();
@@ -415,7 +429,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       auto scores = [&]() {
         xq = qr.next(dead);
         product(tmem, sk, qr.data + xq * kTile);
-        tc_commit(smem_u32(&sh.s_full[0]), on);
+        tc_commit(smem_u32(&sh.s_full), on);
       };
       auto grads = [&]() {
         last_round = gr.round;
@@ -495,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       mbar_wait(smem_u32(&sh.st_full[st]), (it >> 1) & 1, dead);
 #pragma unroll
       for (int e = 0; e < 16; ++e) z[e] = lse[e];
-      mbar_wait(smem_u32(&sh.s_full[0]), it & 1, dead);
+      mbar_wait(smem_u32(&sh.s_full), it & 1, dead);
       tc_fence_after();
       uint32_t p[64];
       tc_ld32(quarter + w * 64, p);
@@ -629,9 +643,12 @@ int64_t cut(BwdArgs& a) {     // returns the workspace's bytes
   a.q_splits = split(q_blocks, a.k_tiles);
   a.k_splits = split(k_blocks, k_walk);
   const int dp = d.D <= 64 ? 64 : 128, tile = dp / 64 * kBlockBytes;
-  const int stages = std::min(2 * kMaxStages, (232448 - 1024 - (int)sizeof(Shared)) / tile - 2);
-  a.k_stages = (stages + 1) / 2;   // K is kept for longer than V, and Q than dO
-  a.v_stages = stages / 2;
+  const int room = (232448 - 1024 - (int)sizeof(Shared)) / tile, stages = std::min(2 * kMaxStages, room - 2);
+  a.q_stages = (stages + 1) / 2;   // Q is kept for longer than dO, and K than V
+  a.go_stages = stages / 2;
+  a.dq_k_stages = std::min(kMaxStages, (room + 1) / 2);
+  a.dq_v_stages = std::min(kMaxStages, room / 2);
+  a.q_tma = kTileRows % G == 0;
   a.G = (int)G;
   const int64_t head = std::max<int64_t>(1, ((int64_t)d.Lk + d.Lq * G) * d.D * 4);
   a.group = (int)std::max<int64_t>(1, std::min<int64_t>(heads, (32 << 20) / head));
@@ -651,12 +668,13 @@ template <int DP, typename T>
 int launch(const BwdArgs& a, cudaStream_t s) {
   const b3r_attention_desc& d = a.d;
   const int64_t G = d.Hq / d.Hkv, heads = (int64_t)d.B * d.Hkv;
-  const int smem = 1024 + (2 + a.k_stages + a.v_stages) * (DP / 64) * kBlockBytes + (int)sizeof(Shared);
+  const int fixed = 1024 + (int)sizeof(Shared), tile = (DP / 64) * kBlockBytes;
+  const int smem_q = fixed + (a.dq_k_stages + a.dq_v_stages) * tile, smem = fixed + (2 + a.q_stages + a.go_stages) * tile;
   B3R_REQUIRE(a.q_tiles * heads * a.q_splits <= 0x7fffffff && a.k_tiles * heads * a.k_splits <= 0x7fffffff,
               "attention backward: too many rows for one call");
   if (a.q_tiles > 0 && (!d.cu_q || d.Tq > 0)) {
-    B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_dq<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention dq"));
-    k_attn_dq<DP, T><<<(unsigned)(a.q_tiles * heads * a.q_splits), kThreads, smem, s>>>(a);
+    B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_dq<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q), "attention dq"));
+    k_attn_dq<DP, T><<<(unsigned)(a.q_tiles * heads * a.q_splits), kThreads, smem_q, s>>>(a);
     B3R_TRY(check_launch("attention dq"));
     if (a.q_splits > 1) {
       k_attn_add<T><<<dim3((unsigned)((d.Lq * G * (d.D / 4) + 255) / 256), (unsigned)heads), 256, 0, s>>>(a, 0);
@@ -701,6 +719,11 @@ extern "C" int b3r_attention_bwd(const b3r_attention_desc* d, void* stream) {
   B3R_TRY(attn_map(&a.go, d->d_o, nq, d->Hq, batch, d->D, d->dtype, kTileRows));
   B3R_TRY(attn_map(&a.k, d->k, nk, d->Hkv, batch, d->D, d->dtype, kTileRows));
   B3R_TRY(attn_map(&a.v, d->v, nk, d->Hkv, batch, d->D, d->dtype, kTileRows));
+  if (a.q_tma) {
+    B3R_TRY(attn_map_groups(&a.qg, d->q, nq, d->Hq, a.G, batch, d->D, d->dtype));
+    B3R_TRY(attn_map_groups(&a.gog, d->d_o, nq, d->Hq, a.G, batch, d->D, d->dtype));
+    B3R_TRY(attn_map_groups(&a.og, d->o, nq, d->Hq, a.G, batch, d->D, d->dtype));
+  }
   cudaStream_t s = as_stream(stream);
   if (d->dtype == B3R_BF16) return d->D <= 64 ? launch<64, __nv_bfloat16>(a, s) : launch<128, __nv_bfloat16>(a, s);
   return d->D <= 64 ? launch<64, __half>(a, s) : launch<128, __half>(a, s);

@@ -133,6 +133,15 @@ __device__ __forceinline__ void tile_product(uint32_t acc, uint32_t a, uint32_t 
       tc_mma(acc, da + (((t >> 2) * kBlockBytes + (t & 3) * 32) >> 4), db + (((t >> 2) * ROWS * 128 + (t & 3) * 32) >> 4), idesc, t > 0,
              on);
 }
+// The same with A in tensor memory (two elements to a column): a left operand in shared memory costs about 100
+// cycles for 16 of the head size, one in tensor memory the 64 that the product takes.
+template <int BLOCKS, int ROWS>
+__device__ __forceinline__ void tile_product_ts(uint32_t acc, uint32_t a, uint32_t b, uint32_t idesc, int steps, uint32_t on) {
+  const uint64_t db = desc_k(b);
+#pragma unroll
+  for (int t = 0; t < BLOCKS * 4; ++t)
+    if (t < steps) tc_mma_ts(acc, a + t * 8, db + (((t >> 2) * ROWS * 128 + (t & 3) * 32) >> 4), idesc, t > 0, on);
+}
 template <int ROWS>
 __device__ __forceinline__ void tile_gather(uint32_t acc, uint32_t a, int half, uint32_t b, uint32_t idesc, bool add, uint32_t on) {
   const uint64_t db = desc_mn(b, ROWS * 128);
