@@ -50,13 +50,18 @@ struct alignas(64) BwdArgs {
   float* part_k;              // [k_splits][2][B Hkv][Lk][D]: dk, dv
 };
 
+constexpr int kStepBytes = kTileRows * 32;
+constexpr float kOne = 64.f;    // the value of `ones`: it keeps the numbers in float16's range
+
 struct Shared {
   uint64_t fix, own_full, full[2][kMaxStages], empty[2][kMaxStages], s_full, s_read, dp_full, p_full, ds_full, done, own_ready;
   uint64_t st_full[2], st_empty[2];
   uint32_t tmem;
   int dead;
   float delta[kTileRows];
-  alignas(16) float stat[2][2][kTileRows];   // k_attn_dkv: per stage, -lse (log2) and -delta of 128 queries
+  // k_attn_dkv: one more step of 16 for S^T and dP^T, which subtracts each query's lse and delta in the tensor
+  // cores: `ones` times (per stage and product) three numbers of the operands' type whose sum, times 64, is it
+  alignas(128) uint4 ones[kStepBytes / 16], stat[2][2][kStepBytes / 16];
 };
 
 // Which head and tile a block works on: heads in groups whose tensors fit L2; `heavy_first`
@@ -78,7 +83,7 @@ __device__ __forceinline__ void init_shared(Shared& sh) {
     }
   for (int i = 0; i < 2; ++i) {
     mbar_init(smem_u32(&sh.st_full[i]), 1);
-    mbar_init(smem_u32(&sh.st_empty[i]), 8);
+    mbar_init(smem_u32(&sh.st_empty[i]), 1);
   }
   mbar_init(smem_u32(&sh.s_full), 1);
   mbar_init(smem_u32(&sh.s_read), 8);
@@ -316,17 +321,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       tc_ld32(at + 160, g + 32);
       tc_wait_ld(g);
       const bool whole = __all_sync(0xffffffffu, lim >= 64);
+#pragma unroll
+      for (int e = 0; e < 64; e += 2) {
+        float2 x = __fadd2_rn(make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), dd);
+        x = __fmul2_rn(x, make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])));
+        g[e] = __float_as_uint(x.x);
+        g[e + 1] = __float_as_uint(x.y);
+      }
+      if (!whole) {                                    // unseen keys: whatever their S and dP are
+#pragma unroll
+        for (int e = 0; e < 64; ++e) g[e] = e < lim ? g[e] : 0u;
+      }
       uint32_t ds[32];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) {
-        float2 x = __fadd2_rn(make_float2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1])), dd);
-        x = __fmul2_rn(x, make_float2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1])));
-        if (!whole) {                                  // unseen keys: whatever their S and dP are
-          x.x = 2 * e < lim ? x.x : 0.f;
-          x.y = 2 * e + 1 < lim ? x.y : 0.f;
-        }
-        ds[e] = pack2(x.x, x.y, T());
-      }
+      for (int e = 0; e < 32; ++e) ds[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), T());
       tc_st32(at + 128, ds);
       tc_wait_st();
       tc_fence_before();
@@ -426,34 +434,39 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         tile_product<kBlocks, kTileRows>(acc, left, right, id_s, steps, on);
       };
       int xq, xg, last_round = 0;
-      auto scores = [&]() {
+      const uint64_t ones = desc_step(smem_u32(sh.ones)), minus = desc_step(smem_u32(sh.stat));
+      auto scores = [&](int it) {
         xq = qr.next(dead);
+        mbar_wait(smem_u32(&sh.st_full[it & 1]), (it >> 1) & 1, dead);
         product(tmem, sk, qr.data + xq * kTile);
+        tc_mma(tmem, ones, minus + ((it & 1) * 2 * kStepBytes >> 4), id_s, true, on);
         tc_commit(smem_u32(&sh.s_full), on);
       };
-      auto grads = [&]() {
+      auto grads = [&](int it) {
         last_round = gr.round;
         xg = gr.next(dead);
         product(tmem + 128, sv, gr.data + xg * kTile);
+        tc_mma(tmem + 128, ones, minus + (((it & 1) * 2 + 1) * kStepBytes >> 4), id_s, true, on);
         tc_commit(smem_u32(&sh.dp_full), on);
+        tc_commit(smem_u32(&sh.st_empty[it & 1]), on);
       };
       mbar_wait(smem_u32(&sh.own_full), 0, dead);
       tc_fence_after();
-      scores();
-      grads();
+      scores(0);
+      grads(0);
       for (int it = 0; it < n; ++it) {
         const int cq = xq, cg = xg, round_g = last_round;
         mbar_wait(smem_u32(&sh.p_full), it & 1, dead);
         tc_fence_after();
         tile_gather<kTileRows>(tmem + 256, tmem, 64, gr.data + cg * kTile, id_o, it > 0, on);             // dv += P^T dO
         tc_commit(smem_u32(&sh.empty[1][cg]), on);
-        if (it + 1 < n) scores();
+        if (it + 1 < n) scores(it + 1);
         mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
         tc_fence_after();
         tile_gather<kTileRows>(tmem + 256 + DP, tmem + 128, 64, qr.data + cq * kTile, id_o, it > 0, on);  // dk += dS^T Q
         tc_commit(smem_u32(&sh.empty[0][cq]), on);
         if (it + 1 < n) {
-          grads();
+          grads(it + 1);
         } else {
           tc_commit(smem_u32(&sh.done), on);
           mbar_wait(smem_u32(&sh.empty[1][cg]), round_g & 1, dead);     // no arrival is left behind
@@ -463,6 +476,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     }
     } else if (warp == 10 && n > 0) {
     // the statistics of each tile's queries, two tiles ahead at most
+    {
+      const T one = t_of<T>(kOne);
+      const uint32_t u = *reinterpret_cast<const uint16_t*>(&one);
+      for (int i = lane; i < kStepBytes / 16; i += 32) {               // bricks of 8: a step's first and second half by turns
+        sh.ones[i] = (i & 8) ? make_uint4(0, 0, 0, 0) : make_uint4(u | u << 16, u, 0, 0);
+        for (int k = 0; k < 4; ++k)
+          if (i & 8) sh.stat[k >> 1][k & 1][i] = make_uint4(0, 0, 0, 0);
+      }
+    }
     int h = kv * G + first / per_head, t = first % per_head;
     for (int it = 0; it < n; ++it) {
       const int st = it & 1, i0 = (t0 + t) * kTileRows;
@@ -476,11 +498,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         y[q] = ok ? dl[q * 32 + lane] : 0.f;
       }
       if (it >= 2) mbar_wait(smem_u32(&sh.st_empty[st]), ((it >> 1) - 1) & 1, dead);
+      auto put = [&](int which, int row, float v) {                    // v as the sum of three
+        const T a0 = t_of<T>(v), a1 = t_of<T>(v - f_of(a0)), a2 = t_of<T>(v - f_of(a0) - f_of(a1));
+        const uint32_t lo = *reinterpret_cast<const uint16_t*>(&a0) | (uint32_t) * reinterpret_cast<const uint16_t*>(&a1) << 16;
+        sh.stat[st][which][(row >> 3) * 16 + (row & 7)] = make_uint4(lo, *reinterpret_cast<const uint16_t*>(&a2), 0, 0);
+      };
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {                                    // nothing seen: P = 2^-inf
-        sh.stat[st][0][q * 32 + lane] = x[q] == -INFINITY ? -INFINITY : kLogScaleP<T> - x[q] * kLog2e;
-        sh.stat[st][1][q * 32 + lane] = x[q] == -INFINITY ? 0.f : -y[q] * (1.f / kScaleP<T>);
+      for (int q = 0; q < 4; ++q) {
+        // a query that sees nothing, or none: its P is masked, or meets zeros; any low score will do
+        const bool none = x[q] == -INFINITY;
+        put(0, q * 32 + lane, none ? -3e4f : (kLogScaleP<T> / kLog2e - x[q]) / (d.scale * kOne));
+        put(1, q * 32 + lane, none ? 0.f : -y[q] * (1.f / kOne));
       }
+      fence_async();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.st_full[st]));
       if (++t == per_head) {
@@ -499,77 +529,58 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     const int see = d.causal ? max(0, j - (s.kl - s.ql)) : 0;         // the first query that sees this key
     int t = n > 0 ? first % per_head : 0;
     for (int it = 0; it < n; ++it) {
-      const int st = it & 1, i0 = (t0 + t) * kTileRows + w * 64;
+      const int i0 = (t0 + t) * kTileRows + w * 64;
       if (++t == per_head) t = 0;
-      // The queries' values, all on their way before the wait that follows: while the tensor cores read
-      // shared memory a load takes hundreds of cycles (fetched as they were needed, dS took 2100).
-      const float4* lse = reinterpret_cast<const float4*>(sh.stat[st][0] + w * 64);
-      const float4* dlt = reinterpret_cast<const float4*>(sh.stat[st][1] + w * 64);
-      float4 z[16];
-      mbar_wait(smem_u32(&sh.st_full[st]), (it >> 1) & 1, dead);
-#pragma unroll
-      for (int e = 0; e < 16; ++e) z[e] = lse[e];
       mbar_wait(smem_u32(&sh.s_full), it & 1, dead);
       tc_fence_after();
-      uint32_t p[64];
+      const int hide = see - i0;                                     // columns before it do not see the key
+      const bool whole = __all_sync(0xffffffffu, hide <= 0);
+      uint32_t p[64], g[64];
       tc_ld32(quarter + w * 64, p);
       tc_ld32(quarter + w * 64 + 32, p + 32);
       tc_wait_ld(p);
-      const int hide = see - i0;                                     // columns before it do not see the key
-      const bool whole = __all_sync(0xffffffffu, hide <= 0);
 #pragma unroll
       for (int e = 0; e < 64; e += 2) {
-        const float4 y = z[e >> 2];
-        const float2 x = __ffma2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), cc,
-                                    (e & 2) ? make_float2(y.z, y.w) : make_float2(y.x, y.y));
+        const float2 x = __fmul2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), cc);
         p[e] = __float_as_uint(ex2(x.x));
         p[e + 1] = __float_as_uint(ex2(x.y));
       }
-      if (!whole) {
+      if (!whole) {                                                  // (apart: within the loops it doubled their time)
 #pragma unroll
         for (int e = 0; e < 64; ++e) p[e] = e >= hide ? p[e] : 0u;
       }
-      {
-        uint32_t h[32];
+      uint32_t h[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]), T());
-        tc_st32(quarter + w * 64, h);
-      }
-#pragma unroll
-      for (int e = 0; e < 16; ++e) z[e] = dlt[e];
+      for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]), T());
+      tc_st32(quarter + w * 64, h);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
       mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
       tc_fence_after();
+      tc_ld32(quarter + 128 + w * 64, g);
+      tc_ld32(quarter + 128 + w * 64 + 32, g + 32);
+      tc_wait_ld(g);
 #pragma unroll
-      for (int e0 = 0; e0 < 64; e0 += 32) {
-        uint32_t g[32], h[16];
-        tc_ld32(quarter + 128 + w * 64 + e0, g);
-        tc_wait_ld(g);
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float4 y = z[(e0 + e) >> 2];
-          float2 x = __ffma2_rn(make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), unscale,
-                                (e & 2) ? make_float2(y.z, y.w) : make_float2(y.x, y.y));
-          x = __fmul2_rn(x, make_float2(__uint_as_float(p[e0 + e]), __uint_as_float(p[e0 + e + 1])));
-          if (!whole) {                                              // (dP may be anything there)
-            x.x = e0 + e >= hide ? x.x : 0.f;
-            x.y = e0 + e + 1 >= hide ? x.y : 0.f;
-          }
-          h[e >> 1] = pack2(x.x, x.y, T());
-        }
-        // dS of these columns lies over dP of columns that have been read: 0-15 first, then 16-31
-        tc_st16(quarter + 128 + w * 64 + (e0 >> 1), h);
+      for (int e = 0; e < 64; e += 2) {
+        float2 x = make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1]));
+        if (kScaleP<T> != 1.f) x = __fmul2_rn(x, unscale);
+        x = __fmul2_rn(x, make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])));
+        g[e] = __float_as_uint(x.x);
+        g[e + 1] = __float_as_uint(x.y);
       }
+      if (!whole) {                                                  // (dP may be anything there)
+#pragma unroll
+        for (int e = 0; e < 64; ++e) g[e] = e >= hide ? g[e] : 0u;
+      }
+#pragma unroll
+      for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), T());
+      tc_st32(quarter + 128 + w * 64, h);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(smem_u32(&sh.ds_full));
-        mbar_arrive(smem_u32(&sh.st_empty[st]));
-      }
+      if (lane == 0) mbar_arrive(smem_u32(&sh.ds_full));
     }
     if (n > 0) {
       mbar_wait(smem_u32(&sh.done), 0, dead);

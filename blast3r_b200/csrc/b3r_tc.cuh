@@ -114,6 +114,11 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr, int block) {
   return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(block >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
          (uint64_t(2) << 61);
 }
+// One step of 16, k-major without swizzle: bricks of 8 rows x 16 bytes, the step's two side by side, 8-row
+// groups 256 bytes apart.
+__device__ __forceinline__ uint64_t desc_step(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t(128 >> 4) << 16) | (uint64_t(256 >> 4) << 32) | (uint64_t(1) << 46);
+}
 // Instruction descriptor: float32 accumulator, both operands bf16 or both f16.
 __host__ __device__ constexpr uint32_t mma_idesc(bool bf16, int M, int N, bool b_mn) {
   return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
