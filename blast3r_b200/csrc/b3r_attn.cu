@@ -52,9 +52,13 @@ static int encode_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, 
   }();
   // the encoder wants a current context, which a thread that has made no runtime call yet (an
   // autograd worker) does not have
+  static thread_local int ready = -1;
   int dev;
   B3R_TRY(check_cuda(cudaGetDevice(&dev), "attention"));
-  B3R_TRY(check_cuda(cudaSetDevice(dev), "attention"));
+  if (dev != ready) {
+    B3R_TRY(check_cuda(cudaSetDevice(dev), "attention"));
+    ready = dev;
+  }
   if (!encode) return fail(B3R_E_CUDA, "attention: the driver has no cuTensorMapEncodeTiled");
   if (rows == 0) {                     // no keys: no load is issued, the map is never read
     *map = CUtensorMap{};

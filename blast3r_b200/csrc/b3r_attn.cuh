@@ -52,6 +52,18 @@ __device__ __forceinline__ __nv_bfloat16 t_of<__nv_bfloat16>(float x) { return _
 template <>
 __device__ __forceinline__ __half t_of<__half>(float x) { return __float2half_rn(x); }
 
+// A kernel's dynamic shared memory limit, raised once on each device.
+template <typename F>
+int attn_smem(F* f, uint64_t& done, const char* what) {
+  int dev;
+  B3R_TRY(check_cuda(cudaGetDevice(&dev), what));
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit)) return B3R_OK;
+  B3R_TRY(check_cuda(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448), what));
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+  return B3R_OK;
+}
+
 // The argument checks: of the sizes alone, and of everything that a direction reads or writes.
 int attn_check_sizes(const b3r_attention_desc* d);
 int attn_check(const b3r_attention_desc* d, bool backward);

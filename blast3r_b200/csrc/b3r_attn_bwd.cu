@@ -684,7 +684,8 @@ int launch(const BwdArgs& a, cudaStream_t s) {
   B3R_REQUIRE(a.q_tiles * heads * a.q_splits <= 0x7fffffff && a.k_tiles * heads * a.k_splits <= 0x7fffffff,
               "attention backward: too many rows for one call");
   if (a.q_tiles > 0 && (!d.cu_q || d.Tq > 0)) {
-    B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_dq<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_q), "attention dq"));
+    static uint64_t ready = 0;
+    B3R_TRY(attn_smem(k_attn_dq<DP, T>, ready, "attention dq"));
     k_attn_dq<DP, T><<<(unsigned)(a.q_tiles * heads * a.q_splits), kThreads, smem_q, s>>>(a);
     B3R_TRY(check_launch("attention dq"));
     if (a.q_splits > 1) {
@@ -693,7 +694,8 @@ int launch(const BwdArgs& a, cudaStream_t s) {
     }
   }
   if (a.k_tiles > 0 && (!d.cu_k || d.Tk > 0)) {
-    B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_dkv<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention dk, dv"));
+    static uint64_t ready = 0;
+    B3R_TRY(attn_smem(k_attn_dkv<DP, T>, ready, "attention dk, dv"));
     k_attn_dkv<DP, T><<<(unsigned)(a.k_tiles * heads * a.k_splits), kThreads, smem, s>>>(a);
     B3R_TRY(check_launch("attention dk, dv"));
     for (int which = 1; which <= 2 && a.k_splits > 1; ++which) {

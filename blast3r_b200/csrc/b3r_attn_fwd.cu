@@ -511,6 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[k % X::kQ]));
       }
+      const bool any = __any_sync(0xffffffffu, row);   // a warp without rows only keeps the others' pace
       float mx = -INFINITY, l = 0.f;       // what the exponentials are taken against (log2), and their sum
       for (int it = 0; it < n; ++it, ++mine) {
         // the step's place among all steps of the block gives its buffer
@@ -519,6 +520,11 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         const int lim = bound - (first + (a.one ? 2 * it + w : it)) * kTileRows;   // keys of this tile that the row sees
         mbar_wait(smem_u32(&sh.s_full[w][bar]), (mine / X::kS) & 1, dead);
         tc_fence_after();
+        if (!any) {
+          if (mine > 0) mbar_wait(smem_u32(&sh.o_done[w]), (mine - 1) & 1, dead);   // (every turn is met)
+          if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[w][bar]));
+          continue;
+        }
         uint32_t s[kTileRows];
 #pragma unroll
         for (int q = 0; q < kTileRows; q += 32) tc_ld32(at + q, s + q);
@@ -606,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         lg = l == 0.f ? -INFINITY : mx + __log2f(l);
       }
       if (w == 0 || !a.one) {
-        const bool has0 = n > 0, has1 = a.one && n1 > 0;
+        const bool has0 = n > 0 && any, has1 = a.one && n1 > 0 && any;
         if (*dead) f0 = f1 = lg = __int_as_float(0x7fffffff);
 #pragma unroll
         for (int q = 0; q < DP; q += 32) {
@@ -754,7 +760,8 @@ template <int DP, typename T>
 int launch(FwdArgs& a, cudaStream_t s) {
   const int smem = 1024 + Cfg<DP>::kQ * (a.one ? 1 : 2) * Cfg<DP>::kTile + (a.k_stages + a.v_stages) * Cfg<DP>::kTile + 8 * kStage +
                    (int)sizeof(Shared);
-  B3R_TRY(check_cuda(cudaFuncSetAttribute(k_attn_fwd<DP, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "attention"));
+  static uint64_t ready = 0;
+  B3R_TRY(attn_smem(k_attn_fwd<DP, T>, ready, "attention"));
   const int64_t jobs = (int64_t)a.tiles * a.heads * a.splits;
   B3R_REQUIRE(jobs <= 0x3fffffff, "attention: too many rows for one call");
   k_attn_fwd<DP, T><<<(unsigned)jobs, kThreads, smem, s>>>(a);

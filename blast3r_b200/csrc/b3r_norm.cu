@@ -165,7 +165,7 @@ __device__ __forceinline__ float2 inside(int v, int j, int tid, int threads, int
 constexpr int kSums = 4;   // values of one row_sum at most
 // Sums of K values over the row's threads: one warp by shuffles, several through `buf` (two sets
 // of kSums x 32 floats used in turn, so one barrier per call is enough), added in the warps' order.
-template <int K>
+template <int K, int MAXW>
 __device__ __forceinline__ void row_sum(float (&s)[K], int warps, float* buf, int& turn) {
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1)
@@ -182,7 +182,9 @@ __device__ __forceinline__ void row_sum(float (&s)[K], int warps, float* buf, in
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     float t = 0.f;
-    for (int q = 0; q < warps; q += 4) {           // entries past the last warp stay zero
+#pragma unroll
+    for (int q = 0; q < MAXW; q += 4) {            // entries past the last warp stay zero
+      if (q >= 8 && q >= warps) break;
       const float4 x = *reinterpret_cast<const float4*>(b + k * 32 + q);
       t += (x.x + x.y) + (x.z + x.w);
     }
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
 #pragma unroll
         for (int j = 0; j < kP; ++j) t = add2(t, n[v][j]);
       float s[1] = {t.x + t.y};
-      row_sum<1>(s, warps, buf, turn);
+      row_sum<1, 8>(s, warps, buf, turn);
       mu = s[0] * inv;
     }
     float2 t = both(0.f);
@@ -251,7 +253,7 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
         t = fma2(n[v][j], n[v][j], t);
       }
     float q[1] = {t.x + t.y};
-    row_sum<1>(q, warps, buf, turn);
+    row_sum<1, 8>(q, warps, buf, turn);
     const float rstd = 1.f / sqrtf(q[0] * inv + a.eps);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
@@ -359,17 +361,18 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
     for (int i = 0; i < a.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
     fence_async();
   }
-  auto own = [&](int which) { return reinterpret_cast<float4*>(weights + which * stride + tid * kE); };
+  // a thread's eight values as two planes of four, so that neighbouring threads meet different banks
+  auto own = [&](int which) { return reinterpret_cast<float4*>(weights + which * stride) + tid; };
   auto keep = [&](int which, const void* p, float none) {   // a weight's columns of this thread to shared memory
     float2 t[kP];
 #pragma unroll
     for (int j = 0; j < kP; ++j) t[j] = both(none);
     if (p) load_w<TY, VEC>(t, p, a.wf32, 0, tid, threads, C);
     own(which)[0] = make_float4(t[0].x, t[0].y, t[1].x, t[1].y);
-    own(which)[1] = make_float4(t[2].x, t[2].y, t[3].x, t[3].y);
+    own(which)[threads] = make_float4(t[2].x, t[2].y, t[3].x, t[3].y);
   };
   auto weight = [&](int which, float2 (&o)[kP]) {
-    const float4 x = own(which)[0], y = own(which)[1];
+    const float4 x = own(which)[0], y = own(which)[threads];
     o[0] = make_float2(x.x, x.y), o[1] = make_float2(x.z, x.w), o[2] = make_float2(y.x, y.y), o[3] = make_float2(y.z, y.w);
   };
   keep(0, a.w_pre, 1.f);
@@ -433,7 +436,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         t[2] = add2(t[2], z[j]);
       }
       float s[3] = {t[0].x + t[0].y, t[1].x + t[1].y, t[2].x + t[2].y};
-      row_sum<3>(s, warps, buf, turn);
+      row_sum<3, MAXT / 32>(s, warps, buf, turn);
       const float mu_r = -s[0] * inv_mean, mu_y = a.post ? -s[1] * inv_mean : 0.f;
       mean_z = s[2] * inv_mean;
 #pragma unroll
@@ -451,7 +454,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
       t[2] = fma2(z[j], r[j], t[2]);
     }
     float q[3] = {t[0].x + t[0].y, t[1].x + t[1].y, t[2].x + t[2].y};
-    row_sum<3>(q, warps, buf, turn);
+    row_sum<3, MAXT / 32>(q, warps, buf, turn);
     if (RING && tid == 0 && row > first) request(row - 1 + a.stages);   // every thread has left the row before
     if (a.pre) {
       const float rstd = 1.f / sqrtf(q[0] * inv + a.eps), proj = -q[2] * inv * rstd;   // -mean(z rhat)
@@ -515,7 +518,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         u[1] = fma2(d[j], y[j], u[1]);
       }
       float s[2] = {u[0].x + u[0].y, u[1].x + u[1].y};
-      row_sum<2>(s, warps, buf, turn);
+      row_sum<2, MAXT / 32>(s, warps, buf, turn);
       const float mz = FULL ? -s[0] * inv_mean : 0.f, proj = -s[1] * inv;
 #pragma unroll
       for (int j = 0; j < kP; ++j) {

@@ -9,8 +9,8 @@
 //
 // One thread owns one slot of a token: V pairs, or V elements that pass through, with V the
 // widest vector that the layout and the alignment allow.  It reads the slot's cosines and
-// sines once and keeps them in registers while it walks over four heads, two heads' loads in
-// flight at a time; neighbouring threads own neighbouring slots.
+// sines once and keeps them in registers while it walks over four heads, the loads
+// of two or four in flight at a time; neighbouring threads own neighbouring slots.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,7 +21,6 @@ namespace {
 
 constexpr int kRotThreads = 256;
 constexpr int kRotHeads = 4;   // heads that a thread walks over
-constexpr int kRotBatch = 2;   // of them, how many have their loads in flight at once
 
 struct RotArgs {
   b3r_rotary_part part[2];
@@ -64,6 +63,7 @@ __global__ void __launch_bounds__(kRotThreads, 4) k_rotary(const __grid_constant
   const uint32_t b = tok / (uint32_t)a.T, t = tok - b * (uint32_t)a.T;
   const bool turns = (int)slot < a.rot_slots;
   constexpr int NP = IL ? V / 2 : V;   // pairs of a slot
+  constexpr int kRotBatch = IL ? 4 : 2;   // heads whose loads are in flight at once
   float c[NP], s[NP];
   int e;                               // the slot's first element
   if (turns) {
