@@ -163,31 +163,48 @@ __device__ __forceinline__ float2 inside(int v, int j, int tid, int threads, int
 }
 
 constexpr int kSums = 4;   // values of one row_sum at most
-// Sums of K values over the row's threads: one warp by shuffles, several through `buf` (two sets
-// of kSums x 32 floats used in turn, so one barrier per call is enough), added in the warps' order.
+// Sums of K values over the row's threads, by shuffles within a warp and through `buf` (two sets of kSums x
+// 32 floats used in turn, so one barrier per call is enough) over the warps, in a fixed order.  Two or
+// more values share their shuffles: after a step that swaps them, half of the lanes go on with each.
 template <int K, int MAXW>
 __device__ __forceinline__ void row_sum(float (&s)[K], int warps, float* buf, int& turn) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  auto swap = [&](float a, float b, int d) {           // lanes without bit d go on with a, the others with b
+    const bool up = lane & d;
+    return (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, d);
+  };
+  float v;
+  int first = 16;                                      // the next step's distance
+  if constexpr (K == 1) {
+    v = s[0];
+  } else if constexpr (K == 2) {
+    v = swap(s[0], s[1], 16);
+    first = 8;
+  } else {
+    v = swap(swap(s[0], s[1], 16), K == 4 ? swap(s[2], s[K - 1], 16) : s[2] + __shfl_xor_sync(0xffffffffu, s[2], 16), 8);
+    first = 4;
+  }
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1)
+    if (d <= first) v += __shfl_xor_sync(0xffffffffu, v, d);
+  // where value k ended up: bit 16 tells 0 from 1 (and 2 from 3), bit 8 the pairs apart
+  auto lane_of = [](int k) { return K == 1 ? 0 : (k & 1) * 16 + (k >> 1) * 8; };
+  if (warps == 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) s[k] += __shfl_xor_sync(0xffffffffu, s[k], d);
-  if (warps == 1) return;
+    for (int k = 0; k < K; ++k) s[k] = K == 1 ? v : __shfl_sync(0xffffffffu, v, lane_of(k));
+    return;
+  }
   float* b = buf + turn * kSums * 32;
   turn ^= 1;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  if (lane == 0)
 #pragma unroll
-    for (int k = 0; k < K; ++k) b[k * 32 + w] = s[k];
+  for (int k = 0; k < K; ++k)
+    if (lane == lane_of(k)) b[k * 32 + w] = v;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    float t = 0.f;
+  for (int k = 0; k < K; ++k) {                        // entries past the last warp stay zero
+    float t = b[k * 32 + (lane & (MAXW - 1))];
 #pragma unroll
-    for (int q = 0; q < MAXW; q += 4) {            // entries past the last warp stay zero
-      if (q >= 8 && q >= warps) break;
-      const float4 x = *reinterpret_cast<const float4*>(b + k * 32 + q);
-      t += (x.x + x.y) + (x.z + x.w);
-    }
+    for (int d = MAXW / 2; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
     s[k] = t;
   }
 }
@@ -254,7 +271,7 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
       }
     float q[1] = {t.x + t.y};
     row_sum<1, 8>(q, warps, buf, turn);
-    const float rstd = 1.f / sqrtf(q[0] * inv + a.eps);
+    const float rstd = rsqrtf(q[0] * inv + a.eps);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
 #pragma unroll
@@ -457,7 +474,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
     row_sum<3, MAXT / 32>(q, warps, buf, turn);
     if (RING && tid == 0 && row > first) request(row - 1 + a.stages);   // every thread has left the row before
     if (a.pre) {
-      const float rstd = 1.f / sqrtf(q[0] * inv + a.eps), proj = -q[2] * inv * rstd;   // -mean(z rhat)
+      const float rstd = rsqrtf(q[0] * inv + a.eps), proj = -q[2] * inv * rstd;   // -mean(z rhat)
 #pragma unroll
       for (int j = 0; j < kP; ++j) {
         const float2 hat = mul2(r[j], both(rstd));
@@ -473,7 +490,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
       for (int j = 0; j < kP; ++j) o[j] = mul2(both(a.alpha), d[j]);
       store8<TX, VEC>(reinterpret_cast<TX*>(a.dx) + row * C, o, 0, tid, threads, C);
     }
-    const float rstd = a.post ? 1.f / sqrtf(q[1] * inv + a.eps) : 1.f;
+    const float rstd = a.post ? rsqrtf(q[1] * inv + a.eps) : 1.f;
 #pragma unroll
     for (int j = 0; j < kP; ++j) y[j] = mul2(y[j], both(rstd));        // yhat
     float2 w[kP];
@@ -517,9 +534,11 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         if (FULL) u[0] = add2(u[0], d[j]);
         u[1] = fma2(d[j], y[j], u[1]);
       }
-      float s[2] = {u[0].x + u[0].y, u[1].x + u[1].y};
-      row_sum<2, MAXT / 32>(s, warps, buf, turn);
-      const float mz = FULL ? -s[0] * inv_mean : 0.f, proj = -s[1] * inv;
+      float s[FULL ? 2 : 1];
+      s[0] = u[1].x + u[1].y;
+      if (FULL) s[FULL ? 1 : 0] = u[0].x + u[0].y;
+      row_sum<FULL ? 2 : 1, MAXT / 32>(s, warps, buf, turn);
+      const float mz = FULL ? -s[FULL ? 1 : 0] * inv_mean : 0.f, proj = -s[0] * inv;
 #pragma unroll
       for (int j = 0; j < kP; ++j) {
         const float2 v = fma2(y[j], both(proj), FULL ? add2(d[j], both(mz)) : d[j]);
