@@ -54,7 +54,7 @@ constexpr int kStepBytes = kTileRows * 32;
 constexpr float kOne = 64.f;    // the value of `ones`: it keeps the numbers in float16's range
 
 struct Shared {
-  uint64_t fix, own_full, full[2][kMaxStages], empty[2][kMaxStages], s_full, s_read, dp_full, p_full, ds_full, done, own_ready;
+  uint64_t fix, own_full, full[2][kMaxStages], empty[2][kMaxStages], s_full[2], s_read, dp_full, p_full, ds_full, done, own_ready;
   uint64_t st_full[2], st_empty[2];
   uint32_t tmem;
   int dead;
@@ -85,7 +85,8 @@ __device__ __forceinline__ void init_shared(Shared& sh) {
     mbar_init(smem_u32(&sh.st_full[i]), 1);
     mbar_init(smem_u32(&sh.st_empty[i]), 1);
   }
-  mbar_init(smem_u32(&sh.s_full), 1);
+  mbar_init(smem_u32(&sh.s_full[0]), 1);
+  mbar_init(smem_u32(&sh.s_full[1]), 1);
   mbar_init(smem_u32(&sh.s_read), 8);
   mbar_init(smem_u32(&sh.dp_full), 1);
   mbar_init(smem_u32(&sh.p_full), 8);
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         k_next = kr.next(dead);
         tc_fence_after();
         tile_product_ts<kBlocks, kTileRows>(tmem, tmem + kQ, kr.data + k_next * kTile, id_s, steps, on);
-        tc_commit(smem_u32(&sh.s_full), on);
+        tc_commit(smem_u32(&sh.s_full[0]), on);
       };
       auto grads = [&]() {                             // dP = dO V^T
         last_round = vr.round;
@@ -300,7 +301,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     for (int it = 0; it < n; ++it) {
       const int lim = bound - (first + it) * kTileRows - w * 64;     // of this thread's 64 keys, how many its row sees
       const uint32_t at = quarter + w * 64;
-      mbar_wait(smem_u32(&sh.s_full), it & 1, dead);
+      mbar_wait(smem_u32(&sh.s_full[0]), it & 1, dead);
       tc_fence_after();
       uint32_t p[64], g[64];
       tc_ld32(at, p);
@@ -360,15 +361,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
 }
 
 // ---------------------------------------------------------------- dk, dv
-// Tensor memory: S^T at 0, dP^T at 128, dv at 256, dk at 256 + DP.  P^T overwrites S^T and dS^T
-// dP^T, each half in place.  While the groups are at P of tile t, the tensor cores are at dk of
-// tile t - 1 and dP of tile t; while they are at dS of t, at dv of t and S of t + 1.
+// Tensor memory: S^T, dP^T, dv, dk; P^T overwrites S^T and dS^T dP^T, each half in place.  While the groups are
+// at P of tile t, the tensor cores are at dk of tile t - 1 and dP of tile t; while they are at dS of t, at
+// dv of t and S of t + 1.  Up to a head size of 64 there is room for two of S^T, and S of t + 1 starts
+// before P of t is there (the groups waited 750 of 2600 cycles for it).
 template <int DP, typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant__ BwdArgs a) {
   extern __shared__ uint8_t raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
   constexpr int kBlocks = DP / 64, kTile = kBlocks * kBlockBytes;
   constexpr bool kBf = __is_same(T, __nv_bfloat16);
+  constexpr int kS = DP == 64 ? 2 : 1, kDp = kS * 128, kDv = kDp + 128, kDk = kDv + DP;   // S's buffers; columns
   const uint32_t sk = smem_u32(base), sv = sk + kTile;
   Shared& sh = *reinterpret_cast<Shared*>(base + (2 + a.q_stages + a.go_stages) * kTile);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // uniform
@@ -438,15 +441,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       auto scores = [&](int it) {
         xq = qr.next(dead);
         mbar_wait(smem_u32(&sh.st_full[it & 1]), (it >> 1) & 1, dead);
-        product(tmem, sk, qr.data + xq * kTile);
-        tc_mma(tmem, ones, minus + ((it & 1) * 2 * kStepBytes >> 4), id_s, true, on);
-        tc_commit(smem_u32(&sh.s_full), on);
+        product(tmem + it % kS * 128, sk, qr.data + xq * kTile);
+        tc_mma(tmem + it % kS * 128, ones, minus + ((it & 1) * 2 * kStepBytes >> 4), id_s, true, on);
+        tc_commit(smem_u32(&sh.s_full[it % kS]), on);
       };
       auto grads = [&](int it) {
         last_round = gr.round;
         xg = gr.next(dead);
-        product(tmem + 128, sv, gr.data + xg * kTile);
-        tc_mma(tmem + 128, ones, minus + (((it & 1) * 2 + 1) * kStepBytes >> 4), id_s, true, on);
+        product(tmem + kDp, sv, gr.data + xg * kTile);
+        tc_mma(tmem + kDp, ones, minus + (((it & 1) * 2 + 1) * kStepBytes >> 4), id_s, true, on);
         tc_commit(smem_u32(&sh.dp_full), on);
         tc_commit(smem_u32(&sh.st_empty[it & 1]), on);
       };
@@ -456,14 +459,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       grads(0);
       for (int it = 0; it < n; ++it) {
         const int cq = xq, cg = xg, round_g = last_round;
+        if (kS == 2 && it + 1 < n) scores(it + 1);
         mbar_wait(smem_u32(&sh.p_full), it & 1, dead);
         tc_fence_after();
-        tile_gather<kTileRows>(tmem + 256, tmem, 64, gr.data + cg * kTile, id_o, it > 0, on);             // dv += P^T dO
+        tile_gather<kTileRows>(tmem + kDv, tmem + it % kS * 128, 64, gr.data + cg * kTile, id_o, it > 0, on);             // dv += P^T dO
         tc_commit(smem_u32(&sh.empty[1][cg]), on);
-        if (it + 1 < n) scores(it + 1);
+        if (kS == 1 && it + 1 < n) scores(it + 1);
         mbar_wait(smem_u32(&sh.ds_full), it & 1, dead);
         tc_fence_after();
-        tile_gather<kTileRows>(tmem + 256 + DP, tmem + 128, 64, qr.data + cq * kTile, id_o, it > 0, on);  // dk += dS^T Q
+        tile_gather<kTileRows>(tmem + kDk, tmem + kDp, 64, qr.data + cq * kTile, id_o, it > 0, on);  // dk += dS^T Q
         tc_commit(smem_u32(&sh.empty[0][cq]), on);
         if (it + 1 < n) {
           grads(it + 1);
@@ -531,13 +535,14 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     for (int it = 0; it < n; ++it) {
       const int i0 = (t0 + t) * kTileRows + w * 64;
       if (++t == per_head) t = 0;
-      mbar_wait(smem_u32(&sh.s_full), it & 1, dead);
+      const uint32_t at = quarter + it % kS * 128 + w * 64, dp = quarter + kDp + w * 64;
+      mbar_wait(smem_u32(&sh.s_full[it % kS]), (it / kS) & 1, dead);
       tc_fence_after();
       const int hide = see - i0;                                     // columns before it do not see the key
       const bool whole = __all_sync(0xffffffffu, hide <= 0);
       uint32_t p[64], g[64];
-      tc_ld32(quarter + w * 64, p);
-      tc_ld32(quarter + w * 64 + 32, p + 32);
+      tc_ld32(at, p);
+      tc_ld32(at + 32, p + 32);
       tc_wait_ld(p);
 #pragma unroll
       for (int e = 0; e < 64; e += 2) {
@@ -552,15 +557,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       uint32_t h[32];
 #pragma unroll
       for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]), T());
-      tc_st32(quarter + w * 64, h);
+      tc_st32(at, h);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
       mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
       tc_fence_after();
-      tc_ld32(quarter + 128 + w * 64, g);
-      tc_ld32(quarter + 128 + w * 64 + 32, g + 32);
+      tc_ld32(dp, g);
+      tc_ld32(dp + 32, g + 32);
       tc_wait_ld(g);
 #pragma unroll
       for (int e = 0; e < 64; e += 2) {
@@ -576,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       }
 #pragma unroll
       for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), T());
-      tc_st32(quarter + 128 + w * 64, h);
+      tc_st32(dp, h);
       tc_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -599,10 +604,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     for (int q = 0; q < DP; q += 32) {
       if (q >= d.D) break;
       // keys past the sequence's end get zeros, whatever their rows of the accumulators hold
-      const uint32_t at = quarter + 256 + w * DP + q;
+      const uint32_t from = quarter + (w ? kDk : kDv) + q;
       uint8_t* const box = base + 2 * kTile + warp * 2048;             // (the rings are idle)
       if (__any_sync(0xffffffffu, row && j >= s.kl)) write32<T>(0, false, f, out, part, d.D, q, row && j >= s.kl, box);
-      if (__any_sync(0xffffffffu, row && j < s.kl)) write32<T>(at, has, f, out, part, d.D, q, row && j < s.kl, box);
+      if (__any_sync(0xffffffffu, row && j < s.kl)) write32<T>(from, has, f, out, part, d.D, q, row && j < s.kl, box);
     }
   }
   finish(sh, d.status, warp, n > 0);
