@@ -667,7 +667,9 @@ int64_t cut(BwdArgs& a) {     // returns the workspace's bytes
   a.q_tma = kTileRows % G == 0;
   a.G = (int)G;
   const int64_t head = std::max<int64_t>(1, ((int64_t)d.Lk + d.Lq * G) * d.D * 4);
-  a.group = (int)std::max<int64_t>(1, std::min<int64_t>(heads, (32 << 20) / head));
+  // Causal blocks differ by up to the whole length of a walk: the longest come first over all heads (in groups
+  // of heads the last group's long ones ended late: 529 against 427 us for dk, dv at 4096 x 4096, 32/8 heads of 128).
+  a.group = d.causal ? (int)std::max<int64_t>(1, heads) : (int)std::max<int64_t>(1, std::min<int64_t>(heads, (32 << 20) / head));
   int64_t n = align256((int64_t)d.B * d.Hq * d.Lq * 4);
   const int64_t q_off = n;
   if (a.q_splits > 1) n += align256((int64_t)a.q_splits * heads * d.Lq * G * d.D * 4);
