@@ -256,33 +256,44 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     const int bound = live ? attn_bound(s, i, d.causal) : 0;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);
     const float c = d.scale * kLog2e;
-    float lse = bound > 0 ? *attn_row<const float>(d.lse, b, s.q0 + i, h) * kLog2e : 0.f;
-    if (lse == -INFINITY) lse = INFINITY;              // nothing seen: P = 0
+    const float lse_in = bound > 0 ? *attn_row<const float>(d.lse, b, s.q0 + i, h) : 0.f;
     // one group brings the rows of Q into tensor memory, the other those of dO and, with O, delta
     {
-      uint4 x[DP / 8];
-      float dot = 0.f;
-      const bool staged = a.q_tma && n > 0;
-      if (staged) mbar_wait(smem_u32(&sh.own_full), 0, dead);
-      const int64_t qr = s.q0 + (live ? i : 0);
-      const int qh = live ? h : kv * G;
-      auto fetch = [&](int at, const b3r_attn_tensor& t, int cb) {
-        if (staged) return *reinterpret_cast<const uint4*>(base + at + (cb >> 3) * kBlockBytes + r * 128 + (((cb & 7) ^ (r & 7)) << 4));
-        return live && cb * 8 < d.D ? reinterpret_cast<const uint4*>(attn_row<const T>(t, b, qr, qh))[cb] : make_uint4(0, 0, 0, 0);
-      };
-#pragma unroll
-      for (int cb = 0; cb < DP / 8; ++cb) x[cb] = w ? fetch(at_go, d.d_o, cb) : fetch(at_q, d.q, cb);
-      if (w) {
+      uint4 x[DP / 8], y[DP / 8];
+      if (a.q_tma && n > 0) {
+        mbar_wait(smem_u32(&sh.own_full), 0, dead);
+        const uint8_t* mine = base + (w ? at_go : at_q) + r * 128;
+        const uint8_t* out = base + at_o + r * 128;
 #pragma unroll
         for (int cb = 0; cb < DP / 8; ++cb) {
-          const uint4 y = fetch(at_o, d.o, cb);
-          const T* xe = reinterpret_cast<const T*>(&x[cb]);
-          const T* ye = reinterpret_cast<const T*>(&y);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) dot += f_of(xe[e]) * f_of(ye[e]);
+          const int at = (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4);
+          x[cb] = *reinterpret_cast<const uint4*>(mine + at);
+          if (w) y[cb] = *reinterpret_cast<const uint4*>(out + at);
         }
-        sh.delta[r] = dot;
-        if (live && split == 0) a.delta[((int64_t)b * d.Hq + h) * d.Lq + i] = dot;
+      } else {
+        const int64_t qr = s.q0 + (live ? i : 0);
+        const int qh = live ? h : kv * G;
+        const uint4* mine = reinterpret_cast<const uint4*>(attn_row<const T>(w ? d.d_o : d.q, b, qr, qh));
+        const uint4* out = reinterpret_cast<const uint4*>(attn_row<const T>(d.o, b, qr, qh));
+#pragma unroll
+        for (int cb = 0; cb < DP / 8; ++cb) {
+          const bool in = live && cb * 8 < d.D;
+          x[cb] = in ? mine[cb] : make_uint4(0, 0, 0, 0);
+          y[cb] = in && w ? out[cb] : make_uint4(0, 0, 0, 0);
+        }
+      }
+      if (w) {
+        float2 dot[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+        for (int cb = 0; cb < DP / 8; ++cb) {
+          const uint32_t* xe = reinterpret_cast<const uint32_t*>(&x[cb]);
+          const uint32_t* ye = reinterpret_cast<const uint32_t*>(&y[cb]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) dot[e & 1] = __ffma2_rn(unpack2(xe[e], T()), unpack2(ye[e], T()), dot[e & 1]);
+        }
+        const float delta = (dot[0].x + dot[0].y) + (dot[1].x + dot[1].y);
+        sh.delta[r] = delta;
+        if (live && split == 0) a.delta[((int64_t)b * d.Hq + h) * d.Lq + i] = delta;
       }
       if (n > 0) {
 #pragma unroll
@@ -296,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       }
       bar_sync(1, 256);
     }
-    const float delta = sh.delta[r];
+    const float delta = sh.delta[r], lse = lse_in == -INFINITY ? INFINITY : lse_in * kLog2e;   // nothing seen: P = 0
     const float2 cc = make_float2(c, c), ll = make_float2(-lse, -lse), dd = make_float2(-delta, -delta);
     for (int it = 0; it < n; ++it) {
       const int lim = bound - (first + it) * kTileRows - w * 64;     // of this thread's 64 keys, how many its row sees
