@@ -34,7 +34,7 @@ def check_attention(device=None):
     s = _status.get(dev.index)
     if s is not None and int(s.item()):
         s.zero_()
-        raise L.B3RError('a bounded wait inside an attention kernel ran out: its outputs are NaN')
+        raise L.B3RError('a bounded wait inside an attention kernel ran out: its outputs are not to be used')
 
 
 def _tensor(t, packed):
@@ -144,7 +144,8 @@ def attention_forward(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=
     past them is not used.  Packed: q (Tq, Hq, D), k and v (Tk, Hkv, D), with cu_q, cu_k
     int32 (sequences + 1,), where each sequence begins and ends, and max_q, max_k, bounds of
     their lengths.  causal: query i sees the keys j <= i + k_len - q_len, so the last query sees
-    the last key.  A query that sees no key has o = 0 and lse = -inf.  scale: D**-0.5."""
+    the last key.  A query that sees no key has o = 0 and lse = -inf.  scale: positive, D**-0.5 by
+    default."""
     d, packed, keep = _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k)
     q, k, v = _readable(q), _readable(k), _readable(v)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -157,7 +158,10 @@ def attention_forward(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=
 
 def attention_backward(do, q, k, v, o, lse, *, causal=False, scale=None, q_lens=None, k_lens=None, cu_q=None, cu_k=None,
                        max_q=None, max_k=None):
-    """(dq, dk, dv) from do, the gradient of o, with the forward call's inputs, outputs and keywords."""
+    """(dq, dk, dv) from do, the gradient of o, with the forward call's inputs, outputs and keywords.
+
+    The probabilities and their gradient are rounded to the inputs' type for the matrix products (in
+    float16 with powers of two that keep small ones out of its subnormal range)."""
     d, packed, keep = _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k)
     for name, t in (('do', do), ('o', o)):
         if not isinstance(t, torch.Tensor) or t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:

@@ -14,7 +14,7 @@ int attn_check_sizes(const b3r_attention_desc* d) {
   // rows (queries x heads of a group) and the blocks' indices are 32-bit integers
   B3R_REQUIRE(d->Tq <= 0x7fffffff && d->Tk <= 0x7fffffff && (int64_t)d->Lq * (d->Hq / d->Hkv) <= 0x7fffff00 && d->Lk <= 0x7fffff00,
               "attention: more rows than 32-bit indices reach");
-  B3R_REQUIRE((int64_t)d->B * d->Hq <= 65535, "attention: more than 65535 sequences x heads");
+  B3R_REQUIRE((int64_t)d->B * d->Hq <= 0x7fffffff, "attention: too many sequences x heads");
   return B3R_OK;
 }
 

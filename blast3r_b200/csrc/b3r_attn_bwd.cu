@@ -35,6 +35,17 @@ constexpr float kLogScaleP = __is_same(T, __half) ? 11.f : 0.f;
 template <typename T>
 constexpr float kScaleP = __is_same(T, __half) ? 2048.f : 1.f;
 
+// In float16 dS is carried 2^k times as large too, with the largest k that cannot overflow: |dS| is at most
+// 2 |do_i| |v_j|, since o is a mean of rows of v.  Gradients of any size then keep their 11 bits.
+template <typename T>
+__device__ __forceinline__ float scale_ds(const float2* range, int head) {
+  if constexpr (!__is_same(T, __half)) return 1.f;
+  const float2 r = range[head];
+  const float most = 2.f * sqrtf(r.x) * sqrtf(r.y);
+  if (!(most > 0.f) || isinf(most)) return 1.f;
+  return exp2f(fminf(fmaxf(floorf(log2f(32768.f / most)), -24.f), 24.f));
+}
+
 struct alignas(64) BwdArgs {
   CUtensorMap q, go, k, v;    // boxes of 128 rows of a head
   CUtensorMap qg, gog, og;    // boxes of whole groups, where q_tma
@@ -46,12 +57,15 @@ struct alignas(64) BwdArgs {
   int q_tma;                       // the heads of a group divide 128
   int G;
   float* delta;               // [B][Hq][Lq]
+  float2* range;              // float16: [B][Hkv], the largest |do|^2 and |v|^2 of a row
   float* part_q;              // [q_splits][B Hkv][rows][D]
   float* part_k;              // [k_splits][2][B Hkv][Lk][D]: dk, dv
 };
 
 constexpr int kStepBytes = kTileRows * 32;
-constexpr float kOne = 64.f;    // the value of `ones`: it keeps the numbers in float16's range
+// A float as 2^8 a + b + 2^-8 c + 2^-14 d with a .. d of the operands' type: to 24 bits at least, in
+// float16 for magnitudes from 1e-6 to 1e7 too (its own numbers end at 6e4, and are coarse below 6e-5).
+__host__ __device__ constexpr float weight_of(int k) { return k == 0 ? 256.f : k == 1 ? 1.f : k == 2 ? 1.f / 256.f : 1.f / 16384.f; }
 
 struct Shared {
   uint64_t fix, own_full, full[2][kMaxStages], empty[2][kMaxStages], s_full[2], s_read, dp_full, p_full, ds_full, done, own_ready;
@@ -60,8 +74,8 @@ struct Shared {
   int dead;
   float delta[kTileRows];
   // k_attn_dkv: one more step of 16 for S^T and dP^T, which subtracts each query's lse and delta in the tensor
-  // cores: `ones` times (per stage and product) three numbers of the operands' type whose sum, times 64, is it
-  alignas(128) uint4 ones[kStepBytes / 16], stat[2][2][kStepBytes / 16];
+  // cores: the weights below times (per stage and product) four numbers of the operands' type each
+  alignas(128) uint4 weights[kStepBytes / 16], stat[2][2][kStepBytes / 16];
 };
 
 // Which head and tile a block works on: heads in groups whose tensors fit L2; `heavy_first`
@@ -144,6 +158,44 @@ __device__ __forceinline__ void write32(uint32_t tmem, bool has, float f, T* out
     T* const to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, row ? reinterpret_cast<uint64_t>(out) : 0, y));
     const uint4 z = box[y * 4 + (c ^ ((y >> 1) & 3))];
     if (to && c0 + c * 8 < D) *reinterpret_cast<uint4*>(to + c0 + c * 8) = z;
+  }
+}
+
+// The largest |do|^2 and |v|^2 of a row among the heads that share keys and values.  A block takes 1024
+// rows of one head; the maximum of non-negative floats is that of their bits, in any order.
+constexpr int kRangeRows = 1024;
+template <typename T>
+__global__ void __launch_bounds__(256) k_attn_range(const __grid_constant__ BwdArgs a, int chunks) {
+  __shared__ float part[8];
+  const b3r_attention_desc& d = a.d;
+  const int b = blockIdx.x / chunks, first = (blockIdx.x - b * chunks) * kRangeRows;
+  const bool of_v = (int)blockIdx.y >= d.Hq;
+  const int h = of_v ? blockIdx.y - d.Hq : blockIdx.y, kv = of_v ? h : h / a.G;
+  const AttnSeq s = attn_seq(d, b);
+  const int last = min(first + kRangeRows, of_v ? s.kl : s.ql);
+  float most = 0.f;
+  for (int i = first + threadIdx.x; i < last; i += 256) {
+    const uint4* x = reinterpret_cast<const uint4*>(attn_row<const T>(of_v ? d.v : d.d_o, b, (of_v ? s.k0 : s.q0) + i, h));
+    float2 sum = make_float2(0.f, 0.f);
+    for (int c = 0; c < d.D / 8; ++c) {
+      const uint4 u = x[c];
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 y = unpack2(w[e], T());
+        sum = __ffma2_rn(y, y, sum);
+      }
+    }
+    most = fmaxf(most, sum.x + sum.y);                 // (a NaN is passed over: it has no size)
+  }
+#pragma unroll
+  for (int t = 16; t > 0; t >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, t));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 8; ++i) most = fmaxf(most, part[i]);
+    float2* r = a.range + (int64_t)b * d.Hkv + kv;
+    atomicMax(reinterpret_cast<int*>(of_v ? &r->y : &r->x), __float_as_int(most));
   }
 }
 
@@ -308,7 +360,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       bar_sync(1, 256);
     }
     const float delta = sh.delta[r], lse = lse_in == -INFINITY ? INFINITY : lse_in * kLog2e;   // nothing seen: P = 0
-    const float2 cc = make_float2(c, c), ll = make_float2(-lse, -lse), dd = make_float2(-delta, -delta);
+    const float up = scale_ds<T>(a.range, head);
+    const float2 cc = make_float2(c, c), ll = make_float2(-lse, -lse), dd = make_float2(-delta * up, -delta * up), uu = make_float2(up, up);
     for (int it = 0; it < n; ++it) {
       const int lim = bound - (first + it) * kTileRows - w * 64;     // of this thread's 64 keys, how many its row sees
       const uint32_t at = quarter + w * 64;
@@ -335,7 +388,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       const bool whole = __all_sync(0xffffffffu, lim >= 64);
 #pragma unroll
       for (int e = 0; e < 64; e += 2) {
-        float2 x = __fadd2_rn(make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1])), dd);
+        float2 x = make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1]));
+        x = __is_same(T, __half) ? __ffma2_rn(x, uu, dd) : __fadd2_rn(x, dd);
         x = __fmul2_rn(x, make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])));
         g[e] = __float_as_uint(x.x);
         g[e + 1] = __float_as_uint(x.y);
@@ -357,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
       mbar_wait(smem_u32(&sh.done), 0, dead);
       tc_fence_after();
     }
-    const float f = *dead ? __int_as_float(0x7fffffff) : d.scale;
+    const float f = *dead ? __int_as_float(0x7fffffff) : d.scale / up;
     T* out = attn_row<T>(d.dq, b, s.q0 + (row ? i : 0), row ? h : 0);
     float* part = a.q_splits > 1
                       ? a.part_q + (((int64_t)split * d.B * d.Hkv + head) * ((int64_t)d.Lq * G) + m) * d.D
@@ -448,19 +502,19 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         tile_product<kBlocks, kTileRows>(acc, left, right, id_s, steps, on);
       };
       int xq, xg, last_round = 0;
-      const uint64_t ones = desc_step(smem_u32(sh.ones)), minus = desc_step(smem_u32(sh.stat));
+      const uint64_t weights = desc_step(smem_u32(sh.weights)), minus = desc_step(smem_u32(sh.stat));
       auto scores = [&](int it) {
         xq = qr.next(dead);
         mbar_wait(smem_u32(&sh.st_full[it & 1]), (it >> 1) & 1, dead);
         product(tmem + it % kS * 128, sk, qr.data + xq * kTile);
-        tc_mma(tmem + it % kS * 128, ones, minus + ((it & 1) * 2 * kStepBytes >> 4), id_s, true, on);
+        tc_mma(tmem + it % kS * 128, weights, minus + ((it & 1) * 2 * kStepBytes >> 4), id_s, true, on);
         tc_commit(smem_u32(&sh.s_full[it % kS]), on);
       };
       auto grads = [&](int it) {
         last_round = gr.round;
         xg = gr.next(dead);
         product(tmem + kDp, sv, gr.data + xg * kTile);
-        tc_mma(tmem + kDp, ones, minus + (((it & 1) * 2 + 1) * kStepBytes >> 4), id_s, true, on);
+        tc_mma(tmem + kDp, weights, minus + (((it & 1) * 2 + 1) * kStepBytes >> 4), id_s, true, on);
         tc_commit(smem_u32(&sh.dp_full), on);
         tc_commit(smem_u32(&sh.st_empty[it & 1]), on);
       };
@@ -492,10 +546,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     } else if (warp == 10 && n > 0) {
     // the statistics of each tile's queries, two tiles ahead at most
     {
-      const T one = t_of<T>(kOne);
-      const uint32_t u = *reinterpret_cast<const uint16_t*>(&one);
+      const uint32_t lo = pack2(weight_of(0), weight_of(1), T()), hi = pack2(weight_of(2), weight_of(3), T());
       for (int i = lane; i < kStepBytes / 16; i += 32) {               // bricks of 8: a step's first and second half by turns
-        sh.ones[i] = (i & 8) ? make_uint4(0, 0, 0, 0) : make_uint4(u | u << 16, u, 0, 0);
+        sh.weights[i] = (i & 8) ? make_uint4(0, 0, 0, 0) : make_uint4(lo, hi, 0, 0);
         for (int k = 0; k < 4; ++k)
           if (i & 8) sh.stat[k >> 1][k & 1][i] = make_uint4(0, 0, 0, 0);
       }
@@ -513,17 +566,21 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         y[q] = ok ? dl[q * 32 + lane] : 0.f;
       }
       if (it >= 2) mbar_wait(smem_u32(&sh.st_empty[st]), ((it >> 1) - 1) & 1, dead);
-      auto put = [&](int which, int row, float v) {                    // v as the sum of three
-        const T a0 = t_of<T>(v), a1 = t_of<T>(v - f_of(a0)), a2 = t_of<T>(v - f_of(a0) - f_of(a1));
-        const uint32_t lo = *reinterpret_cast<const uint16_t*>(&a0) | (uint32_t) * reinterpret_cast<const uint16_t*>(&a1) << 16;
-        sh.stat[st][which][(row >> 3) * 16 + (row & 7)] = make_uint4(lo, *reinterpret_cast<const uint16_t*>(&a2), 0, 0);
+      auto put = [&](int which, int row, float v) {
+        float part[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          part[k] = f_of(t_of<T>(v * (1.f / weight_of(k))));
+          v -= part[k] * weight_of(k);
+        }
+        sh.stat[st][which][(row >> 3) * 16 + (row & 7)] = make_uint4(pack2(part[0], part[1], T()), pack2(part[2], part[3], T()), 0, 0);
       };
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         // a query that sees nothing, or none: its P is masked, or meets zeros; any low score will do
         const bool none = x[q] == -INFINITY;
-        put(0, q * 32 + lane, none ? -3e4f : (kLogScaleP<T> / kLog2e - x[q]) / (d.scale * kOne));
-        put(1, q * 32 + lane, none ? 0.f : -y[q] * (1.f / kOne));
+        put(0, q * 32 + lane, none ? -1e7f : (kLogScaleP<T> / kLog2e - x[q]) / d.scale);
+        put(1, q * 32 + lane, none ? 0.f : -y[q]);
       }
       fence_async();
       __syncwarp();
@@ -540,7 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     const bool row = j < keys;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);
     const float c = d.scale * kLog2e;
-    const float2 cc = make_float2(c, c), unscale = make_float2(1.f / kScaleP<T>, 1.f / kScaleP<T>);
+    const float up = scale_ds<T>(a.range, head), down = up / kScaleP<T>;
+    const float2 cc = make_float2(c, c), unscale = make_float2(down, down);
     const int see = d.causal ? max(0, j - (s.kl - s.ql)) : 0;         // the first query that sees this key
     int t = n > 0 ? first % per_head : 0;
     for (int it = 0; it < n; ++it) {
@@ -603,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       tc_fence_after();
     }
     // one group writes dv, the other dk; keys past the sequence's end get zeros
-    float f = w ? d.scale : 1.f / kScaleP<T>;
+    float f = w ? d.scale / up : 1.f / kScaleP<T>;
     if (*dead) f = __int_as_float(0x7fffffff);
     const bool has = n > 0;
     const b3r_attn_tensor& to = w ? d.dk : d.dv;
@@ -682,12 +740,15 @@ int64_t cut(BwdArgs& a) {     // returns the workspace's bytes
   // of heads the last group's long ones ended late: 529 against 427 us for dk, dv at 4096 x 4096, 32/8 heads of 128).
   a.group = d.causal ? (int)std::max<int64_t>(1, heads) : (int)std::max<int64_t>(1, std::min<int64_t>(heads, (32 << 20) / head));
   int64_t n = align256((int64_t)d.B * d.Hq * d.Lq * 4);
+  const int64_t r_off = n;
+  if (d.dtype == B3R_F16) n += align256(heads * 8);
   const int64_t q_off = n;
   if (a.q_splits > 1) n += align256((int64_t)a.q_splits * heads * d.Lq * G * d.D * 4);
   const int64_t k_off = n;
   if (a.k_splits > 1) n += align256((int64_t)a.k_splits * 2 * heads * d.Lk * d.D * 4);
   uint8_t* w = reinterpret_cast<uint8_t*>(d.work);
   a.delta = reinterpret_cast<float*>(w);
+  a.range = reinterpret_cast<float2*>(w + r_off);
   a.part_q = reinterpret_cast<float*>(w + q_off);
   a.part_k = reinterpret_cast<float*>(w + k_off);
   return n;
@@ -701,6 +762,15 @@ int launch(const BwdArgs& a, cudaStream_t s) {
   const int smem_q = fixed + (a.dq_k_stages + a.dq_v_stages) * tile, smem = fixed + (2 + a.q_stages + a.go_stages) * tile;
   B3R_REQUIRE(a.q_tiles * heads * a.q_splits <= 0x7fffffff && a.k_tiles * heads * a.k_splits <= 0x7fffffff,
               "attention backward: too many rows for one call");
+  if constexpr (__is_same(T, __half)) {
+    B3R_TRY(check_cuda(cudaMemsetAsync(a.range, 0, heads * 8, s), "attention backward"));
+    const int64_t chunks = (std::max(d.Lq, d.Lk) + kRangeRows - 1) / kRangeRows;
+    B3R_REQUIRE(chunks * d.B <= 0x7fffffff && d.Hq + d.Hkv <= 65535, "attention backward: too many rows for one call");
+    if (chunks > 0) {
+      k_attn_range<T><<<dim3((unsigned)(chunks * d.B), d.Hq + d.Hkv), 256, 0, s>>>(a, (int)chunks);
+      B3R_TRY(check_launch("attention backward"));
+    }
+  }
   if (a.q_tiles > 0 && (!d.cu_q || d.Tq > 0)) {
     static uint64_t ready = 0;
     B3R_TRY(attn_smem(k_attn_dq<DP, T>, ready, "attention dq"));

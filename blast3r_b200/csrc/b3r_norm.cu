@@ -618,8 +618,10 @@ __global__ void __launch_bounds__(kRedCols * kRedLanes) k_norm_reduce(const __gr
   }
   if (!out) return;                                // uniform over the block
   float s = 0.f;
-  if (c < a.C)
+  if (c < a.C) {
+#pragma unroll 8
     for (int64_t i = threadIdx.y; i < n; i += kRedLanes) s += p[i * stride + c];
+  }
   sh[threadIdx.y][threadIdx.x] = s;
   __syncthreads();
   if (threadIdx.y == 0 && c < a.C) {
@@ -666,9 +668,12 @@ int fwd_launch(const NormArgs& a, cudaStream_t s) {
 int bwd_threads(int C) { return (C + kE * 32 - 1) / (kE * 32) * 32; }
 
 // Blocks of the backward pass: as many as fit the 148 SMs at once (512 threads an SM, by their
-// registers), each with a run of rows.
+// registers), each with a run of rows; of 16 rows at least where that leaves a block for every SM, since
+// each block writes partial sums of every column.
 int bwd_per_sm(int C) { return std::max(1, std::min(16, 512 / bwd_threads(C))); }
-int bwd_blocks(int64_t rows, int C) { return (int)std::min<int64_t>(rows, 148 * bwd_per_sm(C)); }
+int bwd_blocks(int64_t rows, int C) {
+  return (int)std::min<int64_t>({rows, 148 * bwd_per_sm(C), std::max<int64_t>(148, rows / 16)});
+}
 
 template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>
 int bwd_kernel(const NormArgs& a, int smem, cudaStream_t s) {

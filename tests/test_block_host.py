@@ -46,7 +46,7 @@ def _desc(**kw):
 @pytest.mark.parametrize('kw,what', [(dict(dtype=L.B3R_F32), 'dtype'), (dict(D=60), 'head size'), (dict(D=136), 'head size'),
                                      (dict(Hkv=3), 'evenly'), (dict(Lq=-1), 'negative'), (dict(scale=0.0), 'scale'),
                                      (dict(scale=-1.0), 'scale'), (dict(scale=math.nan), 'scale'), (dict(), 'NULL'),
-                                     (dict(cu_q=16), 'cu_k'), (dict(B=40000), '65535')])
+                                     (dict(cu_q=16), 'cu_k'), (dict(B=1 << 30), 'too many')])
 def test_c_abi_refuses_bad_attention_descriptors(kw, what):
     d = _desc(**kw)
     for f in ('b3r_attention_fwd', 'b3r_attention_bwd'):

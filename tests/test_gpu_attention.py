@@ -152,6 +152,27 @@ def test_large_scores():
     _check(q, k, v, do, [(0, 150, 260)], False, False)
 
 
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('size,scale', [(64.0, None), (2.0 ** -6, None), (1.0, 1e-4), (1.0, 3.0)])
+def test_sizes_of_gradients_and_scales(dtype, size, scale):
+    """Large and small gradients, and scales far from D^-0.5 (many equal scores; one key that takes all)."""
+    q, k, v, do = _dense(1, 200, 300, 4, 2, 64, dtype)
+    _check(q, k, v, do * size, [(0, 200, 300)], False, True, scale=scale)
+
+
+def test_many_sequences():
+    """More sequences x heads than a grid's second dimension holds."""
+    from blast3r_b200.attention import attention_backward, attention_forward
+    B = 70000
+    q, k, v, do = (_rand(B, 2, 1, 8, dtype=torch.float16, seed=s) for s in range(4))
+    o, lse = attention_forward(q, k, v)
+    dq, dk, dv = attention_backward(do, q, k, v, o, lse)
+    at = torch.tensor([0, 1, 65535, 65536, B - 1], device='cuda')
+    want = R.attention(q[at], k[at], v[at], do[at], o[at], False, 8 ** -0.5, [(b, 2, 2) for b in range(5)], False)
+    for name, t in dict(o=o, lse=lse, dq=dq, dk=dk, dv=dv).items():
+        R.close(t[at], *want[name], name)
+
+
 def test_same_results_every_time_and_on_another_stream():
     q, k, v, do = _dense(2, 300, 300, 8, 2, 128, 'bf16')
     from blast3r_b200.attention import attention_backward, attention_forward
