@@ -333,15 +333,20 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
 enum { kDwPost, kDbPost, kDwPre, kDbPre, kCols };
 
 // Rows of the stages of the ring: dr, r (stream type), dh, y, one after the other.
-template <typename TX, typename TY>
+// Without VEC a row may begin anywhere: the whole 16-byte units that hold it are copied, and its
+// place in the first one is kept.
+template <typename T, bool VEC>
+__host__ __device__ inline int slot_bytes(int C) {
+  return VEC ? C * (int)sizeof(T) : (C * (int)sizeof(T) + 30) & ~15;
+}
+template <typename TX, typename TY, bool VEC>
 __host__ __device__ inline int stage_bytes(int C) {
-  return C * (2 * (int)sizeof(TX) + 2 * (int)sizeof(TY));
+  return 2 * slot_bytes<TX, VEC>(C) + 2 * slot_bytes<TY, VEC>(C);
 }
 
 // FULL: with means (layer norm) or biases.  RING: rows come through a ring of `stages` rows in
 // shared memory, filled by bulk copies that run ahead of the arithmetic without holding registers;
-// else (two rows do not fit, or VEC does not hold) each thread reads its columns directly.  Weights
-// lie in shared memory as float32; a thread only touches its own columns of them.
+// else (two rows do not fit) each thread reads its columns directly.  Weights lie in shared memory as float32; a thread only touches its own columns of them.
 template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>
 __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormArgs a) {
   extern __shared__ __align__(128) uint8_t dyn[];
@@ -357,20 +362,29 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
   float* const weights = reinterpret_cast<float*>(dyn);     // w_pre, w_post, gate, and b_post
   uint8_t* const ring = dyn + (FULL ? 4 : 3) * stride * sizeof(float);
   const bool need_y = a.post || a.gate;
-  const int bytes_x = C * (int)sizeof(TX), bytes_y = C * (int)sizeof(TY);
-  const uint32_t expect = bytes_x + (a.pre ? bytes_x + bytes_y : 0) + (need_y ? bytes_y : 0);
+  const int bytes_x = slot_bytes<TX, VEC>(C), bytes_y = slot_bytes<TY, VEC>(C);
   auto request = [&](int64_t row) {                         // one thread: the copies of a row
     if (row >= last) return;
     const int st = (int)((row - first) % a.stages);
     const uint32_t bar = smem_u32(&full[st]);
-    uint8_t* to = ring + (size_t)st * stage_bytes<TX, TY>(C);
-    mbar_expect(bar, expect);
-    bulk_copy(smem_u32(to), reinterpret_cast<const TX*>(a.dr) + row * a.dr_row, bytes_x, bar);
-    if (a.pre) {
-      bulk_copy(smem_u32(to + bytes_x), reinterpret_cast<const TX*>(a.x) + row * a.x_row, bytes_x, bar);
-      bulk_copy(smem_u32(to + 2 * bytes_x), reinterpret_cast<const TY*>(a.dh) + row * a.dh_row, bytes_y, bar);
+    uint8_t* to = ring + (size_t)st * stage_bytes<TX, TY, VEC>(C);
+    const void* from[4] = {reinterpret_cast<const TX*>(a.dr) + row * a.dr_row, reinterpret_cast<const TX*>(a.x) + row * a.x_row,
+                           reinterpret_cast<const TY*>(a.dh) + row * a.dh_row, reinterpret_cast<const TY*>(a.y) + row * a.y_row};
+    const int at[4] = {0, bytes_x, 2 * bytes_x, 2 * bytes_x + bytes_y};
+    uint32_t n[4], all = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t bytes = C * (k < 2 ? sizeof(TX) : sizeof(TY));
+      n[k] = VEC ? bytes : ((uint32_t)(reinterpret_cast<uintptr_t>(from[k]) & 15) + bytes + 15) & ~15u;
+      if (k == 0 || (k == 3 ? need_y : a.pre != 0)) all += n[k];
+      else n[k] = 0;
     }
-    if (need_y) bulk_copy(smem_u32(to + 2 * bytes_x + bytes_y), reinterpret_cast<const TY*>(a.y) + row * a.y_row, bytes_y, bar);
+    mbar_expect(bar, all);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n[k])
+        bulk_copy(smem_u32(to + at[k]), VEC ? from[k] : reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(from[k]) & ~uintptr_t(15)), n[k],
+                  bar);
   };
   clear_sums(buf);
   if (RING && tid == 0) {
@@ -415,13 +429,20 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
   }
   int st = 0, round = 0;
   for (int64_t row = first; row < last; ++row) {
-    const uint8_t* at = ring + (size_t)st * stage_bytes<TX, TY>(C);
+    const uint8_t* at = ring + (size_t)st * stage_bytes<TX, TY, VEC>(C);
     auto fetch = [&](float2 (&o)[kP], int off, auto type, const void* p, int64_t step, bool on) {
       using T = decltype(type);
 #pragma unroll
       for (int j = 0; j < kP; ++j) o[j] = both(0.f);
       if (!on) return;
-      if constexpr (RING) {
+      if constexpr (RING && !VEC) {
+        const T* q = reinterpret_cast<const T*>(at + off + (reinterpret_cast<uintptr_t>(reinterpret_cast<const T*>(p) + row * step) & 15));
+#pragma unroll
+        for (int j = 0; j < kP; ++j) {
+          const int c0 = col_of<false>(0, 2 * j, tid, threads), c1 = col_of<false>(0, 2 * j + 1, tid, threads);
+          o[j] = make_float2(c0 < C ? ld1(q + c0) : 0.f, c1 < C ? ld1(q + c1) : 0.f);
+        }
+      } else if constexpr (RING) {
         if (cols) {
           Raw8<T> d;
           const uint4* q = reinterpret_cast<const uint4*>(at + off + tid * kE * (int)sizeof(T));
@@ -685,12 +706,12 @@ int bwd_kernel(const NormArgs& a, int smem, cudaStream_t s) {
 
 template <typename TX, typename TY, bool FULL, bool VEC>
 int bwd_launch(NormArgs a, cudaStream_t s) {
-  const int threads = bwd_threads(a.C), stage = stage_bytes<TX, TY>(a.C);
+  const int threads = bwd_threads(a.C), stage = stage_bytes<TX, TY, VEC>(a.C);
   const int weights = (FULL ? 4 : 3) * threads * kE * 4, room = (227 * 1024) / bwd_per_sm(a.C) - 3072;
   a.stages = std::min(kMaxStages, (room - weights) / stage);
-  if (VEC && a.stages >= 2) {
+  if (a.stages >= 2) {
     const int smem = weights + a.stages * stage;
-    return threads <= 512 ? bwd_kernel<TX, TY, FULL, VEC, VEC, 512>(a, smem, s) : bwd_kernel<TX, TY, FULL, VEC, VEC, 1024>(a, smem, s);
+    return threads <= 512 ? bwd_kernel<TX, TY, FULL, VEC, true, 512>(a, smem, s) : bwd_kernel<TX, TY, FULL, VEC, true, 1024>(a, smem, s);
   }
   return bwd_kernel<TX, TY, FULL, VEC, false, 1024>(a, weights, s);
 }
