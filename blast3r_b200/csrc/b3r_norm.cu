@@ -162,54 +162,65 @@ __device__ __forceinline__ float2 inside(int v, int j, int tid, int threads, int
   return make_float2(col_of<VEC>(v, 2 * j, tid, threads) < C ? 1.f : 0.f, col_of<VEC>(v, 2 * j + 1, tid, threads) < C ? 1.f : 0.f);
 }
 
-constexpr int kSums = 4;   // values of one row_sum at most
-// Sums of K values over the row's threads, by shuffles within a warp and through `buf` (two sets of kSums x
-// 32 floats used in turn, so one barrier per call is enough) over the warps, in a fixed order.  Two or
+constexpr int kSums = 8;   // room for the values of one row_sum
+template <int MAXW>
+constexpr int kSumRow = MAXW == 32 ? 32 : 16;            // floats of a value's warps
+template <int MAXW>
+constexpr int kSumFloats = 2 * kSums * kSumRow<MAXW>;
+// Sums of K values over the row's threads, by shuffles within a warp and through `buf` (two sets, used in
+// turn, so one barrier per call is enough) over the warps, in a fixed order.  Two or
 // more values share their shuffles: after a step that swaps them, half of the lanes go on with each.
 template <int K, int MAXW>
 __device__ __forceinline__ void row_sum(float (&s)[K], int warps, float* buf, int& turn) {
+  static_assert(K == 1 || K == 2 || K == 3 || K == 6);
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   auto swap = [&](float a, float b, int d) {           // lanes without bit d go on with a, the others with b
     const bool up = lane & d;
     return (up ? b : a) + __shfl_xor_sync(0xffffffffu, up ? a : b, d);
   };
+  auto fold = [&](float a, int d) { return a + __shfl_xor_sync(0xffffffffu, a, d); };
   float v;
-  int first = 16;                                      // the next step's distance
+  constexpr int first = K == 1 ? 16 : K == 2 ? 8 : K == 3 ? 4 : 2;   // the distance at which one value a lane is left
   if constexpr (K == 1) {
     v = s[0];
   } else if constexpr (K == 2) {
     v = swap(s[0], s[1], 16);
-    first = 8;
+  } else if constexpr (K == 3) {
+    v = swap(swap(s[0], s[1], 16), fold(s[2], 16), 8);
   } else {
-    v = swap(swap(s[0], s[1], 16), K == 4 ? swap(s[2], s[K - 1], 16) : s[2] + __shfl_xor_sync(0xffffffffu, s[2], 16), 8);
-    first = 4;
+    v = swap(swap(swap(s[0], s[1], 16), swap(s[2], s[3], 16), 8), fold(swap(s[4], s[5], 16), 8), 4);
   }
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1)
-    if (d <= first) v += __shfl_xor_sync(0xffffffffu, v, d);
-  // where value k ended up: bit 16 tells 0 from 1 (and 2 from 3), bit 8 the pairs apart
-  auto lane_of = [](int k) { return K == 1 ? 0 : (k & 1) * 16 + (k >> 1) * 8; };
+  for (int d = first; d > 0; d >>= 1) v = fold(v, d);
+  // value k ended up in the lanes whose bits 16, 8 and 4 are the bits 1, 2 and 4 of k
   if (warps == 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) s[k] = K == 1 ? v : __shfl_sync(0xffffffffu, v, lane_of(k));
+    for (int k = 0; k < K; ++k) s[k] = K == 1 ? v : __shfl_sync(0xffffffffu, v, (k & 1) * 16 + (k >> 1 & 1) * 8 + (k >> 2) * 4);
     return;
   }
-  float* b = buf + turn * kSums * 32;
+  constexpr int kRow = kSumRow<MAXW>;                  // entries past the last warp stay zero
+  float* b = buf + turn * kSums * kRow;
   turn ^= 1;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-    if (lane == lane_of(k)) b[k * 32 + w] = v;
+  const int mine = (lane >> 4) | (lane >> 2 & 2) | (lane & 4);
+  if ((lane & (2 * first - 1)) == 0 && (K == 1 || mine < K)) b[(K == 1 ? 0 : mine) * kRow + w] = v;
   __syncthreads();
+  if constexpr (MAXW == 32) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {                        // entries past the last warp stay zero
-    float t = b[k * 32 + (lane & (MAXW - 1))];
+    for (int k = 0; k < K; ++k) {
+      float t = b[k * kRow + lane];
 #pragma unroll
-    for (int d = MAXW / 2; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
-    s[k] = t;
+      for (int d = 16; d > 0; d >>= 1) t = fold(t, d);
+      s[k] = t;
+    }
+  } else {                                             // four lanes add up each value's row, four entries to a lane
+    const float4 x = reinterpret_cast<const float4*>(b + (lane >> 2) * kRow)[lane & 3];
+    const float t = fold(fold((x.x + x.y) + (x.z + x.w), 1), 2);
+#pragma unroll
+    for (int k = 0; k < K; ++k) s[k] = __shfl_sync(0xffffffffu, t, 4 * k);
   }
 }
-__device__ __forceinline__ void clear_sums(float* buf) {
-  for (int i = threadIdx.x; i < 2 * kSums * 32; i += blockDim.x) buf[i] = 0.f;
+__device__ __forceinline__ void clear_sums(float* buf, int n) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) buf[i] = 0.f;
 }
 
 struct NormArgs {
@@ -229,12 +240,12 @@ struct NormArgs {
 // POST: with a norm of y, y and x are both held until its statistics are known; without it, only r.
 template <typename TX, typename TY, int VPT, bool VEC, bool POST>
 __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormArgs a) {
-  __shared__ alignas(16) float buf[2 * kSums * 32];
+  __shared__ alignas(16) float buf[kSumFloats<8>];
   // blockDim.x threads to a row; blocks of several rows have one warp to a row
   const int threads = blockDim.x, tid = threadIdx.x, warps = threads >> 5, C = a.C;
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (warps > 1) {
-    clear_sums(buf);
+    clear_sums(buf, kSumFloats<8>);
     __syncthreads();
   }
   if (row >= a.rows) return;                       // uniform over the row's threads
@@ -346,11 +357,19 @@ __host__ __device__ inline int stage_bytes(int C) {
 
 // FULL: with means (layer norm) or biases.  RING: rows come through a ring of `stages` rows in
 // shared memory, filled by bulk copies that run ahead of the arithmetic without holding registers;
-// else (two rows do not fit) each thread reads its columns directly.  Weights lie in shared memory as float32; a thread only touches its own columns of them.
+// else (two rows do not fit) each thread reads its columns directly.  Weights lie in shared memory as
+// float32; a thread only touches its own columns of them.
+//
+// Without means every sum of a row is linear in the raw products, the statistics being factors: with
+// p = w_post g y and rho, sigma the inverse norms of r and y,
+//   sum(dn w_post yhat) = sigma (sum dr p + rho (sum z p - rho^2 mean(z r) sum r p)),
+// so six sums and one barrier a row do (32768 rows of 4096: 381 us, with a second sum after the first 456).
+// With means the centred rows are summed: three barriers.  1024 threads have no registers for the six: two.
 template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>
 __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormArgs a) {
+  constexpr bool kOne = !FULL && MAXT <= 512;   // one sum a row
   extern __shared__ __align__(128) uint8_t dyn[];
-  __shared__ alignas(16) float buf[2 * kSums * 32];
+  __shared__ alignas(16) float buf[kSumFloats<MAXT / 32>];
   __shared__ uint64_t full[kMaxStages];
   __shared__ int dead_flag;
   volatile int* dead = &dead_flag;
@@ -386,7 +405,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         bulk_copy(smem_u32(to + at[k]), VEC ? from[k] : reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(from[k]) & ~uintptr_t(15)), n[k],
                   bar);
   };
-  clear_sums(buf);
+  clear_sums(buf, kSumFloats<MAXT / 32>);
   if (RING && tid == 0) {
     dead_flag = 0;
     for (int i = 0; i < a.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
@@ -484,18 +503,51 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         y[j] = mul2(add2(y[j], both(mu_y)), in);
       }
     }
-    float2 t[3] = {both(0.f), both(0.f), both(0.f)};
+    float2 w[kP], g[kP];
+    auto gate_weights = [&] {
+      if (a.gate && row == group_end) {                      // uniform: the block's rows enter another gate row
+        if (!a.gate_direct && cols) {
+#pragma unroll
+          for (int j = 0; j < kE; ++j) {
+            const int c = col_of<VEC>(0, j, tid, threads);
+            if (c < C) a.gpart[(blockIdx.x + group) * C + c] = (j & 1) ? dg[j / 2].y : dg[j / 2].x;
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kP; ++j) dg[j] = both(0.f);
+        ++group;
+        group_end += a.rows_per_gate;
+        keep(2, reinterpret_cast<const char*>(a.gate) + group * C * (a.wf32 ? 4 : sizeof(TY)), 1.f);
+      }
+      weight(1, w);
+      if (a.gate) weight(2, g);
+    };
+    if (kOne) gate_weights();
+    constexpr int kQ = kOne ? 6 : 3;
+    float2 t[kQ];
+#pragma unroll
+    for (int k = 0; k < kQ; ++k) t[k] = both(0.f);
 #pragma unroll
     for (int j = 0; j < kP; ++j) {
       t[0] = fma2(r[j], r[j], t[0]);
       t[1] = fma2(y[j], y[j], t[1]);
       t[2] = fma2(z[j], r[j], t[2]);
+      if constexpr (kOne) {
+        float2 p = mul2(w[j], y[j]);
+        if (a.gate) p = mul2(g[j], p);
+        t[3] = fma2(d[j], p, t[3]);
+        t[4] = fma2(z[j], p, t[4]);
+        t[5] = fma2(r[j], p, t[5]);
+      }
     }
-    float q[3] = {t[0].x + t[0].y, t[1].x + t[1].y, t[2].x + t[2].y};
-    row_sum<3, MAXT / 32>(q, warps, buf, turn);
+    float q[kQ];
+#pragma unroll
+    for (int k = 0; k < kQ; ++k) q[k] = t[k].x + t[k].y;
+    row_sum<kQ, MAXT / 32>(q, warps, buf, turn);
     if (RING && tid == 0 && row > first) request(row - 1 + a.stages);   // every thread has left the row before
     if (a.pre) {
       const float rstd = rsqrtf(q[0] * inv + a.eps), proj = -q[2] * inv * rstd;   // -mean(z rhat)
+      if constexpr (kOne) q[3] += rstd * (q[4] + proj * rstd * q[5]);
 #pragma unroll
       for (int j = 0; j < kP; ++j) {
         const float2 hat = mul2(r[j], both(rstd));
@@ -514,25 +566,9 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
     const float rstd = a.post ? rsqrtf(q[1] * inv + a.eps) : 1.f;
 #pragma unroll
     for (int j = 0; j < kP; ++j) y[j] = mul2(y[j], both(rstd));        // yhat
-    float2 w[kP];
-    weight(1, w);
+    if (!kOne) gate_weights();
     if (a.gate) {
-      if (row == group_end) {                      // uniform: the block's rows enter another gate row
-        if (!a.gate_direct && cols) {
-#pragma unroll
-          for (int j = 0; j < kE; ++j) {
-            const int c = col_of<VEC>(0, j, tid, threads);
-            if (c < C) a.gpart[(blockIdx.x + group) * C + c] = (j & 1) ? dg[j / 2].y : dg[j / 2].x;
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < kP; ++j) dg[j] = both(0.f);
-        ++group;
-        group_end += a.rows_per_gate;
-        keep(2, reinterpret_cast<const char*>(a.gate) + group * C * (a.wf32 ? 4 : sizeof(TY)), 1.f);
-      }
-      float2 g[kP], b[kP];
-      weight(2, g);
+      float2 b[kP];
       if (FULL) weight(3, b);
 #pragma unroll
       for (int j = 0; j < kP; ++j) {
@@ -552,14 +588,17 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         acc[kDwPost][j] = fma2(d[j], y[j], acc[kDwPost][j]);
         if (FULL) acc[kDbPost][j] = add2(acc[kDbPost][j], d[j]);
         d[j] = mul2(d[j], w[j]);
-        if (FULL) u[0] = add2(u[0], d[j]);
-        u[1] = fma2(d[j], y[j], u[1]);
+        if constexpr (FULL) u[0] = add2(u[0], d[j]);
+        if constexpr (!kOne) u[1] = fma2(d[j], y[j], u[1]);
       }
       float s[FULL ? 2 : 1];
       s[0] = u[1].x + u[1].y;
-      if (FULL) s[FULL ? 1 : 0] = u[0].x + u[0].y;
-      row_sum<FULL ? 2 : 1, MAXT / 32>(s, warps, buf, turn);
-      const float mz = FULL ? -s[FULL ? 1 : 0] * inv_mean : 0.f, proj = -s[0] * inv;
+      if constexpr (FULL) s[1] = u[0].x + u[0].y;
+      if constexpr (kOne) s[0] = rstd * q[3];
+      else row_sum<FULL ? 2 : 1, MAXT / 32>(s, warps, buf, turn);
+      float mz = 0.f;
+      if constexpr (FULL) mz = -s[1] * inv_mean;
+      const float proj = -s[0] * inv;
 #pragma unroll
       for (int j = 0; j < kP; ++j) {
         const float2 v = fma2(y[j], both(proj), FULL ? add2(d[j], both(mz)) : d[j]);
