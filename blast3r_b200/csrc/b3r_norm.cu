@@ -16,6 +16,13 @@
 // next row's loads in flight, and keeps the column sums (dw, db, dg) in registers; it writes them
 // once as a partial, and a second kernel adds the partials in a fixed order: no atomics, so the
 // results do not change from run to run.
+//
+// Measured on one B200, where a copy moves 6.5 TB/s: forward, 49216 layer-norm rows of 1024, float32 stream and
+// bfloat16 branch, 93 us (6.5 TB/s); backward, 32768 RMS rows of 4096, bfloat16, two norms and a gate, 383 us
+// (4.2 TB/s) and 7 us for the partials.  There one block of 512 threads fills an SM's registers, so the
+// latency of a row's sum, barrier included, is hidden by nothing but the copies of the next rows.  Rows
+// without vector alignment are read one element at a time and take twice as long (forward: 18600
+// rows of 2647, 340 us).
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

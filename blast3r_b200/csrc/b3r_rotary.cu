@@ -11,6 +11,12 @@
 // widest vector that the layout and the alignment allow.  It reads the slot's cosines and
 // sines once and keeps them in registers while it walks over four heads, the loads
 // of two or four in flight at a time; neighbouring threads own neighbouring slots.
+//
+// Measured on one B200, where a copy moves 6.5 TB/s: 49152 tokens of 2 x 16 float16 heads of 64, half pairs on two
+// axes, 78 us (5.2 TB/s); 65536 tokens of 32 + 8 bfloat16 heads of 128, 64 of them turned as interleaved pairs, 293 us
+// (4.6 TB/s, at 57 % of the issue slots): latency at 32 warps an SM bounds it; batches of four in
+// the half layout (95 us) and 48 warps (86) were slower.  Where only single pairs line up (17 pairs to a section,
+// heads of 120) the same bytes take four times their copy.  A single token takes 2.9 us.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
