@@ -21,11 +21,11 @@
 // operands' type for the product (its sum is taken before, in float32).
 //
 // What bounds it, measured on one B200 (1669 TFLOP/s, 6.5 TB/s):
-//   one query over 32768 keys (16 sequences, 32/8 heads of 128): 239 us, 5.3 TB/s: HBM
-//   769 x 769 (64 sequences, 16 heads of 64, float16): 440 us, 352 TFLOP/s: the exponentials (16 a cycle and SM: 2048
+//   one query over 32768 keys (16 sequences, 32/8 heads of 128): 228 us, 5.6 TB/s: HBM
+//   769 x 769 (64 sequences, 16 heads of 64, float16): 421 us, 368 TFLOP/s: the exponentials (16 a cycle and SM: 2048
 //     cycles a step of two tiles, which takes 2100 to 2500), tiles that 769 = 6 x 128 + 1 leaves nearly
 //     empty, and 4000 cycles at a job's end
-//   16384 x 16384, causal, 16/4 heads of 128: 885 us in a burst, 1240 TFLOP/s (1050 to 1080 in a long run, at the power
+//   16384 x 16384, causal, 16/4 heads of 128: 885 us in a burst, 1240 TFLOP/s (1030 to 1080 in a long run, at the power
 //     limit): the products, 88 cycles for each 16 of the head size with Q in shared memory
 #include <algorithm>
 #include "b3r_attn.cuh"
@@ -502,7 +502,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       AttnSeq sq_;
       sq_.ql = j.ql;
       sq_.kl = j.kl;
-      const int bound = row && i < j.ql ? attn_bound(sq_, i, d.causal) : 0;
+      // (past the rows nothing is written: such a thread sees what lets its warp take whole tiles)
+      const int bound = !row ? j.kl : i < j.ql ? attn_bound(sq_, i, d.causal) : 0;
       if (!a.q_tma) {
         if (w == 0 || !a.one) {
           // the row of Q into the swizzled tile; zeros past D and past the rows
@@ -533,53 +534,86 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
           if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[w][bar]));
           continue;
         }
-        uint32_t s[kTileRows];
+        auto follow = [&](float top) {                   // moves mx after the true maximum, O and l with it
+          const bool grow = top > mx + kGrow || mx == -INFINITY;   // (mx = -inf: nothing summed yet)
+          if (it > 0 && __any_sync(0xffffffffu, grow && top > mx)) {
+            const float f = grow && top > mx ? ex2(mx - top) : 1.f;      // 0 for the first key that the row sees
+            mbar_wait(smem_u32(&sh.o_done[w]), (mine - 1) & 1, dead);
+            tc_fence_after();
 #pragma unroll
-        for (int q = 0; q < kTileRows; q += 32) tc_ld32(at + q, s + q);
-        tc_wait_ld(s);
-        if (!__all_sync(0xffffffffu, lim >= kTileRows)) {
+            for (int q = 0; q < DP; q += 32) {
+              uint32_t o[32];
+              tc_ld32(quarter + X::kOut + w * DP + q, o);
+              tc_wait_ld(o);
 #pragma unroll
-          for (int q = 0; q < kTileRows; ++q) s[q] = q < lim ? s[q] : 0xff800000u;
-        }
-        float t[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[4 + e]));
-#pragma unroll
-        for (int q = 8; q < kTileRows; q += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(t[e], __uint_as_float(s[q + e])), __uint_as_float(s[q + 4 + e]));
-        const float top = fmaxf(mx, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c);
-        const bool grow = top > mx + kGrow || mx == -INFINITY;   // (mx = -inf: nothing summed yet)
-        if (it > 0 && __any_sync(0xffffffffu, grow && top > mx)) {
-          const float f = grow && top > mx ? ex2(mx - top) : 1.f;      // 0 for the first key that the row sees
-          mbar_wait(smem_u32(&sh.o_done[w]), (mine - 1) & 1, dead);
-          tc_fence_after();
-#pragma unroll
-          for (int q = 0; q < DP; q += 32) {
-            uint32_t o[32];
-            tc_ld32(quarter + X::kOut + w * DP + q, o);
-            tc_wait_ld(o);
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tc_st32(quarter + X::kOut + w * DP + q, o);
+              for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              tc_st32(quarter + X::kOut + w * DP + q, o);
+            }
+            l *= f;
           }
-          l *= f;
-        }
-        if (grow) mx = top;
-        const float2 cc = make_float2(c, c), mm = make_float2(mx == -INFINITY ? 0.f : -mx, mx == -INFINITY ? 0.f : -mx);
+          if (grow) mx = top;
+        };
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-#pragma unroll
-        for (int q0 = 0; q0 < kTileRows / 2; q0 += 16) {
+        auto exps = [&](const uint32_t* s, uint32_t to) {   // 32 columns of P
+          const float2 cc = make_float2(c, c), mm = make_float2(mx == -INFINITY ? 0.f : -mx, mx == -INFINITY ? 0.f : -mx);
           uint32_t p[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) {
-            float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * (q0 + e)]), __uint_as_float(s[2 * (q0 + e) + 1])), cc, mm);
+            float2 x = __ffma2_rn(make_float2(__uint_as_float(s[2 * e]), __uint_as_float(s[2 * e + 1])), cc, mm);
             x.x = ex2(x.x);
             x.y = ex2(x.y);
             sum[e & 1] = __fadd2_rn(sum[e & 1], x);
             p[e] = pack2(x.x, x.y, T());
           }
-          tc_st16(at + q0, p);
+          tc_st16(to, p);
+        };
+        if (__all_sync(0xffffffffu, lim >= kTileRows)) {
+          uint32_t s[kTileRows];
+#pragma unroll
+          for (int q = 0; q < kTileRows; q += 32) tc_ld32(at + q, s + q);
+          tc_wait_ld(s);
+          float t[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) t[e] = fmaxf(__uint_as_float(s[e]), __uint_as_float(s[4 + e]));
+#pragma unroll
+          for (int q = 8; q < kTileRows; q += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = fmaxf(fmaxf(t[e], __uint_as_float(s[q + e])), __uint_as_float(s[q + 4 + e]));
+          follow(fmaxf(mx, fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])) * c));
+#pragma unroll
+          for (int q = 0; q < kTileRows; q += 32) exps(s + q, at + q / 2);
+        } else {
+          // a tile that ends inside: 32 columns at a time, up to the last one that a row of the warp sees (in a body of
+          // its own, 421 us for 64 x 769 x 769 and 16 heads of 64; with masks in one body for all tiles 441, and
+          // with branches around each half of one body 445)
+          const int end = __reduce_max_sync(0xffffffffu, lim);
+          float t = -INFINITY;
+          uint32_t s[32];
+          auto some = [&](int q) {
+            tc_ld32(at + q, s);
+            tc_wait_ld(s);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e] = q + e < lim ? s[e] : 0xff800000u;
+          };
+#pragma unroll 1
+          for (int q = 0; q < min(end, kTileRows); q += 32) {
+            some(q);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) t = fmaxf(t, __uint_as_float(s[e]));
+          }
+          follow(fmaxf(mx, t * c));
+#pragma unroll 1
+          for (int q = 0; q < kTileRows; q += 32) {
+            if (q < end) {
+              some(q);                                   // (P only overwrites scores that have been read)
+              exps(s, at + q / 2);
+            } else {
+              uint32_t p[16];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) p[e] = 0;
+              tc_st16(at + q / 2, p);
+            }
+          }
         }
         tc_wait_st();
         // the last step's product ends long before, but has to be seen: o_done's turns are met one by one
