@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(256) k_attn_range(const __grid_constant__ BwdA
 // shared memory costs about 100 cycles for each 16 of the head size where one in tensor memory costs the product's 64,
 // so Q and dO are copied over once.  Measured on one B200: 2 x 4096 causal, 32/8 heads of 128, 351 us (1170 TFLOP/s over
 // the three products: tensor pipe 59 % busy, the elementwise part beside it); 20 packed sequences of up to 1025,
-// 16 heads of 64, 136 us (a third of a block's time is its start and end).
+// 16 heads of 64, 134 us (a third of a block's time is its start and end).
 template <int DP, typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__ BwdArgs a) {
   extern __shared__ uint8_t raw[];
@@ -366,8 +366,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
     const float delta = sh.delta[r], lse = lse_in == -INFINITY ? INFINITY : lse_in * kLog2e;   // nothing seen: P = 0
     const float up = scale_ds<T>(a.range, head);
     const float2 cc = make_float2(c, c), ll = make_float2(-lse, -lse), dd = make_float2(-delta * up, -delta * up), uu = make_float2(up, up);
+    const int sees = row ? bound : s.kl;               // past the rows nothing is written, so no mask is needed there
     for (int it = 0; it < n; ++it) {
-      const int lim = bound - (first + it) * kTileRows - w * 64;     // of this thread's 64 keys, how many its row sees
+      const int lim = sees - (first + it) * kTileRows - w * 64;      // of this thread's 64 keys, how many its row sees
       const uint32_t at = quarter + w * 64;
       mbar_wait(smem_u32(&sh.s_full[0]), it & 1, dead);
       tc_fence_after();
