@@ -15,8 +15,8 @@
 // Measured on one B200, where a copy moves 6.5 TB/s: 49152 tokens of 2 x 16 float16 heads of 64, half pairs on two
 // axes, 78 us (5.2 TB/s); 65536 tokens of 32 + 8 bfloat16 heads of 128, 64 of them turned as interleaved pairs, 293 us
 // (4.6 TB/s, at 57 % of the issue slots): latency at 32 warps an SM bounds it; batches of four in
-// the half layout (95 us) and 48 warps (86) were slower.  Where only single pairs line up (17 pairs to a section,
-// heads of 120) the same bytes take four times their copy.  A single token takes 2.9 us.
+// the half layout (95 us) and 48 warps (86) were slower.  A single token takes 2.9 us.  Sections that no 16-byte
+// vector divides take the second kernel.
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -139,6 +139,93 @@ __global__ void __launch_bounds__(kRotThreads, 4) k_rotary(const __grid_constant
   }
 }
 
+// Sections that no 16-byte vector divides.  A block takes `per` whole tokens through shared memory: 16-byte pieces
+// of the heads come in with all of a thread's loads in flight, a thread turns one pair of a token in every head
+// with its angle in registers, and the pieces go out again.  Measured on one B200 (and with narrower vectors
+// straight from memory instead): 214478 tokens of 8 + 4 float16 heads of 120, 51 pairs, 351 us, 3.5 TB/s (777);
+// 65536 of 16 + 4 bfloat16 heads of 64, 18 pairs 88 us (189), 20 pairs 89 (124), 20 interleaved 70 (70); 512 of
+// these with 19 pairs 4.9 (7.3).  The pairs' two-byte accesses to shared memory bound it.
+constexpr int kRowPieces = 6;   // of a thread
+constexpr int kRowBytes = kRowPieces * kRotThreads * 16;
+
+// x / d for x d < 2^32: the high half of x ceil(2^32 / d)
+struct Div {
+  uint32_t d, mul;
+  explicit Div(uint32_t n = 1) : d(n), mul(n == 1 ? 0 : (uint32_t)(((uint64_t(1) << 32) + n - 1) / n)) {}
+  __device__ __forceinline__ uint32_t of(uint32_t x) const { return mul ? __umulhi(x, mul) : x; }
+};
+struct RowDivs {
+  Div pieces, heads[2], pairs, half;
+  int per;
+};
+
+template <typename T, bool IL>
+__global__ void __launch_bounds__(kRotThreads) k_rotary_rows(const __grid_constant__ RotArgs a, const __grid_constant__ RowDivs v, uint32_t tokens) {
+  __shared__ alignas(16) uint4 rows[kRowPieces * kRotThreads];
+  const int tid = threadIdx.x;
+  const b3r_rotary_part& pt = a.part[blockIdx.y];
+  if (pt.heads == 0) return;
+  const Div heads = v.heads[blockIdx.y];
+  const uint32_t first = blockIdx.x * v.per, n = min(tokens - first, (uint32_t)v.per), all = n * heads.d * v.pieces.d;
+  const uint32_t b0 = first / (uint32_t)a.T, t0 = first - b0 * (uint32_t)a.T;
+  auto place = [&](uint32_t x, int64_t batch, int64_t token, int64_t head) {   // of piece x, in elements
+    const uint32_t row = v.pieces.of(x), i = heads.of(row), h = row - i * heads.d;
+    uint32_t t = t0 + i, b = b0;
+    if (t >= (uint32_t)a.T) {
+      const uint32_t q = t / (uint32_t)a.T;
+      b += q;
+      t -= q * (uint32_t)a.T;
+    }
+    return b * batch + t * token + h * head + (x - row * v.pieces.d) * (16 / sizeof(T));
+  };
+  uint4 x[kRowPieces];
+#pragma unroll
+  for (int u = 0; u < kRowPieces; ++u)
+    if (tid + u * kRotThreads < all)
+      x[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(pt.x) +
+                                             place(tid + u * kRotThreads, pt.x_batch, pt.x_token, pt.x_head));
+#pragma unroll
+  for (int u = 0; u < kRowPieces; ++u)
+    if (tid + u * kRotThreads < all) rows[tid + u * kRotThreads] = x[u];
+  __syncthreads();
+  for (uint32_t it = tid; it < n * v.pairs.d; it += kRotThreads) {
+    const uint32_t i = v.pairs.of(it), pr = it - i * v.pairs.d, ax = v.half.of(pr), k = pr - ax * v.half.d;
+    const uint32_t tok = first + i, b = tok / (uint32_t)a.T;
+    const int64_t at = b * a.pos_batch + (tok - b * (uint32_t)a.T) * a.pos_token + ax;
+    const int64_t p = a.pos64 ? reinterpret_cast<const int64_t*>(a.pos)[at] : (int64_t) reinterpret_cast<const int32_t*>(a.pos)[at];
+    const float nan = __int_as_float(0x7fffffff);   // (as in k_rotary)
+    const float2 cs = (p >= 0 && p < a.n_pos) ? __ldg(a.table + p * a.half + k) : make_float2(nan, nan);
+    const float s = a.inverse ? -cs.y : cs.y;
+    T* lo = reinterpret_cast<T*>(rows) + i * heads.d * a.D + ax * 2 * a.half + (IL ? 2 * k : k);
+    T* hi = lo + (IL ? 1 : a.half);
+#pragma unroll 4
+    for (uint32_t h = 0; h < heads.d; ++h, lo += a.D, hi += a.D) {
+      const float u = to_f(*lo), w = to_f(*hi);
+      *lo = from_f<T>(u * cs.x - w * s);
+      *hi = from_f<T>(w * cs.x + u * s);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kRowPieces; ++u)
+    if (tid + u * kRotThreads < all)
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(pt.out) + place(tid + u * kRotThreads, pt.out_batch, pt.out_token, pt.out_head)) =
+          rows[tid + u * kRotThreads];
+}
+
+// Whether heads can be moved in 16-byte pieces, and how many tokens fit a block: 0 if none.
+template <typename T>
+int rot_tokens(const RotArgs& a, int n_parts) {
+  int64_t most = 0;
+  for (int p = 0; p < n_parts; ++p) {
+    const b3r_rotary_part& q = a.part[p];
+    const int64_t strides = a.D | q.x_batch | q.x_token | q.x_head | q.out_batch | q.out_token | q.out_head;
+    if (strides * (int64_t)sizeof(T) % 16 || ((uintptr_t)q.x | (uintptr_t)q.out) % 16) return 0;
+    most = std::max(most, (int64_t)q.heads * a.D * (int64_t)sizeof(T));
+  }
+  return most == 0 ? 0 : (int)(kRowBytes / most);
+}
+
 // The widest vector (elements) that every address and section allows: 16 bytes, halved until
 // it divides them.
 int rot_vector(const RotArgs& a, int n_parts, int esz, bool il) {
@@ -181,6 +268,24 @@ template <typename T>
 int rot_run(RotArgs& a, int n_parts, int64_t tokens, bool il, bool copy_rest, cudaStream_t s) {
   const int rot = a.axes * 2 * a.half;
   int v = rot_vector(a, n_parts, sizeof(T), il);
+  // (below a block for every SM the slots are spread over more threads: one token 2.5 us against 3.2)
+  if (v * (int)sizeof(T) < 16 && tokens >= 148) {
+    if (int per = rot_tokens<T>(a, n_parts)) {
+      per = (int)std::max<int64_t>(1, std::min<int64_t>(per, tokens / (148 * 4)));   // few tokens: spread over the SMs
+      const int64_t blocks = (tokens + per - 1) / per;
+      B3R_REQUIRE(tokens <= 0x7fffffff, "rotary: too many tokens for one call");
+      RowDivs dv;
+      dv.pieces = Div(a.D * sizeof(T) / 16);
+      for (int p = 0; p < n_parts; ++p) dv.heads[p] = Div(std::max(1, a.part[p].heads));
+      dv.pairs = Div(a.axes * a.half);
+      dv.half = Div(a.half);
+      dv.per = per;
+      const dim3 grid((unsigned)blocks, n_parts);
+      if (il) k_rotary_rows<T, true><<<grid, kRotThreads, 0, s>>>(a, dv, (uint32_t)tokens);
+      else k_rotary_rows<T, false><<<grid, kRotThreads, 0, s>>>(a, dv, (uint32_t)tokens);
+      return check_launch("rotary");
+    }
+  }
   B3R_REQUIRE(!il || v >= 2, "rotary: interleaved pairs must be aligned to a pair (even strides and head size)");
   a.rot_slots = il ? rot / v : rot / 2 / v;
   a.slots = a.rot_slots + (copy_rest ? (a.D - rot) / v : 0);

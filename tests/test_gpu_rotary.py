@@ -28,6 +28,9 @@ def _setup(B, T, Hq, Hk, D, half, axes, n_pos, dtype, seed=0):
     (2, 19, 3, 2, 40, 6, 1),         # vectors that end inside a section
     (1, 3, 1, 1, 24, 1, 5),          # one pair to a section, more axes
     (1, 600, 2, 2, 6, 3, 1),
+    (3, 700, 12, 4, 120, 17, 3),     # sections that no vector divides: whole tokens, several to a block
+    (1, 5, 64, 2, 96, 5, 2),
+    (700, 1, 2, 1, 64, 19, 1),       # a block's tokens lie in several batches
 ])
 def test_turn_and_back(dtype, interleaved, B, T, Hq, Hk, D, half, axes):
     from blast3r_b200.rotary import rotary
