@@ -21,8 +21,7 @@
 // bfloat16 branch, 93 us (6.5 TB/s); backward, 32768 RMS rows of 4096, bfloat16, two norms and a gate, 383 us
 // (4.2 TB/s) and 7 us for the partials.  There one block of 512 threads fills an SM's registers, so the
 // latency of a row's sum, barrier included, is hidden by nothing but the copies of the next rows.  Rows
-// without vector alignment are read one element at a time and take twice as long (forward: 18600
-// rows of 2647, 340 us).
+// that no vector divides take two to three times as long (forward: 18600 rows of 2647, 268 us).
 #include <algorithm>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -243,10 +242,53 @@ struct NormArgs {
   int post, pre, want_cols, gate_direct, stages, biases;
 };
 
+// Room for a row in shared memory.  Without VEC a row may begin anywhere: the whole 16-byte units that hold it
+// are copied, and its place in the first one is kept.
+template <typename T, bool VEC>
+__host__ __device__ inline int slot_bytes(int C) {
+  return VEC ? C * (int)sizeof(T) : (C * (int)sizeof(T) + 30) & ~15;
+}
+
 // ---------------------------------------------------------------- forward
+// Rows that no vector divides pass through shared memory where they hold 16-bit elements, so that memory sees whole
+// 16-byte units: 165230 rows of 701, float32 stream and bfloat16 branch, no norms, 248 us against 479 one element
+// at a time; 18600 float16 rows of 2647 268 against 350.  Single float32 elements fill a warp's 128 bytes as
+// they are (18600 rows of 7999: 641 us, through shared memory 755).
+template <typename TY, bool VEC>
+__host__ __device__ constexpr bool staged() {
+  return !VEC && sizeof(TY) == 2;
+}
+// Where a row's first element lies in its slot.
+template <typename T>
+__device__ __forceinline__ T* in_slot(uint8_t* slot, const T* p) {
+  return reinterpret_cast<T*>(slot + (reinterpret_cast<uintptr_t>(p) & 15));
+}
+template <typename T>
+__device__ __forceinline__ void ask_row(uint8_t* slot, const T* p, int C, int tid, int threads) {
+  const uint8_t* from = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+  const int end = (int)(reinterpret_cast<uintptr_t>(p) & 15) + C * (int)sizeof(T);
+  for (int u = tid * 16; u < end; u += threads * 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(slot + u)), "l"(from + u) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void put_row(T* p, const uint8_t* slot, int C, int tid, int threads) {
+  uint8_t* to = reinterpret_cast<uint8_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(15));
+  const int first = (int)(reinterpret_cast<uintptr_t>(p) & 15), end = first + C * (int)sizeof(T);
+  for (int u = tid * 16; u < end; u += threads * 16) {
+    if (u >= first && u + 16 <= end) {
+      *reinterpret_cast<uint4*>(to + u) = *reinterpret_cast<const uint4*>(slot + u);
+    } else {                                       // the unit's other bytes are another row's
+      for (int e = max(u, first); e < min(u + 16, end); e += (int)sizeof(T))
+        *reinterpret_cast<T*>(to + e) = *reinterpret_cast<const T*>(slot + e);
+    }
+  }
+}
+
 // POST: with a norm of y, y and x are both held until its statistics are known; without it, only r.
 template <typename TX, typename TY, int VPT, bool VEC, bool POST>
 __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormArgs a) {
+  constexpr bool kStage = staged<TY, VEC>();
+  extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ alignas(16) float buf[kSumFloats<8>];
   // blockDim.x threads to a row; blocks of several rows have one warp to a row
   const int threads = blockDim.x, tid = threadIdx.x, warps = threads >> 5, C = a.C;
@@ -259,6 +301,26 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
   int turn = 0;
   const TY* yp = reinterpret_cast<const TY*>(a.y) + row * a.y_row;
   const TX* xp = reinterpret_cast<const TX*>(a.x) + row * a.x_row;
+  TX* rp = reinterpret_cast<TX*>(a.r) + row * C;
+  TY* hp = reinterpret_cast<TY*>(a.h) + row * C;
+  uint8_t *slot_x = nullptr, *slot_y = nullptr;
+  auto meet = [&] {                                // the row's threads
+    if (warps > 1) __syncthreads();
+    else __syncwarp();
+  };
+  if constexpr (kStage) {
+    slot_x = dyn + threadIdx.y * (slot_bytes<TX, false>(C) + slot_bytes<TY, false>(C));
+    slot_y = slot_x + slot_bytes<TX, false>(C);
+    ask_row(slot_y, yp, C, tid, threads);
+    ask_row(slot_x, xp, C, tid, threads);
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    meet();
+    yp = in_slot(slot_y, yp);
+    xp = in_slot(slot_x, xp);
+  }
+  auto all_read = [&] {                            // the slots become r's and h's
+    if constexpr (kStage) meet();
+  };
   const float inv = 1.f / C;
   const char* gp = reinterpret_cast<const char*>(a.gate);
   if (a.gate && a.rows_per_gate < a.rows)
@@ -317,7 +379,7 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
     }
 #pragma unroll
     for (int j = 0; j < kP; ++j) n[v][j] = fma2(both(a.alpha), x[j], n[v][j]);
-    store8<TX, VEC>(reinterpret_cast<TX*>(a.r) + row * C, n[v], v, tid, threads, C);
+    store8<TX, VEC>(kStage ? in_slot(slot_x, rp) : rp, n[v], v, tid, threads, C);
   };
   if constexpr (POST) {
     float2 x[VPT][kP];
@@ -326,6 +388,7 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
       load8<TY, VEC>(n[v], yp, v, tid, threads, C);
       load8<TX, VEC>(x[v], xp, v, tid, threads, C);
     }
+    all_read();
     normalise(a.w_post, a.b_post);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) join(v, x[v]);
@@ -336,14 +399,23 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
       load8<TY, VEC>(n[v], yp, v, tid, threads, C);
       load8<TX, VEC>(x[v], xp, v, tid, threads, C);
     }
+    all_read();
 #pragma unroll
     for (int v = 0; v < VPT; ++v) join(v, x[v]);
+  }
+  if constexpr (kStage) {
+    meet();
+    put_row(rp, slot_x, C, tid, threads);
   }
   if (!a.pre) return;
   // h is the norm of r before r's rounding to the stream's type
   normalise(a.w_pre, a.b_pre);
 #pragma unroll
-  for (int v = 0; v < VPT; ++v) store8<TY, VEC>(reinterpret_cast<TY*>(a.h) + row * C, n[v], v, tid, threads, C);
+  for (int v = 0; v < VPT; ++v) store8<TY, VEC>(kStage ? in_slot(slot_y, hp) : hp, n[v], v, tid, threads, C);
+  if constexpr (kStage) {
+    meet();
+    put_row(hp, slot_y, C, tid, threads);
+  }
 }
 
 // ---------------------------------------------------------------- backward
@@ -351,12 +423,6 @@ __global__ void __launch_bounds__(256) k_norm_fwd(const __grid_constant__ NormAr
 enum { kDwPost, kDbPost, kDwPre, kDbPre, kCols };
 
 // Rows of the stages of the ring: dr, r (stream type), dh, y, one after the other.
-// Without VEC a row may begin anywhere: the whole 16-byte units that hold it are copied, and its
-// place in the first one is kept.
-template <typename T, bool VEC>
-__host__ __device__ inline int slot_bytes(int C) {
-  return VEC ? C * (int)sizeof(T) : (C * (int)sizeof(T) + 30) & ~15;
-}
 template <typename TX, typename TY, bool VEC>
 __host__ __device__ inline int stage_bytes(int C) {
   return 2 * slot_bytes<TX, VEC>(C) + 2 * slot_bytes<TY, VEC>(C);
@@ -705,9 +771,13 @@ constexpr int kMaxC = 8192;
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename TX, typename TY, int VPT, bool VEC>
-void fwd_kernel(const NormArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
-  if (a.post) k_norm_fwd<TX, TY, VPT, VEC, true><<<grid, block, 0, s>>>(a);
-  else k_norm_fwd<TX, TY, VPT, VEC, false><<<grid, block, 0, s>>>(a);
+int fwd_kernel(const NormArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
+  const int smem = !staged<TY, VEC>() ? 0 : block.y * (slot_bytes<TX, false>(a.C) + slot_bytes<TY, false>(a.C));
+  auto* f = a.post ? k_norm_fwd<TX, TY, VPT, VEC, true> : k_norm_fwd<TX, TY, VPT, VEC, false>;
+  if (smem > 40 * 1024)
+    B3R_TRY(check_cuda(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "residual_norm"));
+  f<<<grid, block, smem, s>>>(a);
+  return check_launch("residual_norm");
 }
 
 template <typename TX, typename TY, bool VEC>
@@ -726,10 +796,9 @@ int fwd_launch(const NormArgs& a, cudaStream_t s) {
   const dim3 block(threads, threads == 32 ? 4 : 1);
   const int64_t grid = (a.rows + block.y - 1) / block.y;
   B3R_REQUIRE(grid <= 0x7fffffff, "residual_norm: too many rows for one call");
-  if (vpt == 1) fwd_kernel<TX, TY, 1, VEC>(a, (unsigned)grid, block, s);
-  else if (vpt == 2) fwd_kernel<TX, TY, 2, VEC>(a, (unsigned)grid, block, s);
-  else fwd_kernel<TX, TY, 4, VEC>(a, (unsigned)grid, block, s);
-  return check_launch("residual_norm");
+  if (vpt == 1) return fwd_kernel<TX, TY, 1, VEC>(a, (unsigned)grid, block, s);
+  if (vpt == 2) return fwd_kernel<TX, TY, 2, VEC>(a, (unsigned)grid, block, s);
+  return fwd_kernel<TX, TY, 4, VEC>(a, (unsigned)grid, block, s);
 }
 
 int bwd_threads(int C) { return (C + kE * 32 - 1) / (kE * 32) * 32; }

@@ -134,6 +134,9 @@ CASES = [  # B, T, C, dtype, stream, kind, post, pre, gate
     (4, 65, 96, 'f32', 'f32', 'rms', False, False, 'sample'),
     (1200, 1, 64, 'bf16', 'bf16', 'layer', True, True, 'sample'),
     (3, 5, 48, 'bf16', 'bf16', 'layer', False, False, None),
+    (31, 90, 701, 'bf16', 'f32', 'layer', False, False, None),
+    (3, 7, 2647, 'f16', 'f32', 'layer', False, True, 'sample'),
+    (3, 70, 4097, 'bf16', 'bf16', 'rms', True, True, 'sample'),
 ]
 
 
