@@ -822,7 +822,7 @@ int bwd_kernel(const NormArgs& a, int smem, cudaStream_t s) {
 template <typename TX, typename TY, bool FULL, bool VEC>
 int bwd_launch(NormArgs a, cudaStream_t s) {
   const int threads = bwd_threads(a.C), stage = stage_bytes<TX, TY, VEC>(a.C);
-  const int weights = (FULL ? 4 : 3) * threads * kE * 4, room = (227 * 1024) / bwd_per_sm(a.C) - 3072;
+  const int weights = (FULL ? 4 : 3) * threads * kE * 4, room = (227 * 1024) / bwd_per_sm(a.C) - 3 * 1024;   // (static and reserved)
   a.stages = std::min(kMaxStages, (room - weights) / stage);
   if (a.stages >= 2) {
     const int smem = weights + a.stages * stage;
