@@ -437,12 +437,13 @@ __host__ __device__ inline int stage_bytes(int C) {
 // p = w_post g y and rho, sigma the inverse norms of r and y,
 //   sum(dn w_post yhat) = sigma (sum dr p + rho (sum z p - rho^2 mean(z r) sum r p)),
 // so six sums and one barrier a row do (32768 rows of 4096: 381 us, with a second sum after the first 456).
-// With means the centred rows are summed: three barriers.  1024 threads have no registers for the six: two.
+// With means the centred rows are summed: three barriers.  More than 512 threads have no registers for the six
+// (640 threads, rows of 5120: 495 us against 393 with two sums): two.
 template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>
 __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormArgs a) {
   constexpr bool kOne = !FULL && MAXT <= 512;   // one sum a row
   extern __shared__ __align__(128) uint8_t dyn[];
-  __shared__ alignas(16) float buf[kSumFloats<MAXT / 32>];
+  __shared__ alignas(16) float buf[kSumFloats<MAXT <= 512 ? 16 : 32>];
   __shared__ uint64_t full[kMaxStages];
   __shared__ int dead_flag;
   volatile int* dead = &dead_flag;
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         bulk_copy(smem_u32(to + at[k]), VEC ? from[k] : reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(from[k]) & ~uintptr_t(15)), n[k],
                   bar);
   };
-  clear_sums(buf, kSumFloats<MAXT / 32>);
+  clear_sums(buf, kSumFloats<MAXT <= 512 ? 16 : 32>);
   if (RING && tid == 0) {
     dead_flag = 0;
     for (int i = 0; i < a.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
@@ -566,7 +567,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         t[2] = add2(t[2], z[j]);
       }
       float s[3] = {t[0].x + t[0].y, t[1].x + t[1].y, t[2].x + t[2].y};
-      row_sum<3, MAXT / 32>(s, warps, buf, turn);
+      row_sum<3, MAXT <= 512 ? 16 : 32>(s, warps, buf, turn);
       const float mu_r = -s[0] * inv_mean, mu_y = a.post ? -s[1] * inv_mean : 0.f;
       mean_z = s[2] * inv_mean;
 #pragma unroll
@@ -616,7 +617,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
     float q[kQ];
 #pragma unroll
     for (int k = 0; k < kQ; ++k) q[k] = t[k].x + t[k].y;
-    row_sum<kQ, MAXT / 32>(q, warps, buf, turn);
+    row_sum<kQ, MAXT <= 512 ? 16 : 32>(q, warps, buf, turn);
     if (RING && tid == 0 && row > first) request(row - 1 + a.stages);   // every thread has left the row before
     if (a.pre) {
       const float rstd = rsqrtf(q[0] * inv + a.eps), proj = -q[2] * inv * rstd;   // -mean(z rhat)
@@ -668,7 +669,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
       s[0] = u[1].x + u[1].y;
       if constexpr (FULL) s[1] = u[0].x + u[0].y;
       if constexpr (kOne) s[0] = rstd * q[3];
-      else row_sum<FULL ? 2 : 1, MAXT / 32>(s, warps, buf, turn);
+      else row_sum<FULL ? 2 : 1, MAXT <= 512 ? 16 : 32>(s, warps, buf, turn);
       float mz = 0.f;
       if constexpr (FULL) mz = -s[1] * inv_mean;
       const float proj = -s[0] * inv;
@@ -826,7 +827,11 @@ int bwd_launch(NormArgs a, cudaStream_t s) {
   a.stages = std::min(kMaxStages, (room - weights) / stage);
   if (a.stages >= 2) {
     const int smem = weights + a.stages * stage;
-    return threads <= 512 ? bwd_kernel<TX, TY, FULL, VEC, true, 512>(a, smem, s) : bwd_kernel<TX, TY, FULL, VEC, true, 1024>(a, smem, s);
+    // registers of a thread: 128, 96 and 64 (18600 bfloat16 rows of 5120 with 96: RMS 393 us, layer norm 525; with
+    // 64, where they do not hold a row's columns and their sums, 508 and 715)
+    if (threads <= 512) return bwd_kernel<TX, TY, FULL, VEC, true, 512>(a, smem, s);
+    if (threads <= 640) return bwd_kernel<TX, TY, FULL, VEC, true, 640>(a, smem, s);
+    return bwd_kernel<TX, TY, FULL, VEC, true, 1024>(a, smem, s);
   }
   return bwd_kernel<TX, TY, FULL, VEC, false, 1024>(a, weights, s);
 }

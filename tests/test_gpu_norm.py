@@ -137,6 +137,8 @@ CASES = [  # B, T, C, dtype, stream, kind, post, pre, gate
     (31, 90, 701, 'bf16', 'f32', 'layer', False, False, None),
     (3, 7, 2647, 'f16', 'f32', 'layer', False, True, 'sample'),
     (3, 70, 4097, 'bf16', 'bf16', 'rms', True, True, 'sample'),
+    (2, 90, 5120, 'bf16', 'f32', 'layer', True, True, 'sample'),
+    (3, 60, 5120, 'bf16', 'bf16', 'rms', True, True, 'channel'),
 ]
 
 
