@@ -81,9 +81,11 @@ struct Job {
 constexpr int kJobs = 3;   // jobs that a block has in hand at most
 
 // The barriers of S and P are each group's own, one for each of its last kS steps: a group that takes
-// no part in a job must not meet a barrier that has turned twice since.
+// no part in a job must not meet a barrier that has turned twice since.  Nor may it turn one for the other
+// group, which it can be two jobs ahead of: where the groups write their rows of Q, each fills its own tile,
+// on barriers and in an order of buffers of its own (q_full[w]), in the jobs that it takes part in alone.
 struct Shared {
-  uint64_t q_full[2], q_empty[2], fix, k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
+  uint64_t q_full[2][2], q_empty[2], fix, k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
   uint64_t s_full[2][kMaxS], p_full[2][kMaxS], s_free[kMaxS], o_done[2];
   uint64_t job_full[kJobs], job_empty[kJobs], want, cancel;
   alignas(16) uint4 answer;
@@ -188,6 +190,29 @@ struct JobList {
   }
 };
 
+// Issuing warp: waits for a job's tiles of Q, and where they are.  By TMA both come to the job's buffer; else each
+// group that takes part has filled the next one of its own.
+template <int DP>
+struct QTiles {
+  uint32_t at[2];
+  int turns[2] = {0, 0};   // jobs of the block (by TMA), or that a group has taken part in
+  __device__ __forceinline__ void get(const FwdArgs& a, Shared& sh, uint32_t sq, int n0, int n1, volatile int* dead) {
+    using X = Cfg<DP>;
+    const uint32_t q_bytes = (a.one ? 1 : 2) * X::kTile;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if (w == 1 && (a.one || a.q_tma)) {
+        at[1] = a.one ? at[0] : at[0] + X::kTile;
+      } else if (a.q_tma || (w ? n1 : n0) > 0) {
+        const int buf = turns[w] % X::kQ;
+        mbar_wait(smem_u32(&sh.q_full[w][buf]), (turns[w] / X::kQ) & 1, dead);
+        at[w] = sq + buf * q_bytes + w * X::kTile;
+        ++turns[w];
+      }
+    }
+  }
+};
+
 template <int DP, typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant__ FwdArgs a) {
   extern __shared__ uint8_t raw[];
@@ -204,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
   if (warp == 9) tc_alloc(smem_u32(&sh.tmem), 512);
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&sh.q_full[i]), a.q_tma ? 1 : 8);
+      for (int w = 0; w < 2; ++w) mbar_init(smem_u32(&sh.q_full[w][i]), a.q_tma ? 1 : 4);   // (by TMA: q_full[0], both tiles)
       mbar_init(smem_u32(&sh.q_empty[i]), 1);
       mbar_init(smem_u32(&sh.o_done[i]), 1);
     }
@@ -249,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       while (const Job* j = list.get(dead)) {
         if (a.q_tma) {                         // rows past the end only reach their own scores
           const int qb = k % X::kQ, use = k / X::kQ;
-          const uint32_t bar = smem_u32(&sh.q_full[qb]);
+          const uint32_t bar = smem_u32(&sh.q_full[0][qb]);
           if (use > 0) mbar_wait(smem_u32(&sh.q_empty[qb]), (use - 1) & 1, dead);
           if (lane == 0) {
             mbar_expect(bar, q_bytes);
@@ -281,16 +306,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       const uint32_t bar_k = smem_u32(sh.k_empty), bar_v = smem_u32(sh.v_empty);
       Ring kr{sk, base + X::kQ * q_bytes, sh.k_full, sh.k_empty, a.k_stages};
       Ring vr{sv, base + X::kQ * q_bytes + a.k_stages * kTile, sh.v_full, sh.v_empty, a.v_stages};
-      int k = 0, hs0 = 0, hs1 = 0, ts0 = 0, ts1 = 0;   // jobs; each group's steps whose S, and O, has been issued
+      int hs0 = 0, hs1 = 0, ts0 = 0, ts1 = 0;   // each group's steps whose S, and O, has been issued
+      QTiles<DP> q;
       int last = -1, last_round = 0;
       JobList list(sh);
       while (const Job* j = list.get(dead)) {
         const int n0 = j->n[0], n1 = j->n[1], n = max(n0, n1);
         list.done(lane);
-        mbar_wait(smem_u32(&sh.q_full[0]), k & 1, dead);
+        q.get(a, sh, sq, n0, n1, dead);
         auto scores = [&](int w, int& hs, int st) {
           tc_fence_after();
-          tile_product<X::kBlocks, kTileRows>(tmem + w * kTileRows, sq + (a.one ? 0 : w) * kTile, sk + st * kTile, id_s, steps, on);
+          tile_product<X::kBlocks, kTileRows>(tmem + w * kTileRows, q.at[w], sk + st * kTile, id_s, steps, on);
           tc_commit(bar_s + (w * kMaxS + (hs & 1)) * 8, on);
           ++hs;
         };
@@ -341,7 +367,6 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
           }
           if (i + 2 == n || n == 1) tc_commit(smem_u32(&sh.q_empty[0]), on);   // the last scores are on their way
         }
-        ++k;
       }
       if (last >= 0) mbar_wait(bar_v + last * 8, last_round & 1, dead);   // no arrival is left behind
     } else if (!X::kOneIssuer && warp == 9) {
@@ -352,12 +377,13 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       Ring kr{sk, base + X::kQ * q_bytes, sh.k_full, sh.k_empty, a.k_stages};
       int k = 0, buf = 0, uses = 0, b0 = 0, b1 = 0;    // S buffer and its turn; each group's barrier
       int last_buf = -1, last_use = 0;
+      QTiles<DP> q_at;
       JobList list(sh);
       while (const Job* j = list.get(dead)) {
         const int n0 = j->n[0], n1 = j->n[1], n = max(n0, n1), qb = k % X::kQ;
         list.done(lane);
-        mbar_wait(smem_u32(&sh.q_full[qb]), (k / X::kQ) & 1, dead);
-        const uint32_t q0 = sq + qb * q_bytes, q1 = a.one ? q0 : q0 + kTile;
+        q_at.get(a, sh, sq, n0, n1, dead);
+        const uint32_t q0 = q_at.at[0], q1 = q_at.at[1];
         auto product = [&](uint32_t q, int w, int& b, int st) {
           if (uses > 0) mbar_wait(bar_f + buf * 8, (uses - 1) & 1, dead);   // until P has been read from it
           tc_fence_after();
@@ -489,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     const int w = warp >> 2, r = threadIdx.x & 127;
     const uint32_t quarter = tmem + ((uint32_t)(warp & 3) << 21);   // this warp's 32 lanes
     const float c = d.scale * kLog2e;
-    int mine = 0;                              // this group's steps so far
+    int mine = 0, turn = 0;                    // this group's steps so far; the jobs that it has written Q for
     JobList list(sh);
     for (int k = 0;; ++k) {
       const Job* jp = list.get(dead);
@@ -504,21 +530,20 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       sq_.kl = j.kl;
       // (past the rows nothing is written: such a thread sees what lets its warp take whole tiles)
       const int bound = !row ? j.kl : i < j.ql ? attn_bound(sq_, i, d.causal) : 0;
-      if (!a.q_tma) {
-        if (w == 0 || !a.one) {
-          // the row of Q into the swizzled tile; zeros past D and past the rows
-          const int h = j.kv * a.G + m - i * a.G;
-          const uint4* q = reinterpret_cast<const uint4*>(attn_row<const T>(d.q, j.b, (int64_t)j.q0 + (row ? i : 0), row ? h : 0));
-          uint8_t* dst = base + (k % X::kQ) * q_bytes + w * kTile + r * 128;
+      if (!a.q_tma && n > 0 && (w == 0 || !a.one)) {
+        // the row of Q into the swizzled tile; zeros past D and past the rows
+        const int h = j.kv * a.G + m - i * a.G;
+        const uint4* q = reinterpret_cast<const uint4*>(attn_row<const T>(d.q, j.b, (int64_t)j.q0 + (row ? i : 0), row ? h : 0));
+        uint8_t* dst = base + (turn % X::kQ) * q_bytes + w * kTile + r * 128;
 #pragma unroll
-          for (int cb = 0; cb < DP / 8; ++cb) {
-            const uint4 x = (row && cb * 8 < d.D) ? q[cb] : make_uint4(0, 0, 0, 0);
-            *reinterpret_cast<uint4*>(dst + (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4)) = x;
-          }
-          fence_async();
+        for (int cb = 0; cb < DP / 8; ++cb) {
+          const uint4 x = (row && cb * 8 < d.D) ? q[cb] : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + (cb >> 3) * kBlockBytes + (((cb & 7) ^ (r & 7)) << 4)) = x;
         }
+        fence_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[k % X::kQ]));
+        if (lane == 0) mbar_arrive(smem_u32(&sh.q_full[w][turn % X::kQ]));
+        ++turn;
       }
       const bool any = __any_sync(0xffffffffu, row);   // a warp without rows only keeps the others' pace
       float mx = -INFINITY, l = 0.f;       // what the exponentials are taken against (log2), and their sum
@@ -632,16 +657,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       // ---------------------------------------------- output
       float f0 = 0.f, f1 = 0.f, lg;                      // factors of O (and of the other group's O); log2 of the sum
       if (a.one) {
-        const int turn = k & 1;
+        const int half = k & 1;
         if (w == 1) {
-          sh.m[turn][r] = mx;
-          sh.l[turn][r] = l;
+          sh.m[half][r] = mx;
+          sh.l[half][r] = l;
         }
         tc_fence_before();
         bar_sync(1, 256);
         tc_fence_after();
         if (w == 0) {
-          const float m1 = sh.m[turn][r], l1 = sh.l[turn][r], top = fmaxf(mx, m1);
+          const float m1 = sh.m[half][r], l1 = sh.l[half][r], top = fmaxf(mx, m1);
           const float e0 = mx == -INFINITY ? 0.f : ex2(mx - top), e1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
           const float sum = l * e0 + l1 * e1;
           f0 = sum > 0.f ? e0 / sum : 0.f;
