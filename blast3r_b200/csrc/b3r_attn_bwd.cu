@@ -14,6 +14,7 @@
 // Splitting the pass in two computes S and dP twice (7 products instead of 5); the
 // alternative adds dq to memory from every key block, which needs atomics or an order to wait for.
 #include <algorithm>
+#include <type_traits>
 #include "b3r_attn.cuh"
 #include "b3r_tc.cuh"
 
@@ -46,6 +47,10 @@ __device__ __forceinline__ float scale_ds(const float2* range, int head) {
   return exp2f(fminf(fmaxf(floorf(log2f(32768.f / most)), -24.f), 24.f));
 }
 
+// What is added to a query's raw scores, so that scale times them is the logarithm of P (as it is carried).
+template <typename T>
+__device__ __forceinline__ float shift_of(float lse, float scale) { return (kLogScaleP<T> / kLog2e - lse) / scale; }
+
 struct alignas(64) BwdArgs {
   CUtensorMap q, go, k, v;    // boxes of 128 rows of a head
   CUtensorMap qg, gog, og;    // boxes of whole groups, where q_tma
@@ -57,22 +62,29 @@ struct alignas(64) BwdArgs {
   int q_tma;                       // the heads of a group divide 128
   int G;
   float* delta;               // [B][Hq][Lq]
-  float2* range;              // float16: [B][Hkv], the largest |do|^2 and |v|^2 of a row
+  float2* range;              // float16: [B][Hkv], the largest |do|^2 and |v|^2 of a row;
+  int* far;                   // and [B][Hkv], whether lse / scale or delta of a row is above kMostInParts
   float* part_q;              // [q_splits][B Hkv][rows][D]
   float* part_k;              // [k_splits][2][B Hkv][Lk][D]: dk, dv
 };
 
 constexpr int kStepBytes = kTileRows * 32;
 // A float as 2^8 a + b + 2^-8 c + 2^-14 d with a .. d of the operands' type: to 24 bits at least, in
-// float16 for magnitudes from 1e-6 to 1e7 too (its own numbers end at 6e4, and are coarse below 6e-5).
+// float16 for magnitudes from 1e-6 to 1.6e7 (its own numbers end at 6e4, and are coarse below 6e-5).
 __host__ __device__ constexpr float weight_of(int k) { return k == 0 ? 256.f : k == 1 ? 1.f : k == 2 ? 1.f / 256.f : 1.f / 16384.f; }
+// Up to 256 * 65504 the parts are float16 numbers.  lse / scale is about the largest raw score, and delta a sum of D
+// products, so both can lie above.  k_attn_dq, which meets every row, marks the heads where one does; there the
+// threads that read S^T and dP^T subtract in float32.  (bfloat16 has float32's range.)
+constexpr float kMostInParts = 1.6e7f;
+constexpr int kPlain = 4;   // stages of those, three of them needed: t + 2 may be written while tile t is at work
 
 struct Shared {
   uint64_t fix, own_full, full[2][kMaxStages], empty[2][kMaxStages], s_full[2], s_read, dp_full, p_full, ds_full, done, own_ready;
-  uint64_t st_full[2], st_empty[2];
+  uint64_t st_full[kPlain], st_empty[2];
   uint32_t tmem;
   int dead;
   float delta[kTileRows];
+  alignas(16) float plain[kPlain][2][kTileRows];      // k_attn_dkv, far statistics: what is added to S^T and to dP^T
   // k_attn_dkv: one more step of 16 for S^T and dP^T, which subtracts each query's lse and delta in the tensor
   // cores: the weights below times (per stage and product) four numbers of the operands' type each
   alignas(128) uint4 weights[kStepBytes / 16], stat[2][2][kStepBytes / 16];
@@ -95,10 +107,8 @@ __device__ __forceinline__ void init_shared(Shared& sh) {
       mbar_init(smem_u32(&sh.full[k][i]), 1);
       mbar_init(smem_u32(&sh.empty[k][i]), 1);
     }
-  for (int i = 0; i < 2; ++i) {
-    mbar_init(smem_u32(&sh.st_full[i]), 1);
-    mbar_init(smem_u32(&sh.st_empty[i]), 1);
-  }
+  for (int i = 0; i < kPlain; ++i) mbar_init(smem_u32(&sh.st_full[i]), 1);
+  for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&sh.st_empty[i]), 1);
   mbar_init(smem_u32(&sh.s_full[0]), 1);
   mbar_init(smem_u32(&sh.s_full[1]), 1);
   mbar_init(smem_u32(&sh.s_read), 8);
@@ -350,6 +360,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         const float delta = (dot[0].x + dot[0].y) + (dot[1].x + dot[1].y);
         sh.delta[r] = delta;
         if (live && split == 0) a.delta[((int64_t)b * d.Hq + h) * d.Lq + i] = delta;
+        if (!kBf && bound > 0 && split == 0 && !(fmaxf(fabsf(shift_of<T>(lse_in, d.scale)), fabsf(delta)) <= kMostInParts))
+          atomicExch(a.far + head, 1);
       }
       if (n > 0) {
 #pragma unroll
@@ -512,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       const uint64_t weights = desc_step(smem_u32(sh.weights)), minus = desc_step(smem_u32(sh.stat));
       auto scores = [&](int it) {
         xq = qr.next(dead);
-        mbar_wait(smem_u32(&sh.st_full[it & 1]), (it >> 1) & 1, dead);
+        mbar_wait(smem_u32(&sh.st_full[it & (kPlain - 1)]), (it / kPlain) & 1, dead);
         product(tmem + it % kS * 128, sk, qr.data + xq * kTile);
         tc_mma(tmem + it % kS * 128, weights, minus + ((it & 1) * 2 * kStepBytes >> 4), id_s, true, on);
         tc_commit(smem_u32(&sh.s_full[it % kS]), on);
@@ -552,6 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     }
     } else if (warp == 10 && n > 0) {
     // the statistics of each tile's queries, two tiles ahead at most
+    const bool apart = !kBf && a.far[head] != 0;
     {
       const uint32_t lo = pack2(weight_of(0), weight_of(1), T()), hi = pack2(weight_of(2), weight_of(3), T());
       for (int i = lane; i < kStepBytes / 16; i += 32) {               // bricks of 8: a step's first and second half by turns
@@ -573,6 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
         y[q] = ok ? dl[q * 32 + lane] : 0.f;
       }
       if (it >= 2) mbar_wait(smem_u32(&sh.st_empty[st]), ((it >> 1) - 1) & 1, dead);
+      const int pl = it & (kPlain - 1);   // (free: st_empty of it - 2 follows dP of that tile, asked for after dS of it - 3)
       auto put = [&](int which, int row, float v) {
         float part[4];
 #pragma unroll
@@ -586,12 +600,17 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
       for (int q = 0; q < 4; ++q) {
         // a query that sees nothing, or none: its P is masked, or meets zeros; any low score will do
         const bool none = x[q] == -INFINITY;
-        put(0, q * 32 + lane, none ? -1e7f : (kLogScaleP<T> / kLog2e - x[q]) / d.scale);
-        put(1, q * 32 + lane, none ? 0.f : -y[q]);
+        const float l_of = none ? -1e7f : shift_of<T>(x[q], d.scale), d_of = none ? 0.f : -y[q];
+        if (apart) {
+          sh.plain[pl][0][q * 32 + lane] = l_of;
+          sh.plain[pl][1][q * 32 + lane] = d_of;
+        }
+        put(0, q * 32 + lane, apart ? 0.f : l_of);
+        put(1, q * 32 + lane, apart ? 0.f : d_of);
       }
       fence_async();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.st_full[st]));
+      if (lane == 0) mbar_arrive(smem_u32(&sh.st_full[pl]));
       if (++t == per_head) {
         t = 0;
         ++h;
@@ -607,62 +626,83 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     const float up = scale_ds<T>(a.range, head), down = up / kScaleP<T>;
     const float2 cc = make_float2(c, c), unscale = make_float2(down, down);
     const int see = d.causal ? max(0, j - (s.kl - s.ql)) : 0;         // the first query that sees this key
-    int t = n > 0 ? first % per_head : 0;
-    for (int it = 0; it < n; ++it) {
-      const int i0 = (t0 + t) * kTileRows + w * 64;
-      if (++t == per_head) t = 0;
-      const uint32_t at = quarter + it % kS * 128 + w * 64, dp = quarter + kDp + w * 64;
-      mbar_wait(smem_u32(&sh.s_full[it % kS]), (it / kS) & 1, dead);
-      tc_fence_after();
-      const int hide = see - i0;                                     // columns before it do not see the key
-      const bool whole = __all_sync(0xffffffffu, hide <= 0);
-      uint32_t p[64], g[64];
-      tc_ld32(at, p);
-      tc_ld32(at + 32, p + 32);
-      tc_wait_ld(p);
+    // (two loops: the test within one cost float16 8 % of the kernel on sequences of a thousand)
+    auto walk = [&](auto far) {
+      int t = n > 0 ? first % per_head : 0;
+      for (int it = 0; it < n; ++it) {
+        const int i0 = (t0 + t) * kTileRows + w * 64;
+        if (++t == per_head) t = 0;
+        const uint32_t at = quarter + it % kS * 128 + w * 64, dp = quarter + kDp + w * 64;
+        mbar_wait(smem_u32(&sh.s_full[it % kS]), (it / kS) & 1, dead);
+        tc_fence_after();
+        const int hide = see - i0;                                     // columns before it do not see the key
+        const bool whole = __all_sync(0xffffffffu, hide <= 0);
+        uint32_t p[64], g[64];
+        auto add = [&](uint32_t (&to)[64], int which) {
+          const float4* f = reinterpret_cast<const float4*>(&sh.plain[it & (kPlain - 1)][which][w * 64]);
 #pragma unroll
-      for (int e = 0; e < 64; e += 2) {
-        const float2 x = __fmul2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), cc);
-        p[e] = __float_as_uint(ex2(x.x));
-        p[e + 1] = __float_as_uint(ex2(x.y));
+          for (int e = 0; e < 64; e += 4) {
+            const float4 z = f[e / 4];
+            to[e] = __float_as_uint(__uint_as_float(to[e]) + z.x);
+            to[e + 1] = __float_as_uint(__uint_as_float(to[e + 1]) + z.y);
+            to[e + 2] = __float_as_uint(__uint_as_float(to[e + 2]) + z.z);
+            to[e + 3] = __float_as_uint(__uint_as_float(to[e + 3]) + z.w);
+          }
+        };
+        tc_ld32(at, p);
+        tc_ld32(at + 32, p + 32);
+        tc_wait_ld(p);
+        if constexpr (decltype(far)::value) {
+          mbar_wait(smem_u32(&sh.st_full[it & (kPlain - 1)]), (it / kPlain) & 1, dead);   // (there before S^T)
+          add(p, 0);
+        }
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          const float2 x = __fmul2_rn(make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])), cc);
+          p[e] = __float_as_uint(ex2(x.x));
+          p[e + 1] = __float_as_uint(ex2(x.y));
+        }
+        if (!whole) {                                                  // (apart: within the loops it doubled their time)
+#pragma unroll
+          for (int e = 0; e < 64; ++e) p[e] = e >= hide ? p[e] : 0u;
+        }
+        uint32_t h[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]), T());
+        tc_st32(at, h);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
+        mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
+        tc_fence_after();
+        tc_ld32(dp, g);
+        tc_ld32(dp + 32, g + 32);
+        tc_wait_ld(g);
+        if constexpr (decltype(far)::value) add(g, 1);
+#pragma unroll
+        for (int e = 0; e < 64; e += 2) {
+          float2 x = make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1]));
+          if (kScaleP<T> != 1.f) x = __fmul2_rn(x, unscale);
+          x = __fmul2_rn(x, make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])));
+          g[e] = __float_as_uint(x.x);
+          g[e + 1] = __float_as_uint(x.y);
+        }
+        if (!whole) {                                                  // (dP may be anything there)
+#pragma unroll
+          for (int e = 0; e < 64; ++e) g[e] = e >= hide ? g[e] : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), T());
+        tc_st32(dp, h);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh.ds_full));
       }
-      if (!whole) {                                                  // (apart: within the loops it doubled their time)
-#pragma unroll
-        for (int e = 0; e < 64; ++e) p[e] = e >= hide ? p[e] : 0u;
-      }
-      uint32_t h[32];
-#pragma unroll
-      for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(p[2 * e]), __uint_as_float(p[2 * e + 1]), T());
-      tc_st32(at, h);
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.p_full));
-      mbar_wait(smem_u32(&sh.dp_full), it & 1, dead);
-      tc_fence_after();
-      tc_ld32(dp, g);
-      tc_ld32(dp + 32, g + 32);
-      tc_wait_ld(g);
-#pragma unroll
-      for (int e = 0; e < 64; e += 2) {
-        float2 x = make_float2(__uint_as_float(g[e]), __uint_as_float(g[e + 1]));
-        if (kScaleP<T> != 1.f) x = __fmul2_rn(x, unscale);
-        x = __fmul2_rn(x, make_float2(__uint_as_float(p[e]), __uint_as_float(p[e + 1])));
-        g[e] = __float_as_uint(x.x);
-        g[e + 1] = __float_as_uint(x.y);
-      }
-      if (!whole) {                                                  // (dP may be anything there)
-#pragma unroll
-        for (int e = 0; e < 64; ++e) g[e] = e >= hide ? g[e] : 0u;
-      }
-#pragma unroll
-      for (int e = 0; e < 32; ++e) h[e] = pack2(__uint_as_float(g[2 * e]), __uint_as_float(g[2 * e + 1]), T());
-      tc_st32(dp, h);
-      tc_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&sh.ds_full));
-    }
+    };
+    if (!kBf && a.far[head] != 0) walk(std::true_type());
+    else walk(std::false_type());
     if (n > 0) {
       mbar_wait(smem_u32(&sh.done), 0, dead);
       tc_fence_after();
@@ -748,7 +788,7 @@ int64_t cut(BwdArgs& a) {     // returns the workspace's bytes
   a.group = d.causal ? (int)std::max<int64_t>(1, heads) : (int)std::max<int64_t>(1, std::min<int64_t>(heads, (32 << 20) / head));
   int64_t n = align256((int64_t)d.B * d.Hq * d.Lq * 4);
   const int64_t r_off = n;
-  if (d.dtype == B3R_F16) n += align256(heads * 8);
+  if (d.dtype == B3R_F16) n += align256(heads * 12);
   const int64_t q_off = n;
   if (a.q_splits > 1) n += align256((int64_t)a.q_splits * heads * d.Lq * G * d.D * 4);
   const int64_t k_off = n;
@@ -756,6 +796,7 @@ int64_t cut(BwdArgs& a) {     // returns the workspace's bytes
   uint8_t* w = reinterpret_cast<uint8_t*>(d.work);
   a.delta = reinterpret_cast<float*>(w);
   a.range = reinterpret_cast<float2*>(w + r_off);
+  a.far = reinterpret_cast<int*>(a.range + heads);
   a.part_q = reinterpret_cast<float*>(w + q_off);
   a.part_k = reinterpret_cast<float*>(w + k_off);
   return n;
@@ -770,7 +811,7 @@ int launch(const BwdArgs& a, cudaStream_t s) {
   B3R_REQUIRE(a.q_tiles * heads * a.q_splits <= 0x7fffffff && a.k_tiles * heads * a.k_splits <= 0x7fffffff,
               "attention backward: too many rows for one call");
   if constexpr (__is_same(T, __half)) {
-    B3R_TRY(check_cuda(cudaMemsetAsync(a.range, 0, heads * 8, s), "attention backward"));
+    B3R_TRY(check_cuda(cudaMemsetAsync(a.range, 0, heads * 12, s), "attention backward"));
     const int64_t chunks = (std::max(d.Lq, d.Lk) + kRangeRows - 1) / kRangeRows;
     B3R_REQUIRE(chunks * d.B <= 0x7fffffff && d.Hq + d.Hkv <= 65535, "attention backward: too many rows for one call");
     if (chunks > 0) {

@@ -45,3 +45,34 @@ def test_idle_first_halves_where_the_groups_write_q(G, D):
     kl = [(13 * b) % 60 + (200 if b % 5 == 0 else 1) for b in range(B)]
     q, k, v, do = _dense(B, Lq, Lk, 4 * G, 4, D, 'f16')
     _check(q, k, v, do, [(b, Lq, kl[b]) for b in range(B)], False, True, k_lens=_i32(kl))
+
+
+# ---------------------------------------------------------------- values far from one
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('size,scale', [(300.0, 1e-6), (3000.0, 2e-8), (0.5, 1e-9), (0.5, 1e-30)])
+def test_statistics_of_any_size_in_raw_scores(dtype, size, scale):
+    """lse / scale on both sides of 1.7e7, the end of 256 times a float16, with scores of ordinary size."""
+    q, k, v, do = _dense(1, 200, 300, 4, 2, 128, dtype)
+    q, k = q * (size / 1.5), k * (size / 1.5)
+    _check(q, k, v, do, [(0, 200, 300)], False, True, scale=scale)
+
+
+def test_large_deltas():
+    """do . o above 1.7e7 in float16, beside queries of ordinary size and hidden ones."""
+    q, k, v, do = _dense(2, 150, 260, 2, 1, 128, 'f16')
+    sign = torch.where(_rand(128, dtype=torch.float32, seed=9) > 0, 1.0, -1.0)
+    v = (20.0 * v + 200.0 * sign).half()
+    do[:, ::3] = (30.0 * do[:, ::3] + 1000.0 * sign).half()
+    q, k = q * 0.01, k * 0.01
+    _check(q, k, v, do, [(0, 150, 260), (1, 90, 40)], False, True, q_lens=_i32([150, 90]), k_lens=_i32([260, 40]))
+
+
+def test_raw_scores_past_float16_stay_finite():
+    """Raw scores of 2e7 and more at the default scale: one key takes everything."""
+    q, k, v, do = _dense(1, 130, 140, 1, 1, 128, 'f16')
+    q, k = q.sign() * 500.0 + q, k.sign() * 500.0 + k
+    k[:, ::7] = q[:, :20]
+    from blast3r_b200.attention import attention_backward, attention_forward
+    o, lse = attention_forward(q, k, v)
+    assert float(lse.max()) > 1.7e7 * 128 ** -0.5
+    assert all(bool(t.isfinite().all()) for t in (o, lse, *attention_backward(do, q, k, v, o, lse)))
