@@ -750,7 +750,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
   }
 }
 
-// Joins the parts of a row: weights 2^(lg_s - max) over their sum.  One warp to a row.  Latency bounds it: 5 us for
+// Joins the parts of a row: weights 2^(lg_s - max) over their sum.  A part that is NaN (its scores were, or a wait
+// ran out) makes the row NaN; the maximum would pass over it.  One warp to a row.  Latency bounds it: 5 us for
 // 96 rows of 64 in 6 parts, 6 us for 512 rows of 128 in 5.
 template <typename T>
 __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ FwdArgs a) {
@@ -762,7 +763,13 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ FwdAr
   if (m >= (int64_t)(d.cu_q ? s.ql : d.Lq) * G) return;
   const int64_t rows = (int64_t)d.Lq * G, step = (int64_t)d.B * d.Hkv * rows, at = head * rows + m;
   float top = -INFINITY;
-  for (int p = lane; p < a.splits; p += 32) top = fmaxf(top, a.part_l[p * step + at]);
+  bool nan = false;
+  for (int p = lane; p < a.splits; p += 32) {
+    const float lg = a.part_l[p * step + at];
+    top = fmaxf(top, lg);
+    nan = nan || isnan(lg);
+  }
+  nan = __any_sync(0xffffffffu, nan);
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
   const int c = lane * 4;
@@ -782,6 +789,7 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ FwdAr
         o.w += f * x.w;
       }
     }
+  if (nan) sum = __int_as_float(0x7fffffff);
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   const int i = (int)(m / G), h = kv * G + (int)(m % G);
   if (c < d.D)

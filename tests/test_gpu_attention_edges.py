@@ -76,3 +76,20 @@ def test_raw_scores_past_float16_stay_finite():
     o, lse = attention_forward(q, k, v)
     assert float(lse.max()) > 1.7e7 * 128 ** -0.5
     assert all(bool(t.isfinite().all()) for t in (o, lse, *attention_backward(do, q, k, v, o, lse)))
+
+
+# ---------------------------------------------------------------- NaN
+@pytest.mark.parametrize('D', [64, 128])
+def test_nan_of_a_split_row_stays(D):
+    """A row of NaN scores is NaN, split along the keys or not; a NaN value or key reaches the rows that see it."""
+    from blast3r_b200.attention import attention_forward
+    q, k, v, _ = _dense(3, 1, 5000, 4, 2, D, 'bf16')
+    q[0, 0, 1] = math.nan
+    k[1, 3, 1] = math.nan
+    kl = [5000, 60, 0]
+    for n in (5000, 100):                       # split along the keys, and not
+        o, lse = attention_forward(q, k[:, :n].contiguous(), v[:, :n].contiguous(), k_lens=_i32([min(n, x) for x in kl]))
+        assert bool(o[0, 0, 1].isnan().all()) and bool(lse[0, 1].isnan())
+        assert bool(o[1, 0, 2:].isnan().all()) and bool(lse[1, 2:].isnan().all())
+        assert bool(o[0, 0, [0, 2, 3]].isfinite().all()) and bool(o[1, 0, :2].isfinite().all())
+        assert float(o[2].abs().max()) == 0 and bool((lse[2] == -math.inf).all())
