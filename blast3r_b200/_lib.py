@@ -187,6 +187,34 @@ def call(name, *args):
     return check(getattr(lib(), name)(*args), name)
 
 
+_status = {}    # (operator, device index) -> int32 [1] in pinned host memory, which kernels reach by its address
+
+
+def status_word(what, index):
+    """The word that a kernel of operator `what` raises on CUDA device `index` when a bounded wait inside it runs
+    out.  Host memory, so that it is there, and clear, under the capture of a graph too."""
+    s = _status.get((what, index))
+    if s is None:
+        import torch
+        s = _status.setdefault((what, index), torch.zeros(1, dtype=torch.int32, pin_memory=True))   # (one for all threads)
+    return s
+
+
+def check_status(what, device):
+    """Waits for the work queued on `device` (the current one for None) and raises, once, if the operator's word is up."""
+    import torch
+    index = None if device is None else torch.device(device).index
+    if index is None:
+        index = torch.cuda.current_device()
+    s = _status.get((what, index))
+    if s is None:
+        return
+    torch.cuda.synchronize(index)
+    if int(s):
+        s.zero_()
+        raise B3RError(f'a bounded wait inside a kernel of {what} ran out: its outputs are not to be used')
+
+
 _fns = {}
 
 

@@ -15,26 +15,11 @@ from . import _lib as L
 
 DTYPES = {torch.bfloat16: L.B3R_BF16, torch.float16: L.B3R_F16}
 
-_status = {}    # device index -> int32 [1], raised by a kernel whose bounded wait ran out
-
-
-def _status_of(dev):
-    s = _status.get(dev.index)
-    if s is None:
-        if torch.cuda.is_current_stream_capturing():
-            return None               # memory of a graph's pool would not outlive the graph
-        s = _status[dev.index] = torch.zeros(1, dtype=torch.int32, device=dev)
-    return s
-
 
 def check_attention(device=None):
     """Raises if a wait inside an attention kernel of this process ran out on ``device`` (the
-    current one by default).  It reads a device flag, so it waits for the work queued so far."""
-    dev = torch.device('cuda', torch.cuda.current_device() if device is None else torch.device(device).index)
-    s = _status.get(dev.index)
-    if s is not None and int(s.item()):
-        s.zero_()
-        raise L.B3RError('a bounded wait inside an attention kernel ran out: its outputs are not to be used')
+    current one by default), in a call or a graph's replay.  It waits for the work queued so far."""
+    L.check_status('attention', device)
 
 
 def _tensor(t, packed):
@@ -123,8 +108,7 @@ def _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k):
 
 
 def _launch(name, d, dev, index):
-    status = _status_of(dev)
-    d.status = None if status is None else status.data_ptr()
+    d.status = L.status_word('attention', index).data_ptr()
     ref = C.byref(d)
     n = getattr(L.lib(), name + '_work_bytes')(ref)
     if n > 0:

@@ -541,8 +541,8 @@ typedef struct {
     b3r_attn_tensor q, k, v, o, lse;
     b3r_attn_tensor d_o, dq, dk, dv; /* backward only */
     void* work;                      /* 256-byte aligned, b3r_attention_*_work_bytes bytes */
-    int32_t* status;                 /* device int32 or NULL: set to 1 if a wait inside a kernel ran
-                                      * out (the outputs are then not to be used) */
+    int32_t* status;                 /* int32 that the device reaches, or NULL: set to 1 if a wait inside
+                                      * a kernel ran out (the outputs are then not to be used) */
 } b3r_attention_desc;
 
 /* o and lse are outputs. */

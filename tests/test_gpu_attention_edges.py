@@ -93,3 +93,51 @@ def test_nan_of_a_split_row_stays(D):
         assert bool(o[1, 0, 2:].isnan().all()) and bool(lse[1, 2:].isnan().all())
         assert bool(o[0, 0, [0, 2, 3]].isfinite().all()) and bool(o[1, 0, :2].isfinite().all())
         assert float(o[2].abs().max()) == 0 and bool((lse[2] == -math.inf).all())
+
+
+# ---------------------------------------------------------------- the status word
+def test_a_raised_status_is_reported_once():
+    from blast3r_b200 import _lib as L
+    from blast3r_b200 import attention as A
+    q, k, v, _ = _dense(1, 5, 7, 2, 2, 64, 'bf16')
+    A.attention_forward(q, k, v)
+    A.check_attention()
+    for device in (None, 'cuda', 0, q.device):
+        L.status_word('attention', q.get_device()).fill_(1)
+        with pytest.raises(L.B3RError, match='ran out'):
+            A.check_attention(device)
+        A.check_attention(device)
+
+
+def test_the_first_call_under_capture_has_a_status():
+    """A graph captured by a process's first call reports failures as every other call."""
+    import subprocess
+    import sys
+    code = '''
+import torch
+from blast3r_b200 import attention as A
+q, k, v = (torch.randn(2, 300, 4, 64, device='cuda').bfloat16() for _ in range(3))
+torch.cuda.synchronize()
+seen = []
+launch, A._launch = A._launch, lambda name, d, *a: (launch(name, d, *a), seen.append(d.status))
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    o, lse = A.attention_forward(q, k, v)
+    grads = A.attention_backward(o, q, k, v, o, lse)
+assert len(seen) == 2 and all(seen)
+from blast3r_b200 import _lib as L
+assert seen[0] == seen[1] == L.status_word('attention', 0).data_ptr()
+g.replay()
+A.check_attention()
+want = A.attention_forward(q, k, v)
+assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+assert all(torch.equal(a, b) for a, b in zip(grads, A.attention_backward(want[0], q, k, v, *want)))
+q.mul_(0.5)
+g.replay()
+assert torch.equal(o, A.attention_forward(q, k, v)[0])
+print('fine')
+'''
+    import os
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    out = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert out.returncode == 0 and 'fine' in out.stdout, out.stderr[-2000:]
