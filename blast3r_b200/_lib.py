@@ -142,6 +142,8 @@ _SIGS = {
     'b3r_residual_norm_fwd': (C.c_int, [C.POINTER(ResidualNorm), _vp, _i64, _vp, _i64, _vp, _vp, _vp]),
     'b3r_residual_norm_work_bytes': (_i64, [C.POINTER(ResidualNorm)]),
     'b3r_residual_norm_bwd': (C.c_int, [C.POINTER(ResidualNorm), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64] + [_vp] * 9),
+    'b3r_residual_norm_bwd_ex': (C.c_int, [C.POINTER(ResidualNorm), _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64] + [_vp] * 9 +
+                                 [C.c_int, C.c_int, _vp]),
     'b3r_attention_fwd_work_bytes': (_i64, [C.POINTER(AttentionDesc)]),
     'b3r_attention_fwd': (C.c_int, [C.POINTER(AttentionDesc), _vp]),
     'b3r_attention_bwd_work_bytes': (_i64, [C.POINTER(AttentionDesc)]),

@@ -240,6 +240,8 @@ struct NormArgs {
   float *part, *gpart;           // backward partials
   void* dgate;
   int post, pre, want_cols, gate_direct, stages, biases;
+  int wait_limit, lose;         // backward: polls of a wait; for a test, copies of a block's last row are not asked for
+  int32_t* status;
 };
 
 // Room for a row in shared memory.  Without VEC a row may begin anywhere: the whole 16-byte units that hold it
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
   extern __shared__ __align__(128) uint8_t dyn[];
   __shared__ alignas(16) float buf[kSumFloats<MAXT <= 512 ? 16 : 32>];
   __shared__ uint64_t full[kMaxStages];
-  __shared__ int dead_flag;
+  __shared__ int dead_flag, asked;                          // (asked: rows whose copies have been asked for, where not all)
   volatile int* dead = &dead_flag;
   const int threads = blockDim.x, tid = threadIdx.x, warps = threads >> 5, C = a.C;
   const int64_t first = a.rows * blockIdx.x / gridDim.x, last = a.rows * (blockIdx.x + 1) / gridDim.x;
@@ -457,7 +459,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
   const bool need_y = a.post || a.gate;
   const int bytes_x = slot_bytes<TX, VEC>(C), bytes_y = slot_bytes<TY, VEC>(C);
   auto request = [&](int64_t row) {                         // one thread: the copies of a row
-    if (row >= last) return;
+    if (row >= last || (a.lose && row == last - 1)) return;
     const int st = (int)((row - first) % a.stages);
     const uint32_t bar = smem_u32(&full[st]);
     uint8_t* to = ring + (size_t)st * stage_bytes<TX, TY, VEC>(C);
@@ -482,6 +484,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
   clear_sums(buf, kSumFloats<MAXT <= 512 ? 16 : 32>);
   if (RING && tid == 0) {
     dead_flag = 0;
+    asked = (int)(last - first) - a.lose;
     for (int i = 0; i < a.stages; ++i) mbar_init(smem_u32(&full[i]), 1);
     fence_async();
   }
@@ -521,6 +524,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
     keep(2, reinterpret_cast<const char*>(a.gate) + group * C * (a.wf32 ? 4 : sizeof(TY)), 1.f);
   }
   int st = 0, round = 0;
+  bool lost = false;                                        // a copy never came
   for (int64_t row = first; row < last; ++row) {
     const uint8_t* at = ring + (size_t)st * stage_bytes<TX, TY, VEC>(C);
     auto fetch = [&](float2 (&o)[kP], int off, auto type, const void* p, int64_t step, bool on) {
@@ -547,7 +551,10 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
         load8<T, VEC>(o, reinterpret_cast<const T*>(p) + row * step, 0, tid, threads, C);
       }
     };
-    if (RING) mbar_wait(smem_u32(&full[st]), round & 1, dead);
+    if (RING && !mbar_wait(smem_u32(&full[st]), round & 1, dead, a.wait_limit)) {
+      if (tid == 0 && !lost) asked = min(asked, max((int)(row - first) - 1, 0) + a.stages);
+      lost = true;
+    }
     float2 r[kP], dh[kP], y[kP], z[kP], d[kP];
     fetch(r, bytes_x, TX(), a.x, a.x_row, a.pre);
     fetch(dh, 2 * bytes_x, TY(), a.dh, a.dh_row, a.pre);
@@ -618,7 +625,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
 #pragma unroll
     for (int k = 0; k < kQ; ++k) q[k] = t[k].x + t[k].y;
     row_sum<kQ, MAXT <= 512 ? 16 : 32>(q, warps, buf, turn);
-    if (RING && tid == 0 && row > first) request(row - 1 + a.stages);   // every thread has left the row before
+    if (RING && tid == 0 && row > first && !lost) request(row - 1 + a.stages);   // every thread has left the row before
     if (a.pre) {
       const float rstd = rsqrtf(q[0] * inv + a.eps), proj = -q[2] * inv * rstd;   // -mean(z rhat)
       if constexpr (kOne) q[3] += rstd * (q[4] + proj * rstd * q[5]);
@@ -685,13 +692,6 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
       ++round;
     }
   }
-  if (RING && *dead) {                              // a copy never came: say so in every result
-#pragma unroll
-    for (int k = 0; k < kCols; ++k)
-#pragma unroll
-      for (int j = 0; j < kP; ++j) acc[k][j] = dg[j] = both(__int_as_float(0x7fffffff));
-    for (int t = 0; t < 100; ++t) __nanosleep(1000);
-  }
 #pragma unroll
   for (int j = 0; j < kE; ++j) {
     const int c = col_of<VEC>(0, j, tid, threads);
@@ -701,6 +701,17 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
       for (int k = 0; k < kCols; ++k)
         a.part[((int64_t)blockIdx.x * kCols + k) * C + c] = (j & 1) ? acc[k][j / 2].y : acc[k][j / 2].x;
     if (a.gate && !a.gate_direct && first < last) a.gpart[(blockIdx.x + group) * C + c] = (j & 1) ? dg[j / 2].y : dg[j / 2].x;
+  }
+  if constexpr (RING) {
+    __syncthreads();
+    if (*dead) {                                    // the copies still on their way end before the block does
+      int none = 0;
+      if (tid == 0) {
+        for (int r = max(0, asked - a.stages); r < asked; ++r) mbar_wait(smem_u32(&full[r % a.stages]), (r / a.stages) & 1, &none);
+        if (a.status) *a.status = 1;
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -932,8 +943,20 @@ extern "C" int b3r_residual_norm_bwd(const b3r_residual_norm* d, const void* dr,
                                      int64_t dh_row, const void* y, int64_t y_row, const void* r, int64_t r_row,
                                      void* dx, void* dy, void* dgate, void* dw_post, void* db_post, void* dw_pre,
                                      void* db_pre, void* work, void* stream) {
+  return b3r_residual_norm_bwd_ex(d, dr, dr_row, dh, dh_row, y, y_row, r, r_row, dx, dy, dgate, dw_post, db_post, dw_pre, db_pre,
+                                  work, nullptr, 0, 0, stream);
+}
+
+extern "C" int b3r_residual_norm_bwd_ex(const b3r_residual_norm* d, const void* dr, int64_t dr_row, const void* dh,
+                                        int64_t dh_row, const void* y, int64_t y_row, const void* r, int64_t r_row,
+                                        void* dx, void* dy, void* dgate, void* dw_post, void* db_post, void* dw_pre,
+                                        void* db_pre, void* work, int32_t* status, int wait_limit, int flags, void* stream) {
   NormArgs a;
   B3R_TRY(common(d, a));
+  B3R_REQUIRE((flags & ~B3R_NORM_TEST_LOST_COPY) == 0, "residual_norm backward: unknown flags");
+  a.status = status;
+  a.wait_limit = wait_limit > 0 ? wait_limit : kWaitLimit;
+  a.lose = flags & B3R_NORM_TEST_LOST_COPY;
   cudaStream_t s = as_stream(stream);
   const int64_t wsz = d->weight_dtype == B3R_F32 ? 4 : 2;
   void* const outs[kCols] = {dw_post, db_post, dw_pre, db_pre};

@@ -22,6 +22,12 @@ KINDS = {'layer': L.NORM_LAYER, 'rms': L.NORM_RMS}
 NormGrads = namedtuple('NormGrads', 'dx, dy, dgate, dw_post, db_post, dw_pre, db_pre')
 
 
+def check_norm(device=None):
+    """Raises if a wait inside a ``residual_norm_backward`` of this process ran out on ``device`` (the
+    current one by default), in a call or a graph's replay.  It waits for the work queued so far."""
+    L.check_status('residual_norm', device)
+
+
 def _rows(t):
     """t as (tensor, row stride) of rows of its last dimension, copied only where its strides
     have no single row stride."""
@@ -148,7 +154,9 @@ def residual_norm_backward(dr, dh, y, r, *, kind='layer', eps=1e-6, post=None, g
         out.dgate.zero_()                # the library sees no rows and does not know the gate's
     ptr = lambda t: None if t is None else t.data_ptr()                                           # noqa: E731
     args = [a for t, s in ts for a in (ptr(t), s)]
-    L.call_on(y.get_device(), 'b3r_residual_norm_bwd', C.byref(d), *args, *[ptr(t) for t in out], wp)
+    index = y.get_device()
+    L.call_on(index, 'b3r_residual_norm_bwd_ex', C.byref(d), *args, *[ptr(t) for t in out], wp,
+              L.status_word('residual_norm', index).data_ptr(), 0, 0)
     return out
 
 

@@ -512,6 +512,17 @@ int b3r_residual_norm_bwd(const b3r_residual_norm* d, const void* dr, int64_t dr
                           const void* y, int64_t y_row, const void* r, int64_t r_row, void* dx, void* dy, void* dgate,
                           void* dw_post, void* db_post, void* dw_pre, void* db_pre, void* work, void* stream);
 
+/* The same with a status word (an int32 that the device reaches, or NULL), set to 1 if a wait for the
+ * copies of a row ran out (the outputs are then not to be used; the context stays usable), and the limit of such
+ * a wait in polls of about 4 us (<= 0: the default, about a second).  flags: 0, or
+ * B3R_NORM_TEST_LOST_COPY, a test of that path in which some rows' copies are never asked for, where rows
+ * come through shared memory. */
+#define B3R_NORM_TEST_LOST_COPY 1
+int b3r_residual_norm_bwd_ex(const b3r_residual_norm* d, const void* dr, int64_t dr_row, const void* dh, int64_t dh_row,
+                             const void* y, int64_t y_row, const void* r, int64_t r_row, void* dx, void* dy, void* dgate,
+                             void* dw_post, void* db_post, void* dw_pre, void* db_pre, void* work, int32_t* status,
+                             int wait_limit, int flags, void* stream);
+
 /* Attention over B sequences with Hq query heads and Hkv key/value heads (Hq a multiple of Hkv;
  * query head h uses head h / (Hq / Hkv)), head size D (a multiple of 8, at most 128), dtype B3R_BF16
  * or B3R_F16:

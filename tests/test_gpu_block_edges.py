@@ -1,0 +1,35 @@
+"""Rotary positions and norms where tensors overlap, gradients go other ways and arguments do not fit."""
+import math
+
+import pytest
+import torch
+
+from tests import block_reference as R
+from tests.test_gpu_norm import _backward, _forward, _make, _sum_of
+from tests.test_gpu_rotary import _setup
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize('C,stream,gate', [(64, 'bf16', None), (1024, 'f32', 'token'), (1000, 'bf16', 'sample'), (1001, 'bf16', 'token'),
+                                           (4096, 'bf16', 'channel'), (5120, 'bf16', None)])
+@pytest.mark.parametrize('kind,weights', [('rms', False), ('layer', True)])
+def test_a_lost_copy_is_reported(monkeypatch, C, stream, gate, kind, weights):
+    """A wait for a row whose copies are never asked for runs out: the call ends, check_norm raises once, and the next
+    call is right."""
+    from blast3r_b200 import _lib as L
+    from blast3r_b200.norm import check_norm, residual_norm_backward
+    y, x, dr, dh, kw = _make(4, 175, C, 'bf16', stream, kind, True, True, gate)
+    if not weights:
+        kw.update(post=True, pre=True)
+    want = residual_norm_backward(dr, dh, y, x, **kw)
+    check_norm()
+    call = L.call_on
+    monkeypatch.setattr(L, 'call_on', lambda index, name, *a: call(index, name, *a[:-2], 100, 1))
+    residual_norm_backward(dr, dh, y, x, **kw)
+    monkeypatch.undo()
+    with pytest.raises(L.B3RError, match='ran out'):
+        check_norm()
+    check_norm()
+    again = residual_norm_backward(dr, dh, y, x, **kw)
+    assert all(t is None or torch.equal(t, w) for t, w in zip(again, want))
