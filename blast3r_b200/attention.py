@@ -126,8 +126,9 @@ def attention_forward(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=
     multiple of 8 up to 128; any strides (a copy is made where D is not contiguous or a row does
     not start on 16 bytes).  q_lens, k_lens: int32 (B,) lengths of padded sequences; what lies
     past them is not used.  Packed: q (Tq, Hq, D), k and v (Tk, Hkv, D), with cu_q, cu_k
-    int32 (sequences + 1,), where each sequence begins and ends, and max_q, max_k, bounds of
-    their lengths.  causal: query i sees the keys j <= i + k_len - q_len, so the last query sees
+    int32 (sequences + 1,), where each sequence begins and ends (they do not decrease), and max_q,
+    max_k, bounds of their lengths: rows past them are not used.  Rows of no sequence have o = 0,
+    lse = -inf and zero gradients.  causal: query i sees the keys j <= i + k_len - q_len, so the last query sees
     the last key.  A query that sees no key has o = 0 and lse = -inf.  scale: positive, D**-0.5 by
     default."""
     d, packed, keep = _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k)

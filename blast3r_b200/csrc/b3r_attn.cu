@@ -1,4 +1,6 @@
-// Part 5 of the C ABI, attention: what both passes check, and the tensor maps that they load by.
+// Part 5 of the C ABI, attention: what both passes check, the tensor maps that they load by, and the packed rows
+// that they do not reach.
+#include <algorithm>
 #include <utility>
 #include "b3r_attn.cuh"
 
@@ -28,14 +30,14 @@ int attn_check(const b3r_attention_desc* d, bool backward) {
   for (int i = 0; i < (backward ? 8 : 4); ++i) {
     const bool of_k = i == 1 || i == 2 || i >= 6;
     const int64_t rows = of_k ? nk : nq, heads = of_k ? d->Hkv : d->Hq;
-    if (d->B == 0 || rows == 0) continue;
+    if ((d->B == 0 && !d->cu_q) || rows == 0) continue;
     B3R_REQUIRE(ts[i]->p, "attention: NULL tensor");
     B3R_REQUIRE(((uintptr_t)ts[i]->p & 15) == 0, "attention: tensors must be 16-byte aligned");
     auto ok = [](int64_t stride, int64_t n) { return n <= 1 || (stride > 0 && stride % 8 == 0); };
     B3R_REQUIRE(ok(ts[i]->row, rows) && ok(ts[i]->head, heads) && (d->cu_q || ok(ts[i]->batch, d->B)),
                 "attention: strides must be positive multiples of 8 elements");
   }
-  B3R_REQUIRE(d->B == 0 || nq == 0 || d->lse.p, "attention: NULL lse");
+  B3R_REQUIRE((d->B == 0 && !d->cu_q) || nq == 0 || d->lse.p, "attention: NULL lse");
   return B3R_OK;
 }
 
@@ -81,6 +83,52 @@ static int encode_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, 
                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS) return fail(B3R_E_CUDA, "attention: cuTensorMapEncodeTiled failed (%d)", (int)rc);
   return B3R_OK;
+}
+
+// Packed rows of no sequence: before the first, past the last, or past the bounds Lq / Lk of a length.  A thread looks
+// one row up among the offsets, and its warp clears those that were found outside.  Nothing to clear is the usual
+// case, and takes a launch's latency (2.2 us for 13 thousand rows in 20 sequences on one B200).
+namespace {
+constexpr int kClearRows = 128;
+__global__ void __launch_bounds__(kClearRows) k_attn_clear(const __grid_constant__ b3r_attention_desc d, int backward) {
+  const bool of_k = blockIdx.y == 1;
+  const int32_t* cu = of_k ? d.cu_k : d.cu_q;
+  const int64_t T = of_k ? d.Tk : d.Tq, row = (int64_t)blockIdx.x * kClearRows + threadIdx.x;
+  const int lane = threadIdx.x & 31, most = of_k ? d.Lk : d.Lq, heads = of_k ? d.Hkv : d.Hq, chunks = d.D / 8;
+  bool off = false;
+  if (row < T) {
+    int lo = 0, hi = d.B + 1;                          // offsets up to this row: those before lo, and none from hi on
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if (cu[mid] <= row) lo = mid + 1;
+      else hi = mid;
+    }
+    off = lo == 0 || lo > d.B || row - max(cu[lo - 1], 0) >= most;
+  }
+  for (uint32_t left = __ballot_sync(0xffffffffu, off); left; left &= left - 1) {
+    const int64_t r = row - lane + __ffs(left) - 1;
+    for (int i = lane; i < heads * chunks; i += 32) {
+      const int h = i / chunks, c = (i - h * chunks) * 8;
+      auto zero = [&](const b3r_attn_tensor& t) { *reinterpret_cast<uint4*>(attn_row<uint16_t>(t, 0, r, h) + c) = make_uint4(0, 0, 0, 0); };
+      if (!backward) {
+        zero(d.o);
+        if (c == 0) *attn_row<float>(d.lse, 0, r, h) = -INFINITY;
+      } else if (!of_k) {
+        zero(d.dq);
+      } else {
+        zero(d.dk);
+        zero(d.dv);
+      }
+    }
+  }
+}
+}  // namespace
+
+int attn_clear(const b3r_attention_desc* d, bool backward, cudaStream_t s) {
+  const int64_t rows = backward ? std::max(d->Tq, d->Tk) : d->Tq;
+  if (!d->cu_q || rows == 0) return B3R_OK;
+  k_attn_clear<<<dim3((unsigned)((rows + kClearRows - 1) / kClearRows), backward ? 2 : 1), kClearRows, 0, s>>>(*d, backward);
+  return check_launch("attention");
 }
 
 int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype, int box) {

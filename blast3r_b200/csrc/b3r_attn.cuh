@@ -68,6 +68,9 @@ int attn_smem(F* f, uint64_t& done, const char* what) {
 int attn_check_sizes(const b3r_attention_desc* d);
 int attn_check(const b3r_attention_desc* d, bool backward);
 
+// Clears the outputs' packed rows that belong to no sequence; before the kernels that write the others.
+int attn_clear(const b3r_attention_desc* d, bool backward, cudaStream_t s);
+
 // The tensor map of a (D, rows, heads, batch) tensor in boxes of 64 elements x `box` rows.
 int attn_map(CUtensorMap* map, const b3r_attn_tensor& t, int64_t rows, int heads, int batch, int D, int dtype, int box);
 // The same tensor as (D, heads, rows, batch), in boxes of 64 elements x G heads x 128 / G rows: row m

@@ -857,6 +857,7 @@ extern "C" int64_t b3r_attention_bwd_work_bytes(const b3r_attention_desc* d) {
 
 extern "C" int b3r_attention_bwd(const b3r_attention_desc* d, void* stream) {
   B3R_TRY(attn_check(d, true));
+  B3R_TRY(attn_clear(d, true, as_stream(stream)));
   if (d->B == 0) return B3R_OK;
   BwdArgs a;
   a.d = *d;

@@ -868,6 +868,7 @@ extern "C" int64_t b3r_attention_fwd_work_bytes(const b3r_attention_desc* d) {
 
 extern "C" int b3r_attention_fwd(const b3r_attention_desc* d, void* stream) {
   B3R_TRY(attn_check(d, false));
+  B3R_TRY(attn_clear(d, false, as_stream(stream)));
   if (d->B == 0 || d->Lq == 0 || (d->cu_q && d->Tq == 0)) return B3R_OK;
   FwdArgs a;
   a.d = *d;

@@ -533,8 +533,9 @@ int b3r_residual_norm_bwd_ex(const b3r_residual_norm* d, const void* dr, int64_t
  *   padded: sequence b is q[b, 0..q_len) of Lq rows and k[b, 0..k_len) of Lk; q_lens / k_lens (device
  *     int32 [B]) or NULL (all of them).  Rows past q_len get o = 0, lse = -inf, dq = 0, rows
  *     past k_len dk = dv = 0.
- *   packed: cu_q, cu_k (device int32 [B + 1], not NULL) hold where each sequence begins and ends
- *     among Tq / Tk rows; the batch strides are not used and Lq / Lk bound the lengths.
+ *   packed: cu_q, cu_k (device int32 [B + 1], not NULL, not decreasing) hold where each sequence begins and
+ *     ends among Tq / Tk rows; the batch strides are not used and Lq / Lk bound the lengths: rows past
+ *     them are not used.  Rows of no sequence get o = 0, lse = -inf and zero gradients.
  * What lies in rows past a sequence's end is not used, NaN included.  Lengths and offsets
  * outside of the tensors are cut to them.  Strides (batch, row, head) in elements, multiples
  * of 8, with 16-byte aligned bases; lse is float with strides of its own. */

@@ -95,6 +95,54 @@ def test_nan_of_a_split_row_stays(D):
         assert float(o[2].abs().max()) == 0 and bool((lse[2] == -math.inf).all())
 
 
+# ---------------------------------------------------------------- packed rows of no sequence
+def _poison(n=64 << 20):
+    """Leaves NaN in the memory that the next outputs are made of."""
+    ts = [torch.full((n >> s,), math.nan, device='cuda') for s in range(0, 20, 2) for _ in range(2)]
+    del ts
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+@pytest.mark.parametrize('lens', [([130, 0, 1, 57], [60, 33, 0, 257]), ([3], [2]), ([0, 0], [0, 0])])
+def test_packed_rows_of_no_sequence(dtype, lens):
+    """Rows before the first sequence, past the last one, and past max_q / max_k: o = 0, lse = -inf, no gradients."""
+    from blast3r_b200.attention import attention_backward, attention_forward
+    ql, kl = lens
+    most_q, most_k = max(max(ql) - 5, 1), max(max(kl) - 9, 1)
+    cq, ck = [17 + sum(ql[:i]) for i in range(len(ql) + 1)], [5 + sum(kl[:i]) for i in range(len(kl) + 1)]
+    q, k, v, do = (t[0] for t in _dense(1, cq[-1] + 300, ck[-1] + 131, 6, 2, 72, dtype))
+    seqs = [(slice(cq[i], cq[i] + min(n, most_q)), slice(ck[i], ck[i] + min(m, most_k))) for i, (n, m) in enumerate(zip(ql, kl))]
+    off_q, off_k = (torch.ones(n, dtype=torch.bool, device='cuda') for n in (len(q), len(k)))
+    for a, b in seqs:
+        off_q[a], off_k[b] = False, False
+    for t, off in ((q, off_q), (do, off_q), (k, off_k), (v, off_k)):
+        t[off] = math.nan
+    kw = dict(cu_q=_i32(cq), cu_k=_i32(ck), max_q=most_q, max_k=most_k)
+    _poison()
+    o, lse = attention_forward(q, k, v, **kw)
+    assert float(o[off_q].abs().max()) == 0 and bool((lse[:, off_q] == -math.inf).all())
+    _poison()
+    grads = attention_backward(do, q, k, v, o, lse, **kw)
+    for g, off in zip(grads, (off_q, off_k, off_k)):
+        assert float(g[off].abs().max()) == 0 and bool(g.isfinite().all())
+    want = R.attention(q, k, v, do, o, False, 72 ** -0.5, seqs, True)
+    for name, t in zip(('o', 'lse', 'dq', 'dk', 'dv'), (o, lse, *grads)):
+        R.close(t, *want[name], name)
+
+
+def test_packed_bounds_of_zero():
+    """max_q or max_k of zero: nothing sees anything, and the outputs are still whole."""
+    from blast3r_b200.attention import attention_backward, attention_forward
+    q, k, v, do = (t[0] for t in _dense(1, 40, 50, 2, 2, 64, 'bf16'))
+    for mq, mk in ((0, 50), (40, 0), (0, 0)):
+        kw = dict(cu_q=_i32([0, 40]), cu_k=_i32([0, 50]), max_q=mq, max_k=mk)
+        _poison()
+        o, lse = attention_forward(q, k, v, **kw)
+        _poison()
+        grads = attention_backward(do, q, k, v, o, lse, **kw)
+        assert all(float(t.abs().max()) == 0 for t in (o, *grads)) and bool((lse == -math.inf).all())
+
+
 # ---------------------------------------------------------------- the status word
 def test_a_raised_status_is_reported_once():
     from blast3r_b200 import _lib as L
@@ -141,3 +189,15 @@ print('fine')
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     out = subprocess.run([sys.executable, '-c', code], cwd=root, capture_output=True, text=True, timeout=300)
     assert out.returncode == 0 and 'fine' in out.stdout, out.stderr[-2000:]
+
+
+def test_packed_without_sequences():
+    """Offsets of no sequence at all: every row is of none."""
+    from blast3r_b200.attention import attention_backward, attention_forward
+    q, k, v, do = (t[0] for t in _dense(1, 40, 50, 2, 2, 64, 'f16'))
+    kw = dict(cu_q=_i32([0]), cu_k=_i32([0]), max_q=40, max_k=50)
+    _poison()
+    o, lse = attention_forward(q, k, v, **kw)
+    _poison()
+    grads = attention_backward(do, q, k, v, o, lse, **kw)
+    assert all(float(t.abs().max()) == 0 for t in (o, *grads)) and bool((lse == -math.inf).all())
