@@ -43,7 +43,7 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   if (mbar_try(bar, parity)) return true;
   for (int n = 0; n < limit; ++n) {
     if (mbar_try(bar, parity)) return true;
-    if (*dead) return false;
+    if ((n & 63) == 63 && *dead) return false;   // (every poll: 4 % of the attention kernels)
   }
   *dead = 1;
   return false;
