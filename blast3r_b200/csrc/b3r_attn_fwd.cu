@@ -18,7 +18,9 @@
 // The maximum that the exponentials are taken against follows the true one only when it has
 // grown by more than 2^8: P, its sum and O then carry the same factor, which cancels in O / l, so
 // O in tensor memory is rescaled a few times at most instead of at every tile.  P is rounded to the
-// operands' type for the product (its sum is taken before, in float32).
+// operands' type for the product (its sum is taken before, in float32).  In float16 it is carried 2^7 times as large
+// besides, 2^15 at most: keys that share little among many would else fall below float16's numbers (30000
+// probabilities of 2^-25, which round to 2^-24, doubled what they add to o).
 //
 // What bounds it, measured on one B200 (1669 TFLOP/s, 6.5 TB/s):
 //   one query over 32768 keys (16 sequences, 32/8 heads of 128): 228 us, 5.6 TB/s: HBM
@@ -38,6 +40,8 @@ constexpr int kThreads = 384;   // three warpgroups: two of softmax, one of load
 constexpr int kMaxStages = 8;
 constexpr int kAskAhead = 4;    // key tiles before its end at which a job's successor is asked for
 constexpr float kGrow = 8.f;    // log2 of how far the maximum may grow before O is rescaled
+template <typename T>
+constexpr float kUp = __is_same(T, __half) ? 7.f : 0.f;   // log2 of P at the maximum that it is taken against
 
 struct alignas(64) FwdArgs {
   CUtensorMap q, k, v;
@@ -559,10 +563,10 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
           if (lane == 0) mbar_arrive(smem_u32(&sh.p_full[w][bar]));
           continue;
         }
-        auto follow = [&](float top) {                   // moves mx after the true maximum, O and l with it
-          const bool grow = top > mx + kGrow || mx == -INFINITY;   // (mx = -inf: nothing summed yet)
+        auto follow = [&](float top) {                   // moves mx after the true maximum (2^kUp below it), O and l with it
+          const bool grow = top > mx + (kGrow + kUp<T>) || mx == -INFINITY;   // (mx = -inf: nothing summed yet)
           if (it > 0 && __any_sync(0xffffffffu, grow && top > mx)) {
-            const float f = grow && top > mx ? ex2(mx - top) : 1.f;      // 0 for the first key that the row sees
+            const float f = grow && top > mx ? ex2(mx - (top - kUp<T>)) : 1.f;      // 0 for the first key that the row sees
             mbar_wait(smem_u32(&sh.o_done[w]), (mine - 1) & 1, dead);
             tc_fence_after();
 #pragma unroll
@@ -576,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
             }
             l *= f;
           }
-          if (grow) mx = top;
+          if (grow) mx = top - kUp<T>;
         };
         float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
         auto exps = [&](const uint32_t* s, uint32_t to) {   // 32 columns of P

@@ -78,6 +78,17 @@ def test_raw_scores_past_float16_stay_finite():
     assert all(bool(t.isfinite().all()) for t in (o, lse, *attention_backward(do, q, k, v, o, lse)))
 
 
+def test_many_small_probabilities_beside_a_large_one():
+    """One key takes nearly all, and many share the rest: their probabilities lie below float16's numbers."""
+    for Lq, Lk in ((1, 30000), (140, 30000)):
+        q = torch.zeros(1, Lq, 2, 64, device='cuda', dtype=torch.float16)
+        k = torch.zeros(1, Lk, 1, 64, device='cuda', dtype=torch.float16)
+        q[..., 0], k[:, 0, :, 0] = 8.0, 17.3 / 8.0
+        v = torch.ones(1, Lk, 1, 64, device='cuda', dtype=torch.float16)
+        v[:, 0] = 0.0
+        _check(q, k, v, torch.ones_like(q), [(0, Lq, Lk)], False, False, scale=1.0)
+
+
 # ---------------------------------------------------------------- NaN
 @pytest.mark.parametrize('D', [64, 128])
 def test_nan_of_a_split_row_stays(D):
