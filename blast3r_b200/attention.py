@@ -129,8 +129,8 @@ def attention_forward(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=
     int32 (sequences + 1,), where each sequence begins and ends (they do not decrease), and max_q,
     max_k, bounds of their lengths: rows past them are not used.  Rows of no sequence have o = 0,
     lse = -inf and zero gradients.  causal: query i sees the keys j <= i + k_len - q_len, so the last query sees
-    the last key.  A query that sees no key has o = 0 and lse = -inf.  scale: positive, D**-0.5 by
-    default."""
+    the last key.  A query that sees no key has o = 0 and lse = -inf.  scale: finite, 2**-100 at least,
+    D**-0.5 by default."""
     d, packed, keep = _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k)
     q, k, v = _readable(q), _readable(k), _readable(v)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)

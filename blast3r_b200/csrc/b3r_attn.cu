@@ -1,6 +1,7 @@
 // Part 5 of the C ABI, attention: what both passes check, the tensor maps that they load by, and the packed rows
 // that they do not reach.
 #include <algorithm>
+#include <cmath>
 #include <utility>
 #include "b3r_attn.cuh"
 
@@ -22,7 +23,8 @@ int attn_check_sizes(const b3r_attention_desc* d) {
 
 int attn_check(const b3r_attention_desc* d, bool backward) {
   B3R_TRY(attn_check_sizes(d));
-  B3R_REQUIRE(d->scale > 0.f, "attention: the scale must be positive");
+  // (from 2^-100 on the backward pass's lse / scale is a float32 too)
+  B3R_REQUIRE(d->scale >= 0x1p-100f && d->scale < INFINITY, "attention: the scale must be positive and finite, 2^-100 at least");
   B3R_REQUIRE((d->cu_q == nullptr) == (d->cu_k == nullptr), "attention: packed sequences need cu_q and cu_k");
   B3R_REQUIRE(!d->cu_q || (!d->q_lens && !d->k_lens), "attention: packed sequences have no q_lens or k_lens");
   const b3r_attn_tensor* ts[] = {&d->q, &d->k, &d->v, &d->o, &d->d_o, &d->dq, &d->dk, &d->dv};

@@ -526,7 +526,7 @@ int b3r_residual_norm_bwd_ex(const b3r_residual_norm* d, const void* dr, int64_t
 /* Attention over B sequences with Hq query heads and Hkv key/value heads (Hq a multiple of Hkv;
  * query head h uses head h / (Hq / Hkv)), head size D (a multiple of 8, at most 128), dtype B3R_BF16
  * or B3R_F16:
- *     S_ij = scale q_i . k_j (scale > 0),   lse_i = log sum_j exp S_ij,   o_i = sum_j exp(S_ij - lse_i) v_j
+ *     S_ij = scale q_i . k_j (scale finite, >= 2^-100),   lse_i = log sum_j exp S_ij,   o_i = sum_j exp(S_ij - lse_i) v_j
  * over the keys j that query i sees: j < k_len and, if causal, j <= i + k_len - q_len (the last
  * query sees the last key).  A query that sees none has o = 0, lse = -inf and zero gradients.
  * Two layouts:

@@ -202,6 +202,15 @@ print('fine')
     assert out.returncode == 0 and 'fine' in out.stdout, out.stderr[-2000:]
 
 
+# ---------------------------------------------------------------- arguments
+def test_scales_out_of_range_are_refused():
+    from blast3r_b200.attention import attention_forward
+    q, k, v, _ = _dense(1, 5, 7, 2, 2, 64, 'bf16')
+    for scale in (math.inf, 1e300, 1e-39, math.nan, 0.0, -1.0):
+        with pytest.raises(RuntimeError, match='scale'):
+            attention_forward(q, k, v, scale=scale)
+
+
 def test_packed_without_sequences():
     """Offsets of no sequence at all: every row is of none."""
     from blast3r_b200.attention import attention_backward, attention_forward
