@@ -90,9 +90,10 @@ def _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k):
             raise RuntimeError('attention: cu_q has one element more than there are sequences')
         keep += [_index(cu_q, 'cu_q', d.B + 1, dev), _index(cu_k, 'cu_k', d.B + 1, dev)]
         d.cu_q, d.cu_k = keep[0].data_ptr(), keep[1].data_ptr()
-        d.Lq, d.Lk, d.Tq, d.Tk = int(max_q), int(max_k), q.shape[0], k.shape[0]
-        if d.Lq < 0 or d.Lk < 0:
+        if max_q < 0 or max_k < 0:
             raise RuntimeError('attention: max_q and max_k must not be negative')
+        d.Tq, d.Tk = q.shape[0], k.shape[0]
+        d.Lq, d.Lk = min(int(max_q), d.Tq), min(int(max_k), d.Tk)      # (no sequence is longer than all rows)
     else:
         if max_q is not None or max_k is not None:
             raise RuntimeError('attention: max_q and max_k go with packed sequences')

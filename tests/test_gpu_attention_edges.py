@@ -211,6 +211,17 @@ def test_scales_out_of_range_are_refused():
             attention_forward(q, k, v, scale=scale)
 
 
+def test_bounds_past_32_bits():
+    """Bounds of any size bound the lengths; they do not wrap to others on their way to the library."""
+    from blast3r_b200.attention import attention_forward
+    q, k, v, _ = (t[0] for t in _dense(1, 50, 50, 2, 2, 64, 'bf16'))
+    cu = dict(cu_q=_i32([0, 13, 50]), cu_k=_i32([0, 13, 50]))
+    want = attention_forward(q, k, v, **cu, max_q=37, max_k=37)
+    for most in (dict(max_q=2 ** 32 + 5, max_k=37), dict(max_q=37, max_k=2 ** 32 + 5), dict(max_q=2 ** 31, max_k=2 ** 40)):
+        got = attention_forward(q, k, v, **cu, **most)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 def test_packed_without_sequences():
     """Offsets of no sequence at all: every row is of none."""
     from blast3r_b200.attention import attention_backward, attention_forward
