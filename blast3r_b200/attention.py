@@ -49,7 +49,7 @@ def _readable(t):
 
 
 def _index(t, name, n, dev):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev:
         raise RuntimeError(f'attention: {name} is an int32 tensor of {n} elements on the tensors\' device')
     return t.contiguous()
 
@@ -85,7 +85,7 @@ def _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k):
             raise RuntimeError('attention: packed sequences need cu_q, cu_k, max_q and max_k')
         if q_lens is not None or k_lens is not None:
             raise RuntimeError('attention: packed sequences have no q_lens or k_lens')
-        d.B = cu_q.shape[0] - 1
+        d.B = cu_q.shape[0] - 1 if isinstance(cu_q, torch.Tensor) and cu_q.dim() == 1 else -1
         if d.B < 0:
             raise RuntimeError('attention: cu_q has one element more than there are sequences')
         keep += [_index(cu_q, 'cu_q', d.B + 1, dev), _index(cu_k, 'cu_k', d.B + 1, dev)]
@@ -153,7 +153,7 @@ def attention_backward(do, q, k, v, o, lse, *, causal=False, scale=None, q_lens=
         if not isinstance(t, torch.Tensor) or t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:
             raise RuntimeError(f'attention backward: {name} has the shape, type and device of q')
     want = (d.Hq, d.Tq) if packed else (d.B, d.Hq, d.Lq)
-    if tuple(lse.shape) != want or lse.dtype != torch.float32 or lse.device != q.device:
+    if not isinstance(lse, torch.Tensor) or tuple(lse.shape) != want or lse.dtype != torch.float32 or lse.device != q.device:
         raise RuntimeError(f'attention backward: lse is the forward call\'s, float32 {want}')
     do, q, k, v, o = (_readable(t) for t in (do, q, k, v, o))
     dq, dk, dv = (torch.empty_like(t, memory_format=torch.contiguous_format) for t in (q, k, v))

@@ -89,7 +89,7 @@ def _describe(y, x, kind, eps, post, gate, residual_scale, pre):
     has_post, w_post, b_post = _pair(post, 'post')
     has_pre, w_pre, b_pre = _pair(pre, 'pre')
     rows, per = (y.numel() // Cn if Cn else 0), 1
-    if gate is not None:
+    if isinstance(gate, torch.Tensor):
         per = _gate_rows(gate, shape)
         if per is None:
             raise RuntimeError(f'residual_norm: the gate {tuple(gate.shape)} is (C,), (B, C), (B, 1, C) or the shape of '
@@ -97,6 +97,8 @@ def _describe(y, x, kind, eps, post, gate, residual_scale, pre):
     wt, keep, ptrs = None, [], []
     for t in (w_post, b_post, gate, w_pre, b_pre):
         if t is not None:
+            if not isinstance(t, torch.Tensor):
+                raise RuntimeError(f'residual_norm: weights, biases and the gate are tensors, got {t!r}')
             if t is not gate and (t.dim() != 1 or t.shape[0] != Cn):
                 raise RuntimeError(f'residual_norm: weights and biases have {Cn} elements')
             if t.get_device() != dev:

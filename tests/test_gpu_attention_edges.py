@@ -222,6 +222,19 @@ def test_bounds_past_32_bits():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_what_is_no_tensor_is_refused():
+    from blast3r_b200.attention import attention_backward, attention_forward
+    q, k, v, do = _dense(1, 5, 7, 2, 2, 64, 'bf16')
+    o, lse = attention_forward(q, k, v)
+    cu = _i32([0, 5])
+    for bad in (lambda: attention_forward(q, k, v, k_lens=[7]), lambda: attention_forward(q, k, v, q_lens=5),
+                lambda: attention_forward(q[0], q[0], q[0], cu_q=[0, 5], cu_k=cu, max_q=5, max_k=5),
+                lambda: attention_forward(q[0], q[0], q[0], cu_q=cu, cu_k=[0, 5], max_q=5, max_k=5),
+                lambda: attention_backward(do, q, k, v, o, None), lambda: attention_backward(None, q, k, v, o, lse)):
+        with pytest.raises(RuntimeError):
+            bad()
+
+
 def test_packed_without_sequences():
     """Offsets of no sequence at all: every row is of none."""
     from blast3r_b200.attention import attention_backward, attention_forward

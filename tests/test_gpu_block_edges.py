@@ -11,6 +11,14 @@ from tests.test_gpu_rotary import _setup
 pytestmark = pytest.mark.gpu
 
 
+def test_norm_refuses_what_is_no_tensor():
+    from blast3r_b200.norm import residual_norm_forward
+    y, x, _, _, kw = _make(2, 6, 64, 'bf16', 'bf16', 'layer', True, True, 'sample')
+    for bad in (dict(gate=1.0), dict(pre=(1.0, None)), dict(post=(None, 0.5))):
+        with pytest.raises(RuntimeError):
+            residual_norm_forward(y, x, **{**kw, **bad})
+
+
 @pytest.mark.parametrize('C,stream,gate', [(64, 'bf16', None), (1024, 'f32', 'token'), (1000, 'bf16', 'sample'), (1001, 'bf16', 'token'),
                                            (4096, 'bf16', 'channel'), (5120, 'bf16', None)])
 @pytest.mark.parametrize('kind,weights', [('rms', False), ('layer', True)])
