@@ -217,6 +217,21 @@ def check_status(what, device):
         raise B3RError(f'a bounded wait inside a kernel of {what} ran out: its outputs are not to be used')
 
 
+_forward_ad = None
+
+
+def refuse_tangents(what, tensors):
+    """Raises if one of the tensors carries a forward-mode tangent: the outputs, written by kernels, would have none."""
+    global _forward_ad
+    if _forward_ad is None:
+        from torch.autograd import forward_ad as _forward_ad
+    if getattr(_forward_ad, '_current_level', 0) < 0:         # (outside of dual levels, without a look at each)
+        return
+    for t in tensors:
+        if hasattr(t, 'data_ptr') and _forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f'{what} has no forward-mode derivative: its tensors must not carry tangents')
+
+
 _fns = {}
 
 

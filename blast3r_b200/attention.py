@@ -183,6 +183,7 @@ class _Attention(torch.autograd.Function):
 def attention(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=None, cu_q=None, cu_k=None, max_q=None, max_k=None):
     """o of ``attention_forward``, differentiable in q, k and v."""
     kw = dict(causal=causal, scale=scale, max_q=max_q, max_k=max_k)
+    L.refuse_tangents('attention', (q, k, v))
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
         return _Attention.apply(q, k, v, q_lens, k_lens, cu_q, cu_k, kw)
     return attention_forward(q, k, v, q_lens=q_lens, k_lens=k_lens, cu_q=cu_q, cu_k=cu_k, **kw)[0]

@@ -188,6 +188,7 @@ def residual_norm(y, x, *, kind='layer', eps=1e-6, post=None, gate=None, residua
     has_post, w_post, b_post = _pair(post, 'post')
     has_pre, w_pre, b_pre = _pair(pre, 'pre')
     ts = (y, x, w_post, b_post, gate, w_pre, b_pre)
+    L.refuse_tangents('residual_norm', ts)
     if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in ts):
         return _ResidualNorm.apply(*ts, has_post, has_pre, kind, eps, residual_scale)
     return residual_norm_forward(y, x, kind=kind, eps=eps, post=post, gate=gate, residual_scale=residual_scale, pre=pre)

@@ -146,6 +146,7 @@ def rotary(xs, table, positions, *, interleaved=False, inverse=False, inplace=Fa
     gradients).  A position outside of the table gives NaN.  Differentiable in xs."""
     pair = isinstance(xs, (tuple, list))
     ts = tuple(xs) if pair else (xs,)
+    L.refuse_tangents('rotary', ts)
     if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad for x in ts):
         if inplace:
             raise RuntimeError('rotary: tensors that need gradients cannot be turned in place')

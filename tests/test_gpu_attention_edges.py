@@ -235,6 +235,22 @@ def test_what_is_no_tensor_is_refused():
             bad()
 
 
+def test_forward_mode_is_refused():
+    """Nothing computes a tangent, so a dual tensor raises instead of losing its own."""
+    import torch.autograd.forward_ad as fwd
+    from blast3r_b200.attention import attention
+    q, k, v, t = _dense(1, 5, 5, 2, 2, 64, 'bf16')
+    with fwd.dual_level():
+        for which in range(3):
+            args = [fwd.make_dual(x, t) if i == which else x for i, x in enumerate((q, k, v))]
+            with pytest.raises(RuntimeError):
+                attention(*args)
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                attention(*args)
+        assert attention(q, k, v).shape == q.shape
+    assert attention(q, k, v).shape == q.shape
+
+
 def test_packed_without_sequences():
     """Offsets of no sequence at all: every row is of none."""
     from blast3r_b200.attention import attention_backward, attention_forward

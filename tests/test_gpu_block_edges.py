@@ -11,6 +11,29 @@ from tests.test_gpu_rotary import _setup
 pytestmark = pytest.mark.gpu
 
 
+def test_rotary_refuses_forward_mode():
+    import torch.autograd.forward_ad as fwd
+    from blast3r_b200.rotary import rotary
+    q, k, table, pos = _setup(1, 6, 2, 2, 16, 8, 1, 10, 'f32')
+    with fwd.dual_level():
+        d = fwd.make_dual(q, torch.ones_like(q))
+        for bad in (lambda: rotary(d, table, pos), lambda: rotary((k, d), table, pos), lambda: rotary(d, table, pos, inplace=True)):
+            with pytest.raises(RuntimeError):
+                bad()
+        assert rotary(q, table, pos).shape == q.shape
+
+
+def test_norm_refuses_forward_mode():
+    import torch.autograd.forward_ad as fwd
+    from blast3r_b200.norm import residual_norm
+    y, x, _, _, kw = _make(2, 6, 64, 'f32', 'f32', 'layer', True, True, 'channel')
+    with fwd.dual_level():
+        for bad in (dict(y=fwd.make_dual(y, x)), dict(x=fwd.make_dual(x, y)), dict(gate=fwd.make_dual(kw['gate'], kw['gate']))):
+            with pytest.raises(RuntimeError):
+                residual_norm(**{'y': y, 'x': x, **kw, **bad})
+        assert residual_norm(y, x, **kw)[0].shape == y.shape
+
+
 def test_norm_refuses_what_is_no_tensor():
     from blast3r_b200.norm import residual_norm_forward
     y, x, _, _, kw = _make(2, 6, 64, 'bf16', 'bf16', 'layer', True, True, 'sample')
