@@ -119,6 +119,8 @@ def _rotate(xs, table, positions, interleaved, inverse, inplace):
         keep.append(x)
     L.call_on(dev, 'b3r_rotary', parts, n, B, T, D, code, table.data_ptr(), n_pos, half, axes, positions.data_ptr(), wide,
               0 if shape[0] == 1 else ps[0], ps[1], bool(interleaved), bool(inverse))
+    if inplace:                              # what autograd keeps of them has changed
+        torch.autograd.graph.increment_version([x for x in xs if not x.is_inference()])
     return outs
 
 

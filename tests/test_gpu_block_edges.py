@@ -11,6 +11,23 @@ from tests.test_gpu_rotary import _setup
 pytestmark = pytest.mark.gpu
 
 
+def test_rotary_in_place_counts_as_a_change():
+    """A tensor that an earlier operator keeps for its backward pass: torch reports the change."""
+    from blast3r_b200.rotary import rotary
+    q, k, table, pos = _setup(1, 6, 2, 2, 16, 8, 1, 10, 'f32')
+    w = torch.ones(16, device='cuda', requires_grad=True)
+    y = (k * w).sum()
+    before = k._version
+    rotary(k, table, pos, inplace=True)
+    assert k._version > before
+    with pytest.raises(RuntimeError, match='inplace'):
+        y.backward()
+    with torch.inference_mode():
+        x = q.clone()
+        rotary(x, table, pos, inplace=True)
+    assert torch.equal(x, rotary(q, table, pos))
+
+
 def test_rotary_refuses_forward_mode():
     import torch.autograd.forward_ad as fwd
     from blast3r_b200.rotary import rotary
