@@ -213,6 +213,64 @@ __global__ void __launch_bounds__(kRotThreads) k_rotary_rows(const __grid_consta
           rows[tid + u * kRotThreads];
 }
 
+// Tensors turned in place: whether two of their elements share memory, or might, where strides are not nested
+// or two tensors lie within each other's memory with different batch or token strides.
+struct Extent {
+  int64_t step, na, nb;   // a dimension's stride in bytes, and its sizes in the two tensors
+};
+// The largest stride first; apart: from the one's start to the other's; end_a, end_b: bytes of a last piece.
+bool rot_meet(const Extent* d, int n, int64_t apart, int64_t end_a, int64_t end_b) {
+  if (n == 0) return -end_b < apart && apart < end_a;
+  int64_t reach = 0;
+  for (int i = 1; i < n; ++i) reach += (std::max(d[i].na, d[i].nb) - 1) * d[i].step;
+  if (end_a + end_b + 2 * reach > 8 * d->step) return true;
+  auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  const int64_t first = std::max(1 - d->na, floor_div(-end_b - reach - apart, d->step));
+  const int64_t last = std::min(d->nb - 1, floor_div(end_a + reach - apart, d->step) + 1);
+  for (int64_t k = first; k <= last; ++k)
+    if (rot_meet(d + 1, n - 1, apart + k * d->step, end_a, end_b)) return true;
+  return false;
+}
+bool rot_overlaps(const b3r_rotary_part* parts, int n_parts, int64_t B, int64_t T, int64_t D, int esz) {
+  int64_t step[2][3], size[2][3], begin[2], end[2];
+  for (int p = 0; p < n_parts; ++p) {
+    const b3r_rotary_part& q = parts[p];
+    if (q.heads == 0) return n_parts == 2 && rot_overlaps(parts + 1 - p, 1, B, T, D, esz);
+    const int64_t st[3] = {q.x_batch, q.x_token, q.x_head}, n[3] = {B, T, q.heads};
+    Extent d[3];
+    int dims = 0;
+    for (int i = 0; i < 3; ++i) {
+      step[p][i] = st[i] * esz;
+      size[p][i] = n[i];
+      if (n[i] > 1) d[dims++] = Extent{step[p][i], n[i], n[i]};
+    }
+    std::sort(d, d + dims, [](const Extent& x, const Extent& y) { return x.step < y.step; });
+    int64_t reach = D * esz;
+    for (int i = 0; i < dims; ++i) {
+      if (d[i].step < reach) return true;
+      reach += (d[i].na - 1) * d[i].step;
+    }
+    begin[p] = (int64_t)(uintptr_t)q.x;
+    end[p] = begin[p] + reach;
+  }
+  if (n_parts == 1 || end[0] <= begin[1] || end[1] <= begin[0]) return false;
+  int64_t end_a = D * esz, end_b = D * esz;
+  Extent d[3];
+  int dims = 0;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t sa = step[0][i], sb = step[1][i], na = size[0][i], nb = size[1][i];
+    if (na > 1 && nb > 1 && sa != sb) {
+      if (i < 2) return true;
+      end_a += (na - 1) * sa;          // heads: a token's as one piece
+      end_b += (nb - 1) * sb;
+    } else if (na > 1 || nb > 1) {
+      d[dims++] = Extent{na > 1 ? sa : sb, na, nb};
+    }
+  }
+  std::sort(d, d + dims, [](const Extent& x, const Extent& y) { return x.step > y.step; });
+  return rot_meet(d, dims, begin[1] - begin[0], end_a, end_b);
+}
+
 // Whether heads can be moved in 16-byte pieces, and how many tokens fit a block: 0 if none.
 template <typename T>
 int rot_tokens(const RotArgs& a, int n_parts) {
@@ -327,6 +385,9 @@ extern "C" int b3r_rotary(const b3r_rotary_part* parts, int n_parts, int64_t B, 
     in_place = in_place && same;
   }
   if (B == 0 || T == 0 || heads == 0) return B3R_OK;
+  if (in_place)
+    B3R_REQUIRE(!rot_overlaps(parts, n_parts, B, T, D, dtype == B3R_F32 ? 4 : 2),
+                "rotary in place: elements of the tensors overlap in memory, or might; turn copies of them");
   B3R_REQUIRE(positions, "rotary: NULL positions");
   a.T = T;
   a.D = D;

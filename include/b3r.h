@@ -459,7 +459,8 @@ int b3r_backsub(b3r_plan* plan, const b3r_params* params, const b3r_lin_opts* op
  * =================================================================================== */
 
 /* One tensor of a rotary call: [B, T, heads, D] in x, written to out (x itself for in place,
- * with the same strides; other overlaps are not allowed). */
+ * with the same strides; other overlaps are not allowed, and elements of tensors in place that share
+ * memory are refused). */
 typedef struct {
     const void* x;
     void* out;

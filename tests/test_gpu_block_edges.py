@@ -81,3 +81,56 @@ def test_a_lost_copy_is_reported(monkeypatch, C, stream, gate, kind, weights):
     check_norm()
     again = residual_norm_backward(dr, dh, y, x, **kw)
     assert all(t is None or torch.equal(t, w) for t, w in zip(again, want))
+
+
+def _apart(D=16):
+    """Pairs that share memory and no element, as projections are cut: (q, k)."""
+    n = lambda *s: torch.randn(*s, device='cuda')                             # noqa: E731
+    fused = n(2, 7, 3, 4, D)                                                  # token, part, head
+    heads = n(2, 3, 4, 7, D).transpose(2, 3)                                  # part, head, token
+    mixed = n(2, 7, 4, 2, D)                                                  # head, part
+    uneven = n(2, 7, 6, D)                                                    # four query and two key heads
+    thin = n(2, 1, 5, D)[:, :, :4].expand(2, 1, 4, D)
+    yield fused[:, :, 0], fused[:, :, 1]
+    yield heads[:, 0], heads[:, 1]
+    yield mixed[:, :, :, 0], mixed[:, :, :, 1]
+    yield uneven[:, :, :4], uneven[:, :, 4:]
+    yield uneven[:, :, 4:], uneven[:, :, :4]
+    yield thin[..., :], n(2, 1, 2, D)
+    batch = n(4, 7, 2, D)
+    yield batch[:2], batch[2:]                                                # halves of a batch
+    yield batch[0::2], batch[1::2]
+    time = n(2, 14, 2, D)
+    yield time[:, :7], time[:, 7:]
+    yield time[:, 0::2], time[:, 1::2]
+    one = n(1, 1, 6, D)
+    yield one[:, :, :3].as_strided((1, 1, 3, D), (1, 1, D, 1)), one[:, :, 3:]  # strides of dimensions of one do not matter
+
+
+def test_rotary_in_place_on_parts_of_one_tensor():
+    from blast3r_b200.rotary import rotary, rotary_table
+    table = rotary_table(20, 16)
+    for q, k in _apart():
+        pos = torch.arange(q.shape[1], device='cuda', dtype=torch.int32)[:, None]
+        want = rotary((q, k), table, pos)
+        got = rotary((q, k), table, pos, inplace=True)
+        assert got[0] is q and got[1] is k
+        assert torch.equal(q, want[0]) and torch.equal(k, want[1])
+
+
+def test_rotary_in_place_refuses_overlaps():
+    """An element that lies in two places would be turned twice, by threads that race for it."""
+    from blast3r_b200.rotary import rotary, rotary_table
+    table, pos = rotary_table(20, 16), torch.arange(6, device='cuda', dtype=torch.int32)[:, None]
+    x = torch.randn(2, 6, 4, 16, device='cuda')
+    flat = torch.randn(2000, device='cuda')
+    one = x[:, :, :1]
+    keep = x.clone(), flat.clone()
+    for bad in (one.expand(2, 6, 4, 16), x[:1].expand(2, 6, 4, 16), x[:, :1].expand(2, 6, 4, 16),
+                flat.as_strided((2, 6, 4, 16), (384, 64, 8, 1)), flat.as_strided((2, 6, 4, 16), (64, 16, 96, 1)),
+                (x, x), (x, x[:, :, 1:3]), (x[:, :, :3], x[:, :, 2:]), (x[:, :, 0:3:2], x[:, :, 2:]),
+                (flat.as_strided((2, 6, 1, 16), (192, 32, 32, 1)), flat.as_strided((2, 6, 1, 16), (192, 32, 32, 1), 8)),
+                (one, one.expand(2, 6, 2, 16))):
+        with pytest.raises(RuntimeError, match='overlap'):
+            rotary(bad, table, pos, inplace=True)
+    assert torch.equal(x, keep[0]) and torch.equal(flat, keep[1])
