@@ -140,10 +140,11 @@ def residual_norm_backward(dr, dh, y, r, *, kind='layer', eps=1e-6, post=None, g
     for what is not there), from dr, the gradient that reaches r other than through h, dh
     (None without ``pre``), the block output y and the forward call's r."""
     d, keep = _describe(y, r, kind, eps, post, gate, residual_scale, pre)
-    if not isinstance(dr, torch.Tensor) or not dr.is_cuda or dr.shape != r.shape or dr.dtype != r.dtype:
-        raise RuntimeError('residual_norm backward: dr has the shape and type of r')
-    if d.pre and (not isinstance(dh, torch.Tensor) or not dh.is_cuda or dh.shape != y.shape or dh.dtype != y.dtype):
-        raise RuntimeError('residual_norm backward: dh has the shape and type of y')
+    index = y.get_device()
+    if not isinstance(dr, torch.Tensor) or dr.get_device() != index or dr.shape != r.shape or dr.dtype != r.dtype:
+        raise RuntimeError('residual_norm backward: dr has the shape, type and device of r')
+    if d.pre and (not isinstance(dh, torch.Tensor) or dh.get_device() != index or dh.shape != y.shape or dh.dtype != y.dtype):
+        raise RuntimeError('residual_norm backward: dh has the shape, type and device of y')
     ts = [_rows(t) if t is not None else (None, 0) for t in (dr, dh if d.pre else None, y, r)]
     new = lambda t: None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)   # noqa: E731
     w_post, b_post, g, w_pre, b_pre = keep
@@ -156,7 +157,6 @@ def residual_norm_backward(dr, dh, y, r, *, kind='layer', eps=1e-6, post=None, g
         out.dgate.zero_()                # the library sees no rows and does not know the gate's
     ptr = lambda t: None if t is None else t.data_ptr()                                           # noqa: E731
     args = [a for t, s in ts for a in (ptr(t), s)]
-    index = y.get_device()
     L.call_on(index, 'b3r_residual_norm_bwd_ex', C.byref(d), *args, *[ptr(t) for t in out], wp,
               L.status_word('residual_norm', index).data_ptr(), 0, 0)
     return out

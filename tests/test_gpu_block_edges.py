@@ -11,6 +11,17 @@ from tests.test_gpu_rotary import _setup
 pytestmark = pytest.mark.gpu
 
 
+class _Elsewhere(torch.Tensor):
+    """A tensor that says it is on another GPU."""
+
+    def get_device(self):
+        return 1
+
+    @property
+    def device(self):
+        return torch.device('cuda', 1)
+
+
 def test_rotary_in_place_counts_as_a_change():
     """A tensor that an earlier operator keeps for its backward pass: torch reports the change."""
     from blast3r_b200.rotary import rotary
@@ -49,6 +60,14 @@ def test_norm_refuses_forward_mode():
             with pytest.raises(RuntimeError):
                 residual_norm(**{'y': y, 'x': x, **kw, **bad})
         assert residual_norm(y, x, **kw)[0].shape == y.shape
+
+
+def test_norm_backward_refuses_another_device():
+    from blast3r_b200.norm import residual_norm_backward
+    y, x, dr, dh, kw = _make(2, 6, 64, 'bf16', 'bf16', 'layer', True, True, 'sample')
+    for a, b in ((dr.as_subclass(_Elsewhere), dh), (dr, dh.as_subclass(_Elsewhere))):
+        with pytest.raises(RuntimeError, match='device'):
+            residual_norm_backward(a, b, y, x, **kw)
 
 
 def test_norm_refuses_what_is_no_tensor():
