@@ -63,9 +63,11 @@ def _gate_rows(gate, shape):
     for n in lead:
         rows *= n
     k = len(g)
-    while k > 0 and g[k - 1] == 1 and (len(g) == len(lead) or k <= len(lead)) and lead[k - 1] != 1:
+    if k > len(lead):
+        return None
+    while k > 0 and g[k - 1] == 1:
         k -= 1                                       # (B, 1, C): one row for each of the first dimensions
-    if k > len(lead) or tuple(g[:k]) != tuple(lead[:k]):
+    if tuple(g[:k]) != tuple(lead[:k]):
         return None
     groups = 1
     for n in g[:k]:
@@ -124,7 +126,8 @@ def residual_norm_forward(y, x, *, kind='layer', eps=1e-6, post=None, gate=None,
     """(r, h) for block output y and residual stream x, (..., C) each; h is None without ``pre``.
 
     post, pre: None (no such norm), True (no weights), a weight, or (weight or None, bias or
-    None).  gate: None, or of shape (C,), (B, C), (B, 1, C) or y's.  x may be float32 beside
+    None).  gate: None, or of shape (C,), (B, C), (B, 1, C) or y's
+    (sizes of 1 at the end of its leading dimensions span y's).  x may be float32 beside
     bfloat16 or float16 blocks; r has x's type, h has y's.  1 to 8192 channels."""
     d, keep = _describe(y, x, kind, eps, post, gate, residual_scale, pre)
     (yt, ys), (xt, xs) = _rows(y), _rows(x)

@@ -56,3 +56,16 @@ def test_rotary_overlaps_are_found():
             assert said or not real, (xs[0].stride(), xs[0].shape)
             found, refused, apart = found + real, refused + (said and not real), apart + (not said)
     assert found > 500 and apart > 2000 and refused < 0.12 * apart
+
+
+@pytest.mark.parametrize('lead,gate,rows', [
+    ((6, 2), (), 12), ((6, 2), (6,), 2), ((6, 2), (6, 1), 2), ((6, 2), (6, 2), 1), ((6, 2), (1, 1), 12), ((6, 2), (1,), 12),
+    ((6, 1), (1, 1), 6), ((6, 1), (6, 1), 1), ((6, 1), (1,), 6), ((6, 1), (6,), 1), ((1, 5), (1, 1), 5), ((1, 5), (1, 5), 1),
+    ((1, 1), (1, 1), 1), ((4, 3, 2), (4, 1, 1), 6), ((4, 3, 2), (4, 3, 1), 2), ((4, 3, 2), (1, 1, 1), 24), ((4, 1, 2), (1, 1, 1), 8),
+    ((6, 0), (6, 1), 1), ((6,), (1,), 6), ((), (), 1),
+    ((6, 2), (1, 2), None), ((6, 2), (2,), None), ((6, 2), (6, 3), None), ((6,), (1, 1), None), ((6, 1), (5, 1), None)])
+def test_rows_of_a_gate(lead, gate, rows):
+    """A gate of sizes 1 fits any y that has the dimensions, prompts and single tokens alike."""
+    import torch
+    from blast3r_b200.norm import _gate_rows
+    assert _gate_rows(torch.zeros(*gate, 8), (*lead, 8)) == rows

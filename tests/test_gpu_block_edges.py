@@ -78,6 +78,22 @@ def test_norm_refuses_what_is_no_tensor():
             residual_norm_forward(y, x, **{**kw, **bad})
 
 
+@pytest.mark.parametrize('shape,gate', [((6, 1, 40), (1, 1, 40)), ((6, 2, 40), (1, 1, 40)), ((1, 5, 40), (1, 1, 40)),
+                                        ((1, 1, 40), (1, 1, 40)), ((6, 1, 40), (6, 1, 40)), ((4, 1, 40), (1, 40))])
+def test_gates_of_one_row(shape, gate):
+    """A gate of one row for all fits a prompt and a single token alike."""
+    from blast3r_b200.norm import residual_norm
+    g = torch.Generator(device='cuda').manual_seed(0)
+    y, x, gt, dr = (torch.randn(*s, device='cuda', generator=g).requires_grad_() for s in (shape, shape, gate, shape))
+    r, _ = residual_norm(y, x, gate=gt)
+    assert float((r - (x + gt * y)).abs().max()) <= 2.0 ** -21 * float((x.abs() + (gt * y).abs()).max())
+    r.backward(dr)
+    over = [i for i in range(3) if ((1,) * (3 - len(gate)) + gate)[i] == 1 and shape[i] > 1]
+    want = dr.double() * y.double()
+    want = (want.sum(over, keepdim=True) if over else want).reshape(gate)
+    assert gt.grad.shape == gate and float((gt.grad - want).abs().max()) <= 2.0 ** -20 * shape[0] * shape[1] * 16
+
+
 @pytest.mark.parametrize('C,stream,gate', [(64, 'bf16', None), (1024, 'f32', 'token'), (1000, 'bf16', 'sample'), (1001, 'bf16', 'token'),
                                            (4096, 'bf16', 'channel'), (5120, 'bf16', None)])
 @pytest.mark.parametrize('kind,weights', [('rms', False), ('layer', True)])
