@@ -780,15 +780,30 @@ __global__ void __launch_bounds__(kRedCols * kRedLanes) k_norm_reduce(const __gr
 // ---------------------------------------------------------------- launches
 constexpr int kMaxC = 8192;
 
+// A kernel's dynamic shared memory limit, raised once on each device to all that its own arrays leave.  (Set to each
+// call's need, it could be lowered by another thread's call before the launch that counted on it.)
+template <auto F>
+int most_smem(const char* what) {
+  static uint64_t done = 0;
+  int dev;
+  B3R_TRY(check_cuda(cudaGetDevice(&dev), what));
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (dev < 64 && (__atomic_load_n(&done, __ATOMIC_RELAXED) & bit)) return B3R_OK;
+  cudaFuncAttributes at;
+  B3R_TRY(check_cuda(cudaFuncGetAttributes(&at, F), what));
+  B3R_TRY(check_cuda(cudaFuncSetAttribute(F, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448 - (int)at.sharedSizeBytes), what));
+  __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+  return B3R_OK;
+}
+
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <typename TX, typename TY, int VPT, bool VEC>
 int fwd_kernel(const NormArgs& a, dim3 grid, dim3 block, cudaStream_t s) {
   const int smem = !staged<TY, VEC>() ? 0 : block.y * (slot_bytes<TX, false>(a.C) + slot_bytes<TY, false>(a.C));
-  auto* f = a.post ? k_norm_fwd<TX, TY, VPT, VEC, true> : k_norm_fwd<TX, TY, VPT, VEC, false>;
-  if (smem > 40 * 1024)
-    B3R_TRY(check_cuda(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "residual_norm"));
-  f<<<grid, block, smem, s>>>(a);
+  constexpr auto with = k_norm_fwd<TX, TY, VPT, VEC, true>, without = k_norm_fwd<TX, TY, VPT, VEC, false>;
+  if (staged<TY, VEC>()) B3R_TRY(a.post ? most_smem<with>("residual_norm") : most_smem<without>("residual_norm"));
+  (a.post ? with : without)<<<grid, block, smem, s>>>(a);
   return check_launch("residual_norm");
 }
 
@@ -825,8 +840,8 @@ int bwd_blocks(int64_t rows, int C) {
 
 template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>
 int bwd_kernel(const NormArgs& a, int smem, cudaStream_t s) {
-  auto* f = k_norm_bwd<TX, TY, FULL, VEC, RING, MAXT>;
-  B3R_TRY(check_cuda(cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, smem), "residual_norm backward"));
+  constexpr auto f = k_norm_bwd<TX, TY, FULL, VEC, RING, MAXT>;
+  B3R_TRY(most_smem<f>("residual_norm backward"));
   f<<<bwd_blocks(a.rows, a.C), bwd_threads(a.C), smem, s>>>(a);
   return check_launch("residual_norm backward");
 }

@@ -94,6 +94,46 @@ def test_gates_of_one_row(shape, gate):
     assert gt.grad.shape == gate and float((gt.grad - want).abs().max()) <= 2.0 ** -20 * shape[0] * shape[1] * 16
 
 
+def test_widths_of_one_kernel_from_several_threads():
+    """Calls of one kernel that need different amounts of shared memory, from six threads at once: none takes away what
+    another's launch counts on."""
+    import ctypes as C
+    import threading
+    from blast3r_b200 import _lib as L
+    from blast3r_b200.norm import _describe
+    lib, errors, made = L.lib(), [], []
+    for width in (8191, 7999, 4096, 2048):
+        y, x, dr, dh, _ = _make(1, 2, width, 'bf16', 'f32', 'rms', True, True, None)
+        d, keep = _describe(y, x, 'rms', 1e-5, True, None, 1.0, True)
+        outs = [torch.empty_like(t) for t in (x, y)]
+        work = torch.empty(int(lib.b3r_residual_norm_work_bytes(C.byref(d))) + 256, dtype=torch.uint8, device='cuda')
+        made.append((d, y, x, dr, dh, outs, work, keep))
+    torch.cuda.synchronize()
+
+    def forward(d, y, x, dr, dh, outs, work, keep, stream):
+        return lib.b3r_residual_norm_fwd(C.byref(d), y.data_ptr(), d.C, x.data_ptr(), d.C, outs[0].data_ptr(), outs[1].data_ptr(), stream)
+
+    def backward(d, y, x, dr, dh, outs, work, keep, stream):
+        return lib.b3r_residual_norm_bwd(C.byref(d), dr.data_ptr(), d.C, dh.data_ptr(), d.C, y.data_ptr(), d.C, x.data_ptr(), d.C,
+                                         outs[0].data_ptr(), outs[1].data_ptr(), None, None, None, None, None,
+                                         work.data_ptr() + (-work.data_ptr()) % 256, stream)
+
+    def work(f, args):
+        stream = torch.cuda.Stream()
+        for i in range(20000):
+            if f(*args, stream.cuda_stream):
+                errors.append(lib.b3r_last_error().decode())
+            if i % 500 == 499:
+                stream.synchronize()
+    for f, (a, b) in ((forward, made[:2]), (backward, made[2:])):
+        ts = [threading.Thread(target=work, args=(f, m)) for m in (a, b) * 3]
+        for t in ts:
+            t.start()
+        for t in ts:
+            t.join()
+    assert not errors, (len(errors), errors[0])
+
+
 @pytest.mark.parametrize('C,stream,gate', [(64, 'bf16', None), (1024, 'f32', 'token'), (1000, 'bf16', 'sample'), (1001, 'bf16', 'token'),
                                            (4096, 'bf16', 'channel'), (5120, 'bf16', None)])
 @pytest.mark.parametrize('kind,weights', [('rms', False), ('layer', True)])
