@@ -94,6 +94,47 @@ def test_gates_of_one_row(shape, gate):
     assert gt.grad.shape == gate and float((gt.grad - want).abs().max()) <= 2.0 ** -20 * shape[0] * shape[1] * 16
 
 
+@pytest.mark.parametrize('dtype,stream', [('bf16', 'bf16'), ('f16', 'f16'), ('bf16', 'f32')])
+@pytest.mark.parametrize('pre', [False, True])
+def test_norm_under_autograd(dtype, stream, pre):
+    """16-bit operands and calls without the second norm, through autograd."""
+    from blast3r_b200.norm import residual_norm
+    B, T, C = 3, 25, 96
+    y, x, dr, dh, kw = _make(B, T, C, dtype, stream, 'layer', True, pre, 'sample')
+    ts = [t for t in (y, x, kw['gate'], *kw['post'], *(kw['pre'] or ())) if t is not None]
+    for t in ts:
+        t.requires_grad_()
+    r, h = residual_norm(y, x, **kw)
+    assert (h is None) == (not pre)
+    torch.autograd.backward((r, h) if pre else (r,), (dr, dh) if pre else (dr,))
+    kw = {n: tuple(t.detach() for t in p) if isinstance(p, tuple) else p.detach() if isinstance(p, torch.Tensor) else p for n, p in kw.items()}
+    want = _backward(dr, dh, y.detach(), r.detach(), kw, _sum_of('sample', B))
+    names = ['dy', 'dx', 'dgate', 'dw_post', 'db_post'] + (['dw_pre', 'db_pre'] if pre else [])
+    for name, t in zip(names, ts):
+        R.close(t.grad, *want[name], name)
+
+
+def test_capture():
+    """Rotations and norms, both directions, in a graph."""
+    from blast3r_b200.norm import residual_norm_backward, residual_norm_forward
+    from blast3r_b200.rotary import rotary
+    y, x, dr, dh, kw = _make(3, 50, 264, 'bf16', 'f32', 'layer', True, True, 'sample')
+    q, k, table, pos = _setup(2, 40, 4, 2, 64, 16, 2, 50, 'bf16')
+
+    def run():
+        r, h = residual_norm_forward(y, x, **kw)
+        return (*rotary((q, k), table, pos), r, h, *residual_norm_backward(dr, dh, y, r, **kw))
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for t in (y, q, k, dh):
+        t.mul_(0.75)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, run()))
+
+
 def test_widths_of_one_kernel_from_several_threads():
     """Calls of one kernel that need different amounts of shared memory, from six threads at once: none takes away what
     another's launch counts on."""
