@@ -146,6 +146,8 @@ _SIGS = {
                                  [C.c_int, C.c_int, _vp]),
     'b3r_attention_fwd_work_bytes': (_i64, [C.POINTER(AttentionDesc)]),
     'b3r_attention_fwd': (C.c_int, [C.POINTER(AttentionDesc), _vp]),
+    'b3r_attention_fwd_ex': (C.c_int, [C.POINTER(AttentionDesc), C.c_int, _vp]),
+    'b3r_attention_bwd_ex': (C.c_int, [C.POINTER(AttentionDesc), C.c_int, _vp]),
     'b3r_attention_bwd_work_bytes': (_i64, [C.POINTER(AttentionDesc)]),
     'b3r_attention_bwd': (C.c_int, [C.POINTER(AttentionDesc), _vp]),
     'b3r_pcg_ex': (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_int, _f64, C.c_int, _i64, C.c_int, _vp, _vp, _vp]),

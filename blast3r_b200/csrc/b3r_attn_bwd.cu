@@ -61,6 +61,7 @@ struct alignas(64) BwdArgs {
   int q_stages, go_stages, group;  // rings of Q and dO in k_attn_dkv
   int q_tma;                       // the heads of a group divide 128
   int G;
+  int lose;                   // a test: the first block of each kernel never gets its first tile
   float* delta;               // [B][Hq][Lq]
   float2* range;              // float16: [B][Hkv], the largest |do|^2 and |v|^2 of a row;
   int* far;                   // and [B][Hkv], whether lse / scale or delta of a row is above kMostInParts
@@ -274,7 +275,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
         const int t = (first + it) * kTileRows;
         if (it == free_until) mbar_wait(smem_u32(&sh.own_ready), 0, dead);
         // dS is zero past the last key and meets K's rows there, so they are cleared
-        ring_load<kBlocks, kTileRows>(kr, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
+        if (a.lose && blockIdx.x + it == 0) kr.step();   // (a test: it never comes)
+        else ring_load<kBlocks, kTileRows>(kr, &a.k, (int)s.k0 + t, kv, batch, s.kl - t, true, &sh.fix, fixes, lane, dead);
         ring_load<kBlocks, kTileRows>(vr, &a.v, (int)s.k0 + t, kv, batch, s.kl - t, false, &sh.fix, fixes, lane, dead);
       }
     } else if (warp == 9 && n > 0) {
@@ -505,7 +507,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant_
     for (int it = 0; it < n; ++it) {
       const int i0 = (t0 + t) * kTileRows;
       // P and dS are zero past the last query and meet the rows of dO and Q there
-      ring_load<kBlocks, kTileRows>(qr, &a.q, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
+      if (a.lose && blockIdx.x + it == 0) qr.step();   // (a test: it never comes)
+      else ring_load<kBlocks, kTileRows>(qr, &a.q, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
       ring_load<kBlocks, kTileRows>(gr, &a.go, (int)s.q0 + i0, h, bq, s.ql - i0, true, &sh.fix, fixes, lane, dead);
       if (++t == per_head) {
         t = 0;
@@ -855,12 +858,16 @@ extern "C" int64_t b3r_attention_bwd_work_bytes(const b3r_attention_desc* d) {
   return cut(a);
 }
 
-extern "C" int b3r_attention_bwd(const b3r_attention_desc* d, void* stream) {
+extern "C" int b3r_attention_bwd(const b3r_attention_desc* d, void* stream) { return b3r_attention_bwd_ex(d, 0, stream); }
+
+extern "C" int b3r_attention_bwd_ex(const b3r_attention_desc* d, int flags, void* stream) {
   B3R_TRY(attn_check(d, true));
+  B3R_REQUIRE((flags & ~B3R_ATTENTION_TEST_LOST_COPY) == 0, "attention backward: unknown flags");
   B3R_TRY(attn_clear(d, true, as_stream(stream)));
   if (d->B == 0) return B3R_OK;
   BwdArgs a;
   a.d = *d;
+  a.lose = flags & B3R_ATTENTION_TEST_LOST_COPY;
   if (cut(a) > 0)
     B3R_REQUIRE(d->work && ((uintptr_t)d->work & 255) == 0, "attention backward: work buffer must be 256-byte aligned");
   const int64_t nq = d->cu_q ? d->Tq : d->Lq, nk = d->cu_q ? d->Tk : d->Lk;

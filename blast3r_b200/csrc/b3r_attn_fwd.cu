@@ -53,6 +53,7 @@ struct alignas(64) FwdArgs {
   uint32_t g_mul, g_shift;   // for divisions by G
   int k_stages, v_stages, group;
   int q_tma;        // the heads of a group divide 128: Q comes by TMA, a box of whole groups
+  int lose;         // a test: block 0 never gets its first keys
   float* part_o;    // [splits][B Hkv][rows][D]
   float* part_l;    // [splits][B Hkv][rows]: log2 of the sum, -inf where a part sees nothing
 };
@@ -91,12 +92,12 @@ constexpr int kJobs = 3;   // jobs that a block has in hand at most
 struct Shared {
   uint64_t q_full[2][2], q_empty[2], fix, k_full[kMaxStages], k_empty[kMaxStages], v_full[kMaxStages], v_empty[kMaxStages];
   uint64_t s_full[2][kMaxS], p_full[2][kMaxS], s_free[kMaxS], o_done[2];
-  uint64_t job_full[kJobs], job_empty[kJobs], want, cancel;
+  uint64_t job_full[kJobs], job_empty[kJobs], want, cancel, half_full, half_free;
   alignas(16) uint4 answer;
   Job job[kJobs];
   uint32_t tmem;
   int dead;
-  float m[2][kTileRows], l[2][kTileRows];   // of the second group, where both share a tile; by turns
+  float m[kTileRows], l[kTileRows];   // of the second group, where both share a tile
 };
 
 __device__ __forceinline__ int div_g(const FwdArgs& a, int m) { return (int)((__umulhi((uint32_t)m, a.g_mul) + (uint32_t)m) >> a.g_shift); }
@@ -181,7 +182,7 @@ struct JobList {
   // The next job, once it is there; nullptr after the last.
   __device__ __forceinline__ const Job* get(volatile int* dead) {
     mbar_wait(smem_u32(&sh.job_full[slot]), round & 1, dead);
-    return sh.job[slot].n[0] < 0 || *dead ? nullptr : &sh.job[slot];
+    return __any_sync(0xffffffffu, sh.job[slot].n[0] < 0 || *dead) ? nullptr : &sh.job[slot];
   }
   // Ends the role's use of it (one lane of a warp that has read all it needs).
   __device__ __forceinline__ void done(int lane) {
@@ -257,6 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
     }
     mbar_init(smem_u32(&sh.want), 1);
     mbar_init(smem_u32(&sh.cancel), 1);
+    mbar_init(smem_u32(&sh.half_full), 4);
+    mbar_init(smem_u32(&sh.half_free), 4);
     sh.dead = 0;
     fence_async();
   }
@@ -279,8 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         if (a.q_tma) {                         // rows past the end only reach their own scores
           const int qb = k % X::kQ, use = k / X::kQ;
           const uint32_t bar = smem_u32(&sh.q_full[0][qb]);
-          if (use > 0) mbar_wait(smem_u32(&sh.q_empty[qb]), (use - 1) & 1, dead);
-          if (lane == 0) {
+          const bool free = use == 0 || mbar_wait(smem_u32(&sh.q_empty[qb]), (use - 1) & 1, dead);
+          if (free && lane == 0) {
             mbar_expect(bar, q_bytes);
             for (int w = 0; w < q_tiles; ++w)
 #pragma unroll
@@ -294,7 +297,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         for (int i = 0; i < tiles; ++i) {
           const int row = (j->first + i) * kTileRows;
           if (i == ask && lane == 0) mbar_arrive(smem_u32(&sh.want));   // near the job's end: the next one, not sooner
-          ring_load<X::kBlocks, kTileRows>(kr, &a.k, j->k0 + row, j->kv, batch, j->kl - row, false, &sh.fix, fixes, lane, dead);
+          if (a.lose && blockIdx.x == 0 && k + i == 0) kr.step();   // (a test: these keys never come)
+          else ring_load<X::kBlocks, kTileRows>(kr, &a.k, j->k0 + row, j->kv, batch, j->kl - row, false, &sh.fix, fixes, lane, dead);
           // P is zero past the last key, so V is cleared there
           ring_load<X::kBlocks, kTileRows>(vr, &a.v, j->k0 + row, j->kv, batch, j->kl - row, true, &sh.fix, fixes, lane, dead);
         }
@@ -488,14 +492,15 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
           j.n[0] = j.n[1] = -1;
         }
         if (id < 0 || j.n[0] + j.n[1] > 0) {
-          if (round > 0) mbar_wait(smem_u32(&sh.job_empty[slot]), (round - 1) & 1, dead);
+          const bool free = round == 0 || mbar_wait(smem_u32(&sh.job_empty[slot]), (round - 1) & 1, dead);
+          if (__any_sync(0xffffffffu, !free || *dead)) break;   // (the others see it for themselves)
           j.buf = buf;
           if (lane == 0) {
             sh.job[slot] = j;
             mbar_arrive(smem_u32(&sh.job_full[slot]));
           }
           __syncwarp();
-          if (id < 0 || *dead) break;
+          if (id < 0) break;
           buf = (buf + j.n[0] + j.n[1]) % X::kS;
           if (++slot == kJobs) {
             slot = 0;
@@ -506,9 +511,9 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         }
         if (lane == 0) ask_next(sh);
         __syncwarp();
-        mbar_wait(smem_u32(&sh.cancel), asks & 1, dead);
+        const bool told = mbar_wait(smem_u32(&sh.cancel), asks & 1, dead);
         ++asks;
-        id = *dead ? -1 : read_next(sh);
+        id = __all_sync(0xffffffffu, told) ? read_next(sh) : -1;
         fence_async();                                   // the answer is read before the next one is written
         __syncwarp();
       }
@@ -661,16 +666,16 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
       // ---------------------------------------------- output
       float f0 = 0.f, f1 = 0.f, lg;                      // factors of O (and of the other group's O); log2 of the sum
       if (a.one) {
-        const int half = k & 1;
         if (w == 1) {
-          sh.m[half][r] = mx;
-          sh.l[half][r] = l;
-        }
-        tc_fence_before();
-        bar_sync(1, 256);
-        tc_fence_after();
-        if (w == 0) {
-          const float m1 = sh.m[half][r], l1 = sh.l[half][r], top = fmaxf(mx, m1);
+          sh.m[r] = mx;
+          sh.l[r] = l;
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&sh.half_full));
+        } else {
+          mbar_wait(smem_u32(&sh.half_full), k & 1, dead);
+          tc_fence_after();
+          const float m1 = sh.m[r], l1 = sh.l[r], top = fmaxf(mx, m1);
           const float e0 = mx == -INFINITY ? 0.f : ex2(mx - top), e1 = m1 == -INFINITY ? 0.f : ex2(m1 - top);
           const float sum = l * e0 + l1 * e1;
           f0 = sum > 0.f ? e0 / sum : 0.f;
@@ -737,7 +742,12 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_fwd(const __grid_constant_
         }
       }
       tc_fence_before();
-      if (a.one) bar_sync(2, 256);                       // the other group's O has been read
+      if (a.one) {                                       // the second group's O and sums have been read
+        __syncwarp();
+        if (w == 0 && lane == 0) mbar_arrive(smem_u32(&sh.half_free));
+        if (w == 1) mbar_wait(smem_u32(&sh.half_free), k & 1, dead);
+        tc_fence_after();
+      }
       list.done(lane);
     }
   }
@@ -870,13 +880,17 @@ extern "C" int64_t b3r_attention_fwd_work_bytes(const b3r_attention_desc* d) {
   return a.splits > 1 ? part_rows(a) * (d->D + 1) * 4 : 0;
 }
 
-extern "C" int b3r_attention_fwd(const b3r_attention_desc* d, void* stream) {
+extern "C" int b3r_attention_fwd(const b3r_attention_desc* d, void* stream) { return b3r_attention_fwd_ex(d, 0, stream); }
+
+extern "C" int b3r_attention_fwd_ex(const b3r_attention_desc* d, int flags, void* stream) {
   B3R_TRY(attn_check(d, false));
+  B3R_REQUIRE((flags & ~B3R_ATTENTION_TEST_LOST_COPY) == 0, "attention: unknown flags");
   B3R_TRY(attn_clear(d, false, as_stream(stream)));
   if (d->B == 0 || d->Lq == 0 || (d->cu_q && d->Tq == 0)) return B3R_OK;
   FwdArgs a;
   a.d = *d;
   cut(a);
+  a.lose = flags & B3R_ATTENTION_TEST_LOST_COPY;
   if (a.splits > 1) {
     B3R_REQUIRE(d->work && ((uintptr_t)d->work & 255) == 0, "attention: work buffer must be 256-byte aligned");
     a.part_o = reinterpret_cast<float*>(d->work);

@@ -18,8 +18,10 @@ constexpr int kBlockBytes = kTileRows * 128;   // 128 rows of 64 elements
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // ---- mbarriers.  No wait is endless: after its limit it raises `dead`, which ends the later
-// waits of every role at once; the loops all have fixed counts, so the kernel then runs to its
-// end, frees its tensor memory and reports the failure.
+// waits of every role soon; the loops all have fixed counts, so the kernel then runs to its
+// end, frees its tensor memory and reports the failure.  What a failed wait was for is not done: no copy to a
+// barrier whose last one is still out, no job over one in use.  Lanes see `dead` at different times, so a warp
+// votes on it, and groups of warps meet on mbarriers alone, never on counted barriers after a choice.
 __device__ __forceinline__ void mbar_init(uint32_t bar, int count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
@@ -246,14 +248,16 @@ __device__ __forceinline__ void ring_load(Ring& g, const CUtensorMap* map, int r
   constexpr int kBytes = ROWS * 128;
   const int at = g.stage * BLOCKS * kBytes;
   const bool cut = clear && valid < ROWS;
-  if (g.round > 0) mbar_wait(smem_u32(g.empty + g.stage), (g.round - 1) & 1, dead);
-  if (lane == 0) {
+  bool go = true;
+  if (g.round > 0) go = mbar_wait(smem_u32(g.empty + g.stage), (g.round - 1) & 1, dead);
+  if (cut) go = __all_sync(0xffffffffu, go && !*dead);     // (bar_fix is met at once, unless a wait has failed)
+  if (lane == 0 && go) {
     const uint32_t bar = cut ? bar_fix : full;
     mbar_expect(bar, BLOCKS * kBytes);
 #pragma unroll
     for (int c = 0; c < BLOCKS; ++c) tma_box(g.data + at + c * kBytes, map, c * 64, row, head, batch, bar);
   }
-  if (cut) {
+  if (cut && go) {
     mbar_wait(bar_fix, fixes & 1, dead);
     ++fixes;
     for (int i = max(valid, 0) * 8 + lane; i < ROWS * 8; i += 32)

@@ -566,6 +566,12 @@ int b3r_attention_fwd(const b3r_attention_desc* d, void* stream);
 int64_t b3r_attention_bwd_work_bytes(const b3r_attention_desc* d);
 int b3r_attention_bwd(const b3r_attention_desc* d, void* stream);
 
+/* The same with flags: 0, or B3R_ATTENTION_TEST_LOST_COPY, a test of the path that sets the status word: one
+ * tile of the first block is never asked for, and the wait for it runs out after about a second. */
+#define B3R_ATTENTION_TEST_LOST_COPY 1
+int b3r_attention_fwd_ex(const b3r_attention_desc* d, int flags, void* stream);
+int b3r_attention_bwd_ex(const b3r_attention_desc* d, int flags, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -261,3 +261,28 @@ def test_packed_without_sequences():
     _poison()
     grads = attention_backward(do, q, k, v, o, lse, **kw)
     assert all(float(t.abs().max()) == 0 for t in (o, *grads)) and bool((lse == -math.inf).all())
+
+
+# ---------------------------------------------------------------- a wait that runs out
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('G,Lq,Lk', [(2, 1, 900), (3, 1, 900), (2, 300, 700), (3, 300, 700)])
+def test_a_lost_copy_is_reported(monkeypatch, D, G, Lq, Lk):
+    """A tile that is never asked for: the wait for it runs out, the call ends, check_attention raises once, and the next
+    call is right.  Both halves on one tile of rows or on their own, Q by TMA or written by them."""
+    from blast3r_b200 import _lib as L
+    from blast3r_b200 import attention as A
+    q, k, v, do = _dense(40, Lq, Lk, 4 * G, 4, D, 'f16')
+    o, lse = A.attention_forward(q, k, v)
+    grads = A.attention_backward(do, q, k, v, o, lse)
+    A.check_attention()
+    call = L.call_on
+    for f in (lambda: A.attention_forward(q, k, v), lambda: A.attention_backward(do, q, k, v, o, lse)):
+        monkeypatch.setattr(L, 'call_on', lambda index, name, d: call(index, name + '_ex', d, 1))
+        f()
+        monkeypatch.undo()
+        with pytest.raises(L.B3RError, match='ran out'):
+            A.check_attention()
+        A.check_attention()
+    again = A.attention_forward(q, k, v)
+    assert torch.equal(again[0], o) and torch.equal(again[1], lse)
+    assert all(torch.equal(a, b) for a, b in zip(A.attention_backward(do, q, k, v, o, lse), grads))
