@@ -18,7 +18,7 @@
 // results do not change from run to run.
 //
 // Measured on one B200, where a copy moves 6.5 TB/s: forward, 49216 layer-norm rows of 1024, float32 stream and
-// bfloat16 branch, 93 us (6.5 TB/s); backward, 32768 RMS rows of 4096, bfloat16, two norms and a gate, 383 us
+// bfloat16 branch, 93 us (6.5 TB/s); backward, 32768 RMS rows of 4096, bfloat16, two norms and a gate, 382 us
 // (4.2 TB/s) and 7 us for the partials.  There one block of 512 threads fills an SM's registers, so the
 // latency of a row's sum, barrier included, is hidden by nothing but the copies of the next rows.  Rows
 // that no vector divides take two to three times as long (forward: 18600 rows of 2647, 268 us).
@@ -438,7 +438,7 @@ __host__ __device__ inline int stage_bytes(int C) {
 // Without means every sum of a row is linear in the raw products, the statistics being factors: with
 // p = w_post g y and rho, sigma the inverse norms of r and y,
 //   sum(dn w_post yhat) = sigma (sum dr p + rho (sum z p - rho^2 mean(z r) sum r p)),
-// so six sums and one barrier a row do (32768 rows of 4096: 381 us, with a second sum after the first 456).
+// so six sums and one barrier a row do (32768 rows of 4096: 382 us, with a second sum after the first 456).
 // With means the centred rows are summed: three barriers.  More than 512 threads have no registers for the six
 // (640 threads, rows of 5120: 495 us against 393 with two sums): two.
 template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>
@@ -524,7 +524,6 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
     keep(2, reinterpret_cast<const char*>(a.gate) + group * C * (a.wf32 ? 4 : sizeof(TY)), 1.f);
   }
   int st = 0, round = 0;
-  bool lost = false;                                        // a copy never came
   for (int64_t row = first; row < last; ++row) {
     const uint8_t* at = ring + (size_t)st * stage_bytes<TX, TY, VEC>(C);
     auto fetch = [&](float2 (&o)[kP], int off, auto type, const void* p, int64_t step, bool on) {
@@ -552,8 +551,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
       }
     };
     if (RING && !mbar_wait(smem_u32(&full[st]), round & 1, dead, a.wait_limit)) {
-      if (tid == 0 && !lost) asked = min(asked, max((int)(row - first) - 1, 0) + a.stages);
-      lost = true;
+      if (tid == 0) asked = min(asked, max((int)(row - first) - 1, 0) + a.stages);
     }
     float2 r[kP], dh[kP], y[kP], z[kP], d[kP];
     fetch(r, bytes_x, TX(), a.x, a.x_row, a.pre);
@@ -625,7 +623,7 @@ __global__ void __launch_bounds__(MAXT) k_norm_bwd(const __grid_constant__ NormA
 #pragma unroll
     for (int k = 0; k < kQ; ++k) q[k] = t[k].x + t[k].y;
     row_sum<kQ, MAXT <= 512 ? 16 : 32>(q, warps, buf, turn);
-    if (RING && tid == 0 && row > first && !lost) request(row - 1 + a.stages);   // every thread has left the row before
+    if (RING && tid == 0 && row > first && !*dead) request(row - 1 + a.stages);   // every thread has left the row before
     if (a.pre) {
       const float rstd = rsqrtf(q[0] * inv + a.eps), proj = -q[2] * inv * rstd;   // -mean(z rhat)
       if constexpr (kOne) q[3] += rstd * (q[4] + proj * rstd * q[5]);
@@ -853,8 +851,8 @@ int bwd_launch(NormArgs a, cudaStream_t s) {
   a.stages = std::min(kMaxStages, (room - weights) / stage);
   if (a.stages >= 2) {
     const int smem = weights + a.stages * stage;
-    // registers of a thread: 128, 96 and 64 (18600 bfloat16 rows of 5120 with 96: RMS 393 us, layer norm 525; with
-    // 64, where they do not hold a row's columns and their sums, 508 and 715)
+    // registers of a thread: 128, 96 and 64 (18600 bfloat16 rows of 5120 beside a float32 stream with 96: RMS 393 us,
+    // layer norm 546; with 64, where they do not hold a row's columns and their sums, 508 and 715)
     if (threads <= 512) return bwd_kernel<TX, TY, FULL, VEC, true, 512>(a, smem, s);
     if (threads <= 640) return bwd_kernel<TX, TY, FULL, VEC, true, 640>(a, smem, s);
     return bwd_kernel<TX, TY, FULL, VEC, true, 1024>(a, smem, s);
