@@ -131,7 +131,8 @@ def attention_forward(q, k, v, *, causal=False, scale=None, q_lens=None, k_lens=
     max_k, bounds of their lengths: rows past them are not used.  Rows of no sequence have o = 0,
     lse = -inf and zero gradients.  causal: query i sees the keys j <= i + k_len - q_len, so the last query sees
     the last key.  A query that sees no key has o = 0 and lse = -inf.  scale: finite, 2**-100 at least,
-    D**-0.5 by default."""
+    D**-0.5 by default.  Scores, their statistics and sums are float32; the probabilities are rounded to
+    the inputs' type for their product with v, and o at the end."""
     d, packed, keep = _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k)
     q, k, v = _readable(q), _readable(k), _readable(v)
     o = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -146,8 +147,9 @@ def attention_backward(do, q, k, v, o, lse, *, causal=False, scale=None, q_lens=
                        max_q=None, max_k=None):
     """(dq, dk, dv) from do, the gradient of o, with the forward call's inputs, outputs and keywords.
 
-    The probabilities and their gradient are rounded to the inputs' type for the matrix products (in
-    float16 with powers of two that keep small ones out of its subnormal range)."""
+    The probabilities are recomputed from lse in float32, and they and their gradient are rounded to the
+    inputs' type for the matrix products (in float16 with powers of two that keep small ones out of
+    its subnormal range); the rounded o gives delta."""
     d, packed, keep = _describe(q, k, v, causal, scale, q_lens, k_lens, cu_q, cu_k, max_q, max_k)
     for name, t in (('do', do), ('o', o)):
         if not isinstance(t, torch.Tensor) or t.shape != q.shape or t.dtype != q.dtype or t.device != q.device:

@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(256) k_attn_range(const __grid_constant__ BwdA
 // Tensor memory: S at 0, dP at 128, dq at 256, and the block's own rows of Q and dO after it, as left operands.
 // The next S starts as soon as this one has been read; dS overwrites dP, each half in place.  A left operand in
 // shared memory costs about 100 cycles for each 16 of the head size where one in tensor memory costs the product's 64,
-// so Q and dO are copied over once.  Measured on one B200: 2 x 4096 causal, 32/8 heads of 128, 351 us (1170 TFLOP/s over
+// so Q and dO are copied over once.  Measured on one B200: 2 x 4096 causal, 32/8 heads of 128, 353 us (1168 TFLOP/s over
 // the three products: tensor pipe 59 % busy, the elementwise part beside it); 20 packed sequences of up to 1025,
 // 16 heads of 64, 134 us (a third of a block's time is its start and end).
 template <int DP, typename T>
@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(kThreads, 1) k_attn_dq(const __grid_constant__
 // at P of tile t, the tensor cores are at dk of tile t - 1 and dP of tile t; while they are at dS of t, at
 // dv of t and S of t + 1.  Up to a head size of 64 there is room for two of S^T, and S of t + 1 starts
 // before P of t is there (the groups waited 750 of 2600 cycles for it).  Measured on one B200: 2 x 4096 causal, 32/8 heads
-// of 128, 430 us (1280 TFLOP/s over the four products, tensor pipe 70 % busy: K and V are left operands in shared
-// memory, since the accumulators fill tensor memory); 20 packed sequences of up to 1025, 16 heads of 64, 176 us.
+// of 128, 436 us (1260 TFLOP/s over the four products, tensor pipe 71 % busy: K and V are left operands in shared
+// memory, since the accumulators fill tensor memory); 20 packed sequences of up to 1025, 16 heads of 64, 178 us.
 template <int DP, typename T>
 __global__ void __launch_bounds__(kThreads, 1) k_attn_dkv(const __grid_constant__ BwdArgs a) {
   extern __shared__ uint8_t raw[];

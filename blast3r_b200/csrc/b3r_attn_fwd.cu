@@ -24,11 +24,14 @@
 //
 // What bounds it, measured on one B200 (1669 TFLOP/s, 6.5 TB/s):
 //   one query over 32768 keys (16 sequences, 32/8 heads of 128): 228 us, 5.6 TB/s: HBM
-//   769 x 769 (64 sequences, 16 heads of 64, float16): 421 us, 368 TFLOP/s: the exponentials (16 a cycle and SM: 2048
-//     cycles a step of two tiles, which takes 2100 to 2500), tiles that 769 = 6 x 128 + 1 leaves nearly
-//     empty, and 4000 cycles at a job's end
-//   16384 x 16384, causal, 16/4 heads of 128: 885 us in a burst, 1240 TFLOP/s (1030 to 1080 in a long run, at the power
+//   769 x 769 (64 sequences, 16 heads of 64, float16): 406 us, 382 TFLOP/s: no pipe (exponentials busy 38 %, tensor cores
+//     24 %).  A step of two tiles takes 2100 to 2500 cycles (its exponentials 2048, 16 a cycle and SM), a job's end
+//     4000; tiles that 769 = 6 x 128 + 1 leaves nearly empty run alone; a third of a mean job's 29 thousand
+//     cycles is not accounted for
+//   16384 x 16384, causal, 16/4 heads of 128: 890 us in a burst, 1235 TFLOP/s (1030 to 1080 in a long run, at the power
 //     limit): the products, 88 cycles for each 16 of the head size with Q in shared memory
+// The softmax groups' 208 registers leave no room for what all roles share: 112 to 148 bytes of it lie in local memory,
+// written once (without their code nothing spills; each other role accounts for some of the loads).
 #include <algorithm>
 #include "b3r_attn.cuh"
 #include "b3r_tc.cuh"

@@ -22,7 +22,7 @@ if __name__ == '__main__':
 
 from blast3r_b200.attention import attention, check_attention   # noqa: E402
 from blast3r_b200.engine import lm_step                          # noqa: E402
-from blast3r_b200.norm import residual_norm                      # noqa: E402
+from blast3r_b200.norm import check_norm, residual_norm                      # noqa: E402
 from blast3r_b200.rotary import rotary, rotary_table             # noqa: E402
 from blast3r_b200.synthetic import make_scene                    # noqa: E402
 
@@ -100,6 +100,7 @@ def main(n_imgs=24, n_tracks=3000, lm_steps=3, train_steps=60, seed=0, verbose=T
         if verbose and step % 10 == 0:
             print(f'step {step:3d}  loss {losses[-1]:.4f}')
     check_attention()
+    check_norm()
     if verbose:
         print(f'{sc.n_obs} observations of {n_imgs} images: loss {losses[0]:.4f} -> {losses[-1]:.4f}')
     assert all(math.isfinite(v) for v in losses)

@@ -491,7 +491,9 @@ int b3r_rotary(const b3r_rotary_part* parts, int n_parts, int64_t B, int64_t T, 
  * gate: [rows / rows_per_gate, C] or NULL (1): one row for all (a channel scale), one per sequence,
  * or one per row.  y, h have dtype; x, r have stream_dtype (dtype or B3R_F32); weights, biases,
  * gate and their gradients have weight_dtype (dtype or B3R_F32).  C <= 8192.  Sums are float32;
- * h is computed from r before r is rounded.  Outputs are contiguous rows. */
+ * h is computed from r before r is rounded.  Outputs are contiguous rows.  Input rows are read in whole 16-byte
+ * units: up to 15 bytes before and after a row, in the aligned units that it begins and ends in, are read and
+ * not used. */
 typedef struct {
     int64_t rows, rows_per_gate;
     int32_t C, kind, dtype, stream_dtype, weight_dtype, post, pre;
@@ -537,6 +539,7 @@ int b3r_residual_norm_bwd_ex(const b3r_residual_norm* d, const void* dr, int64_t
  *   packed: cu_q, cu_k (device int32 [B + 1], not NULL, not decreasing) hold where each sequence begins and
  *     ends among Tq / Tk rows; the batch strides are not used and Lq / Lk bound the lengths: rows past
  *     them are not used.  Rows of no sequence get o = 0, lse = -inf and zero gradients.
+ * Scores, statistics and sums are float32; P and, backward, dS are rounded to dtype for their products.
  * What lies in rows past a sequence's end is not used, NaN included.  Lengths and offsets
  * outside of the tensors are cut to them.  Strides (batch, row, head) in elements, multiples
  * of 8, with 16-byte aligned bases; lse is float with strides of its own. */
