@@ -761,7 +761,6 @@ __global__ void __launch_bounds__(256) k_attn_add(const __grid_constant__ BwdArg
   *reinterpret_cast<uint2*>(out + c) = make_uint2(pack2(t.x, t.y, T()), pack2(t.z, t.w, T()));
 }
 
-constexpr int kSms = 148;
 int64_t align256(int64_t b) { return (b + 255) & ~int64_t(255); }
 
 int64_t cut(BwdArgs& a) {     // returns the workspace's bytes

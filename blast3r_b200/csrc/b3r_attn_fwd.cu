@@ -815,8 +815,6 @@ __global__ void __launch_bounds__(128) k_attn_join(const __grid_constant__ FwdAr
   if (lane == 0) *attn_row<float>(d.lse, b, s.q0 + i, h) = sum == 0.f ? -INFINITY : (top + __log2f(sum)) * kLn2;
 }
 
-constexpr int kSms = 148;
-
 // How the work is cut, from the descriptor alone (the lengths on the device are not known here).
 void cut(FwdArgs& a) {
   const b3r_attention_desc& d = a.d;

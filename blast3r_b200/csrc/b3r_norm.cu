@@ -811,7 +811,7 @@ int fwd_launch(const NormArgs& a, cudaStream_t s) {
   // leave the SMs idle either way, so there they are spread over more threads for latency.
   const int C = a.C;
   int threads, vpt;
-  if (a.rows >= 148 * 4 && C <= 1024) {
+  if (a.rows >= kSms * 4 && C <= 1024) {
     threads = 32;
     vpt = C <= 256 ? 1 : C <= 512 ? 2 : 4;
   } else {
@@ -833,7 +833,7 @@ int bwd_threads(int C) { return (C + kE * 32 - 1) / (kE * 32) * 32; }
 // each block writes partial sums of every column.
 int bwd_per_sm(int C) { return std::max(1, std::min(16, 512 / bwd_threads(C))); }
 int bwd_blocks(int64_t rows, int C) {
-  return (int)std::min<int64_t>({rows, 148 * bwd_per_sm(C), std::max<int64_t>(148, rows / 16)});
+  return (int)std::min<int64_t>({rows, kSms * bwd_per_sm(C), std::max<int64_t>(kSms, rows / 16)});
 }
 
 template <typename TX, typename TY, bool FULL, bool VEC, bool RING, int MAXT>

@@ -311,7 +311,7 @@ int rot_launch(RotArgs& a, int n_parts, int64_t tokens, cudaStream_t s) {
   for (int p = 0; p < n_parts; ++p) {
     const int heads = a.part[p].heads;
     int64_t lanes = (heads + kRotHeads - 1) / kRotHeads;
-    if (tokens * a.slots * lanes < (int64_t)148 * 1024) lanes = heads;
+    if (tokens * a.slots * lanes < (int64_t)kSms * 1024) lanes = heads;
     const int64_t n = tokens * a.slots * lanes;
     B3R_REQUIRE(n <= 0x7fffff00, "rotary: too many tokens for one call");
     a.lanes[p] = (int)lanes;
@@ -327,9 +327,9 @@ int rot_run(RotArgs& a, int n_parts, int64_t tokens, bool il, bool copy_rest, cu
   const int rot = a.axes * 2 * a.half;
   int v = rot_vector(a, n_parts, sizeof(T), il);
   // (below a block for every SM the slots are spread over more threads: one token 2.5 us against 3.2)
-  if (v * (int)sizeof(T) < 16 && tokens >= 148) {
+  if (v * (int)sizeof(T) < 16 && tokens >= kSms) {
     if (int per = rot_tokens<T>(a, n_parts)) {
-      per = (int)std::max<int64_t>(1, std::min<int64_t>(per, tokens / (148 * 4)));   // few tokens: spread over the SMs
+      per = (int)std::max<int64_t>(1, std::min<int64_t>(per, tokens / (kSms * 4)));   // few tokens: spread over the SMs
       const int64_t blocks = (tokens + per - 1) / per;
       B3R_REQUIRE(tokens <= 0x7fffffff, "rotary: too many tokens for one call");
       RowDivs dv;

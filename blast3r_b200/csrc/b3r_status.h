@@ -8,6 +8,8 @@
 
 namespace b3r {
 
+constexpr int kSms = 148;   // of a B200: what the block operators' grids are sized by
+
 std::string& last_error_ref();
 
 inline int fail(int code, const char* fmt, ...) {

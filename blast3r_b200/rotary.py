@@ -145,7 +145,8 @@ def rotary(xs, table, positions, *, interleaved=False, inverse=False, inplace=Fa
     table: ``rotary_table``, whose pairs give the size of a section; axis a turns the a-th section
     of the head, and elements past the sections pass through.  interleaved: pairs side by side
     instead of half a section apart.  inverse turns back.  inplace overwrites xs (not with
-    gradients).  A position outside of the table gives NaN.  Differentiable in xs."""
+    gradients, nor where elements of xs overlap in memory).  A position outside of the table gives
+    NaN.  Differentiable in xs."""
     pair = isinstance(xs, (tuple, list))
     ts = tuple(xs) if pair else (xs,)
     L.refuse_tangents('rotary', ts)
